@@ -204,6 +204,7 @@ int t0_rt_selftest_drop_one_load(t0_runtime* rt);
  *   t0_matmul_f32*, t0_blas_gemm_f32: bf16 copies of the operands, T0_SCRATCH_F32_A / _B = elements * 2 (an operand whose
  *     rows are not a multiple of 8 elements: T0_SCRATCH_OPERAND_A / _B = rows * roundup(columns, 8) * 2), and, for
  *     alpha/beta other than 1/0 or ldc != n, T0_SCRATCH_F32_C = m * n * 4;
+ *   t0_kv4_attention: T0_SCRATCH_KV4, t0_kv4_scratch_bytes(rt) bytes, a fixed size per device, on the first call;
  *   t0_gemm_host and the multi-GPU host entry: pinned staging sets and device operands made on first use per shape.
  * Everything else (aligned shapes of the bf16 GEMM, into however many parts the library cuts their K, the one-launch split-K,
  * t0_w4a16_gemm_static) never allocates.
@@ -217,7 +218,7 @@ int t0_rt_selftest_drop_one_load(t0_runtime* rt);
  * neither allocate nor synchronise. */
 enum {
     T0_SCRATCH_OPERAND_A = 0, T0_SCRATCH_OPERAND_B = 1, T0_SCRATCH_SPLITK_PLANES = 2, T0_SCRATCH_W4_WEIGHTS = 3,
-    T0_SCRATCH_W4_FUSED = 4, T0_SCRATCH_F32_A = 5, T0_SCRATCH_F32_B = 6, T0_SCRATCH_F32_C = 7
+    T0_SCRATCH_W4_FUSED = 4, T0_SCRATCH_F32_A = 5, T0_SCRATCH_F32_B = 6, T0_SCRATCH_F32_C = 7, T0_SCRATCH_KV4 = 8
 };
 int t0_rt_reserve_scratch(t0_runtime* rt, int which, size_t bytes);
 size_t t0_rt_w4_fused_scratch_bytes(const t0_runtime* rt);
@@ -553,6 +554,87 @@ size_t t0_gptq_gpu_buffer_size(uint32_t rows, uint32_t cols, uint32_t group_size
  * Scales are rounded (RNE) to bf16; returns how many were not exactly representable, or -1 on error. */
 long t0_gptq_to_b200(const uint8_t* packed, const float* scales, const int32_t* zero_points, uint32_t rows, uint32_t cols,
                      uint32_t group_size, uint32_t* packed_out, uint16_t* scales_out, uint32_t* zeros_out);
+
+/* ------------------------------------------------------- key/value cache in four bits */
+/* What stands between the projections of a step and its output projection (no counterpart in the reference, which plans attention,
+ * src/t0/tile_ir.rs:8487-8524, and quantises weights, src/t0/quant_kernels.rs:53-171, but keeps no cache): keys and values are kept in
+ * pages, four bits a number, and attended to from there.  The rows these entries take are what t0_w4a16_gemm* (f32) and t0_gemm_launch
+ * (f32 or bf16) write, and the rows t0_kv4_attention writes are the bf16 activations the next W4A16 product reads.
+ *
+ * The cache is an array of n_pages pages of page_size (16, 32 or 64) tokens; t0_kv4_page_bytes gives a page's size.  A page holds one
+ * block of page_size * (head_dim + 8) bytes for each key/value head (head_dim 64 or 128):
+ *   K codes [page_size][head_dim / 2], V codes [page_size][head_dim / 2], K parameters [page_size] {bf16 step, bf16 low}, V parameters
+ *   likewise.  Code e of a row lies in 32-bit word e / 8 of the row, at nibble (e % 8) / 2 + 4 (e % 2) (the order of the tile-major
+ *   weight layout), and stands for step * code + low.
+ * A row x is held as  low = max bf16 <= min(x),  step = min bf16 >= (max(x) - low) / 15 (0 where that is below 2^-126),
+ * code = clamp(rint((x - low) / step), 0, 15), every operation rounded to f32.  A row that holds an infinity or a NaN, or whose range
+ * overflows, is held as NaN throughout (step = low = NaN, codes 0).
+ *
+ * One record describes the batch for all three entries.  Sequence b holds seq_lens[b] tokens, the rows of this call included; token p is
+ * in slot p % page_size of page page_table[b][p / page_size].  Its rows in the call are row_start[b] .. row_start[b + 1] - 1 of the row
+ * arrays (row_start = 0: max_rows rows for every sequence, and n_rows = n_seqs * max_rows), and they are its last tokens: row i of n is
+ * token seq_lens[b] - n + i.  Rows for which that is negative (an empty slot of a recorded batch) have no token; rows that belong to no
+ * sequence are neither read nor written.  page_table, seq_lens and row_start are read on the device when the call runs, so a recorded call may be
+ * replayed with other values in them.  What they hold is checked there: a sequence with a negative length, more tokens than its row of
+ * the table has places, rows outside n_rows or more than max_rows of them is left out, a page outside the cache is left out, and the next
+ * synchronising call returns T0_ERR_BOUNDS (the runtime is not poisoned).  Sequences may share pages that they only read; a token's place
+ * must not be another's whose row is in the same append. */
+typedef struct t0_kv4_batch {
+    uint64_t pages;          /* the cache; 16-byte aligned */
+    uint64_t page_table;     /* i32 [n_seqs][table_stride] */
+    uint64_t seq_lens;       /* i32 [n_seqs] */
+    uint64_t row_start;      /* i32 [n_seqs + 1], or 0 */
+    uint32_t n_pages, page_size, n_kv_heads, head_dim;
+    uint32_t n_seqs, table_stride;
+    uint32_t n_rows;         /* rows of the row arrays */
+    uint32_t max_rows;       /* the most rows of one sequence */
+} t0_kv4_batch;
+/* bytes of one page, all heads; 0 for a page size or head dimension the library has no kernels for */
+size_t t0_kv4_page_bytes(uint32_t page_size, uint32_t n_kv_heads, uint32_t head_dim);
+/* Puts the rows' keys and values into the cache and rotates keys and queries by their positions on the way.  q / k / v: rows of n_q_heads /
+ * n_kv_heads heads of head_dim numbers, bf16 or (in_f32) f32; q = 0 leaves queries out.  q_out receives the rotated queries in bf16 (it may be q itself
+ * where q is bf16 and the strides agree).  Strides are in numbers, 0 = dense, multiples of 8 (f32: 4); rows start on 16-byte boundaries.
+ * rope = 0: no rotation.  Else the first rot_dim numbers (a multiple of 16) of each head are turned in pairs: pair i is (x[i], x[i + rot_dim / 2]),
+ * with `interleaved` (x[2i], x[2i + 1]), and (a, b) becomes (a c - b s, b c + a s), each operation rounded to f32, with (c, s) = rope[position][i].
+ * positions = 0: a row's position is its token's place in the sequence.  Else position a of row r is positions[a][r] and pair i takes the axis
+ * whose run of axis_pairs[a] pairs holds i, in order (n_axes 1 .. 3; axis_pairs sum to rot_dim / 2; with one axis they may be 0).  A row with a position outside the
+ * rope table is left out (T0_ERR_BOUNDS at the next synchronising call), a row without a token too. */
+typedef struct t0_kv4_append_args {
+    uint64_t q, k, v;
+    uint64_t q_out;          /* bf16 */
+    uint64_t rope;           /* f32 [n_positions][rot_dim / 2][2]: cosine, sine; 16-byte aligned; or 0 */
+    uint64_t positions;      /* i32 [n_axes][n_rows], or 0 */
+    uint32_t q_stride, k_stride, v_stride, q_out_stride;
+    uint32_t n_q_heads;
+    uint32_t n_positions, rot_dim, n_axes;
+    uint32_t axis_pairs[3];
+    uint8_t in_f32, interleaved;
+    uint8_t _pad[2];
+} t0_kv4_append_args;
+int t0_kv4_append(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_append_args* args);
+/* Reads the rows' keys and values out of the cache as bf16 (step * code + low, rounded once), into rows of n_kv_heads heads of head_dim: k_out and
+ * v_out, 16-byte aligned, strides multiples of 8 (0 = dense); one of them may be 0.  Rows without a token become zeros.  (With row_start and max_rows
+ * covering whole sequences this moves sequences out of the cache; t0_kv4_append without rope puts them back.) */
+typedef struct t0_kv4_dequant_args {
+    uint64_t k_out, v_out;
+    uint32_t k_out_stride, v_out_stride;
+} t0_kv4_dequant_args;
+int t0_kv4_dequant(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_dequant_args* args);
+/* Attention of the rows over their sequences' cached tokens: row at token p sees the tokens j <= p, with window > 0 those with
+ * j > p - window, and y = sum_j softmax_j(scale * q . k_j) v_j for each of its n_q_heads heads (a multiple of n_kv_heads, at most 64 to a
+ * key/value head; head h reads key/value head h / (n_q_heads / n_kv_heads)).  q and y are bf16 rows, 16-byte aligned, strides multiples of 8 (0 = dense);
+ * y may be q itself.  scale is positive and finite.  A row without a token, or that sees none, becomes zeros.  Sums and softmax statistics are f32.
+ * The rows' own tokens are read from the cache like any other: call t0_kv4_append first.  The work is cut by what the device finds in the batch, not by host
+ * values, so a recorded call stays balanced when its lengths change; sums are added in an order that depends on the batch alone, so a call repeats bit for bit. */
+typedef struct t0_kv4_attention_args {
+    uint64_t q, y;
+    uint32_t q_stride, y_stride;
+    uint32_t n_q_heads, window;
+    float scale;
+    uint32_t _pad;
+} t0_kv4_attention_args;
+int t0_kv4_attention(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_attention_args* args);
+size_t t0_kv4_scratch_bytes(const t0_runtime* rt);
 
 /* ------------------------------------------------------- multi-GPU sharding */
 /* The reference is single-GPU (its MultiGpuManager bounces through host memory, src/universal/runtime/multi_gpu.rs:64-159);

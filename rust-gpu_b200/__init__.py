@@ -272,6 +272,37 @@ class W4A16Args(C.Structure):
                 ("m", C.c_uint32), ("n", C.c_uint32), ("k", C.c_uint32), ("group", C.c_uint32)]
 
 
+class Kv4Batch(C.Structure):
+    """``t0_kv4_batch``: a paged four-bit key/value cache and the rows of one call."""
+    _fields_ = [("pages", C.c_uint64), ("page_table", C.c_uint64), ("seq_lens", C.c_uint64), ("row_start", C.c_uint64),
+                ("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("n_seqs", C.c_uint32), ("table_stride", C.c_uint32), ("n_rows", C.c_uint32), ("max_rows", C.c_uint32)]
+
+
+class Kv4AppendArgs(C.Structure):
+    """``t0_kv4_append_args``."""
+    _fields_ = [("q", C.c_uint64), ("k", C.c_uint64), ("v", C.c_uint64), ("q_out", C.c_uint64), ("rope", C.c_uint64), ("positions", C.c_uint64),
+                ("q_stride", C.c_uint32), ("k_stride", C.c_uint32), ("v_stride", C.c_uint32), ("q_out_stride", C.c_uint32),
+                ("n_q_heads", C.c_uint32), ("n_positions", C.c_uint32), ("rot_dim", C.c_uint32), ("n_axes", C.c_uint32),
+                ("axis_pairs", C.c_uint32 * 3), ("in_f32", C.c_uint8), ("interleaved", C.c_uint8), ("_pad", C.c_uint8 * 2)]
+
+
+class Kv4DequantArgs(C.Structure):
+    """``t0_kv4_dequant_args``."""
+    _fields_ = [("k_out", C.c_uint64), ("v_out", C.c_uint64), ("k_out_stride", C.c_uint32), ("v_out_stride", C.c_uint32)]
+
+
+class Kv4AttentionArgs(C.Structure):
+    """``t0_kv4_attention_args``."""
+    _fields_ = [("q", C.c_uint64), ("y", C.c_uint64), ("q_stride", C.c_uint32), ("y_stride", C.c_uint32),
+                ("n_q_heads", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("_pad", C.c_uint32)]
+
+
+def kv4_page_bytes(page_size: int, n_kv_heads: int, head_dim: int) -> int:
+    """``t0_kv4_page_bytes``: bytes of one page of the cache, 0 where the library has no kernels for the sizes."""
+    return int(lib().t0_kv4_page_bytes(page_size, n_kv_heads, head_dim))
+
+
 class Int4WmmaConfig(C.Structure):
     """``Int4WmmaConfig`` (quant_kernels.rs:316-336): the INT4 tile record and its two constructors."""
     _fields_ = [("tile_m", C.c_uint32), ("tile_n", C.c_uint32), ("tile_k", C.c_uint32)]
@@ -530,7 +561,7 @@ class GpuRuntime:
         _check(lib().t0_rt_selftest_drop_one_load(self._h))
 
     SCRATCH_KINDS = {"operand_a": 0, "operand_b": 1, "splitk_planes": 2, "w4_weights": 3, "w4_fused": 4,
-                     "f32_a": 5, "f32_b": 6, "f32_c": 7}
+                     "f32_a": 5, "f32_b": 6, "f32_c": 7, "kv4": 8}
 
     def reserve_scratch(self, kind: str, n_bytes: int) -> None:
         """Grows one of the runtime's scratch buffers ahead of time so that later launches up to that size neither
@@ -787,6 +818,51 @@ class GpuRuntime:
         """``t0_w4a16_gemm_grouped``: independent problems; one shape with 16 < M <= 128 runs up to 32 per launch."""
         arr = (W4A16Args * len(calls))(*calls)
         _check(lib().t0_w4a16_gemm_grouped(self._h, arr, len(calls)))
+
+    @staticmethod
+    def kv4_batch(pages: int, page_table: int, seq_lens: int, *, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, n_seqs: int,
+                  table_stride: int, n_rows: int, max_rows: int = 1, row_start: int = 0) -> Kv4Batch:
+        """The record all ``kv4_*`` calls take; addresses as integers."""
+        return Kv4Batch(pages, page_table, seq_lens, row_start, n_pages, page_size, n_kv_heads, head_dim, n_seqs, table_stride, n_rows, max_rows)
+
+    @staticmethod
+    def kv4_append_args(k: int, v: int, *, k_stride: int = 0, v_stride: int = 0, in_f32: bool = False, q: int = 0, q_stride: int = 0, q_out: int = 0,
+                        q_out_stride: int = 0, n_q_heads: int = 0, rope: int = 0, n_positions: int = 0, rot_dim: int = 0, interleaved: bool = False,
+                        axis_pairs=(), positions: int = 0) -> Kv4AppendArgs:
+        """``axis_pairs``: pairs of each position axis (one to three; none or one number: a single axis)."""
+        a = Kv4AppendArgs()
+        a.q, a.k, a.v, a.q_out, a.rope, a.positions = q, k, v, q_out, rope, positions
+        a.q_stride, a.k_stride, a.v_stride, a.q_out_stride = q_stride, k_stride, v_stride, q_out_stride
+        a.n_q_heads, a.n_positions, a.rot_dim, a.n_axes = n_q_heads, n_positions, rot_dim, max(1, len(axis_pairs))
+        if len(axis_pairs) > 3:
+            raise ValueError("at most three position axes")
+        for i, n in enumerate(axis_pairs):
+            a.axis_pairs[i] = n
+        a.in_f32, a.interleaved = int(in_f32), int(interleaved)
+        return a
+
+    @staticmethod
+    def kv4_dequant_args(k_out: int, v_out: int, *, k_out_stride: int = 0, v_out_stride: int = 0) -> Kv4DequantArgs:
+        return Kv4DequantArgs(k_out, v_out, k_out_stride, v_out_stride)
+
+    @staticmethod
+    def kv4_attention_args(q: int, y: int, *, n_q_heads: int, scale: float, window: int = 0, q_stride: int = 0, y_stride: int = 0) -> Kv4AttentionArgs:
+        return Kv4AttentionArgs(q, y, q_stride, y_stride, n_q_heads, window, scale, 0)
+
+    def kv4_append(self, batch: Kv4Batch, args: Kv4AppendArgs) -> None:
+        """``t0_kv4_append``: keys and values into the four-bit cache, keys and queries rotated on the way."""
+        _check(lib().t0_kv4_append(self._h, C.byref(batch), C.byref(args)))
+
+    def kv4_dequant(self, batch: Kv4Batch, args: Kv4DequantArgs) -> None:
+        """``t0_kv4_dequant``: the rows' keys and values read out of the cache as bf16."""
+        _check(lib().t0_kv4_dequant(self._h, C.byref(batch), C.byref(args)))
+
+    def kv4_attention(self, batch: Kv4Batch, args: Kv4AttentionArgs) -> None:
+        """``t0_kv4_attention``: attention of the rows over their sequences' cached tokens."""
+        _check(lib().t0_kv4_attention(self._h, C.byref(batch), C.byref(args)))
+
+    def kv4_scratch_bytes(self) -> int:
+        return int(lib().t0_kv4_scratch_bytes(self._h))
 
     def fill_uniform_bf16(self, dst: int, n: int, seed: int, first_index: int = 0) -> None:
         _check(lib().t0_fill_uniform_bf16(self._h, dst, n, seed, first_index))
@@ -1105,6 +1181,11 @@ def _declare(L: C.CDLL) -> None:
     sig("t0_w4a16_gemm_prepacked", i32, vp, u64, u64, u64, u32, u32, u32, u32)
     sig("t0_w4a16_gemm_prepacked_batch", i32, vp, C.POINTER(W4A16Args), sz)
     sig("t0_w4a16_gemm_static_scratch_bytes", sz)
+    sig("t0_kv4_page_bytes", sz, u32, u32, u32)
+    sig("t0_kv4_append", i32, vp, C.POINTER(Kv4Batch), C.POINTER(Kv4AppendArgs))
+    sig("t0_kv4_dequant", i32, vp, C.POINTER(Kv4Batch), C.POINTER(Kv4DequantArgs))
+    sig("t0_kv4_attention", i32, vp, C.POINTER(Kv4Batch), C.POINTER(Kv4AttentionArgs))
+    sig("t0_kv4_scratch_bytes", sz, vp)
     sig("t0_gptq_parse", i32, vp, sz, u32p, u32p, u32p, C.POINTER(sz), C.POINTER(sz), C.POINTER(sz))
     sig("t0_gptq_gpu_buffer_size", sz, u32, u32, u32)
     sig("t0_gptq_to_b200", C.c_long, vp, vp, vp, u32, u32, u32, vp, vp, vp)

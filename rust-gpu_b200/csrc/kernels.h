@@ -10,6 +10,8 @@ namespace t0 {
 
 // Error word written by a kernel whose bounded wait expired: role in the top byte.
 enum : int { kStatusOk = 0, kStatusProducerTimeout = 0x01000000, kStatusMmaTimeout = 0x02000000, kStatusEpilogueTimeout = 0x03000000 };
+// Second status word: a place that a kernel found wrong in arguments on the device and left out, its index in the low 24 bits.
+enum : int { kStatusBadSequence = 0x10000000, kStatusBadPage = 0x11000000, kStatusBadPosition = 0x12000000 };
 
 struct GemmLaunch {
     const void* x;        // bf16 [M,K]; [K,M] with at

@@ -1,0 +1,362 @@
+// The paged key/value cache in four bits: append (with the rotation of keys and queries) and read-out.
+#include "gemm_common.cuh"
+#include "kv4.cuh"
+
+namespace t0 {
+namespace kv4 {
+
+int check_batch(const t0_kv4_batch* b, Batch* out) {
+    if (!b) return fail(T0_ERR_INVALID, "null batch");
+    if (b->page_size != 16 && b->page_size != 32 && b->page_size != 64)
+        return fail(T0_ERR_UNSUPPORTED, "page_size=%u: pages hold 16, 32 or 64 tokens", b->page_size);
+    if (b->head_dim != 64 && b->head_dim != 128) return fail(T0_ERR_UNSUPPORTED, "head_dim=%u: heads have 64 or 128 numbers", b->head_dim);
+    if (b->n_kv_heads == 0 || b->n_kv_heads > 4096) return fail(T0_ERR_INVALID, "n_kv_heads=%u must be in 1 .. 4096", b->n_kv_heads);
+    if (b->n_seqs == 0 || b->n_rows == 0) {
+        *out = Batch{};
+        return T0_OK;
+    }
+    if (b->n_seqs > (1u << 20) || b->n_rows > (1u << 24)) return fail(T0_ERR_INVALID, "%u sequences, %u rows: at most 2^20 and 2^24", b->n_seqs, b->n_rows);
+    if (!b->pages || !b->page_table || !b->seq_lens) return fail(T0_ERR_INVALID, "null device pointer in the batch");
+    if (b->pages & 15) return fail(T0_ERR_INVALID, "the cache must be 16-byte aligned");
+    if ((b->page_table | b->seq_lens | b->row_start) & 3) return fail(T0_ERR_INVALID, "page_table, seq_lens and row_start must be 4-byte aligned");
+    if (b->n_pages == 0 || b->n_pages > 0x7FFFFFFFu) return fail(T0_ERR_INVALID, "n_pages=%u", b->n_pages);
+    if (b->table_stride == 0 || (uint64_t)b->table_stride * b->page_size > 0x40000000ull)
+        return fail(T0_ERR_INVALID, "table_stride=%u: between one page and 2^30 tokens", b->table_stride);
+    if (b->max_rows == 0 || b->max_rows > b->n_rows) return fail(T0_ERR_INVALID, "max_rows=%u must be in 1 .. n_rows=%u", b->max_rows, b->n_rows);
+    if (!b->row_start && (uint64_t)b->n_seqs * b->max_rows != b->n_rows)
+        return fail(T0_ERR_INVALID, "without row_start n_rows=%u must be n_seqs=%u times max_rows=%u", b->n_rows, b->n_seqs, b->max_rows);
+    out->pages = (uint8_t*)b->pages;
+    out->page_table = (const int32_t*)b->page_table;
+    out->seq_lens = (const int32_t*)b->seq_lens;
+    out->row_start = (const int32_t*)b->row_start;
+    out->n_pages = b->n_pages;
+    out->page_log2 = b->page_size == 16 ? 4 : b->page_size == 32 ? 5 : 6;
+    out->n_kv_heads = b->n_kv_heads;
+    out->n_seqs = b->n_seqs; out->table_stride = b->table_stride;
+    out->n_rows = b->n_rows; out->max_rows = b->max_rows;
+    return T0_OK;
+}
+
+int check_rows(const char* name, uint64_t base, uint32_t* stride, uint32_t width, uint32_t bytes) {
+    if (*stride == 0) *stride = width;
+    if (*stride < width) return fail(T0_ERR_INVALID, "%s: a stride of %u numbers, rows have %u", name, *stride, width);
+    if ((base & 15) || (uint64_t)*stride * bytes % 16) return fail(T0_ERR_INVALID, "%s: rows must start on 16-byte boundaries", name);
+    return T0_OK;
+}
+
+bool rows_touch(uint64_t a, uint64_t a_bytes, uint64_t a_stride, uint64_t b, uint64_t b_bytes, uint64_t b_stride, uint64_t rows) {
+    const uint64_t a_end = a + (rows - 1) * a_stride + a_bytes, b_end = b + (rows - 1) * b_stride + b_bytes;
+    if (a_end <= b || b_end <= a) return false;
+    if (a_stride != b_stride || rows == 1) return true;
+    const uint64_t d = b >= a ? (b - a) % a_stride : (a_stride - (a - b) % a_stride) % a_stride;       // columns of one wider array
+    return d < a_bytes || d + b_bytes > a_stride;
+}
+
+namespace {
+
+struct Append {
+    Batch B;
+    const void *q, *k, *v;
+    __nv_bfloat16* q_out;
+    const float2* rope;
+    const int32_t* positions;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride;
+    uint32_t n_q_heads, n_positions, rot_dim;
+    uint32_t end0, end1;                    // first pair of the second and of the third axis
+    uint32_t n_axes;
+    bool interleaved;
+};
+
+template <bool F32>
+__device__ __forceinline__ void load8(float (&x)[8], const void* base, uint64_t at) {
+    if constexpr (F32) {
+        const float4* p = (const float4*)((const float*)base + at);
+        const float4 a = p[0], b = p[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 w = *(const uint4*)((const __nv_bfloat16*)base + at);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(u[i] << 16);
+            x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        }
+    }
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&p;
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+
+// A group of D / 8 lanes takes one head of one row, eight numbers a lane: it turns them, and either rounds them to bf16 (queries) or finds the row's
+// range and cuts it to four bits, a 32-bit word of codes a lane.
+template <int D, bool F32>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Append P) {
+    constexpr uint32_t kLanes = D / 8;
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const Batch& B = P.B;
+    const uint32_t heads = P.n_q_heads + 2 * B.n_kv_heads;
+    const uint64_t unit = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
+    const uint32_t e = threadIdx.x % kLanes;
+    const uint32_t group_mask = (uint32_t)((1ull << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes);
+    const uint32_t r = (uint32_t)(unit / heads), h = (uint32_t)(unit % heads);
+    if (r >= B.n_rows) return;
+    uint32_t b;
+    Sequence s;
+    if (!sequence_of_row(B, r, &b, &s)) return;
+    const int token = s.len - s.rows + ((int)r - s.first_row);
+    if (token < 0) return;
+
+    // the row's positions
+    int pos[3] = {token, token, token};
+    if (P.rope) {
+        if (P.positions)
+            for (uint32_t a = 0; a < P.n_axes; ++a) pos[a] = P.positions[(uint64_t)a * B.n_rows + r];
+        bool bad = false;
+        for (uint32_t a = 0; a < P.n_axes; ++a) bad |= (uint32_t)pos[a] >= P.n_positions;
+        if (bad) {
+            if (e == 0) report(B, kStatusBadPosition, r);
+            return;
+        }
+    }
+    float x[8];
+    const bool is_q = h < P.n_q_heads, is_k = !is_q && h < P.n_q_heads + B.n_kv_heads;
+    const uint32_t head = is_q ? h : is_k ? h - P.n_q_heads : h - P.n_q_heads - B.n_kv_heads;
+    if (is_q) load8<F32>(x, P.q, r * P.q_stride + head * D + 8 * e);
+    else if (is_k) load8<F32>(x, P.k, r * P.k_stride + head * D + 8 * e);
+    else load8<F32>(x, P.v, r * P.v_stride + head * D + 8 * e);
+
+    if ((is_q || is_k) && P.rope) {
+        const uint32_t pairs = P.rot_dim / 2;
+        auto cs = [&](uint32_t pair) {
+            const int p = pair < P.end0 ? pos[0] : pair < P.end1 ? pos[1] : pos[2];
+            return P.rope[(uint64_t)p * pairs + pair];
+        };
+        if (P.interleaved) {
+            if (e < P.rot_dim / 8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 t = cs(e * 4 + i);
+                    const float u = x[2 * i], w = x[2 * i + 1];
+                    x[2 * i] = __fsub_rn(__fmul_rn(u, t.x), __fmul_rn(w, t.y));
+                    x[2 * i + 1] = __fadd_rn(__fmul_rn(w, t.x), __fmul_rn(u, t.y));
+                }
+            }
+        } else {
+            const uint32_t away = P.rot_dim / 16;          // lanes between the two numbers of a pair
+            const bool first = e < away, second = !first && e < 2 * away;
+            const uint32_t from = threadIdx.x % 32 - e + (first ? e + away : second ? e - away : e);
+            float other[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(group_mask, x[i], from);
+            if (first || second) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 t = cs((first ? e : e - away) * 8 + i);
+                    x[i] = first ? __fsub_rn(__fmul_rn(x[i], t.x), __fmul_rn(other[i], t.y)) : __fadd_rn(__fmul_rn(x[i], t.x), __fmul_rn(other[i], t.y));
+                }
+            }
+        }
+    }
+    if (is_q) {
+        *(uint4*)(P.q_out + r * P.q_out_stride + head * D + 8 * e) = pack8(x);
+        return;
+    }
+    // the range
+    float mn = x[0], mx = x[0];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        mn = fminf(mn, x[i]);
+        mx = fmaxf(mx, x[i]);
+        bad |= !(fabsf(x[i]) < __int_as_float(0x7F800000));
+    }
+#pragma unroll
+    for (uint32_t d = 1; d < kLanes; d *= 2) {
+        mn = fminf(mn, __shfl_xor_sync(group_mask, mn, d));
+        mx = fmaxf(mx, __shfl_xor_sync(group_mask, mx, d));
+    }
+    bad = (__ballot_sync(group_mask, bad) & group_mask) != 0;
+    const float low = bf16_down(mn), range = __fsub_rn(mx, low);
+    bad |= !(range < __int_as_float(0x7F800000));
+    float step = -bf16_down(-__fdiv_rn(range, 15.0f));
+    if (step < 1.17549435e-38f) step = 0.0f;
+    uint32_t codes = 0;
+    if (!bad && step > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], low), step)), 0.0f), 15.0f);
+            codes |= (uint32_t)c << code_shift(i);
+        }
+    }
+    uint8_t* block = block_of<D>(B, b, (uint32_t)token >> B.page_log2, head);
+    if (!block) return;
+    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1), which = is_k ? 0 : 1;
+    *(uint32_t*)(block + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e) = codes;
+    if (e == 0)
+        *(uint32_t*)(block + params_at<D>(B.page_log2, which) + 4 * slot) =
+            bad ? 0x7FC07FC0u : (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
+}
+
+struct Dequant {
+    Batch B;
+    __nv_bfloat16 *k_out, *v_out;
+    uint64_t k_stride, v_stride;
+};
+
+// A group of D / 8 lanes reads one head of one row of the keys or of the values, a word of eight codes a lane.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_dequant_kernel(const __grid_constant__ Dequant P) {
+    constexpr uint32_t kLanes = D / 8;
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const Batch& B = P.B;
+    const uint64_t unit = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
+    const uint32_t e = threadIdx.x % kLanes;
+    const uint32_t r = (uint32_t)(unit / (2 * B.n_kv_heads)), h = (uint32_t)(unit % (2 * B.n_kv_heads));
+    if (r >= B.n_rows) return;
+    const uint32_t which = h < B.n_kv_heads ? 0 : 1, head = which ? h - B.n_kv_heads : h;
+    __nv_bfloat16* out = which ? P.v_out : P.k_out;
+    if (!out) return;
+    uint32_t b;
+    Sequence s;
+    if (!sequence_of_row(B, r, &b, &s)) return;
+    const int token = s.len - s.rows + ((int)r - s.first_row);
+    uint4* to = (uint4*)(out + r * (which ? P.v_stride : P.k_stride) + head * D + 8 * e);
+    if (token < 0) {
+        *to = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const uint8_t* block = block_of<D>(B, b, (uint32_t)token >> B.page_log2, head);
+    if (!block) return;
+    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1);
+    const uint32_t w = *(const uint32_t*)(block + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e);
+    const uint32_t p = *(const uint32_t*)(block + params_at<D>(B.page_log2, which) + 4 * slot);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(__fmul_rn((float)((w >> code_shift(i)) & 15), param_step(p)), param_low(p));
+    *to = pack8(x);
+}
+
+}  // namespace
+}  // namespace kv4
+
+const char* kv4_status_text(int code) {
+    switch (code & 0x7F000000) {
+        case kStatusBadSequence: return "the length or the rows of sequence";
+        case kStatusBadPage: return "a page outside the cache, of sequence";
+        case kStatusBadPosition: return "a position outside the rope table, of row";
+        default: return "place";
+    }
+}
+
+}  // namespace t0
+
+using namespace t0;
+using namespace t0::kv4;
+
+extern "C" {
+
+size_t t0_kv4_page_bytes(uint32_t page_size, uint32_t n_kv_heads, uint32_t head_dim) {
+    if ((page_size != 16 && page_size != 32 && page_size != 64) || (head_dim != 64 && head_dim != 128)) return 0;
+    return (size_t)page_size * (head_dim + 8) * n_kv_heads;
+}
+
+int t0_kv4_append(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_append_args* args) {
+    Append P;
+    memset(&P, 0, sizeof P);
+    if (!args) return fail(T0_ERR_INVALID, "null arguments");
+    int rc = check_batch(batch, &P.B);
+    if (rc != T0_OK) return rc;
+    if (P.B.n_rows == 0) return check_rt(rt);
+    t0_kv4_append_args a = *args;
+    const uint32_t D = batch->head_dim, size = a.in_f32 ? 4 : 2;
+    if (!a.k || !a.v) return fail(T0_ERR_INVALID, "null device pointer");
+    if (a.q && (!a.q_out || a.n_q_heads == 0 || a.n_q_heads > 65536)) return fail(T0_ERR_INVALID, "queries need q_out and n_q_heads (%u) in 1 .. 65536", a.n_q_heads);
+    if (!a.q) a.n_q_heads = 0;
+    if ((rc = check_rows("k", a.k, &a.k_stride, batch->n_kv_heads * D, size)) != T0_OK) return rc;
+    if ((rc = check_rows("v", a.v, &a.v_stride, batch->n_kv_heads * D, size)) != T0_OK) return rc;
+    if (a.q) {
+        if ((rc = check_rows("q", a.q, &a.q_stride, a.n_q_heads * D, size)) != T0_OK) return rc;
+        if ((rc = check_rows("q_out", a.q_out, &a.q_out_stride, a.n_q_heads * D, 2)) != T0_OK) return rc;
+        const uint64_t q_bytes = (uint64_t)a.n_q_heads * D * size, kv_bytes = (uint64_t)batch->n_kv_heads * D * size, out_bytes = (uint64_t)a.n_q_heads * D * 2;
+        const uint64_t out_stride = (uint64_t)a.q_out_stride * 2, n = batch->n_rows;
+        const bool in_place = a.q_out == a.q && !a.in_f32 && (a.q_out_stride == a.q_stride || n == 1);
+        if ((!in_place && rows_touch(a.q_out, out_bytes, out_stride, a.q, q_bytes, (uint64_t)a.q_stride * size, n)) ||
+            rows_touch(a.q_out, out_bytes, out_stride, a.k, kv_bytes, (uint64_t)a.k_stride * size, n) ||
+            rows_touch(a.q_out, out_bytes, out_stride, a.v, kv_bytes, (uint64_t)a.v_stride * size, n))
+            return fail(T0_ERR_INVALID, "q_out overlaps q, k or v (it may be q itself where q is bf16)");
+    }
+    if (a.rope) {
+        if ((a.rope & 15) || (a.positions & 3)) return fail(T0_ERR_INVALID, "the rope table must be 16-byte aligned, positions 4-byte");
+        if (a.rot_dim == 0 || a.rot_dim % 16 || a.rot_dim > D) return fail(T0_ERR_INVALID, "rot_dim=%u must be a multiple of 16, at most head_dim=%u", a.rot_dim, D);
+        if (a.n_positions == 0 || a.n_positions > 0x7FFFFFFFu) return fail(T0_ERR_INVALID, "n_positions=%u", a.n_positions);
+        if (a.n_axes > 3) return fail(T0_ERR_INVALID, "n_axes=%u: one to three", a.n_axes);
+        if (a.n_axes <= 1) {
+            if (a.n_axes == 1 && a.axis_pairs[0] && a.axis_pairs[0] != a.rot_dim / 2)
+                return fail(T0_ERR_INVALID, "one axis has all %u pairs, not %u", a.rot_dim / 2, a.axis_pairs[0]);
+            a.n_axes = 1;
+            a.axis_pairs[0] = a.rot_dim / 2;
+        } else if (!a.positions) {
+            return fail(T0_ERR_INVALID, "several axes need positions");
+        }
+        uint64_t sum = 0;
+        for (uint32_t i = 0; i < a.n_axes; ++i) sum += a.axis_pairs[i];
+        if (sum != a.rot_dim / 2) return fail(T0_ERR_INVALID, "the axes have %llu pairs, rot_dim=%u", (unsigned long long)sum, a.rot_dim);
+    }
+    P.q = (const void*)a.q; P.k = (const void*)a.k; P.v = (const void*)a.v;
+    P.q_out = (__nv_bfloat16*)a.q_out;
+    P.rope = (const float2*)a.rope;
+    P.positions = (const int32_t*)a.positions;
+    P.q_stride = a.q_stride; P.k_stride = a.k_stride; P.v_stride = a.v_stride; P.q_out_stride = a.q_out_stride;
+    P.n_q_heads = a.n_q_heads; P.n_positions = a.n_positions; P.rot_dim = a.rot_dim;
+    P.n_axes = a.n_axes;
+    P.interleaved = a.interleaved != 0;
+    P.end0 = a.axis_pairs[0]; P.end1 = a.n_axes == 1 ? P.end0 : a.axis_pairs[0] + a.axis_pairs[1];
+    if ((rc = check_rt(rt)) != T0_OK) return rc;
+    P.B.status = rt->d_status + 1;
+    DeviceGuard guard(rt->device);
+    const uint64_t threads = (uint64_t)batch->n_rows * (a.n_q_heads + 2 * batch->n_kv_heads) * (D / 8);
+    const uint64_t grid = (threads + 255) / 256;
+    if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "too many rows and heads for one launch");
+    auto go = [&](auto kernel) { return gemm::launch_pdl(kernel, (uint32_t)grid, 256, 0, rt->stream, P); };
+    const cudaError_t e = D == 64 ? (a.in_f32 ? go(kv4_append_kernel<64, true>) : go(kv4_append_kernel<64, false>))
+                                  : (a.in_f32 ? go(kv4_append_kernel<128, true>) : go(kv4_append_kernel<128, false>));
+    if (e != cudaSuccess) return fail(T0_ERR_CUDA, "append launch failed: %s", cudaGetErrorString(e));
+    rt->launches.fetch_add(1);
+    return T0_OK;
+}
+
+int t0_kv4_dequant(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_dequant_args* args) {
+    Dequant P;
+    memset(&P, 0, sizeof P);
+    if (!args) return fail(T0_ERR_INVALID, "null arguments");
+    int rc = check_batch(batch, &P.B);
+    if (rc != T0_OK) return rc;
+    if (P.B.n_rows == 0) return check_rt(rt);
+    t0_kv4_dequant_args a = *args;
+    const uint32_t D = batch->head_dim, width = batch->n_kv_heads * D;
+    if (!a.k_out && !a.v_out) return fail(T0_ERR_INVALID, "null device pointer: neither keys nor values are asked for");
+    if (a.k_out && (rc = check_rows("k_out", a.k_out, &a.k_out_stride, width, 2)) != T0_OK) return rc;
+    if (a.v_out && (rc = check_rows("v_out", a.v_out, &a.v_out_stride, width, 2)) != T0_OK) return rc;
+    if (a.k_out && a.v_out && rows_touch(a.k_out, 2ull * width, 2ull * a.k_out_stride, a.v_out, 2ull * width, 2ull * a.v_out_stride, batch->n_rows))
+        return fail(T0_ERR_INVALID, "k_out and v_out overlap");
+    P.k_out = (__nv_bfloat16*)a.k_out; P.v_out = (__nv_bfloat16*)a.v_out;
+    P.k_stride = a.k_out_stride; P.v_stride = a.v_out_stride;
+    if ((rc = check_rt(rt)) != T0_OK) return rc;
+    P.B.status = rt->d_status + 1;
+    DeviceGuard guard(rt->device);
+    const uint64_t grid = ((uint64_t)batch->n_rows * 2 * batch->n_kv_heads * (D / 8) + 255) / 256;
+    if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "too many rows and heads for one launch");
+    const cudaError_t e = D == 64 ? gemm::launch_pdl(kv4_dequant_kernel<64>, (uint32_t)grid, 256, 0, rt->stream, P)
+                                  : gemm::launch_pdl(kv4_dequant_kernel<128>, (uint32_t)grid, 256, 0, rt->stream, P);
+    if (e != cudaSuccess) return fail(T0_ERR_CUDA, "read-out launch failed: %s", cudaGetErrorString(e));
+    rt->launches.fetch_add(1);
+    return T0_OK;
+}
+
+}  // extern "C"

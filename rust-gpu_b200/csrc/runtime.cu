@@ -373,8 +373,8 @@ int t0_rt_new(int device, t0_runtime** out) {
     T0_CUDA(cudaEventCreate(&rt->ev_stop));
     T0_CUDA(cudaMalloc(&rt->d_probe, (2 + 64) * sizeof(unsigned long long)));   // clock words + eight launches' trace stamps
     T0_CUDA(cudaMemset(rt->d_probe, 0, (2 + 64) * sizeof(unsigned long long)));
-    T0_CUDA(cudaHostAlloc(&rt->h_status, sizeof(int), cudaHostAllocMapped));
-    *rt->h_status = 0;
+    T0_CUDA(cudaHostAlloc(&rt->h_status, 2 * sizeof(int), cudaHostAllocMapped));
+    rt->h_status[0] = rt->h_status[1] = 0;
     T0_CUDA(cudaHostGetDevicePointer(&rt->d_status, rt->h_status, 0));
     if (w4a16_umma_reserve(rt.get()) != T0_OK) cudaGetLastError();     // (without room the W4A16 calls take forms that need none)
     *out = rt.release();
@@ -387,7 +387,7 @@ void t0_rt_free(t0_runtime* rt) {
     cudaStreamSynchronize(rt->stream);
     host_pipe_free(rt);
     t0_rt_pool_clear(rt);
-    for (Scratch* s : {&rt->scratch_a, &rt->scratch_b, &rt->scratch_planes, &rt->scratch_w4, &rt->scratch_um, &rt->scratch_w, &rt->scratch_cvt_a, &rt->scratch_cvt_b, &rt->scratch_cvt_c})
+    for (Scratch* s : {&rt->scratch_a, &rt->scratch_b, &rt->scratch_planes, &rt->scratch_w4, &rt->scratch_um, &rt->scratch_w, &rt->scratch_cvt_a, &rt->scratch_cvt_b, &rt->scratch_cvt_c, &rt->scratch_kv4})
         if (s->ptr) cudaFree(s->ptr);
     if (rt->d_probe) cudaFree(rt->d_probe);
     if (rt->d_peer_maps) cudaFree(rt->d_peer_maps);
@@ -449,6 +449,17 @@ int t0_rt_reserve_scratch(t0_runtime* rt, int which, size_t bytes) {
                 T0_CUDA(cudaMemsetAsync(rt->scratch_w4.ptr, 0, w4a16_counter_region_bytes(), rt->stream));
             }
             return bytes >= all ? w4a16_umma_reserve(rt) : T0_OK;
+        }
+        case T0_SCRATCH_KV4: {
+            // arrival counters (must start at zero), then the parts; the size depends only on the device, so less is made whole
+            const size_t need = std::max(bytes, t0_kv4_scratch_bytes(rt));
+            if (need <= rt->scratch_kv4.size) return T0_OK;
+            rc = ensure_scratch(rt, rt->scratch_kv4, need);
+            if (rc != T0_OK) return rc;
+            const cudaError_t e = cudaMemsetAsync(rt->scratch_kv4.ptr, 0, kv4_counter_bytes(), rt->stream);
+            if (e != cudaSuccess) rt->scratch_kv4.size = 0;      // not usable: the next call makes it again
+            T0_CUDA(e);
+            return T0_OK;
         }
         default: return fail(T0_ERR_INVALID, "unknown scratch kind %d", which);
     }

@@ -50,7 +50,7 @@ struct t0_runtime {
     std::atomic<int> drop_next_load{0};       // self-test hook: the next GEMM launch leaves out one operand load
     bool static_scratch_cleared = false;      // t0_w4a16_gemm_static: this runtime has zeroed the shared counters once
     int* h_status = nullptr;     // error word, in mapped host memory: written by kernels whose bounded wait expired, read after a synchronisation
-    int* d_status = nullptr;     // ... its device address
+    int* d_status = nullptr;     // ... its device address; the second word: what a kernel found wrong in device-side arguments (kernels.h, kStatusBad*)
     unsigned long long* d_probe = nullptr;   // {cycles, ns} of the last GEMM kernel's CTA 0
     void* d_peer_maps = nullptr;             // gathered output: device slot for the destinations' tensor maps (made on first use)
     std::vector<uint64_t> peer_maps_key;     // destinations and shape the slot currently describes
@@ -59,6 +59,7 @@ struct t0_runtime {
     Scratch scratch_um;          // tcgen05 W4A16: counters + partial sums of the cut tiles (made with the runtime)
     Scratch scratch_w;           // W4A16 general path: dequantised weights
     Scratch scratch_cvt_a, scratch_cvt_b, scratch_cvt_c;   // f32 entries: bf16 copies of the operands, f32 product before alpha/beta
+    Scratch scratch_kv4;         // attention over the four-bit cache: arrival counters + parts of cut sums
     void* host_pipe = nullptr;   // host-operand GEMM pipeline (streams, events, staging sets), made on first use
 };
 
@@ -67,6 +68,8 @@ namespace t0 {
 void host_pipe_free(t0_runtime* rt);   // host_pipeline.cu
 size_t w4a16_umma_scratch_bytes(const t0_runtime* rt);   // w4a16_umma_cut.cu
 int w4a16_umma_reserve(t0_runtime* rt);
+size_t kv4_counter_bytes();                              // kv4_attention.cu
+const char* kv4_status_text(int code);                   // kv4_cache.cu
 // runtime.cu: one bf16 product of operands with row strides, everything else chosen by the library
 int gemm_strided(t0_runtime* rt, uint64_t a, uint32_t lda, bool at, uint64_t b, uint32_t ldb, bool nn, uint64_t y, uint32_t m, uint32_t n, uint32_t k);
 
@@ -125,6 +128,12 @@ inline int check_status_after_sync(t0_runtime* rt) {
         *(volatile int*)rt->h_status = 0;
         return fail(T0_ERR_TIMEOUT, "a bounded device-side wait expired (status 0x%08x: role %d, work item %d)", code,
                     (code >> 24) & 0xFF, code & 0xFFFFFF);
+    }
+    // what a call found wrong in arguments that lie on the device: reported, and the runtime goes on (the kernels left the place out)
+    const int bad = ((volatile int*)rt->h_status)[1];
+    if (bad != 0) {
+        ((volatile int*)rt->h_status)[1] = 0;
+        return fail(T0_ERR_BOUNDS, "%s %d of an earlier call on the key/value cache was left out", kv4_status_text(bad), bad & 0xFFFFFF);
     }
     return T0_OK;
 }

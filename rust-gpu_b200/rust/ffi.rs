@@ -33,6 +33,7 @@ pub const T0_SCRATCH_W4_FUSED: u32 = 4;
 pub const T0_SCRATCH_F32_A: u32 = 5;
 pub const T0_SCRATCH_F32_B: u32 = 6;
 pub const T0_SCRATCH_F32_C: u32 = 7;
+pub const T0_SCRATCH_KV4: u32 = 8;
 pub const T0_WARP_ROW_DOMINANT: u32 = 0;
 pub const T0_WARP_COL_DOMINANT: u32 = 1;
 pub const T0_WARP_SQUARE: u32 = 2;
@@ -172,6 +173,68 @@ pub struct t0_int4_wmma_config {
     pub tile_m: u32,
     pub tile_n: u32,
     pub tile_k: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_kv4_batch {
+    pub pages: u64,
+    pub page_table: u64,
+    pub seq_lens: u64,
+    pub row_start: u64,
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub n_kv_heads: u32,
+    pub head_dim: u32,
+    pub n_seqs: u32,
+    pub table_stride: u32,
+    pub n_rows: u32,
+    pub max_rows: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_kv4_append_args {
+    pub q: u64,
+    pub k: u64,
+    pub v: u64,
+    pub q_out: u64,
+    pub rope: u64,
+    pub positions: u64,
+    pub q_stride: u32,
+    pub k_stride: u32,
+    pub v_stride: u32,
+    pub q_out_stride: u32,
+    pub n_q_heads: u32,
+    pub n_positions: u32,
+    pub rot_dim: u32,
+    pub n_axes: u32,
+    pub axis_pairs: [u32; 3],
+    pub in_f32: u8,
+    pub interleaved: u8,
+    pub _pad: [u8; 2],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_kv4_dequant_args {
+    pub k_out: u64,
+    pub v_out: u64,
+    pub k_out_stride: u32,
+    pub v_out_stride: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_kv4_attention_args {
+    pub q: u64,
+    pub y: u64,
+    pub q_stride: u32,
+    pub y_stride: u32,
+    pub n_q_heads: u32,
+    pub window: u32,
+    pub scale: f32,
+    pub _pad: u32,
 }
 
 extern "C" {
@@ -329,6 +392,11 @@ extern "C" {
     pub fn t0_gptq_parse(raw: *const u8, len: usize, rows: *mut u32, cols: *mut u32, group_size: *mut u32, packed_off: *mut usize, scales_off: *mut usize, zero_points_off: *mut usize) -> c_int;
     pub fn t0_gptq_gpu_buffer_size(rows: u32, cols: u32, group_size: u32) -> usize;
     pub fn t0_gptq_to_b200(packed: *const u8, scales: *const f32, zero_points: *const i32, rows: u32, cols: u32, group_size: u32, packed_out: *mut u32, scales_out: *mut u16, zeros_out: *mut u32) -> c_long;
+    pub fn t0_kv4_page_bytes(page_size: u32, n_kv_heads: u32, head_dim: u32) -> usize;
+    pub fn t0_kv4_append(rt: *mut t0_runtime, batch: *const t0_kv4_batch, args: *const t0_kv4_append_args) -> c_int;
+    pub fn t0_kv4_dequant(rt: *mut t0_runtime, batch: *const t0_kv4_batch, args: *const t0_kv4_dequant_args) -> c_int;
+    pub fn t0_kv4_attention(rt: *mut t0_runtime, batch: *const t0_kv4_batch, args: *const t0_kv4_attention_args) -> c_int;
+    pub fn t0_kv4_scratch_bytes(rt: *const t0_runtime) -> usize;
     pub fn t0_shard_columns(n: u32, n_gpus: u32, rank: u32, first_col: *mut u32, n_cols: *mut u32) -> c_int;
     pub fn t0_mg_new(n_gpus: c_int, out: *mut *mut t0_mg) -> c_int;
     pub fn t0_mg_free(mg: *mut t0_mg);
