@@ -576,7 +576,8 @@ long t0_gptq_to_b200(const uint8_t* packed, const float* scales, const int32_t* 
  * token seq_lens[b] - n + i.  Rows for which that is negative (an empty slot of a recorded batch) have no token; rows that belong to no
  * sequence are neither read nor written.  page_table, seq_lens and row_start are read on the device when the call runs, so a recorded call may be
  * replayed with other values in them.  What they hold is checked there: a sequence with a negative length, more tokens than its row of
- * the table has places, rows outside n_rows or more than max_rows of them is left out, a page outside the cache is left out, and the next
+ * the table has places, rows outside n_rows or more than max_rows of them is left out; a page outside the cache is neither read nor written
+ * (what the sequence's rows get is then of no use, other sequences' are as ever); in either case the next
  * synchronising call returns T0_ERR_BOUNDS (the runtime is not poisoned).  Sequences may share pages that they only read; a token's place
  * must not be another's whose row is in the same append. */
 typedef struct t0_kv4_batch {

@@ -80,6 +80,12 @@ __device__ __forceinline__ uint8_t* block_of(const Batch& B, uint32_t b, uint32_
     }
     return B.pages + ((uint64_t)page * B.n_kv_heads + head) * ((uint64_t)(D + 8) << B.page_log2);
 }
+// The same for kernels that read whole chunks: in place of a page outside the cache, page 0.
+template <int D>
+__device__ __forceinline__ const uint8_t* block_to_read(const Batch& B, uint32_t b, uint32_t table_column, uint32_t head) {
+    const uint8_t* block = block_of<D>(B, b, table_column, head);
+    return block ? block : B.pages + (uint64_t)head * ((D + 8) << B.page_log2);
+}
 template <int D> __device__ __forceinline__ uint32_t codes_at(uint32_t page_log2, uint32_t which) { return which * ((D / 2) << page_log2); }           // 0 keys, 1 values
 template <int D> __device__ __forceinline__ uint32_t params_at(uint32_t page_log2, uint32_t which) { return (D + 4 * which) << page_log2; }
 

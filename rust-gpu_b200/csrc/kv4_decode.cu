@@ -1,0 +1,574 @@
+// Attention of few rows (rows x group <= 16) over the paged four-bit cache: reading the cache once is all that counts.
+//
+// Transposed products on mma.sync: S^T = K Q^T with sixteen tokens as the rows of a tile and eight (row, head) columns, and O^T = V^T P^T
+// with sixteen numbers of the head as rows.  Columns that no query fills cost a product nothing it would not cost anyway, and the cache's codes are
+// the A operands of both: a nibble in the mantissa of a bf16 128 is 128 + code, so the codes of two neighbours become a register of the operand with a shift and a
+// logical operation.  Steps and lows stay outside of the products:
+//   score_j = a_j (q . (128 + c_j)) + b_j sum(q),   a_j = step_j, b_j = low_j - 128 step_j    (f32)
+//   o       = sum_j (p_j step_j) (c_j - 8) + sum_j p_j (low_j + 8 step_j)
+// where p_j step_j is rounded to bf16 (one rounding for each token and row, off by at most 2^-9 of its weight either way; the second sum stays f32).
+// A code is never an infinity or a NaN, so a token that a row must not see can be cut off by its factors alone, whatever its parameters are.
+//
+// The work is the list of all (sequence, key/value head) items' chunks of 64 tokens, cut into equal contiguous runs, one for each warp: whatever the lengths, every warp
+// reads as much as the next.  A warp has its own two buffers, filled by bulk copies (the blocks of a chunk are contiguous pieces of the pages), and its own running
+// maximum and sums.  Items that end up in several warps are joined, first inside the CTA, then between CTAs by the one that arrives last, always in order.
+#include "kv4_attention.cuh"
+
+namespace t0 {
+namespace kv4 {
+namespace {
+
+constexpr int kTok = 64;                                  // tokens of a chunk
+constexpr int kStages = 2;
+
+template <int D> constexpr int stage_bytes() { return kTok * (D + 8); }
+template <int D, int NT> constexpr int warps() { return D == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 ? 16 : 12); }
+template <int D, int NT> constexpr int record_floats() { return 8 * NT * (D + 2); }
+
+// position of tile row r among the sixteen tokens of a tile: neighbouring rows, and every second row, then lie in both halves of the 32 banks
+__device__ __forceinline__ int token_of(int r) { return r ^ ((r >> 1) & 1); }
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// 128 + code of nibbles i and i + 4
+__device__ __forceinline__ uint32_t codes_128(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u; }
+// code - 8, exactly
+__device__ __forceinline__ uint32_t codes_centred(uint32_t w, int i) {
+    const uint32_t x = codes_128(w, i);
+    const __nv_bfloat162 r = __hsub2(*(const __nv_bfloat162*)&x, __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
+    return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&p;
+}
+
+// The chunks of every sequence, in order, and how they are cut: made by the CTA for itself.
+struct Plan {
+    uint32_t prefix[1024 + 1];       // chunks (one head's) before the sequences that each thread looked at
+    uint32_t warp_sum[32];
+    uint32_t per_thread;             // sequences that one thread looked at
+};
+
+// chunks of sequence b for one head; rows it is to be left out for have none
+__device__ __forceinline__ uint32_t chunks_of(const Attention& P, const Sequence& s) {
+    if (s.rows == 0 || (uint32_t)s.rows * P.group > P.few) return 0;
+    const int lo = first_seen(s, P.window) / kTok, hi = (s.len + kTok - 1) / kTok;
+    return hi > lo ? hi - lo : 1;                         // at least one: rows that see nothing are written too
+}
+
+struct Item {
+    uint32_t b, head;
+    Sequence s;
+    uint32_t chunks, c0;             // chunks of the item; the first chunk's number in the sequence
+    uint64_t first;                  // its first unit
+};
+
+template <int kThreads>
+__device__ __forceinline__ uint64_t make_plan(const Attention& P, Plan& plan) {
+    const uint32_t n = P.B.n_seqs, per = (n + kThreads - 1) / kThreads, tid = threadIdx.x;
+    uint32_t mine = 0;
+    for (uint32_t b = tid * per; b < min(n, (tid + 1) * per); ++b) mine += chunks_of(P, sequence(P.B, b));
+    uint32_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint32_t other = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if ((tid & 31) >= d) upto += other;
+    }
+    if ((tid & 31) == 31) plan.warp_sum[tid / 32] = upto;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < tid / 32; ++w) before += plan.warp_sum[w];
+    plan.prefix[tid + 1] = before + upto;
+    if (tid == 0) {
+        plan.prefix[0] = 0;
+        plan.per_thread = per;
+    }
+    __syncthreads();
+    return (uint64_t)plan.prefix[kThreads] * P.B.n_kv_heads;
+}
+
+// The item that unit u belongs to (u < all units).
+template <int kThreads>
+__device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, uint64_t u) {
+    const uint32_t H = P.B.n_kv_heads;
+    uint32_t lo = 0, hi = kThreads;                       // the last thread whose prefix does not exceed u
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if ((uint64_t)plan.prefix[mid] * H <= u) lo = mid; else hi = mid;
+    }
+    Item it;
+    it.b = lo * plan.per_thread;
+    uint64_t at = (uint64_t)plan.prefix[lo] * H;
+    for (;; ++it.b) {
+        it.s = sequence(P.B, it.b);
+        it.chunks = chunks_of(P, it.s);
+        const uint64_t next = at + (uint64_t)it.chunks * H;
+        if (u < next || it.b + 1 >= P.B.n_seqs) break;
+        at = next;
+    }
+    it.chunks = max(it.chunks, 1u);
+    it.head = (uint32_t)((u - at) / it.chunks);
+    it.first = at + (uint64_t)it.head * it.chunks;
+    it.c0 = first_seen(it.s, P.window) / kTok;
+    return it;
+}
+
+template <int D, int NT>
+struct Params {
+    Attention P;
+    float* records;                  // two for each warp of the grid, then two for each CTA
+    int* counters;                   // one for each CTA: parts that have arrived of the item it begins and does not end
+    uint32_t min_warps;
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(const __grid_constant__ Params<D, NT> G) {
+    constexpr int kWarps = warps<D, NT>(), kThreads = kWarps * 32, kCols = 8 * NT;
+    constexpr int kKeyWords = D / 32, kSteps = D / 16;    // words of a row in a lane; k steps of the scores
+    constexpr int kValueWords = D / 64;
+    constexpr int kRecord = record_floats<D, NT>();
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Plan plan;
+    __shared__ __align__(8) uint64_t bars[kWarps * kStages];
+    __shared__ int abort_flag, rec_item[2 * kWarps], rec_open[2 * kWarps], is_last;
+    __shared__ float weight[2 * kWarps + 2][kCols];
+    const Attention& P = G.P;
+    const Batch& B = P.B;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const uint32_t ring = ptx::smem_u32(smem) + warp * kStages * stage_bytes<D>();
+    const uint8_t* ring_ptr = smem + warp * kStages * stage_bytes<D>();
+    const uint32_t bar = ptx::smem_u32(bars) + warp * kStages * 8;
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) ptx::mbar_init(bar + 8 * i, 1);
+        ptx::fence_barrier_init();
+    }
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const uint64_t units = make_plan<kThreads>(P, plan);
+    if (units == 0) return;
+    // how many warps of a CTA work: all, or fewer where that spreads the chunks over more SMs
+    const uint32_t per_cta = (uint32_t)min((uint64_t)kWarps, max((uint64_t)G.min_warps, (units + gridDim.x - 1) / gridDim.x));
+    const uint64_t workers = min(units, (uint64_t)gridDim.x * per_cta);
+    const uint64_t me = (uint64_t)blockIdx.x * per_cta + warp;
+    const bool active = warp < per_cta && me < workers;
+    auto start_of = [&](uint64_t w) { return w * units / workers; };
+    auto worker_of = [&](uint64_t u) { return ((u + 1) * workers + units - 1) / units - 1; };
+    if ((uint64_t)blockIdx.x * per_cta >= workers) return;
+    if (lane == 0) {
+        rec_item[2 * warp] = rec_item[2 * warp + 1] = -1;
+        rec_open[2 * warp] = rec_open[2 * warp + 1] = 0;
+    }
+
+    bool ok = true;
+    if (active) {
+        const uint64_t begin = start_of(me), end = start_of(me + 1);
+        const uint32_t pl = B.page_log2, pages_per_chunk = kTok >> pl, block_bytes = (D + 8) << pl;
+        // ---- copies: chunk u of the run into stage s; item and chunk of the copies run ahead of the ones worked on
+        Item ahead = item_of<kThreads>(P, plan, begin);
+        uint64_t ahead_u = begin;
+        auto issue = [&](int s) {                          // the next chunk of the run, if there is one
+            if (ahead_u >= end) return;
+            if (ahead_u >= ahead.first + ahead.chunks) ahead = item_of<kThreads>(P, plan, ahead_u);
+            const uint32_t c = ahead.c0 + (uint32_t)(ahead_u - ahead.first);
+            const int left = ahead.s.len - (int)(c * kTok);                      // may be <= 0: nothing to read
+            const uint32_t blocks = left <= 0 ? 0 : min(pages_per_chunk, ((uint32_t)left + (1u << pl) - 1) >> pl);
+            const uint8_t* src = nullptr;
+            if (lane < blocks) src = block_to_read<D>(B, ahead.b, (c * kTok >> pl) + lane, ahead.head);
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * s, blocks * block_bytes);
+            __syncwarp();
+            if (src) ptx::bulk_load(ring + s * stage_bytes<D>() + lane * block_bytes, src, block_bytes, bar + 8 * s);
+            ++ahead_u;
+        };
+        for (int s = 0; s < kStages; ++s) issue(s);
+
+        uint32_t qf[NT][kSteps][2];                        // the queries' fragments
+        float q_sum[NT][2];                                // sums of the columns that this lane's scores are of
+        float o[NT][D / 16][4], m[NT][2], l[NT][2], low[NT][2];
+        Item it = item_of<kThreads>(P, plan, begin);
+        int p_row[NT][2];                                  // the tokens of those columns' rows
+
+        auto begin_item = [&]() {
+            const uint32_t cols = (uint32_t)it.s.rows * P.group;
+            float part[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t col = 8 * n + g;
+                const bool real = col < cols;
+                const uint32_t row = real ? col / P.group : 0, head = it.head * P.group + (real ? col % P.group : 0);
+                const uint4* src = (const uint4*)(P.q + (uint64_t)(it.s.first_row + row) * P.q_stride + head * D + t * (D / 4));
+                part[n] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const uint4 w = real ? src[i] : make_uint4(0, 0, 0, 0);
+                    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        qf[n][2 * i + j / 2][j % 2] = x[j];
+                        part[n] += __uint_as_float(x[j] << 16) + __uint_as_float(x[j] & 0xFFFF0000u);
+                    }
+                }
+                part[n] += __shfl_xor_sync(0xFFFFFFFFu, part[n], 1);
+                part[n] += __shfl_xor_sync(0xFFFFFFFFu, part[n], 2);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    q_sum[n][i] = __shfl_sync(0xFFFFFFFFu, part[n], 4 * (2 * t + i));
+                    const uint32_t c = 8 * n + 2 * t + i;
+                    p_row[n][i] = it.s.len - it.s.rows + (int)min(c / P.group, (uint32_t)it.s.rows - 1);
+                    m[n][i] = -INFINITY;
+                    l[n][i] = low[n][i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
+            }
+        };
+
+        auto work_on = [&](const uint8_t* stage, uint32_t c) {
+            const int first = (int)(c * kTok);
+            // whether every row sees every token of the chunk
+            const int p_first = it.s.len - it.s.rows, p_last = it.s.len - 1;
+            const bool whole = first + kTok - 1 <= p_first && (P.window == 0 || first > p_last - (int)P.window);
+            float x[NT][kTok / 16][4];
+            uint32_t v_param[kTok / 16][2];
+#pragma unroll
+            for (int i = 0; i < kTok / 16; ++i) {
+                const uint8_t* block = stage + (16 * i >> pl) * block_bytes;
+                const uint32_t slot = (16 * i) & ((1u << pl) - 1);
+                uint32_t wa[kKeyWords], wb[kKeyWords];
+                const uint8_t* row = block + (slot + token_of(g)) * (D / 2) + t * (D / 8);
+                if constexpr (D == 128) {
+                    const uint4 a = *(const uint4*)row, b = *(const uint4*)(row + 8 * (D / 2));
+                    wa[0] = a.x; wa[1] = a.y; wa[2] = a.z; wa[3] = a.w;
+                    wb[0] = b.x; wb[1] = b.y; wb[2] = b.z; wb[3] = b.w;
+                } else {
+                    const uint2 a = *(const uint2*)row, b = *(const uint2*)(row + 8 * (D / 2));
+                    wa[0] = a.x; wa[1] = a.y;
+                    wb[0] = b.x; wb[1] = b.y;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[n][i][j] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+                    const uint32_t a0 = codes_128(wa[s / 2], 2 * (s % 2)), a1 = codes_128(wb[s / 2], 2 * (s % 2));
+                    const uint32_t a2 = codes_128(wa[s / 2], 2 * (s % 2) + 1), a3 = codes_128(wb[s / 2], 2 * (s % 2) + 1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_bf16(x[n][i], a0, a1, a2, a3, qf[n][s][0], qf[n][s][1]);
+                }
+                // scores, in powers of two
+                const uint32_t* params = (const uint32_t*)(block + params_at<D>(pl, 0)) + slot + token_of(g);
+                const uint32_t* v_params = (const uint32_t*)(block + params_at<D>(pl, 1)) + slot + token_of(g);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t p = params[8 * r];
+                    v_param[i][r] = v_params[8 * r];
+                    const float a = param_step(p) * P.scale_log2, b = fmaf(-128.0f, a, param_low(p) * P.scale_log2);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) x[n][i][2 * r + k] = fmaf(x[n][i][2 * r + k], a, b * q_sum[n][k]);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < kTok / 16; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int j = first + 16 * i + 8 * r + token_of(g);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                if (j > p_row[n][k] || (P.window && j <= p_row[n][k] - (int)P.window)) x[n][i][2 * r + k] = -INFINITY;
+                    }
+            }
+            // running maximum
+            float top[NT][2];
+            bool moved = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float y = m[n][k];
+#pragma unroll
+                    for (int i = 0; i < kTok / 16; ++i) y = fmaxf(y, fmaxf(x[n][i][k], x[n][i][2 + k]));
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, d));
+                    top[n][k] = y;
+                    moved |= y > m[n][k];
+                }
+            if (__any_sync(0xFFFFFFFFu, moved)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float keep = m[n][k] == top[n][k] ? 1.0f : exp2_fast(m[n][k] - top[n][k]);
+                        m[n][k] = top[n][k];
+                        l[n][k] *= keep;
+                        low[n][k] *= keep;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            o[n][i][k] *= keep;
+                            o[n][i][2 + k] *= keep;
+                        }
+                    }
+            }
+            // weights, and the values' steps in them
+            uint32_t pf[NT][kTok / 16][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+#pragma unroll
+                for (int i = 0; i < kTok / 16; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float step = param_step(v_param[i][r]), base = fmaf(8.0f, step, param_low(v_param[i][r]));
+                        const float p0 = exp2_fast(x[n][i][2 * r] - m0), p1 = exp2_fast(x[n][i][2 * r + 1] - m1);
+                        l[n][0] += p0;
+                        l[n][1] += p1;
+                        float w0 = p0 * step, w1 = p1 * step, e0 = p0 * base, e1 = p1 * base;
+                        if (!whole) {                      // the parameters of what is not seen may be anything
+                            if (x[n][i][2 * r] == -INFINITY) w0 = e0 = 0.0f;
+                            if (x[n][i][2 * r + 1] == -INFINITY) w1 = e1 = 0.0f;
+                        }
+                        low[n][0] += e0;
+                        low[n][1] += e1;
+                        pf[n][i][r] = transpose8x8(pack(w0, w1));
+                    }
+            }
+            // values
+#pragma unroll
+            for (int i = 0; i < kTok / 16; ++i) {
+                const uint8_t* block = stage + (16 * i >> pl) * block_bytes;
+                const uint32_t slot = (16 * i) & ((1u << pl) - 1);
+                uint32_t w[4][kValueWords];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int token = token_of(2 * t + (r & 1)) + 8 * (r >> 1);
+                    const uint8_t* row = block + codes_at<D>(pl, 1) + (slot + token) * (D / 2) + g * (D / 16);
+                    if constexpr (D == 128) {
+                        const uint2 a = *(const uint2*)row;
+                        w[r][0] = a.x; w[r][1] = a.y;
+                    } else {
+                        w[r][0] = *(const uint32_t*)row;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kValueWords; ++j) {
+                    const uint32_t even0 = __byte_perm(w[0][j], w[1][j], 0x5410), odd0 = __byte_perm(w[0][j], w[1][j], 0x7632);
+                    const uint32_t even1 = __byte_perm(w[2][j], w[3][j], 0x5410), odd1 = __byte_perm(w[2][j], w[3][j], 0x7632);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t a0 = codes_centred(even0, k), a1 = codes_centred(odd0, k), a2 = codes_centred(even1, k), a3 = codes_centred(odd1, k);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_bf16(o[n][4 * j + k], a0, a1, a2, a3, pf[n][i][0], pf[n][i][1]);
+                    }
+                }
+            }
+        };
+
+        // the item is done as far as this warp goes: sums over the lanes, then to y, or to a record
+        auto end_item = [&](bool opens, bool goes_on) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) {
+                        l[n][k] += __shfl_xor_sync(0xFFFFFFFFu, l[n][k], d);
+                        low[n][k] += __shfl_xor_sync(0xFFFFFFFFu, low[n][k], d);
+                    }
+            if (opens && !goes_on) {
+                const uint32_t cols = (uint32_t)it.s.rows * P.group;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t c = 8 * n + 2 * t + k;
+                        if (c >= cols) continue;
+                        __nv_bfloat16* to = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + g * (D / 8);
+                        const float inverse = l[n][k] == 0.0f ? 0.0f : 1.0f / l[n][k];
+                        uint32_t out[D / 16];
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) out[i] = pack((o[n][i][k] + low[n][k]) * inverse, (o[n][i][2 + k] + low[n][k]) * inverse);
+#pragma unroll
+                        for (int i = 0; i < D / 64; ++i) *(uint4*)(to + 8 * i) = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
+                    }
+                return;
+            }
+            const uint32_t which = opens ? 1 : 0;          // 0: begun before this run, 1: begun in it
+            float* rec = G.records + (uint64_t)(2 * (blockIdx.x * kWarps + warp) + which) * kRecord;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t c = 8 * n + 2 * t + k;
+                    float4* to = (float4*)(rec + c * D + g * (D / 8));
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+                        to[i] = make_float4(o[n][2 * i][k] + low[n][k], o[n][2 * i][2 + k] + low[n][k], o[n][2 * i + 1][k] + low[n][k], o[n][2 * i + 1][2 + k] + low[n][k]);
+                    if (g == 0) {
+                        rec[kCols * D + c] = m[n][k];
+                        rec[kCols * D + kCols + c] = l[n][k];
+                    }
+                }
+            if (lane == 0) {
+                rec_item[2 * warp + which] = (int)(it.b * B.n_kv_heads + it.head);
+                rec_open[2 * warp + which] = goes_on;
+            }
+        };
+
+        uint64_t u = begin;
+        uint32_t phase = 0;
+        while (u < end) {
+            if (u != begin) it = item_of<kThreads>(P, plan, u);
+            const uint64_t item_end = it.first + it.chunks;
+            const bool opens = u == it.first;
+            begin_item();
+            for (; u < end && u < item_end; ++u) {
+                const int s = (int)((u - begin) % kStages);
+                ok = ok && ptx::mbar_wait_warp(bar + 8 * s, (phase >> s) & 1, &abort_flag, P.wait_limit_ns);
+                if (!ok) break;
+                phase ^= 1u << s;
+                work_on(ring_ptr + s * stage_bytes<D>(), it.c0 + (uint32_t)(u - it.first));
+                __syncwarp();
+                issue(s);
+            }
+            if (!ok) break;
+            end_item(opens, u < item_end);
+        }
+        if (!ok) {                                         // copies in flight end before the CTA does
+            for (int s = 0; s < kStages; ++s) {
+                volatile int never = 0;
+                ptx::mbar_wait_warp(bar + 8 * s, (phase >> s) & 1, &never, P.wait_limit_ns);
+            }
+            if (lane == 0) *(volatile int*)P.timeout_status = kStatusProducerTimeout | (int)blockIdx.x;
+        }
+    }
+    __syncthreads();
+    if (abort_flag) return;
+
+    // ---- joining.  Records of one item follow one another in the order (warp, begun before / begun in); a run of them that has both ends is finished here,
+    // one that is open on a side becomes a record of the CTA.
+    float* const cta_records = G.records + (uint64_t)2 * gridDim.x * kWarps * kRecord;
+    auto join = [&](uint32_t count, auto record, bool finish, const Item& it, float* to) {
+        // record(i): the i-th record in order; weights of the records, then every number of the sum by one thread
+        for (uint32_t c = threadIdx.x; c < kCols; c += kThreads) {
+            float top = -INFINITY, sum = 0.0f;
+            for (uint32_t i = 0; i < count; ++i) top = fmaxf(top, __ldcg(record(i) + kCols * D + c));
+            if (!finish) to[kCols * D + c] = top;
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (uint32_t i = 0; i < count; ++i) sum += exp2_fast(__ldcg(record(i) + kCols * D + c) - base) * __ldcg(record(i) + kCols * D + kCols + c);
+            if (!finish) to[kCols * D + kCols + c] = sum;
+            weight[0][c] = base;
+            weight[1][c] = finish ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+        }
+        __syncthreads();
+        const uint32_t cols = finish ? (uint32_t)it.s.rows * P.group : kCols;
+        for (uint32_t e = threadIdx.x * 4; e < cols * D; e += kThreads * 4) {
+            const uint32_t c = e / D;
+            float4 sum = make_float4(0, 0, 0, 0);
+            for (uint32_t i = 0; i < count; ++i) {
+                const float w = exp2_fast(__ldcg(record(i) + kCols * D + c) - weight[0][c]);
+                const float4 x = __ldcg((const float4*)(record(i) + e));
+                sum.x = fmaf(w, x.x, sum.x); sum.y = fmaf(w, x.y, sum.y); sum.z = fmaf(w, x.z, sum.z); sum.w = fmaf(w, x.w, sum.w);
+            }
+            const float f = weight[1][c];
+            if (finish) {
+                __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
+                *(uint2*)y = make_uint2(pack(sum.x * f, sum.y * f), pack(sum.z * f, sum.w * f));
+            } else {
+                *(float4*)(to + e) = sum;
+            }
+        }
+        __syncthreads();
+    };
+    const uint64_t cta_begin = start_of((uint64_t)blockIdx.x * per_cta);
+    const uint64_t cta_end = start_of(min(workers, (uint64_t)(blockIdx.x + 1) * per_cta));
+    for (int r = 0; r < 2 * kWarps;) {
+        if (rec_item[r] < 0) { ++r; continue; }
+        const int item = rec_item[r], from = r;
+        int last = r;
+        uint32_t count = 0;
+        for (; r < 2 * kWarps && (rec_item[r] < 0 || rec_item[r] == item); ++r)
+            if (rec_item[r] == item) { last = r; ++count; }
+        const bool open_start = (from & 1) == 0, open_end = rec_open[last] != 0;
+        // the records' numbers in order: a run is the first one, then one a warp
+        const float* base = G.records + (uint64_t)2 * blockIdx.x * kWarps * kRecord;
+        auto record = [&](uint32_t i) { return base + (uint64_t)(i == 0 ? from : 2 * (from / 2 + (int)i)) * kRecord; };
+        if (!open_start && !open_end) {
+            // (its first unit: the begin of the last run with it, less what came before; found again from the unit before that run)
+            const Item it = item_of<kThreads>(P, plan, start_of((uint64_t)blockIdx.x * per_cta + last / 2));
+            join(count, record, true, it, nullptr);
+            continue;
+        }
+        float* mine = cta_records + (uint64_t)(2 * blockIdx.x + (open_start ? 0 : 1)) * kRecord;
+        join(count, record, false, Item{}, mine);
+        const Item it = item_of<kThreads>(P, plan, open_start ? cta_begin : cta_end - 1);
+        const uint32_t first_cta = (uint32_t)(worker_of(it.first) / per_cta), last_cta = (uint32_t)(worker_of(it.first + it.chunks - 1) / per_cta);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const int before = atomicAdd(G.counters + first_cta, 1);
+            is_last = before == (int)(last_cta - first_cta);
+            if (is_last) G.counters[first_cta] = 0;
+            __threadfence();
+        }
+        __syncthreads();
+        if (is_last) {
+            auto part = [&](uint32_t i) { return cta_records + (uint64_t)(2 * (first_cta + i) + (i == 0 ? 1 : 0)) * kRecord; };
+            join(last_cta - first_cta + 1, part, true, it, nullptr);
+        }
+        __syncthreads();
+    }
+}
+
+template <int D, int NT>
+int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
+    constexpr int smem = warps<D, NT>() * kStages * stage_bytes<D>();
+    static bool attr_set[64] = {};   // per instantiation, per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return fail(T0_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", smem, cudaGetErrorString(e));
+        if (dev >= 0 && dev < 64) attr_set[dev] = true;
+    }
+    Params<D, NT> g;
+    g.P = p;
+    g.counters = (int*)p.scratch;
+    g.records = (float*)(p.scratch + kv4_counter_bytes());
+    g.min_warps = 4;
+    const cudaError_t e = gemm::launch_pdl(kv4_decode_kernel<D, NT>, std::min(sms, kMaxCtas), warps<D, NT>() * 32, smem, stream, g);
+    if (e != cudaSuccess) return fail(T0_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
+    return T0_OK;
+}
+
+}  // namespace
+
+size_t decode_scratch_bytes(uint32_t sms) {
+    const size_t n = std::min(sms, kMaxCtas);
+    auto one = [&](size_t warps, size_t record) { return (2 * n * warps + 2 * n) * record * sizeof(float); };
+    return std::max(std::max(one(warps<128, 1>(), record_floats<128, 1>()), one(warps<128, 2>(), record_floats<128, 2>())),
+                    std::max(one(warps<64, 1>(), record_floats<64, 1>()), one(warps<64, 2>(), record_floats<64, 2>())));
+}
+
+int launch_decode(const Attention& p, uint32_t head_dim, uint32_t columns, uint32_t sms, cudaStream_t stream) {
+    if (head_dim == 128) return columns <= 8 ? launch<128, 1>(p, sms, stream) : launch<128, 2>(p, sms, stream);
+    return columns <= 8 ? launch<64, 1>(p, sms, stream) : launch<64, 2>(p, sms, stream);
+}
+
+}  // namespace kv4
+}  // namespace t0
