@@ -22,7 +22,7 @@ struct Attention {
 };
 
 constexpr uint32_t kFewColumns = 16;                     // rows x group that kv4_decode takes
-constexpr uint32_t kMaxCtas = 1024;                      // arrival counters
+constexpr uint32_t kMaxCtas = 160;                       // of a persistent launch, one for each SM: arrival counters, parts of one item
 
 size_t decode_scratch_bytes(uint32_t sms);               // behind the counters
 int launch_decode(const Attention& p, uint32_t head_dim, uint32_t columns, uint32_t sms, cudaStream_t stream);

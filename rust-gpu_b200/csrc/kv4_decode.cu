@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kTok = 64;                                  // tokens of a chunk
 constexpr int kStages = 2;
+constexpr uint32_t kMaxParts = kMaxCtas;                  // parts of one item: at most one for each CTA
 
 template <int D> constexpr int stage_bytes() { return kTok * (D + 8); }
 template <int D, int NT> constexpr int warps() { return D == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 ? 16 : 12); }
@@ -38,14 +39,26 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// 128 + code of nibbles i and i + 4
-__device__ __forceinline__ uint32_t codes_128(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u; }
+// 128 + code of nibbles i and i + 4.  (x & mask) | k128 is one instruction where one of the two constants is in a register: k128, made by keep().
+__device__ __forceinline__ uint32_t keep(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t codes_128(uint32_t w, int i, uint32_t k128) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(k128));
+    return x;
+}
 // code - 8, exactly
-__device__ __forceinline__ uint32_t codes_centred(uint32_t w, int i) {
-    const uint32_t x = codes_128(w, i);
+__device__ __forceinline__ uint32_t codes_centred(uint32_t w, int i, uint32_t k128) {
+    const uint32_t x = codes_128(w, i, k128);
     const __nv_bfloat162 r = __hsub2(*(const __nv_bfloat162*)&x, __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
     return *(const uint32_t*)&r;
 }
+// two f32 at once
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&p;
@@ -125,7 +138,7 @@ __device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, ui
 template <int D, int NT>
 struct Params {
     Attention P;
-    float* records;                  // two for each warp of the grid, then two for each CTA
+    float* records;                  // one for each warp of the grid, then two for each CTA
     int* counters;                   // one for each CTA: parts that have arrived of the item it begins and does not end
     uint32_t min_warps;
 };
@@ -140,7 +153,9 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     __shared__ Plan plan;
     __shared__ __align__(8) uint64_t bars[kWarps * kStages];
     __shared__ int abort_flag, rec_item[2 * kWarps], rec_open[2 * kWarps], is_last;
-    __shared__ float weight[2 * kWarps + 2][kCols];
+    __shared__ float2 part_ml[kMaxParts][kCols];          // joining: maximum and sum of each part, then its weight
+    __shared__ float scale_of[kCols];
+    __shared__ const float* rec_at[2 * kWarps];
     const Attention& P = G.P;
     const Batch& B = P.B;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
@@ -172,28 +187,39 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     bool ok = true;
     if (active) {
         const uint64_t begin = start_of(me), end = start_of(me + 1);
-        const uint32_t pl = B.page_log2, pages_per_chunk = kTok >> pl, block_bytes = (D + 8) << pl;
-        // ---- copies: chunk u of the run into stage s; item and chunk of the copies run ahead of the ones worked on
+        const uint32_t pl = B.page_log2, page_mask = (1u << pl) - 1;
+        // ---- copies: chunk u of the run into stage s; item and chunk of the copies run ahead of the ones worked on.  A stage is laid out as a block of
+        // 64 tokens whatever the page size, so that its addresses are constants: a block of fewer tokens is copied in four pieces, one for each lane.
         Item ahead = item_of<kThreads>(P, plan, begin);
-        uint64_t ahead_u = begin;
+        uint32_t ahead_c = (uint32_t)(begin - ahead.first), ahead_left = (uint32_t)(end - begin);
+        const uint32_t piece = lane & 3, piece_row = piece < 2 ? D / 2 : 4;                     // bytes of a token in this lane's piece
+        const uint32_t piece_src = (piece == 0 ? 0 : piece == 1 ? D / 2 : piece == 2 ? D : D + 4) << pl, piece_dst = (piece == 0 ? 0 : piece == 1 ? D / 2 : piece == 2 ? D : D + 4) * kTok;
         auto issue = [&](int s) {                          // the next chunk of the run, if there is one
-            if (ahead_u >= end) return;
-            if (ahead_u >= ahead.first + ahead.chunks) ahead = item_of<kThreads>(P, plan, ahead_u);
-            const uint32_t c = ahead.c0 + (uint32_t)(ahead_u - ahead.first);
-            const int left = ahead.s.len - (int)(c * kTok);                      // may be <= 0: nothing to read
-            const uint32_t blocks = left <= 0 ? 0 : min(pages_per_chunk, ((uint32_t)left + (1u << pl) - 1) >> pl);
-            const uint8_t* src = nullptr;
-            if (lane < blocks) src = block_to_read<D>(B, ahead.b, (c * kTok >> pl) + lane, ahead.head);
-            if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * s, blocks * block_bytes);
+            if (ahead_left == 0) return;
+            if (ahead_c == ahead.chunks) {
+                ahead = item_of<kThreads>(P, plan, ahead.first + ahead.chunks);
+                ahead_c = 0;
+            }
+            const uint32_t first = (ahead.c0 + ahead_c) * kTok;
+            const uint32_t left = ahead.s.len > (int)first ? min((uint32_t)ahead.s.len - first, (uint32_t)kTok) : 0;
+            const uint32_t blocks = (left + page_mask) >> pl;
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * s, blocks * ((D + 8) << pl));
             __syncwarp();
-            if (src) ptx::bulk_load(ring + s * stage_bytes<D>() + lane * block_bytes, src, block_bytes, bar + 8 * s);
-            ++ahead_u;
+            const uint32_t mine = pl == 6 ? lane : lane >> 2;
+            if (mine < blocks) {
+                const uint8_t* src = block_to_read<D>(B, ahead.b, (first >> pl) + mine, ahead.head);
+                if (pl == 6) ptx::bulk_load(ring + s * stage_bytes<D>(), src, stage_bytes<D>(), bar + 8 * s);
+                else ptx::bulk_load(ring + s * stage_bytes<D>() + piece_dst + ((mine * piece_row) << pl), src + piece_src, piece_row << pl, bar + 8 * s);
+            }
+            ++ahead_c;
+            --ahead_left;
         };
         for (int s = 0; s < kStages; ++s) issue(s);
 
         uint32_t qf[NT][kSteps][2];                        // the queries' fragments
-        float q_sum[NT][2];                                // sums of the columns that this lane's scores are of
-        float o[NT][D / 16][4], m[NT][2], l[NT][2], low[NT][2];
+        float2 q_sum[NT];                                  // sums of the columns that this lane's scores are of
+        float o[NT][D / 16][4], m[NT][2];
+        float2 l[NT], low[NT];
         Item it = item_of<kThreads>(P, plan, begin);
         int p_row[NT][2];                                  // the tokens of those columns' rows
 
@@ -221,12 +247,12 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                 part[n] += __shfl_xor_sync(0xFFFFFFFFu, part[n], 2);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    q_sum[n][i] = __shfl_sync(0xFFFFFFFFu, part[n], 4 * (2 * t + i));
+                    (i ? q_sum[n].y : q_sum[n].x) = __shfl_sync(0xFFFFFFFFu, part[n], 4 * (2 * t + i));
                     const uint32_t c = 8 * n + 2 * t + i;
                     p_row[n][i] = it.s.len - it.s.rows + (int)min(c / P.group, (uint32_t)it.s.rows - 1);
                     m[n][i] = -INFINITY;
-                    l[n][i] = low[n][i] = 0.0f;
                 }
+                l[n] = low[n] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -234,19 +260,18 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             }
         };
 
-        auto work_on = [&](const uint8_t* stage, uint32_t c) {
-            const int first = (int)(c * kTok);
-            // whether every row sees every token of the chunk
-            const int p_first = it.s.len - it.s.rows, p_last = it.s.len - 1;
-            const bool whole = first + kTok - 1 <= p_first && (P.window == 0 || first > p_last - (int)P.window);
-            float x[NT][kTok / 16][4];
+        const uint32_t k128 = keep(0x43004300u);
+        const uint32_t key_at = token_of(g) * (D / 2) + t * (D / 8), param_at = D * kTok + 4 * token_of(g);
+        const uint32_t value_at = kTok * (D / 2) + token_of(2 * t) * (D / 2) + g * (D / 16);
+        // `whole`: every row sees every token of the chunk
+        auto work_on = [&](const uint8_t* stage, int first, auto whole) {
+            constexpr bool kWhole = decltype(whole)::value;
+            float2 x[NT][kTok / 16][2];
             uint32_t v_param[kTok / 16][2];
 #pragma unroll
             for (int i = 0; i < kTok / 16; ++i) {
-                const uint8_t* block = stage + (16 * i >> pl) * block_bytes;
-                const uint32_t slot = (16 * i) & ((1u << pl) - 1);
                 uint32_t wa[kKeyWords], wb[kKeyWords];
-                const uint8_t* row = block + (slot + token_of(g)) * (D / 2) + t * (D / 8);
+                const uint8_t* row = stage + key_at + i * (16 * D / 2);
                 if constexpr (D == 128) {
                     const uint4 a = *(const uint4*)row, b = *(const uint4*)(row + 8 * (D / 2));
                     wa[0] = a.x; wa[1] = a.y; wa[2] = a.z; wa[3] = a.w;
@@ -256,108 +281,102 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                     wa[0] = a.x; wa[1] = a.y;
                     wb[0] = b.x; wb[1] = b.y;
                 }
+                float acc[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[n][i][j] = 0.0f;
+                    for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
-                    const uint32_t a0 = codes_128(wa[s / 2], 2 * (s % 2)), a1 = codes_128(wb[s / 2], 2 * (s % 2));
-                    const uint32_t a2 = codes_128(wa[s / 2], 2 * (s % 2) + 1), a3 = codes_128(wb[s / 2], 2 * (s % 2) + 1);
+                    const uint32_t a0 = codes_128(wa[s / 2], 2 * (s % 2), k128), a1 = codes_128(wb[s / 2], 2 * (s % 2), k128);
+                    const uint32_t a2 = codes_128(wa[s / 2], 2 * (s % 2) + 1, k128), a3 = codes_128(wb[s / 2], 2 * (s % 2) + 1, k128);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_bf16(x[n][i], a0, a1, a2, a3, qf[n][s][0], qf[n][s][1]);
+                    for (int n = 0; n < NT; ++n) mma_bf16(acc[n], a0, a1, a2, a3, qf[n][s][0], qf[n][s][1]);
                 }
                 // scores, in powers of two
-                const uint32_t* params = (const uint32_t*)(block + params_at<D>(pl, 0)) + slot + token_of(g);
-                const uint32_t* v_params = (const uint32_t*)(block + params_at<D>(pl, 1)) + slot + token_of(g);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint32_t p = params[8 * r];
-                    v_param[i][r] = v_params[8 * r];
+                    const uint32_t p = *(const uint32_t*)(stage + param_at + 4 * (16 * i + 8 * r));
+                    v_param[i][r] = *(const uint32_t*)(stage + param_at + 4 * (kTok + 16 * i + 8 * r));
                     const float a = param_step(p) * P.scale_log2, b = fmaf(-128.0f, a, param_low(p) * P.scale_log2);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
+                        x[n][i][r] = fma2(make_float2(acc[n][2 * r], acc[n][2 * r + 1]), make_float2(a, a), mul2(make_float2(b, b), q_sum[n]));
+                    if constexpr (!kWhole) {
+                        const int j = first + 16 * i + 8 * r + token_of(g);
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) x[n][i][2 * r + k] = fmaf(x[n][i][2 * r + k], a, b * q_sum[n][k]);
+                        for (int n = 0; n < NT; ++n) {
+                            if (j > p_row[n][0] || (P.window && j <= p_row[n][0] - (int)P.window)) x[n][i][r].x = -INFINITY;
+                            if (j > p_row[n][1] || (P.window && j <= p_row[n][1] - (int)P.window)) x[n][i][r].y = -INFINITY;
+                        }
+                    }
                 }
             }
-            if (!whole) {
+            // running maximum
+            float2 top[NT];
+            bool moved = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                top[n] = make_float2(m[n][0], m[n][1]);
 #pragma unroll
                 for (int i = 0; i < kTok / 16; ++i)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const int j = first + 16 * i + 8 * r + token_of(g);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k)
-                                if (j > p_row[n][k] || (P.window && j <= p_row[n][k] - (int)P.window)) x[n][i][2 * r + k] = -INFINITY;
+                        top[n].x = fmaxf(top[n].x, x[n][i][r].x);
+                        top[n].y = fmaxf(top[n].y, x[n][i][r].y);
                     }
-            }
-            // running maximum
-            float top[NT][2];
-            bool moved = false;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float y = m[n][k];
-#pragma unroll
-                    for (int i = 0; i < kTok / 16; ++i) y = fmaxf(y, fmaxf(x[n][i][k], x[n][i][2 + k]));
-#pragma unroll
-                    for (int d = 4; d < 32; d *= 2) y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, d));
-                    top[n][k] = y;
-                    moved |= y > m[n][k];
+                for (int d = 4; d < 32; d *= 2) {
+                    top[n].x = fmaxf(top[n].x, __shfl_xor_sync(0xFFFFFFFFu, top[n].x, d));
+                    top[n].y = fmaxf(top[n].y, __shfl_xor_sync(0xFFFFFFFFu, top[n].y, d));
                 }
+                moved |= top[n].x > m[n][0] || top[n].y > m[n][1];
+            }
             if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                    const float2 less = make_float2(m[n][0] == top[n].x ? 1.0f : exp2_fast(m[n][0] - top[n].x), m[n][1] == top[n].y ? 1.0f : exp2_fast(m[n][1] - top[n].y));
+                    m[n][0] = top[n].x;
+                    m[n][1] = top[n].y;
+                    l[n] = mul2(l[n], less);
+                    low[n] = mul2(low[n], less);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float keep = m[n][k] == top[n][k] ? 1.0f : exp2_fast(m[n][k] - top[n][k]);
-                        m[n][k] = top[n][k];
-                        l[n][k] *= keep;
-                        low[n][k] *= keep;
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i) {
-                            o[n][i][k] *= keep;
-                            o[n][i][2 + k] *= keep;
-                        }
+                    for (int i = 0; i < D / 16; ++i) {
+                        o[n][i][0] *= less.x; o[n][i][1] *= less.y;
+                        o[n][i][2] *= less.x; o[n][i][3] *= less.y;
                     }
+                }
             }
             // weights, and the values' steps in them
             uint32_t pf[NT][kTok / 16][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+                const float2 minus = make_float2(m[n][0] == -INFINITY ? 0.0f : -m[n][0], m[n][1] == -INFINITY ? 0.0f : -m[n][1]);
 #pragma unroll
                 for (int i = 0; i < kTok / 16; ++i)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float step = param_step(v_param[i][r]), base = fmaf(8.0f, step, param_low(v_param[i][r]));
-                        const float p0 = exp2_fast(x[n][i][2 * r] - m0), p1 = exp2_fast(x[n][i][2 * r + 1] - m1);
-                        l[n][0] += p0;
-                        l[n][1] += p1;
-                        float w0 = p0 * step, w1 = p1 * step, e0 = p0 * base, e1 = p1 * base;
-                        if (!whole) {                      // the parameters of what is not seen may be anything
-                            if (x[n][i][2 * r] == -INFINITY) w0 = e0 = 0.0f;
-                            if (x[n][i][2 * r + 1] == -INFINITY) w1 = e1 = 0.0f;
+                        const float2 y = add2(x[n][i][r], minus), p = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                        l[n] = add2(l[n], p);
+                        float2 w = mul2(p, make_float2(step, step));
+                        if constexpr (kWhole) {
+                            low[n] = fma2(p, make_float2(base, base), low[n]);
+                        } else {                           // the parameters of what is not seen may be anything
+                            if (x[n][i][r].x == -INFINITY) w.x = 0.0f; else low[n].x = fmaf(p.x, base, low[n].x);
+                            if (x[n][i][r].y == -INFINITY) w.y = 0.0f; else low[n].y = fmaf(p.y, base, low[n].y);
                         }
-                        low[n][0] += e0;
-                        low[n][1] += e1;
-                        pf[n][i][r] = transpose8x8(pack(w0, w1));
+                        pf[n][i][r] = transpose8x8(pack(w.x, w.y));
                     }
             }
             // values
 #pragma unroll
             for (int i = 0; i < kTok / 16; ++i) {
-                const uint8_t* block = stage + (16 * i >> pl) * block_bytes;
-                const uint32_t slot = (16 * i) & ((1u << pl) - 1);
                 uint32_t w[4][kValueWords];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int token = token_of(2 * t + (r & 1)) + 8 * (r >> 1);
-                    const uint8_t* row = block + codes_at<D>(pl, 1) + (slot + token) * (D / 2) + g * (D / 16);
+                for (int r = 0; r < 4; ++r) {              // (token_of(2 t + 1) is token_of(2 t) + 1 or - 1)
+                    const int away = (r & 1) ? (t & 1 ? -(D / 2) : D / 2) : 0;
+                    const uint8_t* row = stage + value_at + away + (16 * i + 8 * (r >> 1)) * (D / 2);
                     if constexpr (D == 128) {
                         const uint2 a = *(const uint2*)row;
                         w[r][0] = a.x; w[r][1] = a.y;
@@ -371,7 +390,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                     const uint32_t even1 = __byte_perm(w[2][j], w[3][j], 0x5410), odd1 = __byte_perm(w[2][j], w[3][j], 0x7632);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const uint32_t a0 = codes_centred(even0, k), a1 = codes_centred(odd0, k), a2 = codes_centred(even1, k), a3 = codes_centred(odd1, k);
+                        const uint32_t a0 = codes_centred(even0, k, k128), a1 = codes_centred(odd0, k, k128), a2 = codes_centred(even1, k, k128), a3 = codes_centred(odd1, k, k128);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) mma_bf16(o[n][4 * j + k], a0, a1, a2, a3, pf[n][i][0], pf[n][i][1]);
                     }
@@ -380,16 +399,20 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
         };
 
         // the item is done as far as this warp goes: sums over the lanes, then to y, or to a record
-        auto end_item = [&](bool opens, bool goes_on) {
+        auto end_item = [&](bool opens, bool goes_on, bool last) {
+            float sum[NT][2], rest[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < 2; ++k) {
+                    sum[n][k] = k ? l[n].y : l[n].x;
+                    rest[n][k] = k ? low[n].y : low[n].x;
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) {
-                        l[n][k] += __shfl_xor_sync(0xFFFFFFFFu, l[n][k], d);
-                        low[n][k] += __shfl_xor_sync(0xFFFFFFFFu, low[n][k], d);
+                        sum[n][k] += __shfl_xor_sync(0xFFFFFFFFu, sum[n][k], d);
+                        rest[n][k] += __shfl_xor_sync(0xFFFFFFFFu, rest[n][k], d);
                     }
+                }
             if (opens && !goes_on) {
                 const uint32_t cols = (uint32_t)it.s.rows * P.group;
 #pragma unroll
@@ -399,17 +422,19 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                         const uint32_t c = 8 * n + 2 * t + k;
                         if (c >= cols) continue;
                         __nv_bfloat16* to = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + g * (D / 8);
-                        const float inverse = l[n][k] == 0.0f ? 0.0f : 1.0f / l[n][k];
+                        const float inverse = sum[n][k] == 0.0f ? 0.0f : 1.0f / sum[n][k];
                         uint32_t out[D / 16];
 #pragma unroll
-                        for (int i = 0; i < D / 16; ++i) out[i] = pack((o[n][i][k] + low[n][k]) * inverse, (o[n][i][2 + k] + low[n][k]) * inverse);
+                        for (int i = 0; i < D / 16; ++i) out[i] = pack((o[n][i][k] + rest[n][k]) * inverse, (o[n][i][2 + k] + rest[n][k]) * inverse);
 #pragma unroll
                         for (int i = 0; i < D / 64; ++i) *(uint4*)(to + 8 * i) = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
                     }
                 return;
             }
             const uint32_t which = opens ? 1 : 0;          // 0: begun before this run, 1: begun in it
-            float* rec = G.records + (uint64_t)(2 * (blockIdx.x * kWarps + warp) + which) * kRecord;
+            // after the last chunk of the run the warp's buffers are free; before, the record has to go out
+            float* rec = last ? (float*)ring_ptr : G.records + (uint64_t)(blockIdx.x * kWarps + warp) * kRecord;
+            if (last) __syncwarp();
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -418,15 +443,16 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                     float4* to = (float4*)(rec + c * D + g * (D / 8));
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i)
-                        to[i] = make_float4(o[n][2 * i][k] + low[n][k], o[n][2 * i][2 + k] + low[n][k], o[n][2 * i + 1][k] + low[n][k], o[n][2 * i + 1][2 + k] + low[n][k]);
+                        to[i] = make_float4(o[n][2 * i][k] + rest[n][k], o[n][2 * i][2 + k] + rest[n][k], o[n][2 * i + 1][k] + rest[n][k], o[n][2 * i + 1][2 + k] + rest[n][k]);
                     if (g == 0) {
                         rec[kCols * D + c] = m[n][k];
-                        rec[kCols * D + kCols + c] = l[n][k];
+                        rec[kCols * D + kCols + c] = sum[n][k];
                     }
                 }
             if (lane == 0) {
                 rec_item[2 * warp + which] = (int)(it.b * B.n_kv_heads + it.head);
                 rec_open[2 * warp + which] = goes_on;
+                rec_at[2 * warp + which] = rec;
             }
         };
 
@@ -442,12 +468,15 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                 ok = ok && ptx::mbar_wait_warp(bar + 8 * s, (phase >> s) & 1, &abort_flag, P.wait_limit_ns);
                 if (!ok) break;
                 phase ^= 1u << s;
-                work_on(ring_ptr + s * stage_bytes<D>(), it.c0 + (uint32_t)(u - it.first));
+                const int first = (int)(it.c0 + (uint32_t)(u - it.first)) * kTok, p_first = it.s.len - it.s.rows;
+                const uint8_t* stage = ring_ptr + s * stage_bytes<D>();
+                if (first + kTok - 1 <= p_first && (P.window == 0 || first > it.s.len - 1 - (int)P.window)) work_on(stage, first, std::true_type{});
+                else work_on(stage, first, std::false_type{});
                 __syncwarp();
                 issue(s);
             }
             if (!ok) break;
-            end_item(opens, u < item_end);
+            end_item(opens, u < item_end, u == end);
         }
         if (!ok) {                                         // copies in flight end before the CTA does
             for (int s = 0; s < kStages; ++s) {
@@ -462,30 +491,49 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
 
     // ---- joining.  Records of one item follow one another in the order (warp, begun before / begun in); a run of them that has both ends is finished here,
     // one that is open on a side becomes a record of the CTA.
-    float* const cta_records = G.records + (uint64_t)2 * gridDim.x * kWarps * kRecord;
+    float* const cta_records = G.records + (uint64_t)gridDim.x * kWarps * kRecord;
     auto join = [&](uint32_t count, auto record, bool finish, const Item& it, float* to) {
-        // record(i): the i-th record in order; weights of the records, then every number of the sum by one thread
-        for (uint32_t c = threadIdx.x; c < kCols; c += kThreads) {
-            float top = -INFINITY, sum = 0.0f;
-            for (uint32_t i = 0; i < count; ++i) top = fmaxf(top, __ldcg(record(i) + kCols * D + c));
-            if (!finish) to[kCols * D + c] = top;
-            const float base = top == -INFINITY ? 0.0f : top;
-            for (uint32_t i = 0; i < count; ++i) sum += exp2_fast(__ldcg(record(i) + kCols * D + c) - base) * __ldcg(record(i) + kCols * D + kCols + c);
-            if (!finish) to[kCols * D + kCols + c] = sum;
-            weight[0][c] = base;
-            weight[1][c] = finish ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+        // record(i): the i-th part in order.  Maxima and sums of all parts, their weights, then every number of the sum by one thread.
+        for (uint32_t e = threadIdx.x; e < count * kCols; e += kThreads) {
+            const float* r = record(e / kCols) + kCols * D + e % kCols;
+            part_ml[e / kCols][e % kCols] = make_float2(r[0], r[kCols]);
+        }
+        __syncthreads();
+        if (warp < kCols) {
+            for (uint32_t c = warp; c < kCols; c += kWarps) {
+                float top = -INFINITY, sum = 0.0f;
+                for (uint32_t i = lane; i < count; i += 32) top = fmaxf(top, part_ml[i][c].x);
+#pragma unroll
+                for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                const float base = top == -INFINITY ? 0.0f : top;
+                for (uint32_t i = lane; i < count; i += 32) {
+                    const float w = exp2_fast(part_ml[i][c].x - base);
+                    sum += w * part_ml[i][c].y;
+                    part_ml[i][c].x = w;
+                }
+#pragma unroll
+                for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+                if (lane == 0) {
+                    scale_of[c] = !finish ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+                    if (!finish) {
+                        to[kCols * D + c] = top;
+                        to[kCols * D + kCols + c] = sum;
+                    }
+                }
+            }
         }
         __syncthreads();
         const uint32_t cols = finish ? (uint32_t)it.s.rows * P.group : kCols;
         for (uint32_t e = threadIdx.x * 4; e < cols * D; e += kThreads * 4) {
             const uint32_t c = e / D;
             float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 8
             for (uint32_t i = 0; i < count; ++i) {
-                const float w = exp2_fast(__ldcg(record(i) + kCols * D + c) - weight[0][c]);
-                const float4 x = __ldcg((const float4*)(record(i) + e));
+                const float w = part_ml[i][c].x;
+                const float4 x = *(const float4*)(record(i) + e);
                 sum.x = fmaf(w, x.x, sum.x); sum.y = fmaf(w, x.y, sum.y); sum.z = fmaf(w, x.z, sum.z); sum.w = fmaf(w, x.w, sum.w);
             }
-            const float f = weight[1][c];
+            const float f = scale_of[c];
             if (finish) {
                 __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
                 *(uint2*)y = make_uint2(pack(sum.x * f, sum.y * f), pack(sum.z * f, sum.w * f));
@@ -506,8 +554,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             if (rec_item[r] == item) { last = r; ++count; }
         const bool open_start = (from & 1) == 0, open_end = rec_open[last] != 0;
         // the records' numbers in order: a run is the first one, then one a warp
-        const float* base = G.records + (uint64_t)2 * blockIdx.x * kWarps * kRecord;
-        auto record = [&](uint32_t i) { return base + (uint64_t)(i == 0 ? from : 2 * (from / 2 + (int)i)) * kRecord; };
+        auto record = [&](uint32_t i) { return rec_at[i == 0 ? from : 2 * (from / 2 + (int)i)]; };
         if (!open_start && !open_end) {
             // (its first unit: the begin of the last run with it, less what came before; found again from the unit before that run)
             const Item it = item_of<kThreads>(P, plan, start_of((uint64_t)blockIdx.x * per_cta + last / 2));
@@ -515,7 +562,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             continue;
         }
         float* mine = cta_records + (uint64_t)(2 * blockIdx.x + (open_start ? 0 : 1)) * kRecord;
-        join(count, record, false, Item{}, mine);
+        join(count, record, false, Item{}, mine);          // (also where it is one part: it may lie in shared memory)
         const Item it = item_of<kThreads>(P, plan, open_start ? cta_begin : cta_end - 1);
         const uint32_t first_cta = (uint32_t)(worker_of(it.first) / per_cta), last_cta = (uint32_t)(worker_of(it.first + it.chunks - 1) / per_cta);
         __threadfence();
@@ -560,7 +607,7 @@ int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
 
 size_t decode_scratch_bytes(uint32_t sms) {
     const size_t n = std::min(sms, kMaxCtas);
-    auto one = [&](size_t warps, size_t record) { return (2 * n * warps + 2 * n) * record * sizeof(float); };
+    auto one = [&](size_t warps, size_t record) { return (n * warps + 2 * n) * record * sizeof(float); };
     return std::max(std::max(one(warps<128, 1>(), record_floats<128, 1>()), one(warps<128, 2>(), record_floats<128, 2>())),
                     std::max(one(warps<64, 1>(), record_floats<64, 1>()), one(warps<64, 2>(), record_floats<64, 2>())));
 }
