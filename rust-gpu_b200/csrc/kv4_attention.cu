@@ -79,6 +79,10 @@ int t0_kv4_attention(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_att
     const bool in_place = a.y == a.q && (a.y_stride == a.q_stride || batch->n_rows == 1);
     if (!in_place && rows_touch(a.q, 2ull * width, 2ull * a.q_stride, a.y, 2ull * width, 2ull * a.y_stride, batch->n_rows))
         return fail(T0_ERR_INVALID, "y overlaps q (it may be q itself)");
+    // the most chunks of 64 tokens that the batch may hold: the kernels count them, for every head, in 32 bits
+    if ((uint64_t)batch->n_seqs * ((uint64_t)batch->table_stride * batch->page_size / 64 + 1) * batch->n_kv_heads >= 1ull << 31)
+        return fail(T0_ERR_UNSUPPORTED, "%u sequences of up to %llu tokens, %u heads: too much for one call", batch->n_seqs,
+                    (unsigned long long)batch->table_stride * batch->page_size, batch->n_kv_heads);
     P.q = (const __nv_bfloat16*)a.q; P.y = (__nv_bfloat16*)a.y;
     P.q_stride = a.q_stride; P.y_stride = a.y_stride;
     P.group = a.n_q_heads / batch->n_kv_heads; P.window = a.window;

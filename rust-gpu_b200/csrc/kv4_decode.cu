@@ -82,11 +82,11 @@ struct Item {
     uint32_t b, head;
     Sequence s;
     uint32_t chunks, c0;             // chunks of the item; the first chunk's number in the sequence
-    uint64_t first;                  // its first unit
+    uint32_t first;                  // its first unit
 };
 
 template <int kThreads>
-__device__ __forceinline__ uint64_t make_plan(const Attention& P, Plan& plan) {
+__device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
     const uint32_t n = P.B.n_seqs, per = (n + kThreads - 1) / kThreads, tid = threadIdx.x;
     uint32_t mine = 0;
     for (uint32_t b = tid * per; b < min(n, (tid + 1) * per); ++b) mine += chunks_of(P, sequence(P.B, b));
@@ -106,31 +106,31 @@ __device__ __forceinline__ uint64_t make_plan(const Attention& P, Plan& plan) {
         plan.per_thread = per;
     }
     __syncthreads();
-    return (uint64_t)plan.prefix[kThreads] * P.B.n_kv_heads;
+    return plan.prefix[kThreads] * P.B.n_kv_heads;           // (less than 2^31: checked on the host)
 }
 
 // The item that unit u belongs to (u < all units).
 template <int kThreads>
-__device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, uint64_t u) {
+__device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, uint32_t u) {
     const uint32_t H = P.B.n_kv_heads;
     uint32_t lo = 0, hi = kThreads;                       // the last thread whose prefix does not exceed u
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
-        if ((uint64_t)plan.prefix[mid] * H <= u) lo = mid; else hi = mid;
+        if (plan.prefix[mid] * H <= u) lo = mid; else hi = mid;
     }
     Item it;
     it.b = lo * plan.per_thread;
-    uint64_t at = (uint64_t)plan.prefix[lo] * H;
+    uint32_t at = plan.prefix[lo] * H;
     for (;; ++it.b) {
         it.s = sequence(P.B, it.b);
         it.chunks = chunks_of(P, it.s);
-        const uint64_t next = at + (uint64_t)it.chunks * H;
+        const uint32_t next = at + it.chunks * H;
         if (u < next || it.b + 1 >= P.B.n_seqs) break;
         at = next;
     }
     it.chunks = max(it.chunks, 1u);
-    it.head = (uint32_t)((u - at) / it.chunks);
-    it.first = at + (uint64_t)it.head * it.chunks;
+    it.head = (u - at) / it.chunks;
+    it.first = at + it.head * it.chunks;
     it.c0 = first_seen(it.s, P.window) / kTok;
     return it;
 }
@@ -152,7 +152,9 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Plan plan;
     __shared__ __align__(8) uint64_t bars[kWarps * kStages];
-    __shared__ int abort_flag, rec_item[2 * kWarps], rec_open[2 * kWarps], is_last;
+    __shared__ int abort_flag, rec_there[2 * kWarps], rec_open[2 * kWarps], is_last[2];
+    __shared__ uint32_t parts_from[2], parts_of[2];
+    __shared__ Item edge_item[2];                           // the items that the CTA may have begun in, and may end in
     __shared__ float2 part_ml[kMaxParts][kCols];          // joining: maximum and sum of each part, then its weight
     __shared__ float scale_of[kCols];
     __shared__ const float* rec_at[2 * kWarps];
@@ -169,29 +171,31 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     }
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const uint64_t units = make_plan<kThreads>(P, plan);
+    const uint32_t units = make_plan<kThreads>(P, plan);
     if (units == 0) return;
     // how many warps of a CTA work: all, or fewer where that spreads the chunks over more SMs
-    const uint32_t per_cta = (uint32_t)min((uint64_t)kWarps, max((uint64_t)G.min_warps, (units + gridDim.x - 1) / gridDim.x));
-    const uint64_t workers = min(units, (uint64_t)gridDim.x * per_cta);
-    const uint64_t me = (uint64_t)blockIdx.x * per_cta + warp;
+    const uint32_t per_cta = min((uint32_t)kWarps, max(G.min_warps, (units + gridDim.x - 1) / gridDim.x));
+    const uint32_t workers = min(units, gridDim.x * per_cta), whole = units / workers, rest = units % workers;
+    const uint32_t me = blockIdx.x * per_cta + warp;
     const bool active = warp < per_cta && me < workers;
-    auto start_of = [&](uint64_t w) { return w * units / workers; };
-    auto worker_of = [&](uint64_t u) { return ((u + 1) * workers + units - 1) / units - 1; };
-    if ((uint64_t)blockIdx.x * per_cta >= workers) return;
+    auto start_of = [&](uint32_t w) { return w * whole + w * rest / workers; };       // w units / workers, rounded down
+    auto worker_of = [&](uint32_t u) { return (uint32_t)(((uint64_t)(u + 1) * workers + units - 1) / units - 1); };
+    if (blockIdx.x * per_cta >= workers) return;
+    const uint32_t here = min(per_cta, workers - blockIdx.x * per_cta);               // warps of this CTA that work
     if (lane == 0) {
-        rec_item[2 * warp] = rec_item[2 * warp + 1] = -1;
+        rec_there[2 * warp] = rec_there[2 * warp + 1] = 0;
         rec_open[2 * warp] = rec_open[2 * warp + 1] = 0;
     }
 
     bool ok = true;
     if (active) {
-        const uint64_t begin = start_of(me), end = start_of(me + 1);
+        const uint32_t begin = start_of(me), end = start_of(me + 1);
         const uint32_t pl = B.page_log2, page_mask = (1u << pl) - 1;
         // ---- copies: chunk u of the run into stage s; item and chunk of the copies run ahead of the ones worked on.  A stage is laid out as a block of
         // 64 tokens whatever the page size, so that its addresses are constants: a block of fewer tokens is copied in four pieces, one for each lane.
-        Item ahead = item_of<kThreads>(P, plan, begin);
-        uint32_t ahead_c = (uint32_t)(begin - ahead.first), ahead_left = (uint32_t)(end - begin);
+        const Item ahead_first = item_of<kThreads>(P, plan, begin);
+        Item ahead = ahead_first;
+        uint32_t ahead_c = begin - ahead.first, ahead_left = end - begin;
         const uint32_t piece = lane & 3, piece_row = piece < 2 ? D / 2 : 4;                     // bytes of a token in this lane's piece
         const uint32_t piece_src = (piece == 0 ? 0 : piece == 1 ? D / 2 : piece == 2 ? D : D + 4) << pl, piece_dst = (piece == 0 ? 0 : piece == 1 ? D / 2 : piece == 2 ? D : D + 4) * kTok;
         auto issue = [&](int s) {                          // the next chunk of the run, if there is one
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
         float2 q_sum[NT];                                  // sums of the columns that this lane's scores are of
         float o[NT][D / 16][4], m[NT][2];
         float2 l[NT], low[NT];
-        Item it = item_of<kThreads>(P, plan, begin);
+        Item it = ahead_first;
         int p_row[NT][2];                                  // the tokens of those columns' rows
 
         auto begin_item = [&]() {
@@ -450,25 +454,25 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                     }
                 }
             if (lane == 0) {
-                rec_item[2 * warp + which] = (int)(it.b * B.n_kv_heads + it.head);
+                rec_there[2 * warp + which] = 1;
                 rec_open[2 * warp + which] = goes_on;
                 rec_at[2 * warp + which] = rec;
             }
         };
 
-        uint64_t u = begin;
-        uint32_t phase = 0;
+        if (warp == 0 && lane == 0) edge_item[0] = it;
+        uint32_t u = begin, phase = 0;
         while (u < end) {
             if (u != begin) it = item_of<kThreads>(P, plan, u);
-            const uint64_t item_end = it.first + it.chunks;
+            const uint32_t item_end = it.first + it.chunks;
             const bool opens = u == it.first;
             begin_item();
             for (; u < end && u < item_end; ++u) {
-                const int s = (int)((u - begin) % kStages);
+                const int s = (u - begin) % kStages;
                 ok = ok && ptx::mbar_wait_warp(bar + 8 * s, (phase >> s) & 1, &abort_flag, P.wait_limit_ns);
                 if (!ok) break;
                 phase ^= 1u << s;
-                const int first = (int)(it.c0 + (uint32_t)(u - it.first)) * kTok, p_first = it.s.len - it.s.rows;
+                const int first = (int)(it.c0 + (u - it.first)) * kTok, p_first = it.s.len - it.s.rows;
                 const uint8_t* stage = ring_ptr + s * stage_bytes<D>();
                 if (first + kTok - 1 <= p_first && (P.window == 0 || first > it.s.len - 1 - (int)P.window)) work_on(stage, first, std::true_type{});
                 else work_on(stage, first, std::false_type{});
@@ -478,6 +482,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             if (!ok) break;
             end_item(opens, u < item_end, u == end);
         }
+        if (warp == here - 1 && lane == 0) edge_item[1] = it;
         if (!ok) {                                         // copies in flight end before the CTA does
             for (int s = 0; s < kStages; ++s) {
                 volatile int never = 0;
@@ -489,95 +494,152 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     __syncthreads();
     if (abort_flag) return;
 
-    // ---- joining.  Records of one item follow one another in the order (warp, begun before / begun in); a run of them that has both ends is finished here,
-    // one that is open on a side becomes a record of the CTA.
+    // ---- joining.  A record a warp begins in (index 2 w) continues what the warp before has as the record it ends in (2 w + 1), or, where the warp lies in the item as a
+    // whole, as its own 2 w.  So a run of parts of one item is the record 2 a + 1, then 2 (a + 1), 2 (a + 2), ... to the one that is not open.  Runs with both ends in the
+    // CTA are finished by the warp they begin in, all at the same time; at most two are open, at the CTA's begin and at its end: they become records of the CTA.
+    auto index_of = [&](int from, uint32_t i) { return i == 0 ? from : 2 * (from / 2 + (int)i); };
+    auto parts = [&](int from, bool* closed) {              // of the run that begins at record `from`
+        uint32_t n = 1;
+        *closed = rec_open[from] == 0;
+        for (uint32_t w = from / 2 + 1; !*closed && w < here; ++w, ++n) *closed = rec_open[2 * w] == 0;
+        return n;
+    };
+    auto store = [&](const Item& it, uint32_t e, float4 sum, float f) {
+        const uint32_t c = e / D;
+        __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
+        *(uint2*)y = make_uint2(pack(sum.x * f, sum.y * f), pack(sum.z * f, sum.w * f));
+    };
+    bool closed = false;
+    if (active && rec_there[2 * warp + 1]) {
+        const int from = 2 * warp + 1;
+        const uint32_t n = parts(from, &closed);
+        if (closed) {
+            const Item it = item_of<kThreads>(P, plan, start_of(me + 1) - 1);
+            for (int c = 0; c < kCols; ++c) {
+                const float* r = rec_at[index_of(from, min(lane, n - 1))] + kCols * D + c;
+                const float m = lane < n ? r[0] : -INFINITY;
+                float top = m;
+#pragma unroll
+                for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                const float w = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
+                float sum = lane < n ? w * r[kCols] : 0.0f;
+#pragma unroll
+                for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+                if (lane < n) part_ml[index_of(from, lane)][c] = make_float2(w, sum == 0.0f ? 0.0f : 1.0f / sum);
+            }
+            __syncwarp();
+            const uint32_t cols = (uint32_t)it.s.rows * P.group;
+            for (uint32_t e = lane * 4; e < cols * D; e += 128) {
+                float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+                for (uint32_t i = 0; i < n; ++i) {
+                    const float w = part_ml[index_of(from, i)][e / D].x;
+                    const float4 x = *(const float4*)(rec_at[index_of(from, i)] + e);
+                    sum.x = fmaf(w, x.x, sum.x); sum.y = fmaf(w, x.y, sum.y); sum.z = fmaf(w, x.z, sum.z); sum.w = fmaf(w, x.w, sum.w);
+                }
+                store(it, e, sum, part_ml[from][e / D].y);
+            }
+        }
+    }
+    // the open runs: the one that record 0 begins, and the one that the last record belongs to
+    int open_from[2] = {-1, -1};
+    uint32_t open_parts[2] = {0, 0};
+    bool ends;
+    if (rec_there[0]) {
+        open_from[0] = 0;
+        open_parts[0] = parts(0, &ends);
+    }
+    const int tail = 2 * (here - 1) + 1;
+    if (rec_there[tail]) {
+        open_from[1] = tail;
+        open_parts[1] = 1;
+    } else if (rec_there[tail - 1] && rec_open[tail - 1]) {
+        int w = here - 1;
+        while (w > 0 && !rec_there[2 * w + 1]) --w;
+        if (rec_there[2 * w + 1]) {                     // (else it is the run of record 0)
+            open_from[1] = 2 * w + 1;
+            open_parts[1] = here - w;
+        }
+    }
+    if (open_from[0] < 0 && open_from[1] < 0) return;
     float* const cta_records = G.records + (uint64_t)gridDim.x * kWarps * kRecord;
-    auto join = [&](uint32_t count, auto record, bool finish, const Item& it, float* to) {
-        // record(i): the i-th part in order.  Maxima and sums of all parts, their weights, then every number of the sum by one thread.
-        for (uint32_t e = threadIdx.x; e < count * kCols; e += kThreads) {
+    // the weights of `n` parts, a warp to a column; with `finish` the inverse of the whole sum
+    auto weigh = [&](uint32_t n, auto record, bool finish, float* to) {
+        for (uint32_t e = threadIdx.x; e < n * kCols; e += kThreads) {
             const float* r = record(e / kCols) + kCols * D + e % kCols;
             part_ml[e / kCols][e % kCols] = make_float2(r[0], r[kCols]);
         }
         __syncthreads();
-        if (warp < kCols) {
-            for (uint32_t c = warp; c < kCols; c += kWarps) {
-                float top = -INFINITY, sum = 0.0f;
-                for (uint32_t i = lane; i < count; i += 32) top = fmaxf(top, part_ml[i][c].x);
+        for (uint32_t c = warp; c < kCols; c += kWarps) {
+            float top = -INFINITY, sum = 0.0f;
+            for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, part_ml[i][c].x);
 #pragma unroll
-                for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                const float base = top == -INFINITY ? 0.0f : top;
-                for (uint32_t i = lane; i < count; i += 32) {
-                    const float w = exp2_fast(part_ml[i][c].x - base);
-                    sum += w * part_ml[i][c].y;
-                    part_ml[i][c].x = w;
-                }
+            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (uint32_t i = lane; i < n; i += 32) {
+                const float w = exp2_fast(part_ml[i][c].x - base);
+                sum += w * part_ml[i][c].y;
+                part_ml[i][c].x = w;
+            }
 #pragma unroll
-                for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-                if (lane == 0) {
-                    scale_of[c] = !finish ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-                    if (!finish) {
-                        to[kCols * D + c] = top;
-                        to[kCols * D + kCols + c] = sum;
-                    }
+            for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+            if (lane == 0) {
+                scale_of[c] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (!finish) {
+                    to[kCols * D + c] = top;
+                    to[kCols * D + kCols + c] = sum;
                 }
-            }
-        }
-        __syncthreads();
-        const uint32_t cols = finish ? (uint32_t)it.s.rows * P.group : kCols;
-        for (uint32_t e = threadIdx.x * 4; e < cols * D; e += kThreads * 4) {
-            const uint32_t c = e / D;
-            float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-            for (uint32_t i = 0; i < count; ++i) {
-                const float w = part_ml[i][c].x;
-                const float4 x = *(const float4*)(record(i) + e);
-                sum.x = fmaf(w, x.x, sum.x); sum.y = fmaf(w, x.y, sum.y); sum.z = fmaf(w, x.z, sum.z); sum.w = fmaf(w, x.w, sum.w);
-            }
-            const float f = scale_of[c];
-            if (finish) {
-                __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
-                *(uint2*)y = make_uint2(pack(sum.x * f, sum.y * f), pack(sum.z * f, sum.w * f));
-            } else {
-                *(float4*)(to + e) = sum;
             }
         }
         __syncthreads();
     };
-    const uint64_t cta_begin = start_of((uint64_t)blockIdx.x * per_cta);
-    const uint64_t cta_end = start_of(min(workers, (uint64_t)(blockIdx.x + 1) * per_cta));
-    for (int r = 0; r < 2 * kWarps;) {
-        if (rec_item[r] < 0) { ++r; continue; }
-        const int item = rec_item[r], from = r;
-        int last = r;
-        uint32_t count = 0;
-        for (; r < 2 * kWarps && (rec_item[r] < 0 || rec_item[r] == item); ++r)
-            if (rec_item[r] == item) { last = r; ++count; }
-        const bool open_start = (from & 1) == 0, open_end = rec_open[last] != 0;
-        // the records' numbers in order: a run is the first one, then one a warp
-        auto record = [&](uint32_t i) { return rec_at[i == 0 ? from : 2 * (from / 2 + (int)i)]; };
-        if (!open_start && !open_end) {
-            // (its first unit: the begin of the last run with it, less what came before; found again from the unit before that run)
-            const Item it = item_of<kThreads>(P, plan, start_of((uint64_t)blockIdx.x * per_cta + last / 2));
-            join(count, record, true, it, nullptr);
+    auto add_up = [&](uint32_t n, auto record, uint32_t e) {
+        float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+        for (uint32_t i = 0; i < n; ++i) {
+            const float w = part_ml[i][e / D].x;
+            const float4 x = *(const float4*)(record(i) + e);
+            sum.x = fmaf(w, x.x, sum.x); sum.y = fmaf(w, x.y, sum.y); sum.z = fmaf(w, x.z, sum.z); sum.w = fmaf(w, x.w, sum.w);
+        }
+        return sum;
+    };
+    for (int k = 0; k < 2; ++k) {
+        if (open_from[k] < 0) continue;
+        float* to = cta_records + (uint64_t)(2 * blockIdx.x + k) * kRecord;
+        if (open_parts[k] == 1) {
+            const float* from = rec_at[open_from[k]];
+            for (uint32_t e = threadIdx.x * 2; e < kRecord; e += kThreads * 2) *(float2*)(to + e) = *(const float2*)(from + e);
             continue;
         }
-        float* mine = cta_records + (uint64_t)(2 * blockIdx.x + (open_start ? 0 : 1)) * kRecord;
-        join(count, record, false, Item{}, mine);          // (also where it is one part: it may lie in shared memory)
-        const Item it = item_of<kThreads>(P, plan, open_start ? cta_begin : cta_end - 1);
-        const uint32_t first_cta = (uint32_t)(worker_of(it.first) / per_cta), last_cta = (uint32_t)(worker_of(it.first + it.chunks - 1) / per_cta);
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const int before = atomicAdd(G.counters + first_cta, 1);
-            is_last = before == (int)(last_cta - first_cta);
-            if (is_last) G.counters[first_cta] = 0;
+        auto record = [&](uint32_t i) { return rec_at[index_of(open_from[k], i)]; };
+        __syncthreads();                                    // (the table of weights may be in use)
+        weigh(open_parts[k], record, false, to);
+        for (uint32_t e = threadIdx.x * 4; e < kCols * D; e += kThreads * 4) *(float4*)(to + e) = add_up(open_parts[k], record, e);
+    }
+    // the CTA that arrives last finishes the item
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const int k = threadIdx.x;
+        is_last[k] = 0;
+        if (open_from[k] >= 0) {
+            const Item& it = edge_item[k];
+            const uint32_t first_cta = worker_of(it.first) / per_cta, last_cta = worker_of(it.first + it.chunks - 1) / per_cta;
+            parts_from[k] = first_cta;
+            parts_of[k] = last_cta - first_cta + 1;
+            is_last[k] = atomicAdd(G.counters + first_cta, 1) == (int)(last_cta - first_cta);
+            if (is_last[k]) G.counters[first_cta] = 0;
             __threadfence();
         }
-        __syncthreads();
-        if (is_last) {
-            auto part = [&](uint32_t i) { return cta_records + (uint64_t)(2 * (first_cta + i) + (i == 0 ? 1 : 0)) * kRecord; };
-            join(last_cta - first_cta + 1, part, true, it, nullptr);
-        }
+    }
+    __syncthreads();
+    for (int k = 0; k < 2; ++k) {
+        if (!is_last[k]) continue;
+        const Item it = edge_item[k];
+        const uint32_t from = parts_from[k], n = parts_of[k];
+        auto part = [&](uint32_t i) { return cta_records + (uint64_t)(2 * (from + i) + (i == 0 ? 1 : 0)) * kRecord; };
+        weigh(n, part, true, nullptr);
+        for (uint32_t e = threadIdx.x * 4; e < (uint32_t)it.s.rows * P.group * D; e += kThreads * 4) store(it, e, add_up(n, part, e), scale_of[e / D]);
         __syncthreads();
     }
 }
