@@ -515,29 +515,47 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
         const uint32_t n = parts(from, &closed);
         if (closed) {
             const Item it = item_of<kThreads>(P, plan, start_of(me + 1) - 1);
-            for (int c = 0; c < kCols; ++c) {
-                const float* r = rec_at[index_of(from, min(lane, n - 1))] + kCols * D + c;
-                const float m = lane < n ? r[0] : -INFINITY;
-                float top = m;
+            // weights: a lane to a column, the parts dealt to the lanes of a column
+            constexpr uint32_t kEach = 32 / kCols;
+            const uint32_t c = lane % kCols;
+            float top = -INFINITY, sum = 0.0f;
+            for (uint32_t i = lane / kCols; i < n; i += kEach) top = fmaxf(top, rec_at[index_of(from, i)][kCols * D + c]);
 #pragma unroll
-                for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                const float w = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
-                float sum = lane < n ? w * r[kCols] : 0.0f;
-#pragma unroll
-                for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-                if (lane < n) part_ml[index_of(from, lane)][c] = make_float2(w, sum == 0.0f ? 0.0f : 1.0f / sum);
+            for (uint32_t d = kCols; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (uint32_t i = lane / kCols; i < n; i += kEach) {
+                const float* r = rec_at[index_of(from, i)] + kCols * D + c;
+                const float w = exp2_fast(r[0] - base);
+                sum += w * r[kCols];
+                part_ml[index_of(from, i)][c].x = w;
             }
+#pragma unroll
+            for (uint32_t d = kCols; d < 32; d *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
             __syncwarp();
-            const uint32_t cols = (uint32_t)it.s.rows * P.group;
-            for (uint32_t e = lane * 4; e < cols * D; e += 128) {
-                float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-                for (uint32_t i = 0; i < n; ++i) {
-                    const float w = part_ml[index_of(from, i)][e / D].x;
-                    const float4 x = *(const float4*)(rec_at[index_of(from, i)] + e);
-                    sum.x = fmaf(w, x.x, sum.x); sum.y = fmaf(w, x.y, sum.y); sum.z = fmaf(w, x.z, sum.z); sum.w = fmaf(w, x.w, sum.w);
+            // every lane takes four numbers of every column, all columns of a part at once
+            constexpr int kPieces = kCols * D / 128;
+            float4 total[kPieces];
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) total[j] = make_float4(0, 0, 0, 0);
+            for (uint32_t i = 0; i < n; ++i) {
+                const float4* r = (const float4*)rec_at[index_of(from, i)] + lane;
+                float4 x[kPieces];
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) x[j] = r[32 * j];
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const float w = part_ml[index_of(from, i)][(128 * j + 4 * lane) / D].x;
+                    total[j].x = fmaf(w, x[j].x, total[j].x); total[j].y = fmaf(w, x[j].y, total[j].y);
+                    total[j].z = fmaf(w, x[j].z, total[j].z); total[j].w = fmaf(w, x[j].w, total[j].w);
                 }
-                store(it, e, sum, part_ml[from][e / D].y);
+            }
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const uint32_t cols = (uint32_t)it.s.rows * P.group;
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                const uint32_t e = 128 * j + 4 * lane;
+                const float f = __shfl_sync(0xFFFFFFFFu, inverse, e / D);
+                if (e / D < cols) store(it, e, total[j], f);
             }
         }
     }
