@@ -25,6 +25,8 @@ constexpr uint32_t kFewColumns = 16;                     // rows x group that kv
 constexpr uint32_t kMaxCtas = 160;                       // of a persistent launch, one for each SM: arrival counters, parts of one item
 
 size_t decode_scratch_bytes(uint32_t sms);               // behind the counters
+size_t prompt_scratch_bytes(uint32_t sms);
+int launch_prompt(const Attention& p, uint32_t head_dim, uint32_t sms, cudaStream_t stream);      // two kernels
 int launch_decode(const Attention& p, uint32_t head_dim, uint32_t columns, uint32_t sms, cudaStream_t stream);
 
 // First token that any row of the sequence sees.

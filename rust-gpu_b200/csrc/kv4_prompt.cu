@@ -1,0 +1,614 @@
+// Attention of many rows (rows x group > 16) over the paged four-bit cache: tcgen05 products, the cache's codes made bf16 on the way into shared memory.
+//
+// An item is 256 rows (pairs of token and query head of one key/value head, two tiles of 128) against the chunks of 128 tokens that any of them sees.  Per chunk
+//   S = Q K^T (shared memory x shared memory -> tensor memory),  P = 2^(S - m) (one thread a row),  O += P V (P in tensor memory, over S's own columns)
+// with the two tiles half a step apart: while the softmax warps of one work on its S, the tensor cores work for the other.  512 columns of tensor memory are S and O
+// of both tiles.  The maximum a row's weights are taken against only moves when it is left behind by more than 2^8 (then O is read, scaled and written back), so the sums
+// stay far inside f32 and O is rarely touched.
+//   warps 0-3, 4-7  softmax of tile 0 and 1, and their results     warps 8-11  codes -> bf16, K and V into rings of two stages
+//   warp 12         issues the products                            warp 13     queries of the next item into shared memory
+// Keys and values are rounded to bf16 here (step * code + low, once), which a score feels by at most 2^-8 of sum |q k|.  A value row that is NaN is put in as zeros and
+// its key as NaN: a row that sees the token becomes NaN through its score, a row that must not see it has weight 0, and 0 x 0 adds nothing.
+//
+// The units of work are all items' chunks, in equal contiguous runs, one for each CTA.  Items that end up in several CTAs leave parts (O, m, l) that a second kernel joins.
+#include "kv4_attention.cuh"
+
+namespace t0 {
+namespace kv4 {
+namespace {
+
+constexpr int kTok = 128, kRows = 256, kTile = 128;
+constexpr int kThreads = 14 * 32;
+constexpr float kLag = 8.0f;                              // powers of two by which a row's maximum may be left behind
+
+template <int D> constexpr uint32_t tile_bytes() { return kTile * D * 2; }
+template <int D> constexpr uint32_t smem_bytes() { return 6 * tile_bytes<D>() + 1024 + 512; }
+template <int D> constexpr uint32_t record_floats() { return kRows * (D + 2); }          // [D][256] sums, [256] maxima, [256] sums of weights
+
+// The items of one head in the order (sequence, tile), and their chunks: what every thread found in its share, summed up.
+struct Plan {
+    uint32_t tiles[kThreads + 1];    // tiles before the sequences of each thread
+    uint32_t chunks[kThreads + 1];   // chunks before the tiles of each thread
+    uint32_t warp_sum[kThreads / 32];
+    uint32_t seqs_each, tiles_each;
+};
+
+__device__ __forceinline__ uint32_t tiles_of(const Attention& P, const Sequence& s) {
+    const uint32_t n = (uint32_t)s.rows * P.group;
+    return n <= P.few ? 0 : (n + kRows - 1) / kRows;
+}
+
+struct Item {
+    Sequence s;
+    uint32_t b, tile, head;
+    int c0, c1;                      // its chunks
+    __device__ __forceinline__ void range(const Attention& P) {
+        const int i0 = (int)(tile * kRows / P.group), i1 = min(s.rows - 1, (int)((tile * kRows + kRows - 1) / P.group));
+        const int p0 = s.len - s.rows + i0, p1 = s.len - s.rows + i1;
+        c0 = P.window && p0 >= (int)P.window ? (p0 - (int)P.window + 1) / kTok : 0;
+        c1 = p1 < 0 ? c0 + 1 : p1 / kTok + 1;             // at least one, also where no row sees anything: its rows are written
+    }
+    // the next tile; sequences that have none here are passed over
+    __device__ __forceinline__ void advance(const Attention& P) {
+        if (++tile >= tiles_of(P, s)) {
+            tile = 0;
+            for (uint32_t i = 0; i < P.B.n_seqs; ++i) {
+                if (++b == P.B.n_seqs) {
+                    b = 0;
+                    ++head;
+                }
+                s = sequence(P.B, b);
+                if (tiles_of(P, s)) break;
+            }
+        }
+        range(P);
+    }
+};
+
+__device__ __forceinline__ uint32_t scan(uint32_t mine, uint32_t* warp_sum, uint32_t* out) {
+    uint32_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint32_t other = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if ((threadIdx.x & 31) >= d) upto += other;
+    }
+    if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x / 32] = upto;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < threadIdx.x / 32; ++w) before += warp_sum[w];
+    out[threadIdx.x + 1] = before + upto;
+    if (threadIdx.x == 0) out[0] = 0;
+    __syncthreads();
+    return out[kThreads];
+}
+__device__ __forceinline__ uint32_t last_not_above(const uint32_t* prefix, uint32_t x) {
+    uint32_t lo = 0, hi = kThreads;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (prefix[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+// tile number `at` of one head
+__device__ __forceinline__ Item tile_at(const Attention& P, const Plan& plan, uint32_t at) {
+    const uint32_t th = last_not_above(plan.tiles, at);
+    Item it;
+    it.head = 0;
+    it.b = th * plan.seqs_each;
+    uint32_t n = plan.tiles[th];
+    for (;; ++it.b) {
+        it.s = sequence(P.B, it.b);
+        const uint32_t next = n + tiles_of(P, it.s);
+        if (at < next || it.b + 1 >= P.B.n_seqs) break;
+        n = next;
+    }
+    it.tile = at - n;
+    it.range(P);
+    return it;
+}
+// returns the chunks of one head
+__device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
+    const uint32_t n = P.B.n_seqs, each = (n + kThreads - 1) / kThreads, tid = threadIdx.x;
+    if (tid == 0) plan.seqs_each = each;
+    uint32_t mine = 0;
+    for (uint32_t b = tid * each; b < min(n, (tid + 1) * each); ++b) mine += tiles_of(P, sequence(P.B, b));
+    const uint32_t tiles = scan(mine, plan.warp_sum, plan.tiles);
+    const uint32_t tiles_each = (tiles + kThreads - 1) / kThreads;
+    if (tid == 0) plan.tiles_each = tiles_each;
+    mine = 0;
+    if (tid * tiles_each < tiles) {
+        Item it = tile_at(P, plan, tid * tiles_each);
+        for (uint32_t i = tid * tiles_each;;) {
+            mine += it.c1 - it.c0;
+            if (++i >= min(tiles, (tid + 1) * tiles_each)) break;
+            it.advance(P);
+        }
+    }
+    return scan(mine, plan.warp_sum, plan.chunks);
+}
+// the item that unit u (of all heads) belongs to, and the unit it begins with
+__device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, uint32_t per_head, uint32_t u, uint32_t* first) {
+    const uint32_t head = u / per_head, at = u % per_head, th = last_not_above(plan.chunks, at);
+    Item it = tile_at(P, plan, th * plan.tiles_each);
+    uint32_t n = plan.chunks[th];
+    while (at >= n + (uint32_t)(it.c1 - it.c0)) {
+        n += it.c1 - it.c0;
+        it.advance(P);
+    }
+    it.head = head;
+    *first = head * per_head + n;
+    return it;
+}
+// the run of CTA c: units * c / ctas, rounded down
+__device__ __forceinline__ uint32_t start_of(uint32_t c, uint32_t units, uint32_t ctas) { return c * (units / ctas) + c * (units % ctas) / ctas; }
+
+struct Params {
+    Attention P;
+    float* records;                  // two for each CTA: of the item it begins in, of the item it ends in
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&p;
+}
+// step * code + low, rounded once, of nibbles i and i + 4: 128 + code in a bf16, less 128, times step plus low
+__device__ __forceinline__ uint32_t value_of(uint32_t w, int i, uint32_t k128, __nv_bfloat162 step, __nv_bfloat162 low) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(k128));
+    const __nv_bfloat162 k = __nv_bfloat162(__ushort_as_bfloat16(0x4300), __ushort_as_bfloat16(0x4300));
+    const __nv_bfloat162 v = __hfma2(__hsub2(*(const __nv_bfloat162*)&x, k), step, low);
+    return *(const uint32_t*)&v;
+}
+__device__ __forceinline__ __nv_bfloat162 twice(uint32_t bits16) {
+    const uint32_t x = bits16 * 0x10001u;
+    return *(const __nv_bfloat162*)&x;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_constant__ Params G) {
+    constexpr uint32_t kTileBytes = tile_bytes<D>(), kPanel = kTile * 128, kTmem = 512;
+    constexpr uint32_t kS = 0, kO = 2 * kTok;             // columns of tensor memory: S of both tiles (P over them), O of both
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Plan plan;
+    const Attention& P = G.P;
+    const Batch& B = P.B;
+    const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = (uint64_t*)(smem + 6 * kTileBytes);
+    const uint32_t q_smem = ptx::smem_u32(smem), k_smem = q_smem + 2 * kTileBytes, v_smem = k_smem + 2 * kTileBytes, bar = ptx::smem_u32(bars);
+    // barriers
+    const uint32_t q_full = bar, q_empty = bar + 8;
+    auto k_full = [&](uint32_t s) { return bar + 16 + 8 * s; };
+    auto k_empty = [&](uint32_t s) { return bar + 32 + 8 * s; };
+    auto v_full = [&](uint32_t s) { return bar + 48 + 8 * s; };
+    auto v_empty = [&](uint32_t s) { return bar + 64 + 8 * s; };
+    auto s_full = [&](uint32_t t) { return bar + 80 + 8 * t; };
+    auto p_full = [&](uint32_t t) { return bar + 96 + 8 * t; };
+    auto o_full = [&](uint32_t t) { return bar + 112 + 8 * t; };
+    const uint32_t drained = bar + 128;
+    uint32_t* tmem_holder = (uint32_t*)(bars + 17);
+    volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(q_full, 1);
+        ptx::mbar_init(q_empty, 1);
+        ptx::mbar_init(drained, 1);
+        for (uint32_t s = 0; s < 2; ++s) {
+            ptx::mbar_init(k_full(s), 4);
+            ptx::mbar_init(k_empty(s), 1);
+            ptx::mbar_init(v_full(s), 4);
+            ptx::mbar_init(v_empty(s), 1);
+            ptx::mbar_init(s_full(s), 1);
+            ptx::mbar_init(p_full(s), 4);
+            ptx::mbar_init(o_full(s), 1);
+        }
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+    }
+    if (warp == 12) {
+        ptx::tmem_alloc(ptx::smem_u32(tmem_holder), kTmem);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_holder, 0);
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+
+    const uint32_t per_head = make_plan(P, plan), units = per_head * B.n_kv_heads;
+    const uint32_t begin = units ? start_of(blockIdx.x, units, gridDim.x) : 0, end = units ? start_of(blockIdx.x + 1, units, gridDim.x) : 0;
+    bool ok = true;
+    auto wait = [&](uint32_t b, uint32_t parity) {
+        if (ok) ok = ptx::mbar_wait_warp(b, parity, abort_flag, P.wait_limit_ns);
+        return ok;
+    };
+    if (begin < end) {
+        uint32_t item_first;
+        Item it = item_of(P, plan, per_head, begin, &item_first);
+        int c = it.c0 + (int)(begin - item_first);        // the chunk at hand
+        uint32_t u = begin;
+
+        if (warp < 8) {
+            // ------------------------------------------------------------ softmax: a thread has a row
+            const uint32_t t = warp / 4, r = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
+            const uint32_t s_col = tmem + kS + t * kTok + lanes, o_col = tmem + kO + t * D + lanes;
+            uint32_t s_phase = 0, o_phase = 0;
+            while (ok && u < end) {
+                const bool opens = c == it.c0;
+                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group;
+                const bool closes = c + (int)n == it.c1;
+                const uint32_t row = it.tile * kRows + t * kTile + r;
+                if (it.tile * kRows + t * kTile < total) {
+                    const int last = (int)min(row, total - 1);
+                    const int p = it.s.len - it.s.rows + last / (int)P.group;                      // the row's token
+                    const int p_low = it.s.len - it.s.rows + (int)((it.tile * kRows + t * kTile) / P.group);     // the tile's first and last
+                    const int p_high = it.s.len - it.s.rows + (int)(min(it.tile * kRows + t * kTile + kTile, total) - 1) / (int)P.group;
+                    float m = -INFINITY, l = 0.0f;
+                    for (uint32_t i = 0; i < n; ++i) {
+                        if (!wait(s_full(t), s_phase)) break;
+                        s_phase ^= 1;
+                        ptx::tc_fence_after_sync();
+                        const int first = (c + (int)i) * kTok;
+                        const bool whole = first + kTok - 1 <= p_low && (P.window == 0 || first > p_high - (int)P.window);
+                        const int from = P.window ? p - (int)P.window + 1 - first : -1, to = p - first;          // columns the row sees
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int q = 0; q < kTok / 32; ++q) {
+                            uint32_t x[32];
+                            ptx::tmem_ld_32x32b_x32(s_col + 32 * q, x);
+                            ptx::tmem_ld_wait();
+                            if (whole) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (32 * q + j >= from && 32 * q + j <= to) top = fmaxf(top, __uint_as_float(x[j]));
+                            }
+                        }
+                        top *= P.scale_log2;              // (the scale is positive)
+                        const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
+                        if (__any_sync(0xFFFFFFFFu, left_behind)) {
+                            const float m_new = left_behind ? top : m, less = m == m_new ? 1.0f : exp2_fast(m - m_new);
+                            m = m_new;
+                            l *= less;
+                            if (i > 0) {
+#pragma unroll
+                                for (int q = 0; q < D / 32; ++q) {
+                                    uint32_t x[32];
+                                    ptx::tmem_ld_32x32b_x32(o_col + 32 * q, x);
+                                    ptx::tmem_ld_wait();
+#pragma unroll
+                                    for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * less);
+                                    ptx::tmem_st_32x32b_x32(o_col + 32 * q, x);
+                                }
+                            }
+                        }
+                        const float minus = m == -INFINITY ? 0.0f : -m;
+                        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                        for (int q = 0; q < kTok / 64; ++q) {
+                            uint32_t y[32];
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                uint32_t x[32];
+                                ptx::tmem_ld_32x32b_x32(s_col + 64 * q + 32 * half, x);
+                                ptx::tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    const int at = 64 * q + 32 * half + 2 * j;
+                                    float a = exp2_fast(fmaf(__uint_as_float(x[2 * j]), P.scale_log2, minus)), b = exp2_fast(fmaf(__uint_as_float(x[2 * j + 1]), P.scale_log2, minus));
+                                    if (!whole) {
+                                        if (at < from || at > to) a = 0.0f;
+                                        if (at + 1 < from || at + 1 > to) b = 0.0f;
+                                    }
+                                    sum0 += a;
+                                    sum1 += b;
+                                    y[16 * half + j] = pack(a, b);
+                                }
+                            }
+                            ptx::tmem_st_32x32b_x32(s_col + 32 * q, y);          // over columns that have been read
+                        }
+                        l += sum0 + sum1;
+                        ptx::tmem_st_wait();
+                        ptx::tc_fence_before_sync();
+                        __syncwarp();
+                        ptx::mbar_arrive_if(p_full(t), lane == 0);
+                    }
+                    if (!wait(o_full(t), o_phase)) break;
+                    o_phase ^= 1;
+                    ptx::tc_fence_after_sync();
+                    if (opens && closes) {
+                        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+                        __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + last / (int)P.group) * P.y_stride + (it.head * P.group + last % P.group) * D;
+#pragma unroll
+                        for (int q = 0; q < D / 32; ++q) {
+                            uint32_t x[32];
+                            ptx::tmem_ld_32x32b_x32(o_col + 32 * q, x);
+                            ptx::tmem_ld_wait();
+                            if (row < total) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    uint32_t w[4];
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) w[k] = pack(__uint_as_float(x[8 * j + 2 * k]) * inverse, __uint_as_float(x[8 * j + 2 * k + 1]) * inverse);
+                                    *(uint4*)(y + 32 * q + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+                                }
+                            }
+                        }
+                    } else {
+                        float* rec = G.records + (uint64_t)(2 * blockIdx.x + (opens ? 1 : 0)) * record_floats<D>() + t * kTile + r;
+#pragma unroll
+                        for (int q = 0; q < D / 32; ++q) {
+                            uint32_t x[32];
+                            ptx::tmem_ld_32x32b_x32(o_col + 32 * q, x);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) rec[(32 * q + j) * kRows] = __uint_as_float(x[j]);
+                        }
+                        rec[D * kRows] = m;
+                        rec[(D + 1) * kRows] = l;
+                    }
+                    ptx::tc_fence_before_sync();           // the next item's first product writes O after this warp's next p_full
+                }
+                u += n;
+                if (u < end) {
+                    it.advance(P);
+                    c = it.c0;
+                }
+            }
+        } else if (warp < 12) {
+            // ------------------------------------------------------------ codes to bf16
+            const uint32_t tid = threadIdx.x - 256, part = tid & 3;       // a quarter of rows tid / 4, + 32, + 64, + 96
+            constexpr int kWords = D / 32;                                  // words of a quarter
+            uint32_t k128;
+            asm volatile("mov.b32 %0, 0x43004300;" : "=r"(k128));
+            uint32_t raw[2][4][kWords], kp[4], vp[4];
+            Item ahead = it;
+            int ahead_c = c;
+            uint32_t ahead_u = u;
+            auto load = [&](int which) {                    // K or V codes, and the parameters of both with K, of the chunk that is ahead
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t row = tid / 4 + 32 * i, token = (uint32_t)ahead_c * kTok + row;
+                    const bool there = token < (uint32_t)ahead.s.len;
+                    const uint32_t slot = token & ((1u << B.page_log2) - 1);
+                    const uint8_t* block = there ? block_to_read<D>(B, ahead.b, token >> B.page_log2, ahead.head) : nullptr;
+                    if (which == 0) {
+                        kp[i] = there ? *(const uint32_t*)(block + params_at<D>(B.page_log2, 0) + 4 * slot) : 0;
+                        vp[i] = there ? *(const uint32_t*)(block + params_at<D>(B.page_log2, 1) + 4 * slot) : 0;
+                    }
+                    const uint8_t* src = block + codes_at<D>(B.page_log2, which) + slot * (D / 2) + part * (D / 8);
+                    if constexpr (kWords == 4) {
+                        const uint4 w = there ? *(const uint4*)src : make_uint4(0, 0, 0, 0);
+                        raw[which][i][0] = w.x; raw[which][i][1] = w.y; raw[which][i][2] = w.z; raw[which][i][3] = w.w;
+                    } else {
+                        const uint2 w = there ? *(const uint2*)src : make_uint2(0, 0);
+                        raw[which][i][0] = w.x; raw[which][i][1] = w.y;
+                    }
+                }
+            };
+            auto store = [&](int which, uint32_t base, const uint32_t (&params)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t row = tid / 4 + 32 * i;
+                    const __nv_bfloat162 step = twice(params[i] & 0xFFFFu), low = twice(params[i] >> 16);
+#pragma unroll
+                    for (int j = 0; j < kWords; ++j) {
+                        // 16-byte units of the row: quarter `part` has kWords of them; the order of its stores differs between lanes, so that eight lanes hit all banks
+                        const uint32_t jj = D == 128 ? j ^ ((part >> 1) << 1) : j;
+                        uint32_t w = raw[which][i][j];
+                        if (D == 128 && (part >> 1)) w = raw[which][i][j ^ 2];
+                        const uint32_t unit = part * kWords + jj, panel = unit / 8, at = unit % 8;
+                        const uint32_t dst = base + panel * kPanel + row * 128 + ((at ^ (row & 7)) << 4);
+                        const uint32_t v0 = value_of(w, 0, k128, step, low), v1 = value_of(w, 1, k128, step, low), v2 = value_of(w, 2, k128, step, low), v3 = value_of(w, 3, k128, step, low);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
+                    }
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+            };
+            load(0);
+            load(1);
+            uint32_t stage = 0, phase = 0;
+            for (; ok && u < end; ++u) {
+                // parameters of this chunk; those of a NaN value go into its key
+                uint32_t kq[4], vq[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool bad = (vp[i] & 0x7F800000u) == 0x7F800000u || (vp[i] & 0x7F80u) == 0x7F80u;
+                    kq[i] = bad ? 0x7FC07FC0u : kp[i];
+                    vq[i] = bad ? 0u : vp[i];
+                }
+                if (++ahead_u < end && ++ahead_c == ahead.c1) {
+                    ahead.advance(P);
+                    ahead_c = ahead.c0;
+                }
+                if (!wait(k_empty(stage), phase ^ 1)) break;
+                store(0, k_smem + stage * kTileBytes, kq);
+                ptx::mbar_arrive_if(k_full(stage), lane == 0);
+                if (ahead_u < end) load(0);
+                if (!wait(v_empty(stage), phase ^ 1)) break;
+                store(1, v_smem + stage * kTileBytes, vq);
+                ptx::mbar_arrive_if(v_full(stage), lane == 0);
+                if (ahead_u < end) load(1);
+                stage ^= 1;
+                phase ^= stage == 0;
+            }
+        } else if (warp == 12) {
+            // ------------------------------------------------------------ the products
+            constexpr uint32_t kIdescS = ptx::make_idesc_bf16_f32(kTile, kTok, 0), kIdescO = ptx::make_idesc_bf16_f32(kTile, D, 1);
+            const uint32_t issue = ptx::elect_one();
+            uint32_t stage = 0, phase = 0, q_phase = 0, p_phase[2] = {0, 0};
+            auto scores = [&](uint32_t t) {
+                const uint32_t a = ptx::smem_desc_lo(q_smem + t * kTileBytes, 16), b = ptx::smem_desc_lo(k_smem + stage * kTileBytes, 16);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = (k / 4) * (kPanel / 16) + (k % 4) * 2;
+                    ptx::umma_bf16_ss_if(issue, tmem + kS + t * kTok, a + at, b + at, kIdescS, k > 0);
+                }
+                ptx::umma_commit_if(issue, s_full(t));
+            };
+            auto sums = [&](uint32_t t, uint32_t v_stage, bool more) {
+                const uint32_t b = ptx::smem_desc_lo(v_smem + v_stage * kTileBytes, kPanel);
+#pragma unroll
+                for (int k = 0; k < kTok / 16; ++k) ptx::umma_bf16_ts_mn_if(issue, tmem + kO + t * D, tmem + kS + t * kTok + k * 8, b + k * 128, kIdescO, k > 0 || more);
+            };
+            while (ok && u < end) {
+                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group;
+                const uint32_t tiles = it.tile * kRows + kTile < total ? 2 : 1;
+                if (!wait(q_full, q_phase)) break;
+                q_phase ^= 1;
+                for (uint32_t i = 0; i <= n && ok; ++i) {   // scores of chunk i, sums of chunk i - 1
+                    const uint32_t before = stage ^ 1, before_phase = phase ^ (stage == 0);
+                    if (i < n && !wait(k_full(stage), phase)) break;
+                    if (i > 0 && !wait(v_full(before), before_phase)) break;
+                    ptx::tc_fence_after_sync();
+                    for (uint32_t t = 0; t < tiles && ok; ++t) {
+                        if (i > 0) {
+                            if (!wait(p_full(t), p_phase[t])) break;
+                            p_phase[t] ^= 1;
+                            ptx::tc_fence_after_sync();
+                            sums(t, before, i > 1);
+                            if (i == n) ptx::umma_commit_if(issue, o_full(t));
+                        }
+                        if (i < n) scores(t);
+                    }
+                    if (!ok) break;
+                    if (i > 0) ptx::umma_commit_if(issue, v_empty(before));
+                    if (i < n) {
+                        ptx::umma_commit_if(issue, k_empty(stage));
+                        if (i + 1 == n) ptx::umma_commit_if(issue, q_empty);
+                        stage ^= 1;
+                        phase ^= stage == 0;
+                    }
+                }
+                u += n;
+                if (u < end) {
+                    it.advance(P);
+                    c = it.c0;
+                }
+            }
+            // what is in flight ends before the memory it uses is given back: in a run that went well the last sums have been waited for by the softmax warps
+            if (!ok) {
+                volatile int never = 0;
+                ptx::umma_commit_if(issue, drained);
+                ptx::mbar_wait_warp(drained, 0, &never, P.wait_limit_ns);
+            }
+        } else {
+            // ------------------------------------------------------------ queries
+            uint32_t phase = 1;
+            while (ok && u < end) {
+                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group;
+                if (!wait(q_empty, phase)) break;
+                phase ^= 1;
+                const uint32_t rows = min(total - it.tile * kRows, (uint32_t)kRows) <= kTile ? kTile : kRows;
+                for (uint32_t e = lane; e < rows * (D / 8); e += 32) {
+                    const uint32_t r = e / (D / 8), unit = e % (D / 8), row = it.tile * kRows + r;
+                    const bool there = row < total;
+                    const uint32_t i = there ? row / P.group : 0, g = there ? row % P.group : 0;
+                    const __nv_bfloat16* src = P.q + (uint64_t)(it.s.first_row + i) * P.q_stride + (it.head * P.group + g) * D + unit * 8;
+                    cp_async16(q_smem + (r / kTile) * kTileBytes + (unit / 8) * kPanel + (r % kTile) * 128 + (((unit % 8) ^ (r & 7)) << 4), src, there ? 16 : 0);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                ptx::mbar_arrive_if(q_full, lane == 0);
+                u += n;
+                if (u < end) {
+                    it.advance(P);
+                    c = it.c0;
+                }
+            }
+        }
+        if (!ok && lane == 0) atomicCAS(P.timeout_status, 0, (warp == 12 ? kStatusMmaTimeout : warp < 8 ? kStatusEpilogueTimeout : kStatusProducerTimeout) | (int)(u & 0xFFFFFF));
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 12) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem, kTmem);
+    }
+}
+
+// Joins the parts of the items that several CTAs of the launch before worked on.  Block (c, z): the item that the boundary before CTA c cuts, if c is the first one to cut it;
+// z: a slice of its rows.  A thread has a row and a quarter of its numbers.
+constexpr int kJoinRows = 32, kJoinThreads = kThreads;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) kv4_prompt_join_kernel(const __grid_constant__ Params G, uint32_t ctas) {
+    __shared__ Plan plan;
+    const Attention& P = G.P;
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const uint32_t per_head = make_plan(P, plan), units = per_head * P.B.n_kv_heads;
+    if (units == 0) return;
+    const uint32_t slices = kRows / kJoinRows, c = blockIdx.x / slices + 1, z = blockIdx.x % slices, cut = start_of(c, units, ctas);
+    if (cut >= units || cut == start_of(c - 1, units, ctas)) return;
+    uint32_t first;
+    const Item it = item_of(P, plan, per_head, cut, &first);
+    const uint32_t last = first + (it.c1 - it.c0) - 1;
+    if (first == cut || start_of(c - 1, units, ctas) > first) return;      // no cut, or an earlier boundary's item
+    const uint32_t total = (uint32_t)it.s.rows * P.group;
+    if (it.tile * kRows + z * kJoinRows >= total || threadIdx.x >= kJoinRows * 8) return;
+    const uint32_t r = z * kJoinRows + threadIdx.x % kJoinRows, quarter = threadIdx.x / kJoinRows, row = it.tile * kRows + r;
+    constexpr int kEach = D / 8;
+    auto record = [&](uint32_t i) { return G.records + (uint64_t)(2 * i + (i == c - 1 ? 1 : 0)) * record_floats<D>() + r; };
+    float top = -INFINITY, l = 0.0f, sum[kEach] = {};
+    for (uint32_t i = c - 1; i < ctas && start_of(i, units, ctas) <= last; ++i)
+        if (start_of(i, units, ctas) < start_of(i + 1, units, ctas)) top = fmaxf(top, record(i)[D * kRows]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    for (uint32_t i = c - 1; i < ctas && start_of(i, units, ctas) <= last; ++i) {
+        if (start_of(i, units, ctas) == start_of(i + 1, units, ctas)) continue;
+        const float* rec = record(i);
+        const float w = exp2_fast(rec[D * kRows] - base);
+        l = fmaf(w, rec[(D + 1) * kRows], l);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) sum[j] = fmaf(w, rec[(quarter * kEach + j) * kRows], sum[j]);
+    }
+    if (row >= total) return;
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + row / P.group) * P.y_stride + (it.head * P.group + row % P.group) * D + quarter * kEach;
+#pragma unroll
+    for (int j = 0; j < kEach / 8; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = pack(sum[8 * j + 2 * k] * inverse, sum[8 * j + 2 * k + 1] * inverse);
+        *(uint4*)(y + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <int D>
+int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
+    constexpr int smem = smem_bytes<D>();
+    static bool attr_set[64] = {};   // per instantiation, per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return fail(T0_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", smem, cudaGetErrorString(e));
+        if (dev >= 0 && dev < 64) attr_set[dev] = true;
+    }
+    Params g;
+    g.P = p;
+    g.records = (float*)(p.scratch + kv4_counter_bytes());
+    const uint32_t ctas = std::min(sms, kMaxCtas);
+    cudaError_t e = gemm::launch_pdl(kv4_prompt_kernel<D>, ctas, kThreads, smem, stream, g);
+    if (e == cudaSuccess && ctas > 1) e = gemm::launch_pdl(kv4_prompt_join_kernel<D>, (ctas - 1) * (kRows / kJoinRows), kJoinThreads, 0, stream, g, ctas);
+    if (e != cudaSuccess) return fail(T0_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
+    return T0_OK;
+}
+
+}  // namespace
+
+size_t prompt_scratch_bytes(uint32_t sms) { return (size_t)2 * std::min(sms, kMaxCtas) * record_floats<128>() * sizeof(float); }
+
+int launch_prompt(const Attention& p, uint32_t head_dim, uint32_t sms, cudaStream_t stream) {
+    return head_dim == 128 ? launch<128>(p, sms, stream) : launch<64>(p, sms, stream);
+}
+
+}  // namespace kv4
+}  // namespace t0

@@ -301,6 +301,20 @@ __device__ __forceinline__ void umma_bf16_ts_if(uint32_t issue, uint32_t tmem_d,
 }
 // Low word of a descriptor of make_smem_desc with groups of eight rows 1024 bytes apart: start address and leading offset, in 16-byte units.
 __device__ __forceinline__ uint32_t smem_desc_lo(uint32_t smem_addr, uint32_t lbo_bytes) { return ((smem_addr & 0x3FFFFu) >> 4) | ((lbo_bytes >> 4) << 16); }
+// D[tmem] (+)= A[tmem] * B[smem] with B N-contiguous in shared memory: the low word of its descriptor carries the distance between 64-column atoms.
+__device__ __forceinline__ void umma_bf16_ts_mn_if(uint32_t issue, uint32_t tmem_d, uint32_t tmem_a, uint32_t desc_b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        ".reg .b64 d;\n\t"
+        "mov.b64 d, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %3, p;\n\t"
+        "}"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(desc_b_lo), "r"(idesc), "r"(accumulate), "n"((1024 >> 4) | (1 << 14) | (2 << 29)), "r"(issue)
+        : "memory");
+}
 // D[tmem] (+)= A[smem] * B[smem], issued where `issue` holds, both descriptors given by their low words.
 __device__ __forceinline__ void umma_bf16_ss_if(uint32_t issue, uint32_t tmem_d, uint32_t desc_a_lo, uint32_t desc_b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
