@@ -6,7 +6,7 @@
 // of both tiles.  The maximum a row's weights are taken against only moves when it is left behind by more than 2^8 (then O is read, scaled and written back), so the sums
 // stay far inside f32 and O is rarely touched.
 //   warps 0-3, 4-7  softmax of tile 0 and 1, and their results     warps 8-11  codes -> bf16, K and V into rings of two stages
-//   warp 12         issues the products                            warp 13     queries of the next item into shared memory
+//   warp 12         issues the products                            warps 13-15  queries of the next item into shared memory
 // Keys and values are rounded to bf16 here (step * code + low, once), which a score feels by at most 2^-8 of sum |q k|.  A value row that is NaN is put in as zeros and
 // its key as NaN: a row that sees the token becomes NaN through its score, a row that must not see it has weight 0, and 0 x 0 adds nothing.
 //
@@ -18,7 +18,7 @@ namespace kv4 {
 namespace {
 
 constexpr int kTok = 128, kRows = 256, kTile = 128;
-constexpr int kThreads = 14 * 32;
+constexpr int kThreads = 16 * 32;
 constexpr float kLag = 8.0f;                              // powers of two by which a row's maximum may be left behind
 
 template <int D> constexpr uint32_t tile_bytes() { return kTile * D * 2; }
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     uint32_t* tmem_holder = (uint32_t*)(bars + 17);
     volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
     if (threadIdx.x == 0) {
-        ptx::mbar_init(q_full, 1);
+        ptx::mbar_init(q_full, 3);
         ptx::mbar_init(q_empty, 1);
         ptx::mbar_init(drained, 1);
         for (uint32_t s = 0; s < 2; ++s) {
@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 
         if (warp < 8) {
             // ------------------------------------------------------------ softmax: a thread has a row
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
             const uint32_t t = warp / 4, r = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
             const uint32_t s_col = tmem + kS + t * kTok + lanes, o_col = tmem + kO + t * D + lanes;
             uint32_t s_phase = 0, o_phase = 0;
@@ -255,21 +256,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         const int first = (c + (int)i) * kTok;
                         const bool whole = first + kTok - 1 <= p_low && (P.window == 0 || first > p_high - (int)P.window);
                         const int from = P.window ? p - (int)P.window + 1 - first : -1, to = p - first;          // columns the row sees
-                        float top = -INFINITY;
+                        float x[kTok];
 #pragma unroll
-                        for (int q = 0; q < kTok / 32; ++q) {
-                            uint32_t x[32];
-                            ptx::tmem_ld_32x32b_x32(s_col + 32 * q, x);
-                            ptx::tmem_ld_wait();
-                            if (whole) {
+                        for (int q = 0; q < kTok / 32; ++q) ptx::tmem_ld_32x32b_x32(s_col + 32 * q, *(uint32_t(*)[32])(x + 32 * q));
+                        ptx::tmem_ld_wait();
+                        if (!whole) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(x[j]));
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (32 * q + j >= from && 32 * q + j <= to) top = fmaxf(top, __uint_as_float(x[j]));
-                            }
+                            for (int j = 0; j < kTok; ++j)
+                                if (j < from || j > to) x[j] = -INFINITY;
                         }
+                        float tops[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                        for (int j = 4; j < kTok; ++j) tops[j % 4] = fmaxf(tops[j % 4], x[j]);
+                        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                         top *= P.scale_log2;              // (the scale is positive)
                         const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
                         if (__any_sync(0xFFFFFFFFu, left_behind)) {
@@ -278,42 +277,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                             l *= less;
                             if (i > 0) {
 #pragma unroll
-                                for (int q = 0; q < D / 32; ++q) {
-                                    uint32_t x[32];
-                                    ptx::tmem_ld_32x32b_x32(o_col + 32 * q, x);
+                                for (int q = 0; q < D / 8; ++q) {
+                                    uint32_t y[8];
+                                    ptx::tmem_ld_32x32b_x8(o_col + 8 * q, y);
                                     ptx::tmem_ld_wait();
 #pragma unroll
-                                    for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * less);
-                                    ptx::tmem_st_32x32b_x32(o_col + 32 * q, x);
+                                    for (int j = 0; j < 8; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * less);
+                                    ptx::tmem_st_32x32b_x8(o_col + 8 * q, y);
                                 }
                             }
                         }
                         const float minus = m == -INFINITY ? 0.0f : -m;
-                        float sum0 = 0.0f, sum1 = 0.0f;
+                        float2 sums[2] = {make_float2(0, 0), make_float2(0, 0)};
 #pragma unroll
                         for (int q = 0; q < kTok / 64; ++q) {
                             uint32_t y[32];
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                uint32_t x[32];
-                                ptx::tmem_ld_32x32b_x32(s_col + 64 * q + 32 * half, x);
-                                ptx::tmem_ld_wait();
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    const int at = 64 * q + 32 * half + 2 * j;
-                                    float a = exp2_fast(fmaf(__uint_as_float(x[2 * j]), P.scale_log2, minus)), b = exp2_fast(fmaf(__uint_as_float(x[2 * j + 1]), P.scale_log2, minus));
-                                    if (!whole) {
-                                        if (at < from || at > to) a = 0.0f;
-                                        if (at + 1 < from || at + 1 > to) b = 0.0f;
-                                    }
-                                    sum0 += a;
-                                    sum1 += b;
-                                    y[16 * half + j] = pack(a, b);
-                                }
+                            for (int j = 0; j < 32; ++j) {
+                                const float2 e = __ffma2_rn(make_float2(x[64 * q + 2 * j], x[64 * q + 2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
+                                const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                                sums[j % 2] = __fadd2_rn(sums[j % 2], w);
+                                y[j] = pack(w.x, w.y);
                             }
-                            ptx::tmem_st_32x32b_x32(s_col + 32 * q, y);          // over columns that have been read
+                            ptx::tmem_st_32x32b_x32(s_col + 32 * q, y);
                         }
-                        l += sum0 + sum1;
+                        l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                         ptx::tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -363,31 +351,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             }
         } else if (warp < 12) {
             // ------------------------------------------------------------ codes to bf16
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
             const uint32_t tid = threadIdx.x - 256, part = tid & 3;       // a quarter of rows tid / 4, + 32, + 64, + 96
             constexpr int kWords = D / 32;                                  // words of a quarter
             uint32_t k128;
             asm volatile("mov.b32 %0, 0x43004300;" : "=r"(k128));
             uint32_t raw[2][4][kWords], kp[4], vp[4];
+            // A chunk's codes are asked for half a chunk's work before they are used, and its pages' numbers a whole one before that: `pages` are those of the chunk
+            // that is loaded next.  A page outside the cache is read as page 0 and reported at the end.
             Item ahead = it;
             int ahead_c = c;
-            uint32_t ahead_u = u;
-            auto load = [&](int which) {                    // K or V codes, and the parameters of both with K, of the chunk that is ahead
+            uint32_t ahead_u = u, left_out = 0xFFFFFFFFu;
+            uint32_t pages[4], pages_len = 0, pages_head = 0, pages_c = 0;
+            const uint32_t pl = B.page_log2, page_mask = (1u << pl) - 1, block_bytes = (D + 8) << pl;
+            auto look_up = [&]() {                          // pages of the chunk that is ahead, and that chunk's place; then on to the next
+                pages_len = (uint32_t)ahead.s.len;
+                pages_head = ahead.head;
+                pages_c = (uint32_t)ahead_c;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t row = tid / 4 + 32 * i, token = (uint32_t)ahead_c * kTok + row;
-                    const bool there = token < (uint32_t)ahead.s.len;
-                    const uint32_t slot = token & ((1u << B.page_log2) - 1);
-                    const uint8_t* block = there ? block_to_read<D>(B, ahead.b, token >> B.page_log2, ahead.head) : nullptr;
-                    if (which == 0) {
-                        kp[i] = there ? *(const uint32_t*)(block + params_at<D>(B.page_log2, 0) + 4 * slot) : 0;
-                        vp[i] = there ? *(const uint32_t*)(block + params_at<D>(B.page_log2, 1) + 4 * slot) : 0;
+                    const uint32_t token = (uint32_t)ahead_c * kTok + tid / 4 + 32 * i;
+                    pages[i] = token < pages_len ? (uint32_t)B.page_table[(uint64_t)ahead.b * B.table_stride + (token >> pl)] : 0;
+                    if (pages[i] >= B.n_pages) {
+                        left_out = ahead.b;
+                        pages[i] = 0;
                     }
-                    const uint8_t* src = block + codes_at<D>(B.page_log2, which) + slot * (D / 2) + part * (D / 8);
+                }
+                if (++ahead_u < end && ++ahead_c == ahead.c1) {
+                    ahead.advance(P);
+                    ahead_c = ahead.c0;
+                }
+            };
+            const uint8_t* rows[4];                         // where the four rows' blocks begin; null: no such token
+            uint32_t slots[4];
+            auto load = [&](int which) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (which == 0) {
+                        const uint32_t token = pages_c * kTok + tid / 4 + 32 * i;
+                        slots[i] = token & page_mask;
+                        rows[i] = token < pages_len ? B.pages + ((uint64_t)pages[i] * B.n_kv_heads + pages_head) * block_bytes : nullptr;
+                        kp[i] = rows[i] ? *(const uint32_t*)(rows[i] + params_at<D>(pl, 0) + 4 * slots[i]) : 0;
+                        vp[i] = rows[i] ? *(const uint32_t*)(rows[i] + params_at<D>(pl, 1) + 4 * slots[i]) : 0;
+                    }
+                    const uint8_t* src = rows[i] + codes_at<D>(pl, which) + slots[i] * (D / 2) + part * (D / 8);
                     if constexpr (kWords == 4) {
-                        const uint4 w = there ? *(const uint4*)src : make_uint4(0, 0, 0, 0);
+                        const uint4 w = rows[i] ? *(const uint4*)src : make_uint4(0, 0, 0, 0);
                         raw[which][i][0] = w.x; raw[which][i][1] = w.y; raw[which][i][2] = w.z; raw[which][i][3] = w.w;
                     } else {
-                        const uint2 w = there ? *(const uint2*)src : make_uint2(0, 0);
+                        const uint2 w = rows[i] ? *(const uint2*)src : make_uint2(0, 0);
                         raw[which][i][0] = w.x; raw[which][i][1] = w.y;
                     }
                 }
@@ -412,8 +424,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
             };
+            look_up();
             load(0);
             load(1);
+            if (u + 1 < end) look_up();
             uint32_t stage = 0, phase = 0;
             for (; ok && u < end; ++u) {
                 // parameters of this chunk; those of a NaN value go into its key
@@ -424,22 +438,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     kq[i] = bad ? 0x7FC07FC0u : kp[i];
                     vq[i] = bad ? 0u : vp[i];
                 }
-                if (++ahead_u < end && ++ahead_c == ahead.c1) {
-                    ahead.advance(P);
-                    ahead_c = ahead.c0;
-                }
                 if (!wait(k_empty(stage), phase ^ 1)) break;
                 store(0, k_smem + stage * kTileBytes, kq);
                 ptx::mbar_arrive_if(k_full(stage), lane == 0);
-                if (ahead_u < end) load(0);
+                if (u + 1 < end) load(0);
                 if (!wait(v_empty(stage), phase ^ 1)) break;
                 store(1, v_smem + stage * kTileBytes, vq);
                 ptx::mbar_arrive_if(v_full(stage), lane == 0);
-                if (ahead_u < end) load(1);
+                if (u + 1 < end) load(1);
+                if (u + 2 < end) look_up();
                 stage ^= 1;
                 phase ^= stage == 0;
             }
-        } else if (warp == 12) {
+            if (left_out != 0xFFFFFFFFu) report(B, kStatusBadPage, left_out);
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");          // (2 x 168 + 2 x 88 registers a thread are the 4 x 128 of the launch)
+        }
+        if (warp == 12) {
             // ------------------------------------------------------------ the products
             constexpr uint32_t kIdescS = ptx::make_idesc_bf16_f32(kTile, kTok, 0), kIdescO = ptx::make_idesc_bf16_f32(kTile, D, 1);
             const uint32_t issue = ptx::elect_one();
@@ -499,20 +514,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 ptx::umma_commit_if(issue, drained);
                 ptx::mbar_wait_warp(drained, 0, &never, P.wait_limit_ns);
             }
-        } else {
-            // ------------------------------------------------------------ queries
+        } else if (warp > 12) {
+            // ------------------------------------------------------------ queries: a lane has the same 16 bytes of every sixth (twelfth) row
+            constexpr uint32_t kLanes = D / 8, kStep = 3 * 32 / kLanes;
+            const uint32_t unit = lane % kLanes, r0 = (warp - 13) * (32 / kLanes) + lane / kLanes;
+            const uint32_t step_i = kStep / P.group, step_g = kStep % P.group;
             uint32_t phase = 1;
             while (ok && u < end) {
-                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group;
+                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group, base = it.tile * kRows;
                 if (!wait(q_empty, phase)) break;
                 phase ^= 1;
-                const uint32_t rows = min(total - it.tile * kRows, (uint32_t)kRows) <= kTile ? kTile : kRows;
-                for (uint32_t e = lane; e < rows * (D / 8); e += 32) {
-                    const uint32_t r = e / (D / 8), unit = e % (D / 8), row = it.tile * kRows + r;
-                    const bool there = row < total;
-                    const uint32_t i = there ? row / P.group : 0, g = there ? row % P.group : 0;
-                    const __nv_bfloat16* src = P.q + (uint64_t)(it.s.first_row + i) * P.q_stride + (it.head * P.group + g) * D + unit * 8;
-                    cp_async16(q_smem + (r / kTile) * kTileBytes + (unit / 8) * kPanel + (r % kTile) * 128 + (((unit % 8) ^ (r & 7)) << 4), src, there ? 16 : 0);
+                const uint32_t rows = total - base <= kTile ? kTile : kRows;
+                uint32_t i = (base + r0) / P.group, g = (base + r0) % P.group;
+                const __nv_bfloat16* q = P.q + (uint64_t)it.s.first_row * P.q_stride + it.head * P.group * D + unit * 8;
+                for (uint32_t r = r0; r < rows; r += kStep) {
+                    const bool there = base + r < total;
+                    cp_async16(q_smem + (r / kTile) * kTileBytes + (unit / 8) * kPanel + (r % kTile) * 128 + (((unit % 8) ^ (r & 7)) << 4),
+                               there ? q + i * P.q_stride + g * D : q, there ? 16 : 0);
+                    i += step_i;
+                    g += step_g;
+                    if (g >= P.group) {
+                        g -= P.group;
+                        ++i;
+                    }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 ptx::fence_proxy_async_smem();
