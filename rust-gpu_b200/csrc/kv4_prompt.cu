@@ -5,7 +5,7 @@
 // with the two tiles half a step apart: while the softmax warps of one work on its S, the tensor cores work for the other.  512 columns of tensor memory are S and O
 // of both tiles.  The maximum a row's weights are taken against only moves when it is left behind by more than 2^8 (then O is read, scaled and written back), so the sums
 // stay far inside f32 and O is rarely touched.
-//   warps 0-3, 4-7  softmax of tile 0 and 1, and their results     warps 8-11  codes -> bf16, K and V into rings of two stages
+//   warps 0-3, 4-7  softmax of tile 0 and 1, and their results     warps 8-11   codes -> bf16, K and V into rings of two stages
 //   warp 12         issues the products                            warps 13-15  queries of the next item into shared memory
 // Keys and values are rounded to bf16 here (step * code + low, once), which a score feels by at most 2^-8 of sum |q k|.  A value row that is NaN is put in as zeros and
 // its key as NaN: a row that sees the token becomes NaN through its score, a row that must not see it has weight 0, and 0 x 0 adds nothing.
@@ -18,8 +18,10 @@ namespace kv4 {
 namespace {
 
 constexpr int kTok = 128, kRows = 256, kTile = 128;
-constexpr int kThreads = 16 * 32;
-constexpr float kLag = 8.0f;                              // powers of two by which a row's maximum may be left behind
+constexpr int kDequantWarps = 4;
+constexpr int kThreads = (12 + kDequantWarps) * 32;
+constexpr uint32_t kIssuer = 8 + kDequantWarps;           // the warp that issues the products
+constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed what a row's weights are taken against
 
 template <int D> constexpr uint32_t tile_bytes() { return kTile * D * 2; }
 template <int D> constexpr uint32_t smem_bytes() { return 6 * tile_bytes<D>() + 1024 + 512; }
@@ -196,9 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         ptx::mbar_init(q_empty, 1);
         ptx::mbar_init(drained, 1);
         for (uint32_t s = 0; s < 2; ++s) {
-            ptx::mbar_init(k_full(s), 4);
+            ptx::mbar_init(k_full(s), kDequantWarps);
             ptx::mbar_init(k_empty(s), 1);
-            ptx::mbar_init(v_full(s), 4);
+            ptx::mbar_init(v_full(s), kDequantWarps);
             ptx::mbar_init(v_empty(s), 1);
             ptx::mbar_init(s_full(s), 1);
             ptx::mbar_init(p_full(s), 4);
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         ptx::fence_barrier_init();
         ptx::fence_proxy_async_smem();
     }
-    if (warp == 12) {
+    if (warp == kIssuer) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_holder), kTmem);
         ptx::tmem_relinquish();
     }
@@ -234,7 +236,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 
         if (warp < 8) {
             // ------------------------------------------------------------ softmax: a thread has a row
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
             const uint32_t t = warp / 4, r = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
             const uint32_t s_col = tmem + kS + t * kTok + lanes, o_col = tmem + kO + t * D + lanes;
             uint32_t s_phase = 0, o_phase = 0;
@@ -248,7 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     const int p = it.s.len - it.s.rows + last / (int)P.group;                      // the row's token
                     const int p_low = it.s.len - it.s.rows + (int)((it.tile * kRows + t * kTile) / P.group);     // the tile's first and last
                     const int p_high = it.s.len - it.s.rows + (int)(min(it.tile * kRows + t * kTile + kTile, total) - 1) / (int)P.group;
-                    float m = -INFINITY, l = 0.0f;
+                    float m = -INFINITY;
+                    float2 l = make_float2(0.0f, 0.0f);
                     for (uint32_t i = 0; i < n; ++i) {
                         if (!wait(s_full(t), s_phase)) break;
                         s_phase ^= 1;
@@ -256,52 +258,73 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         const int first = (c + (int)i) * kTok;
                         const bool whole = first + kTok - 1 <= p_low && (P.window == 0 || first > p_high - (int)P.window);
                         const int from = P.window ? p - (int)P.window + 1 - first : -1, to = p - first;          // columns the row sees
-                        float x[kTok];
+                        // 32 columns at a time, the next ones on their way: weights against the maximum as it is, the largest score beside them.  A row that the
+                        // maximum has left behind moves it, to a whole power of two: what there is of O, l and of this chunk's P is then scaled without rounding.
+                        uint32_t x[2][32];
+                        ptx::tmem_ld_32x32b_x32(s_col, x[0]);
 #pragma unroll
-                        for (int q = 0; q < kTok / 32; ++q) ptx::tmem_ld_32x32b_x32(s_col + 32 * q, *(uint32_t(*)[32])(x + 32 * q));
-                        ptx::tmem_ld_wait();
-                        if (!whole) {
+                        for (int q = 0; q < kTok / 32; ++q) {
+                            ptx::tmem_ld_wait();
+                            if (q + 1 < kTok / 32) ptx::tmem_ld_32x32b_x32(s_col + 32 * (q + 1), x[(q + 1) % 2]);
+                            float* z = (float*)x[q % 2];
+                            if (!whole) {
 #pragma unroll
-                            for (int j = 0; j < kTok; ++j)
-                                if (j < from || j > to) x[j] = -INFINITY;
-                        }
-                        float tops[4] = {x[0], x[1], x[2], x[3]};
+                                for (int j = 0; j < 32; ++j)
+                                    if (32 * q + j < from || 32 * q + j > to) z[j] = -INFINITY;
+                            }
+                            uint32_t y[16];
+                            float2 sum;
+                            float top = -INFINITY;
+                            auto weigh = [&]() {
+                                const float minus = m == -INFINITY ? 0.0f : -m;
+                                sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                        for (int j = 4; j < kTok; ++j) tops[j % 4] = fmaxf(tops[j % 4], x[j]);
-                        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                        top *= P.scale_log2;              // (the scale is positive)
-                        const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
-                        if (__any_sync(0xFFFFFFFFu, left_behind)) {
-                            const float m_new = left_behind ? top : m, less = m == m_new ? 1.0f : exp2_fast(m - m_new);
-                            m = m_new;
-                            l *= less;
-                            if (i > 0) {
+                                for (int j = 0; j < 16; ++j) {
+                                    const float2 e = __ffma2_rn(make_float2(z[2 * j], z[2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
+                                    const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                                    sum = __fadd2_rn(sum, w);
+                                    y[j] = pack(w.x, w.y);
+                                }
+                            };
 #pragma unroll
-                                for (int q = 0; q < D / 8; ++q) {
-                                    uint32_t y[8];
-                                    ptx::tmem_ld_32x32b_x8(o_col + 8 * q, y);
+                            for (int j = 0; j < 16; ++j) top = fmaxf(fmaxf(top, z[2 * j]), z[2 * j + 1]);
+                            weigh();
+                            top *= P.scale_log2;          // (the scale is positive)
+                            const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
+                            if (__any_sync(0xFFFFFFFFu, left_behind)) {          // once or twice an item
+                                const float m_new = left_behind ? ceilf(top) : m, gap = m_new - m;
+                                const float less = m == m_new ? 1.0f : gap < 126.0f ? __int_as_float((127 - (int)gap) << 23) : 0.0f;
+                                m = m_new;
+                                l.x *= less;
+                                l.y *= less;
+                                ptx::tmem_st_wait();
+                                const __nv_bfloat162 less2 = __float2bfloat162_rn(less);
+#pragma unroll 1
+                                for (int k = 0; k < 2 * q; ++k) {
+                                    uint32_t o[8];
+                                    ptx::tmem_ld_32x32b_x8(s_col + 8 * k, o);
                                     ptx::tmem_ld_wait();
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * less);
-                                    ptx::tmem_st_32x32b_x8(o_col + 8 * q, y);
+                                    for (int j = 0; j < 8; ++j) {
+                                        const __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&o[j], less2);
+                                        o[j] = *(const uint32_t*)&v;
+                                    }
+                                    ptx::tmem_st_32x32b_x8(s_col + 8 * k, o);
                                 }
-                            }
-                        }
-                        const float minus = m == -INFINITY ? 0.0f : -m;
-                        float2 sums[2] = {make_float2(0, 0), make_float2(0, 0)};
+#pragma unroll 1
+                                for (int k = 0; i > 0 && k < D / 8; ++k) {
+                                    uint32_t o[8];
+                                    ptx::tmem_ld_32x32b_x8(o_col + 8 * k, o);
+                                    ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int q = 0; q < kTok / 64; ++q) {
-                            uint32_t y[32];
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const float2 e = __ffma2_rn(make_float2(x[64 * q + 2 * j], x[64 * q + 2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
-                                const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                                sums[j % 2] = __fadd2_rn(sums[j % 2], w);
-                                y[j] = pack(w.x, w.y);
+                                    for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * less);
+                                    ptx::tmem_st_32x32b_x8(o_col + 8 * k, o);
+                                }
+                                weigh();
                             }
-                            ptx::tmem_st_32x32b_x32(s_col + 32 * q, y);
+                            l = __fadd2_rn(l, sum);
+                            ptx::tmem_st_32x32b_x16(s_col + 16 * q, y);          // over columns that have been read
                         }
-                        l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                         ptx::tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
@@ -311,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     o_phase ^= 1;
                     ptx::tc_fence_after_sync();
                     if (opens && closes) {
-                        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+                        const float inverse = l.x + l.y == 0.0f ? 0.0f : 1.0f / (l.x + l.y);
                         __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + last / (int)P.group) * P.y_stride + (it.head * P.group + last % P.group) * D;
 #pragma unroll
                         for (int q = 0; q < D / 32; ++q) {
@@ -339,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                             for (int j = 0; j < 32; ++j) rec[(32 * q + j) * kRows] = __uint_as_float(x[j]);
                         }
                         rec[D * kRows] = m;
-                        rec[(D + 1) * kRows] = l;
+                        rec[(D + 1) * kRows] = l.x + l.y;
                     }
                     ptx::tc_fence_before_sync();           // the next item's first product writes O after this warp's next p_full
                 }
@@ -349,76 +372,83 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     c = it.c0;
                 }
             }
-        } else if (warp < 12) {
+        } else if (warp < kIssuer) {
             // ------------------------------------------------------------ codes to bf16
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-            const uint32_t tid = threadIdx.x - 256, part = tid & 3;       // a quarter of rows tid / 4, + 32, + 64, + 96
+            const uint32_t tid = threadIdx.x - 256, part = tid & 3;       // a quarter of rows tid / 4 + kRowStep i
             constexpr int kWords = D / 32;                                  // words of a quarter
+            constexpr int kRowStep = kDequantWarps * 8, kEach = kTok / kRowStep;
             uint32_t k128;
             asm volatile("mov.b32 %0, 0x43004300;" : "=r"(k128));
-            uint32_t raw[2][4][kWords], kp[4], vp[4];
-            // A chunk's codes are asked for half a chunk's work before they are used, and its pages' numbers a whole one before that: `pages` are those of the chunk
-            // that is loaded next.  A page outside the cache is read as page 0 and reported at the end.
+            const uint32_t pl = B.page_log2;
+            // places of the rows, the same in every chunk: their parameters and codes in a block, their 16-byte units in a stage.  The order in which a quarter's units are
+            // stored differs between lanes, so that eight lanes hit all banks.
+            uint32_t param_off[kEach], code_off[kEach], unit_off[kWords];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const uint32_t slot = (tid / 4 + kRowStep * i) & ((1u << pl) - 1);
+                param_off[i] = params_at<D>(pl, 0) + 4 * slot;
+                code_off[i] = slot * (D / 2) + part * (D / 8);
+            }
+            const bool swapped = D == 128 && part >= 2;
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                const uint32_t unit = part * kWords + (swapped ? j ^ 2 : j);
+                unit_off[j] = unit / 8 * kPanel + tid / 4 * 128 + ((unit % 8 ^ (tid / 4 & 7)) << 4);
+            }
+            // A chunk's codes are asked for half a chunk's work before they are used, and its pages' numbers a whole one before that.  A page outside the cache is read
+            // as page 0 and reported at the end; where there is no token page 0 is read too, and the parameters are zeros.
             Item ahead = it;
             int ahead_c = c;
-            uint32_t ahead_u = u, left_out = 0xFFFFFFFFu;
-            uint32_t pages[4], pages_len = 0, pages_head = 0, pages_c = 0;
-            const uint32_t pl = B.page_log2, page_mask = (1u << pl) - 1, block_bytes = (D + 8) << pl;
-            auto look_up = [&]() {                          // pages of the chunk that is ahead, and that chunk's place; then on to the next
-                pages_len = (uint32_t)ahead.s.len;
-                pages_head = ahead.head;
-                pages_c = (uint32_t)ahead_c;
+            uint32_t ahead_u = u, left_out = 0xFFFFFFFFu, next_pages[kEach];
+            bool next_there[kEach], there[kEach];
+            uint32_t next_head = 0, next_seq = 0, raw[2][kEach][kWords], kp[kEach], vp[kEach];
+            const uint8_t* block[kEach];
+            auto look_up = [&]() {                          // of the chunk that is ahead; then on to the next
+                next_head = ahead.head;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t token = (uint32_t)ahead_c * kTok + tid / 4 + 32 * i;
-                    pages[i] = token < pages_len ? (uint32_t)B.page_table[(uint64_t)ahead.b * B.table_stride + (token >> pl)] : 0;
-                    if (pages[i] >= B.n_pages) {
-                        left_out = ahead.b;
-                        pages[i] = 0;
-                    }
+                for (int i = 0; i < kEach; ++i) {
+                    const uint32_t token = (uint32_t)ahead_c * kTok + tid / 4 + kRowStep * i;
+                    next_there[i] = token < (uint32_t)ahead.s.len;
+                    next_pages[i] = next_there[i] ? (uint32_t)B.page_table[(uint64_t)ahead.b * B.table_stride + (token >> pl)] : 0;
                 }
+                next_seq = ahead.b;
                 if (++ahead_u < end && ++ahead_c == ahead.c1) {
                     ahead.advance(P);
                     ahead_c = ahead.c0;
                 }
             };
-            const uint8_t* rows[4];                         // where the four rows' blocks begin; null: no such token
-            uint32_t slots[4];
             auto load = [&](int which) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kEach; ++i) {
                     if (which == 0) {
-                        const uint32_t token = pages_c * kTok + tid / 4 + 32 * i;
-                        slots[i] = token & page_mask;
-                        rows[i] = token < pages_len ? B.pages + ((uint64_t)pages[i] * B.n_kv_heads + pages_head) * block_bytes : nullptr;
-                        kp[i] = rows[i] ? *(const uint32_t*)(rows[i] + params_at<D>(pl, 0) + 4 * slots[i]) : 0;
-                        vp[i] = rows[i] ? *(const uint32_t*)(rows[i] + params_at<D>(pl, 1) + 4 * slots[i]) : 0;
+                        if (next_pages[i] >= B.n_pages) {
+                            left_out = next_seq;
+                            next_pages[i] = 0;
+                        }
+                        block[i] = B.pages + ((uint64_t)next_pages[i] * B.n_kv_heads + next_head) * ((D + 8) << pl);
+                        there[i] = next_there[i];
+                        kp[i] = *(const uint32_t*)(block[i] + param_off[i]);
+                        vp[i] = *(const uint32_t*)(block[i] + param_off[i] + (4u << pl));
                     }
-                    const uint8_t* src = rows[i] + codes_at<D>(pl, which) + slots[i] * (D / 2) + part * (D / 8);
+                    const uint8_t* src = block[i] + code_off[i] + (which ? (D / 2) << pl : 0);
                     if constexpr (kWords == 4) {
-                        const uint4 w = rows[i] ? *(const uint4*)src : make_uint4(0, 0, 0, 0);
+                        const uint4 w = *(const uint4*)src;
                         raw[which][i][0] = w.x; raw[which][i][1] = w.y; raw[which][i][2] = w.z; raw[which][i][3] = w.w;
                     } else {
-                        const uint2 w = rows[i] ? *(const uint2*)src : make_uint2(0, 0);
+                        const uint2 w = *(const uint2*)src;
                         raw[which][i][0] = w.x; raw[which][i][1] = w.y;
                     }
                 }
             };
-            auto store = [&](int which, uint32_t base, const uint32_t (&params)[4]) {
+            auto store = [&](int which, uint32_t base, const uint32_t (&params)[kEach]) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t row = tid / 4 + 32 * i;
+                for (int i = 0; i < kEach; ++i) {
                     const __nv_bfloat162 step = twice(params[i] & 0xFFFFu), low = twice(params[i] >> 16);
 #pragma unroll
                     for (int j = 0; j < kWords; ++j) {
-                        // 16-byte units of the row: quarter `part` has kWords of them; the order of its stores differs between lanes, so that eight lanes hit all banks
-                        const uint32_t jj = D == 128 ? j ^ ((part >> 1) << 1) : j;
-                        uint32_t w = raw[which][i][j];
-                        if (D == 128 && (part >> 1)) w = raw[which][i][j ^ 2];
-                        const uint32_t unit = part * kWords + jj, panel = unit / 8, at = unit % 8;
-                        const uint32_t dst = base + panel * kPanel + row * 128 + ((at ^ (row & 7)) << 4);
+                        const uint32_t w = swapped ? raw[which][i][(j ^ 2) % kWords] : raw[which][i][j];
                         const uint32_t v0 = value_of(w, 0, k128, step, low), v1 = value_of(w, 1, k128, step, low), v2 = value_of(w, 2, k128, step, low), v3 = value_of(w, 3, k128, step, low);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + unit_off[j] + i * (kRowStep * 128)), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
                     }
                 }
                 ptx::fence_proxy_async_smem();
@@ -431,12 +461,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             uint32_t stage = 0, phase = 0;
             for (; ok && u < end; ++u) {
                 // parameters of this chunk; those of a NaN value go into its key
-                uint32_t kq[4], vq[4];
+                uint32_t kq[kEach], vq[kEach];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kEach; ++i) {
                     const bool bad = (vp[i] & 0x7F800000u) == 0x7F800000u || (vp[i] & 0x7F80u) == 0x7F80u;
-                    kq[i] = bad ? 0x7FC07FC0u : kp[i];
-                    vq[i] = bad ? 0u : vp[i];
+                    kq[i] = !there[i] ? 0u : bad ? 0x7FC07FC0u : kp[i];
+                    vq[i] = !there[i] || bad ? 0u : vp[i];
                 }
                 if (!wait(k_empty(stage), phase ^ 1)) break;
                 store(0, k_smem + stage * kTileBytes, kq);
@@ -451,10 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 phase ^= stage == 0;
             }
             if (left_out != 0xFFFFFFFFu) report(B, kStatusBadPage, left_out);
-        } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");          // (2 x 168 + 2 x 88 registers a thread are the 4 x 128 of the launch)
-        }
-        if (warp == 12) {
+        } else if (warp == kIssuer) {
             // ------------------------------------------------------------ the products
             constexpr uint32_t kIdescS = ptx::make_idesc_bf16_f32(kTile, kTok, 0), kIdescO = ptx::make_idesc_bf16_f32(kTile, D, 1);
             const uint32_t issue = ptx::elect_one();
@@ -514,10 +541,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 ptx::umma_commit_if(issue, drained);
                 ptx::mbar_wait_warp(drained, 0, &never, P.wait_limit_ns);
             }
-        } else if (warp > 12) {
+        } else if (warp > kIssuer) {
             // ------------------------------------------------------------ queries: a lane has the same 16 bytes of every sixth (twelfth) row
             constexpr uint32_t kLanes = D / 8, kStep = 3 * 32 / kLanes;
-            const uint32_t unit = lane % kLanes, r0 = (warp - 13) * (32 / kLanes) + lane / kLanes;
+            const uint32_t unit = lane % kLanes, r0 = (warp - kIssuer - 1) * (32 / kLanes) + lane / kLanes;
             const uint32_t step_i = kStep / P.group, step_g = kStep % P.group;
             uint32_t phase = 1;
             while (ok && u < end) {
@@ -549,11 +576,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 }
             }
         }
-        if (!ok && lane == 0) atomicCAS(P.timeout_status, 0, (warp == 12 ? kStatusMmaTimeout : warp < 8 ? kStatusEpilogueTimeout : kStatusProducerTimeout) | (int)(u & 0xFFFFFF));
+        if (!ok && lane == 0) atomicCAS(P.timeout_status, 0, (warp == kIssuer ? kStatusMmaTimeout : warp < 8 ? kStatusEpilogueTimeout : kStatusProducerTimeout) | (int)(u & 0xFFFFFF));
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kIssuer) {
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc(tmem, kTmem);
     }
