@@ -260,24 +260,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         const int from = P.window ? p - (int)P.window + 1 - first : -1, to = p - first;          // columns the row sees
                         // 32 columns at a time, the next ones on their way: weights against the maximum as it is, the largest score beside them.  A row that the
                         // maximum has left behind moves it, to a whole power of two: what there is of O, l and of this chunk's P is then scaled without rounding.
-                        uint32_t x[2][32];
-                        ptx::tmem_ld_32x32b_x32(s_col, x[0]);
-#pragma unroll
-                        for (int q = 0; q < kTok / 32; ++q) {
-                            ptx::tmem_ld_wait();
-                            if (q + 1 < kTok / 32) ptx::tmem_ld_32x32b_x32(s_col + 32 * (q + 1), x[(q + 1) % 2]);
-                            float* z = (float*)x[q % 2];
+                        auto block = [&](int q, uint32_t (&x)[32]) {
+                            float* z = (float*)x;
                             if (!whole) {
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)
-                                    if (32 * q + j < from || 32 * q + j > to) z[j] = -INFINITY;
+                                    if (j < from - 32 * q || j > to - 32 * q) z[j] = -INFINITY;
                             }
-                            uint32_t y[16];
-                            float2 sum;
                             float top = -INFINITY;
-                            auto weigh = [&]() {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) top = fmaxf(fmaxf(top, z[2 * j]), z[2 * j + 1]);
+                            top *= P.scale_log2;          // (the scale is positive)
+                            for (;;) {
                                 const float minus = m == -INFINITY ? 0.0f : -m;
-                                sum = make_float2(0.0f, 0.0f);
+                                float2 sum = make_float2(0.0f, 0.0f);
+                                uint32_t y[16];
 #pragma unroll
                                 for (int j = 0; j < 16; ++j) {
                                     const float2 e = __ffma2_rn(make_float2(z[2 * j], z[2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
@@ -285,13 +282,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                     sum = __fadd2_rn(sum, w);
                                     y[j] = pack(w.x, w.y);
                                 }
-                            };
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) top = fmaxf(fmaxf(top, z[2 * j]), z[2 * j + 1]);
-                            weigh();
-                            top *= P.scale_log2;          // (the scale is positive)
-                            const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
-                            if (__any_sync(0xFFFFFFFFu, left_behind)) {          // once or twice an item
+                                const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
+                                if (!__any_sync(0xFFFFFFFFu, left_behind)) {
+                                    l = __fadd2_rn(l, sum);
+                                    ptx::tmem_st_32x32b_x16(s_col + 16 * q, y);      // over columns that have been read
+                                    return;
+                                }
+                                // once or twice an item; then the block again
                                 const float m_new = left_behind ? ceilf(top) : m, gap = m_new - m;
                                 const float less = m == m_new ? 1.0f : gap < 126.0f ? __int_as_float((127 - (int)gap) << 23) : 0.0f;
                                 m = m_new;
@@ -320,10 +317,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                     for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * less);
                                     ptx::tmem_st_32x32b_x8(o_col + 8 * k, o);
                                 }
-                                weigh();
                             }
-                            l = __fadd2_rn(l, sum);
-                            ptx::tmem_st_32x32b_x16(s_col + 16 * q, y);          // over columns that have been read
+                        };
+#pragma unroll 1
+                        for (int q = 0; q < kTok / 32; ++q) {
+                            uint32_t x[32];
+                            ptx::tmem_ld_32x32b_x32(s_col + 32 * q, x);
+                            ptx::tmem_ld_wait();
+                            block(q, x);
                         }
                         ptx::tmem_st_wait();
                         ptx::tc_fence_before_sync();
