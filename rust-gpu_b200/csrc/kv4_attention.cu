@@ -41,7 +41,7 @@ int t0_kv4_attention(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_att
     // the kernels count the chunks (64 tokens for few rows, 128 against 256 rows for many) that a batch of this shape may hold, for every head, in 32 bits
     const uint64_t places = (uint64_t)batch->table_stride * batch->page_size;
     if ((uint64_t)batch->n_seqs * (places / 64 + 1) * batch->n_kv_heads >= 1ull << 31 ||
-        ((uint64_t)batch->n_rows * a.n_q_heads / batch->n_kv_heads / 256 + batch->n_seqs) * (places / 128 + 1) * batch->n_kv_heads >= 1ull << 31)
+        ((uint64_t)batch->n_rows * a.n_q_heads / batch->n_kv_heads / 256 + batch->n_seqs) * (places / 128 + 4) * batch->n_kv_heads >= 1ull << 31)
         return fail(T0_ERR_UNSUPPORTED, "%u sequences of up to %llu tokens, %u heads: too much for one call", batch->n_seqs,
                     (unsigned long long)places, batch->n_kv_heads);
     P.q = (const __nv_bfloat16*)a.q; P.y = (__nv_bfloat16*)a.y;

@@ -10,7 +10,8 @@
 // Keys and values are rounded to bf16 here (step * code + low, once), which a score feels by at most 2^-8 of sum |q k|.  A value row that is NaN is put in as zeros and
 // its key as NaN: a row that sees the token becomes NaN through its score, a row that must not see it has weight 0, and 0 x 0 adds nothing.
 //
-// The units of work are all items' chunks, in equal contiguous runs, one for each CTA.  Items that end up in several CTAs leave parts (O, m, l) that a second kernel joins.
+// The units of work are all items' chunks, and kItemUnits for what an item costs beside them, in equal contiguous runs, one for each CTA.  Items whose chunks end up in
+// several CTAs leave parts (O, m, l) that a second kernel joins.
 #include "kv4_attention.cuh"
 
 namespace t0 {
@@ -21,6 +22,7 @@ constexpr int kTok = 128, kRows = 256, kTile = 128;
 constexpr int kDequantWarps = 4;
 constexpr int kThreads = (12 + kDequantWarps) * 32;
 constexpr uint32_t kIssuer = 8 + kDequantWarps;           // the warp that issues the products
+constexpr uint32_t kItemUnits = 2;                        // an item's queries, results and idle times in chunks' time (10600 of 4400 clocks, measured on a prompt of 8192 tokens)
 constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed what a row's weights are taken against
 
 template <int D> constexpr uint32_t tile_bytes() { return kTile * D * 2; }
@@ -30,7 +32,7 @@ template <int D> constexpr uint32_t record_floats() { return kRows * (D + 2); } 
 // The items of one head in the order (sequence, tile), and their chunks: what every thread found in its share, summed up.
 struct Plan {
     uint32_t tiles[kThreads + 1];    // tiles before the sequences of each thread
-    uint32_t chunks[kThreads + 1];   // chunks before the tiles of each thread
+    uint32_t units[kThreads + 1];    // units before the tiles of each thread
     uint32_t warp_sum[kThreads / 32];
     uint32_t seqs_each, tiles_each;
 };
@@ -44,6 +46,7 @@ struct Item {
     Sequence s;
     uint32_t b, tile, head;
     int c0, c1;                      // its chunks
+    __device__ __forceinline__ uint32_t units() const { return (uint32_t)(c1 - c0) + kItemUnits; }
     __device__ __forceinline__ void range(const Attention& P) {
         const int i0 = (int)(tile * kRows / P.group), i1 = min(s.rows - 1, (int)((tile * kRows + kRows - 1) / P.group));
         const int p0 = s.len - s.rows + i0, p1 = s.len - s.rows + i1;
@@ -76,8 +79,7 @@ __device__ __forceinline__ uint32_t scan(uint32_t mine, uint32_t* warp_sum, uint
     }
     if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x / 32] = upto;
     __syncthreads();
-    uint32_t before = 0;
-    for (uint32_t w = 0; w < threadIdx.x / 32; ++w) before += warp_sum[w];
+    const uint32_t before = __reduce_add_sync(0xFFFFFFFFu, (threadIdx.x & 31) < threadIdx.x / 32 ? warp_sum[threadIdx.x & 31] : 0);
     out[threadIdx.x + 1] = before + upto;
     if (threadIdx.x == 0) out[0] = 0;
     __syncthreads();
@@ -108,7 +110,7 @@ __device__ __forceinline__ Item tile_at(const Attention& P, const Plan& plan, ui
     it.range(P);
     return it;
 }
-// returns the chunks of one head
+// returns the units of one head
 __device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
     const uint32_t n = P.B.n_seqs, each = (n + kThreads - 1) / kThreads, tid = threadIdx.x;
     if (tid == 0) plan.seqs_each = each;
@@ -121,32 +123,67 @@ __device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
     if (tid * tiles_each < tiles) {
         Item it = tile_at(P, plan, tid * tiles_each);
         for (uint32_t i = tid * tiles_each;;) {
-            mine += it.c1 - it.c0;
+            mine += it.units();
             if (++i >= min(tiles, (tid + 1) * tiles_each)) break;
             it.advance(P);
         }
     }
-    return scan(mine, plan.warp_sum, plan.chunks);
+    return scan(mine, plan.warp_sum, plan.units);
 }
 // the item that unit u (of all heads) belongs to, and the unit it begins with
 __device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, uint32_t per_head, uint32_t u, uint32_t* first) {
-    const uint32_t head = u / per_head, at = u % per_head, th = last_not_above(plan.chunks, at);
+    const uint32_t head = u / per_head, at = u % per_head, th = last_not_above(plan.units, at);
     Item it = tile_at(P, plan, th * plan.tiles_each);
-    uint32_t n = plan.chunks[th];
-    while (at >= n + (uint32_t)(it.c1 - it.c0)) {
-        n += it.c1 - it.c0;
+    uint32_t n = plan.units[th];
+    while (at >= n + it.units()) {
+        n += it.units();
         it.advance(P);
     }
     it.head = head;
     *first = head * per_head + n;
     return it;
 }
-// the run of CTA c: units * c / ctas, rounded down
-__device__ __forceinline__ uint32_t start_of(uint32_t c, uint32_t units, uint32_t ctas) { return c * (units / ctas) + c * (units % ctas) / ctas; }
+// where run c of `runs` begins: units * c / runs, rounded down.  There are no more runs than units, so that none is empty.
+__device__ __forceinline__ uint32_t start_of(uint32_t c, uint32_t units, uint32_t runs) { return c * (units / runs) + c * (units % runs) / runs; }
+
+// A run's way through its items: the chunks c .. c + n - 1 of one after the other.
+struct Walk {
+    Item it;
+    uint32_t first, end;             // the item's first unit; the run's end
+    int c;
+    uint32_t n;                      // 0: the run is over
+    __device__ __forceinline__ void count() {
+        const int upto = (int)min(end - first, it.units()) - (int)kItemUnits;
+        n = max(it.c0 + upto - c, 0);
+    }
+    __device__ __forceinline__ Walk(const Attention& P, const Plan& plan, uint32_t per_head, uint32_t begin, uint32_t end_) : end(end_) {
+        it = item_of(P, plan, per_head, begin, &first);
+        c = it.c0 + max((int)(begin - first) - (int)kItemUnits, 0);
+        count();
+    }
+    __device__ __forceinline__ void next(const Attention& P) {
+        first += it.units();
+        n = 0;
+        if (first >= end) return;
+        it.advance(P);
+        c = it.c0;
+        count();
+    }
+};
+
+// What the joining kernel needs to know of the item that a CTA's run begins in.
+struct Cut {
+    uint32_t units, first, chunks;   // of the launch; the item's first, and its chunks (0: the run is empty)
+    uint32_t tile, head;
+    int first_row;
+    uint32_t total;                  // rows x group of the sequence
+    uint32_t _pad;
+};
 
 struct Params {
     Attention P;
     float* records;                  // two for each CTA: of the item it begins in, of the item it ends in
+    Cut* cuts;                       // one for each CTA
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -221,28 +258,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
 
-    const uint32_t per_head = make_plan(P, plan), units = per_head * B.n_kv_heads;
-    const uint32_t begin = units ? start_of(blockIdx.x, units, gridDim.x) : 0, end = units ? start_of(blockIdx.x + 1, units, gridDim.x) : 0;
+    const uint32_t per_head = make_plan(P, plan), units = per_head * B.n_kv_heads, runs = min(gridDim.x, units);
+    const uint32_t begin = blockIdx.x < runs ? start_of(blockIdx.x, units, runs) : 0, end = blockIdx.x < runs ? start_of(blockIdx.x + 1, units, runs) : 0;
     bool ok = true;
     auto wait = [&](uint32_t b, uint32_t parity) {
         if (ok) ok = ptx::mbar_wait_warp(b, parity, abort_flag, P.wait_limit_ns);
         return ok;
     };
+    if (begin >= end && threadIdx.x == 0) G.cuts[blockIdx.x] = Cut{};
     if (begin < end) {
-        uint32_t item_first;
-        Item it = item_of(P, plan, per_head, begin, &item_first);
-        int c = it.c0 + (int)(begin - item_first);        // the chunk at hand
-        uint32_t u = begin;
+        Walk walk(P, plan, per_head, begin, end);
+        const Item& it = walk.it;
+        if (threadIdx.x == 0)
+            G.cuts[blockIdx.x] = Cut{units, walk.first, (uint32_t)(it.c1 - it.c0), it.tile, it.head, it.s.first_row, (uint32_t)it.s.rows * P.group, 0};
 
         if (warp < 8) {
             // ------------------------------------------------------------ softmax: a thread has a row
             const uint32_t t = warp / 4, r = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
             const uint32_t s_col = tmem + kS + t * kTok + lanes, o_col = tmem + kO + t * D + lanes;
             uint32_t s_phase = 0, o_phase = 0;
-            while (ok && u < end) {
-                const bool opens = c == it.c0;
-                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group;
-                const bool closes = c + (int)n == it.c1;
+            for (; ok && walk.n; walk.next(P)) {
+                const int c = walk.c;
+                const uint32_t n = walk.n, total = (uint32_t)it.s.rows * P.group;
+                const bool opens = c == it.c0, closes = c + (int)n == it.c1;
                 const uint32_t row = it.tile * kRows + t * kTile + r;
                 if (it.tile * kRows + t * kTile < total) {
                     const int last = (int)min(row, total - 1);
@@ -367,11 +405,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     }
                     ptx::tc_fence_before_sync();           // the next item's first product writes O after this warp's next p_full
                 }
-                u += n;
-                if (u < end) {
-                    it.advance(P);
-                    c = it.c0;
-                }
             }
         } else if (warp < kIssuer) {
             // ------------------------------------------------------------ codes to bf16
@@ -398,25 +431,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             }
             // A chunk's codes are asked for half a chunk's work before they are used, and its pages' numbers a whole one before that.  A page outside the cache is read
             // as page 0 and reported at the end; where there is no token page 0 is read too, and the parameters are zeros.
-            Item ahead = it;
-            int ahead_c = c;
-            uint32_t ahead_u = u, left_out = 0xFFFFFFFFu, next_pages[kEach];
+            Walk ahead = walk;
+            uint32_t left_out = 0xFFFFFFFFu, next_pages[kEach];
             bool next_there[kEach], there[kEach];
             uint32_t next_head = 0, next_seq = 0, raw[2][kEach][kWords], kp[kEach], vp[kEach];
             const uint8_t* block[kEach];
-            auto look_up = [&]() {                          // of the chunk that is ahead; then on to the next
-                next_head = ahead.head;
+            bool more = ahead.n != 0;                       // whether pages have been looked up that are not loaded yet
+            auto look_up = [&]() {                          // of the chunk that is ahead, if there is one; then on to the next
+                more = ahead.n != 0;
+                if (!more) return;
+                next_head = ahead.it.head;
 #pragma unroll
                 for (int i = 0; i < kEach; ++i) {
-                    const uint32_t token = (uint32_t)ahead_c * kTok + tid / 4 + kRowStep * i;
-                    next_there[i] = token < (uint32_t)ahead.s.len;
-                    next_pages[i] = next_there[i] ? (uint32_t)B.page_table[(uint64_t)ahead.b * B.table_stride + (token >> pl)] : 0;
+                    const uint32_t token = (uint32_t)ahead.c * kTok + tid / 4 + kRowStep * i;
+                    next_there[i] = token < (uint32_t)ahead.it.s.len;
+                    next_pages[i] = next_there[i] ? (uint32_t)B.page_table[(uint64_t)ahead.it.b * B.table_stride + (token >> pl)] : 0;
                 }
-                next_seq = ahead.b;
-                if (++ahead_u < end && ++ahead_c == ahead.c1) {
-                    ahead.advance(P);
-                    ahead_c = ahead.c0;
-                }
+                next_seq = ahead.it.b;
+                ++ahead.c;
+                if (--ahead.n == 0) ahead.next(P);
             };
             auto load = [&](int which) {
 #pragma unroll
@@ -456,11 +489,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 __syncwarp();
             };
             look_up();
-            load(0);
-            load(1);
-            if (u + 1 < end) look_up();
+            bool at_hand = more;                            // whether there is a chunk whose codes are loaded
+            if (at_hand) {
+                load(0);
+                load(1);
+                look_up();
+            }
             uint32_t stage = 0, phase = 0;
-            for (; ok && u < end; ++u) {
+            while (ok && at_hand) {
                 // parameters of this chunk; those of a NaN value go into its key
                 uint32_t kq[kEach], vq[kEach];
 #pragma unroll
@@ -472,12 +508,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 if (!wait(k_empty(stage), phase ^ 1)) break;
                 store(0, k_smem + stage * kTileBytes, kq);
                 ptx::mbar_arrive_if(k_full(stage), lane == 0);
-                if (u + 1 < end) load(0);
+                at_hand = more;
+                if (more) load(0);
                 if (!wait(v_empty(stage), phase ^ 1)) break;
                 store(1, v_smem + stage * kTileBytes, vq);
                 ptx::mbar_arrive_if(v_full(stage), lane == 0);
-                if (u + 1 < end) load(1);
-                if (u + 2 < end) look_up();
+                if (more) {
+                    load(1);
+                    look_up();
+                }
                 stage ^= 1;
                 phase ^= stage == 0;
             }
@@ -501,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 #pragma unroll
                 for (int k = 0; k < kTok / 16; ++k) ptx::umma_bf16_ts_mn_if(issue, tmem + kO + t * D, tmem + kS + t * kTok + k * 8, b + k * 128, kIdescO, k > 0 || more);
             };
-            while (ok && u < end) {
-                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group;
+            for (; ok && walk.n; walk.next(P)) {
+                const uint32_t n = walk.n, total = (uint32_t)it.s.rows * P.group;
                 const uint32_t tiles = it.tile * kRows + kTile < total ? 2 : 1;
                 if (!wait(q_full, q_phase)) break;
                 q_phase ^= 1;
@@ -530,11 +569,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         phase ^= stage == 0;
                     }
                 }
-                u += n;
-                if (u < end) {
-                    it.advance(P);
-                    c = it.c0;
-                }
             }
             // what is in flight ends before the memory it uses is given back: in a run that went well the last sums have been waited for by the softmax warps
             if (!ok) {
@@ -548,8 +582,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             const uint32_t unit = lane % kLanes, r0 = (warp - kIssuer - 1) * (32 / kLanes) + lane / kLanes;
             const uint32_t step_i = kStep / P.group, step_g = kStep % P.group;
             uint32_t phase = 1;
-            while (ok && u < end) {
-                const uint32_t n = min(end - u, (uint32_t)(it.c1 - c)), total = (uint32_t)it.s.rows * P.group, base = it.tile * kRows;
+            for (; ok && walk.n; walk.next(P)) {
+                const uint32_t total = (uint32_t)it.s.rows * P.group, base = it.tile * kRows;
                 if (!wait(q_empty, phase)) break;
                 phase ^= 1;
                 const uint32_t rows = total - base <= kTile ? kTile : kRows;
@@ -570,14 +604,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 ptx::mbar_arrive_if(q_full, lane == 0);
-                u += n;
-                if (u < end) {
-                    it.advance(P);
-                    c = it.c0;
-                }
             }
         }
-        if (!ok && lane == 0) atomicCAS(P.timeout_status, 0, (warp == kIssuer ? kStatusMmaTimeout : warp < 8 ? kStatusEpilogueTimeout : kStatusProducerTimeout) | (int)(u & 0xFFFFFF));
+        if (!ok && lane == 0) atomicCAS(P.timeout_status, 0, (warp == kIssuer ? kStatusMmaTimeout : warp < 8 ? kStatusEpilogueTimeout : kStatusProducerTimeout) | (int)blockIdx.x);
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
@@ -587,43 +616,40 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     }
 }
 
-// Joins the parts of the items that several CTAs of the launch before worked on.  Block (c, z): the item that the boundary before CTA c cuts, if c is the first one to cut it;
-// z: a slice of its rows.  A thread has a row and a quarter of its numbers.
-constexpr int kJoinRows = 32, kJoinThreads = kThreads;
+// Joins the parts of the items whose chunks several CTAs of the launch before worked on.  Block (c, z): the item that the boundary before CTA c cuts, if c is the first one
+// to cut it; z: a slice of its rows.  A thread has a row and an eighth of its numbers.
+constexpr int kJoinRows = 32, kJoinThreads = kJoinRows * 8;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) kv4_prompt_join_kernel(const __grid_constant__ Params G, uint32_t ctas) {
-    __shared__ Plan plan;
+__global__ void __launch_bounds__(kJoinThreads) kv4_prompt_join_kernel(const __grid_constant__ Params G) {
     const Attention& P = G.P;
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const uint32_t per_head = make_plan(P, plan), units = per_head * P.B.n_kv_heads;
-    if (units == 0) return;
-    const uint32_t slices = kRows / kJoinRows, c = blockIdx.x / slices + 1, z = blockIdx.x % slices, cut = start_of(c, units, ctas);
-    if (cut >= units || cut == start_of(c - 1, units, ctas)) return;
-    uint32_t first;
-    const Item it = item_of(P, plan, per_head, cut, &first);
-    const uint32_t last = first + (it.c1 - it.c0) - 1;
-    if (first == cut || start_of(c - 1, units, ctas) > first) return;      // no cut, or an earlier boundary's item
-    const uint32_t total = (uint32_t)it.s.rows * P.group;
-    if (it.tile * kRows + z * kJoinRows >= total || threadIdx.x >= kJoinRows * 8) return;
-    const uint32_t r = z * kJoinRows + threadIdx.x % kJoinRows, quarter = threadIdx.x / kJoinRows, row = it.tile * kRows + r;
+    const uint32_t slices = kRows / kJoinRows, c = blockIdx.x / slices + 1, z = blockIdx.x % slices;
+    const Cut cut = G.cuts[c];
+    if (cut.chunks == 0) return;
+    const uint32_t runs = min(gridDim.x / slices + 1, cut.units);
+    const uint32_t at = start_of(c, cut.units, runs), chunk0 = cut.first + kItemUnits, behind = chunk0 + cut.chunks;
+    if (at <= chunk0 || start_of(c - 1, cut.units, runs) > chunk0) return;      // all chunks lie in this run, or an earlier boundary cuts them
+    if (cut.tile * kRows + z * kJoinRows >= cut.total) return;
+    const uint32_t r = z * kJoinRows + threadIdx.x % kJoinRows, part = threadIdx.x / kJoinRows, row = cut.tile * kRows + r;
     constexpr int kEach = D / 8;
     auto record = [&](uint32_t i) { return G.records + (uint64_t)(2 * i + (i == c - 1 ? 1 : 0)) * record_floats<D>() + r; };
     float top = -INFINITY, l = 0.0f, sum[kEach] = {};
-    for (uint32_t i = c - 1; i < ctas && start_of(i, units, ctas) <= last; ++i)
-        if (start_of(i, units, ctas) < start_of(i + 1, units, ctas)) top = fmaxf(top, record(i)[D * kRows]);
+    uint32_t parts_end = c;                                // the run behind the last one with a part
+    while (parts_end < runs && start_of(parts_end, cut.units, runs) < behind) ++parts_end;
+    for (uint32_t i = c - 1; i < parts_end; ++i) top = fmaxf(top, record(i)[D * kRows]);
     const float base = top == -INFINITY ? 0.0f : top;
-    for (uint32_t i = c - 1; i < ctas && start_of(i, units, ctas) <= last; ++i) {
-        if (start_of(i, units, ctas) == start_of(i + 1, units, ctas)) continue;
+#pragma unroll 2
+    for (uint32_t i = c - 1; i < parts_end; ++i) {
         const float* rec = record(i);
         const float w = exp2_fast(rec[D * kRows] - base);
         l = fmaf(w, rec[(D + 1) * kRows], l);
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) sum[j] = fmaf(w, rec[(quarter * kEach + j) * kRows], sum[j]);
+        for (int j = 0; j < kEach; ++j) sum[j] = fmaf(w, rec[(part * kEach + j) * kRows], sum[j]);
     }
-    if (row >= total) return;
+    if (row >= cut.total) return;
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-    __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + row / P.group) * P.y_stride + (it.head * P.group + row % P.group) * D + quarter * kEach;
+    __nv_bfloat16* y = P.y + (uint64_t)(cut.first_row + row / P.group) * P.y_stride + (cut.head * P.group + row % P.group) * D + part * kEach;
 #pragma unroll
     for (int j = 0; j < kEach / 8; ++j) {
         uint32_t w[4];
@@ -646,17 +672,18 @@ int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
     }
     Params g;
     g.P = p;
-    g.records = (float*)(p.scratch + kv4_counter_bytes());
+    g.cuts = (Cut*)(p.scratch + kv4_counter_bytes());
+    g.records = (float*)(g.cuts + kMaxCtas);
     const uint32_t ctas = std::min(sms, kMaxCtas);
     cudaError_t e = gemm::launch_pdl(kv4_prompt_kernel<D>, ctas, kThreads, smem, stream, g);
-    if (e == cudaSuccess && ctas > 1) e = gemm::launch_pdl(kv4_prompt_join_kernel<D>, (ctas - 1) * (kRows / kJoinRows), kJoinThreads, 0, stream, g, ctas);
+    if (e == cudaSuccess && ctas > 1) e = gemm::launch_pdl(kv4_prompt_join_kernel<D>, (ctas - 1) * (kRows / kJoinRows), kJoinThreads, 0, stream, g);
     if (e != cudaSuccess) return fail(T0_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
     return T0_OK;
 }
 
 }  // namespace
 
-size_t prompt_scratch_bytes(uint32_t sms) { return (size_t)2 * std::min(sms, kMaxCtas) * record_floats<128>() * sizeof(float); }
+size_t prompt_scratch_bytes(uint32_t sms) { return kMaxCtas * sizeof(Cut) + (size_t)2 * std::min(sms, kMaxCtas) * record_floats<128>() * sizeof(float); }
 
 int launch_prompt(const Attention& p, uint32_t head_dim, uint32_t sms, cudaStream_t stream) {
     return head_dim == 128 ? launch<128>(p, sms, stream) : launch<64>(p, sms, stream);
