@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     const int p_low = it.s.len - it.s.rows + (int)((it.tile * kRows + t * kTile) / P.group);     // the tile's first and last
                     const int p_high = it.s.len - it.s.rows + (int)(min(it.tile * kRows + t * kTile + kTile, total) - 1) / (int)P.group;
                     float m = -INFINITY;
-                    float2 l = make_float2(0.0f, 0.0f);
+                    float2 l[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                     for (uint32_t i = 0; i < n; ++i) {
                         if (!wait(s_full(t), s_phase)) break;
                         s_phase ^= 1;
@@ -296,84 +296,84 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                         const int first = (c + (int)i) * kTok;
                         const bool whole = first + kTok - 1 <= p_low && (P.window == 0 || first > p_high - (int)P.window);
                         const int from = P.window ? p - (int)P.window + 1 - first : -1, to = p - first;          // columns the row sees
-                        // 32 columns at a time, the next ones on their way: weights against the maximum as it is, the largest score beside them.  A row that the
-                        // maximum has left behind moves it, to a whole power of two: what there is of O, l and of this chunk's P is then scaled without rounding.
-                        auto block = [&](int q, uint32_t (&x)[32]) {
-                            float* z = (float*)x;
-                            if (!whole) {
+                        // 64 columns at a time.  A row whose maximum has been left behind moves it, to a whole power of two: what there is of O, l and of this chunk's P is
+                        // then scaled without rounding.
+                        auto keep_up = [&](int q, float top) {                  // the maximum for half q and all behind it
+                            const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
+                            if (!__any_sync(0xFFFFFFFFu, left_behind)) return;  // (all but once or twice an item)
+                            const float m_new = left_behind ? ceilf(top) : m, gap = m_new - m;
+                            const float less = m == m_new ? 1.0f : gap < 126.0f ? __int_as_float((127 - (int)gap) << 23) : 0.0f;
+                            m = m_new;
+                            l[0] = __fmul2_rn(l[0], make_float2(less, less));
+                            l[1] = __fmul2_rn(l[1], make_float2(less, less));
+                            ptx::tmem_st_wait();
+                            const __nv_bfloat162 less2 = __float2bfloat162_rn(less);
+#pragma unroll 1
+                            for (int k = 0; k < 4 * q; ++k) {
+                                uint32_t o[8];
+                                ptx::tmem_ld_32x32b_x8(s_col + 8 * k, o);
+                                ptx::tmem_ld_wait();
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (j < from - 32 * q || j > to - 32 * q) z[j] = -INFINITY;
+                                for (int j = 0; j < 8; ++j) {
+                                    const __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&o[j], less2);
+                                    o[j] = *(const uint32_t*)&v;
+                                }
+                                ptx::tmem_st_32x32b_x8(s_col + 8 * k, o);
                             }
-                            float top = -INFINITY;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) top = fmaxf(fmaxf(top, z[2 * j]), z[2 * j + 1]);
-                            top *= P.scale_log2;          // (the scale is positive)
-                            for (;;) {
-                                const float minus = m == -INFINITY ? 0.0f : -m;
-                                float2 sum = make_float2(0.0f, 0.0f);
-                                uint32_t y[16];
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    const float2 e = __ffma2_rn(make_float2(z[2 * j], z[2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
-                                    const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                                    sum = __fadd2_rn(sum, w);
-                                    y[j] = pack(w.x, w.y);
-                                }
-                                const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
-                                if (!__any_sync(0xFFFFFFFFu, left_behind)) {
-                                    l = __fadd2_rn(l, sum);
-                                    ptx::tmem_st_32x32b_x16(s_col + 16 * q, y);      // over columns that have been read
-                                    return;
-                                }
-                                // once or twice an item; then the block again
-                                const float m_new = left_behind ? ceilf(top) : m, gap = m_new - m;
-                                const float less = m == m_new ? 1.0f : gap < 126.0f ? __int_as_float((127 - (int)gap) << 23) : 0.0f;
-                                m = m_new;
-                                l.x *= less;
-                                l.y *= less;
-                                ptx::tmem_st_wait();
-                                const __nv_bfloat162 less2 = __float2bfloat162_rn(less);
 #pragma unroll 1
-                                for (int k = 0; k < 2 * q; ++k) {
-                                    uint32_t o[8];
-                                    ptx::tmem_ld_32x32b_x8(s_col + 8 * k, o);
-                                    ptx::tmem_ld_wait();
+                            for (int k = 0; i > 0 && k < D / 8; ++k) {
+                                uint32_t o[8];
+                                ptx::tmem_ld_32x32b_x8(o_col + 8 * k, o);
+                                ptx::tmem_ld_wait();
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j) {
-                                        const __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&o[j], less2);
-                                        o[j] = *(const uint32_t*)&v;
-                                    }
-                                    ptx::tmem_st_32x32b_x8(s_col + 8 * k, o);
-                                }
-#pragma unroll 1
-                                for (int k = 0; i > 0 && k < D / 8; ++k) {
-                                    uint32_t o[8];
-                                    ptx::tmem_ld_32x32b_x8(o_col + 8 * k, o);
-                                    ptx::tmem_ld_wait();
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * less);
-                                    ptx::tmem_st_32x32b_x8(o_col + 8 * k, o);
-                                }
+                                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * less);
+                                ptx::tmem_st_32x32b_x8(o_col + 8 * k, o);
                             }
                         };
 #pragma unroll 1
-                        for (int q = 0; q < kTok / 32; ++q) {
-                            uint32_t x[32];
-                            ptx::tmem_ld_32x32b_x32(s_col + 32 * q, x);
+                        for (int q = 0; q < kTok / 64; ++q) {
+                            float x[64];
+                            ptx::tmem_ld_32x32b_x32(s_col + 64 * q, *(uint32_t(*)[32])x);
+                            ptx::tmem_ld_32x32b_x32(s_col + 64 * q + 32, *(uint32_t(*)[32])(x + 32));
                             ptx::tmem_ld_wait();
-                            block(q, x);
+                            if (!whole) {
+#pragma unroll
+                                for (int j = 0; j < 64; ++j)
+                                    if (j < from - 64 * q || j > to - 64 * q) x[j] = -INFINITY;
+                            }
+                            float tops[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) tops[j] = x[16 * j];
+#pragma unroll
+                            for (int j = 1; j < 16; ++j)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], x[16 * k + j]);
+                            keep_up(q, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * P.scale_log2);      // (the scale is positive)
+                            const float minus = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                uint32_t y[16];
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    const float2 e = __ffma2_rn(make_float2(x[32 * k + 2 * j], x[32 * k + 2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
+                                    const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                                    l[j % 2] = __fadd2_rn(l[j % 2], w);
+                                    y[j] = pack(w.x, w.y);
+                                }
+                                ptx::tmem_st_32x32b_x16(s_col + 32 * q + 16 * k, y);          // over columns that have been read
+                            }
                         }
                         ptx::tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
                         ptx::mbar_arrive_if(p_full(t), lane == 0);
                     }
+                    const float sum = (l[0].x + l[0].y) + (l[1].x + l[1].y);
                     if (!wait(o_full(t), o_phase)) break;
                     o_phase ^= 1;
                     ptx::tc_fence_after_sync();
                     if (opens && closes) {
-                        const float inverse = l.x + l.y == 0.0f ? 0.0f : 1.0f / (l.x + l.y);
+                        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
                         __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + last / (int)P.group) * P.y_stride + (it.head * P.group + last % P.group) * D;
 #pragma unroll
                         for (int q = 0; q < D / 32; ++q) {
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                             for (int j = 0; j < 32; ++j) rec[(32 * q + j) * kRows] = __uint_as_float(x[j]);
                         }
                         rec[D * kRows] = m;
-                        rec[(D + 1) * kRows] = l.x + l.y;
+                        rec[(D + 1) * kRows] = sum;
                     }
                     ptx::tc_fence_before_sync();           // the next item's first product writes O after this warp's next p_full
                 }
