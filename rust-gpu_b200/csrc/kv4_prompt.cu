@@ -2,9 +2,9 @@
 //
 // An item is 256 rows (pairs of token and query head of one key/value head, two tiles of 128) against the chunks of 128 tokens that any of them sees.  Per chunk
 //   S = Q K^T (shared memory x shared memory -> tensor memory),  P = 2^(S - m) (one thread a row),  O += P V (P in tensor memory, over S's own columns)
-// with the two tiles half a step apart: while the softmax warps of one work on its S, the tensor cores work for the other.  512 columns of tensor memory are S and O
-// of both tiles.  The maximum a row's weights are taken against only moves when it is left behind by more than 2^8 (then O is read, scaled and written back), so the sums
-// stay far inside f32 and O is rarely touched.
+// half a chunk at a time: the 512 columns of tensor memory are O of both tiles and, for each, S of two halves, so that the scores of one half are there when the softmax
+// warps are done with the other.  The maximum a row's weights are taken against only moves when it is left behind by more than 2^8 (then O is read, scaled and written
+// back), so the sums stay far inside f32 and O is rarely touched.
 //   warps 0-3, 4-7  softmax of tile 0 and 1, and their results     warps 8-11   codes -> bf16, K and V into rings of two stages
 //   warp 12         issues the products                            warps 13-15  queries of the next item into shared memory
 // Keys and values are rounded to bf16 here (step * code + low, once), which a score feels by at most 2^-8 of sum |q k|.  A value row that is NaN is put in as zeros and
@@ -219,16 +219,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     uint64_t* bars = (uint64_t*)(smem + 6 * kTileBytes);
     const uint32_t q_smem = ptx::smem_u32(smem), k_smem = q_smem + 2 * kTileBytes, v_smem = k_smem + 2 * kTileBytes, bar = ptx::smem_u32(bars);
     // barriers
-    const uint32_t q_full = bar, q_empty = bar + 8;
-    auto k_full = [&](uint32_t s) { return bar + 16 + 8 * s; };
-    auto k_empty = [&](uint32_t s) { return bar + 32 + 8 * s; };
-    auto v_full = [&](uint32_t s) { return bar + 48 + 8 * s; };
-    auto v_empty = [&](uint32_t s) { return bar + 64 + 8 * s; };
-    auto s_full = [&](uint32_t t) { return bar + 80 + 8 * t; };
-    auto p_full = [&](uint32_t t) { return bar + 96 + 8 * t; };
-    auto o_full = [&](uint32_t t) { return bar + 112 + 8 * t; };
-    const uint32_t drained = bar + 128;
-    uint32_t* tmem_holder = (uint32_t*)(bars + 17);
+    const uint32_t q_full = bar, q_empty = bar + 8, drained = bar + 16;
+    auto k_full = [&](uint32_t s) { return bar + 24 + 8 * s; };
+    auto k_empty = [&](uint32_t s) { return bar + 40 + 8 * s; };
+    auto v_full = [&](uint32_t s) { return bar + 56 + 8 * s; };
+    auto v_empty = [&](uint32_t s) { return bar + 72 + 8 * s; };
+    auto s_full = [&](uint32_t t, uint32_t half) { return bar + 88 + 16 * t + 8 * half; };
+    auto p_full = [&](uint32_t t, uint32_t half) { return bar + 120 + 16 * t + 8 * half; };
+    // The sums of one more half are in O: waited for only where O is scaled, by a warp that has not yet given the next half's weights away, so that no more than the phase it
+    // asks for can be open or over.  The end of an item has a barrier of its own: two phases may end there before a warp looks.
+    auto o_step = [&](uint32_t t) { return bar + 152 + 8 * t; };
+    auto o_full = [&](uint32_t t) { return bar + 168 + 8 * t; };
+    uint32_t* tmem_holder = (uint32_t*)(bars + 23);
     volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
     if (threadIdx.x == 0) {
         ptx::mbar_init(q_full, 3);
@@ -239,8 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             ptx::mbar_init(k_empty(s), 1);
             ptx::mbar_init(v_full(s), kDequantWarps);
             ptx::mbar_init(v_empty(s), 1);
-            ptx::mbar_init(s_full(s), 1);
-            ptx::mbar_init(p_full(s), 4);
+            for (uint32_t half = 0; half < 2; ++half) {
+                ptx::mbar_init(s_full(s, half), 1);
+                ptx::mbar_init(p_full(s, half), 4);
+            }
+            ptx::mbar_init(o_step(s), 1);
             ptx::mbar_init(o_full(s), 1);
         }
         *abort_flag = 0;
@@ -276,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             // ------------------------------------------------------------ softmax: a thread has a row
             const uint32_t t = warp / 4, r = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
             const uint32_t s_col = tmem + kS + t * kTok + lanes, o_col = tmem + kO + t * D + lanes;
-            uint32_t s_phase = 0, o_phase = 0;
+            uint32_t s_phase = 0, o_phase = 0, halves = 0;             // halves this tile has had
             for (; ok && walk.n; walk.next(P)) {
                 const int c = walk.c;
                 const uint32_t n = walk.n, total = (uint32_t)it.s.rows * P.group;
@@ -289,36 +294,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     const int p_high = it.s.len - it.s.rows + (int)(min(it.tile * kRows + t * kTile + kTile, total) - 1) / (int)P.group;
                     float m = -INFINITY;
                     float2 l[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                    for (uint32_t i = 0; i < n; ++i) {
-                        if (!wait(s_full(t), s_phase)) break;
-                        s_phase ^= 1;
+                    for (uint32_t i = 0; i < 2 * n; ++i) {
+                        const uint32_t half = i & 1, col = s_col + 64 * half;
+                        if (!wait(s_full(t, half), s_phase)) break;
+                        s_phase ^= half;
                         ptx::tc_fence_after_sync();
-                        const int first = (c + (int)i) * kTok;
-                        const bool whole = first + kTok - 1 <= p_low && (P.window == 0 || first > p_high - (int)P.window);
-                        const int from = P.window ? p - (int)P.window + 1 - first : -1, to = p - first;          // columns the row sees
-                        // 64 columns at a time.  A row whose maximum has been left behind moves it, to a whole power of two: what there is of O, l and of this chunk's P is
-                        // then scaled without rounding.
-                        auto keep_up = [&](int q, float top) {                  // the maximum for half q and all behind it
-                            const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
-                            if (!__any_sync(0xFFFFFFFFu, left_behind)) return;  // (all but once or twice an item)
-                            const float m_new = left_behind ? ceilf(top) : m, gap = m_new - m;
-                            const float less = m == m_new ? 1.0f : gap < 126.0f ? __int_as_float((127 - (int)gap) << 23) : 0.0f;
+                        const int first = c * kTok + (int)i * 64;
+                        const bool whole = first + 63 <= p_low && (P.window == 0 || first > p_high - (int)P.window);
+                        float x[64];
+                        ptx::tmem_ld_32x32b_x32(col, *(uint32_t(*)[32])x);
+                        ptx::tmem_ld_32x32b_x32(col + 32, *(uint32_t(*)[32])(x + 32));
+                        ptx::tmem_ld_wait();
+                        if (!whole) {
+                            const int from = P.window ? p - (int)P.window + 1 - first : -1, to = p - first;      // columns the row sees
+#pragma unroll
+                            for (int j = 0; j < 64; ++j)
+                                if (j < from || j > to) x[j] = -INFINITY;
+                        }
+                        float tops[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) tops[j] = x[16 * j];
+#pragma unroll
+                        for (int j = 1; j < 16; ++j)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], x[16 * k + j]);
+                        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * P.scale_log2;         // (the scale is positive)
+                        const bool left_behind = top > m + kLag || (m == -INFINITY && top > m);
+                        if (__any_sync(0xFFFFFFFFu, left_behind)) {          // once or twice an item
+                            const float m_new = left_behind ? ceilf(top) : m, less = m == m_new ? 1.0f : exp2_fast(m - m_new);
                             m = m_new;
                             l[0] = __fmul2_rn(l[0], make_float2(less, less));
                             l[1] = __fmul2_rn(l[1], make_float2(less, less));
-                            ptx::tmem_st_wait();
-                            const __nv_bfloat162 less2 = __float2bfloat162_rn(less);
-#pragma unroll 1
-                            for (int k = 0; k < 4 * q; ++k) {
-                                uint32_t o[8];
-                                ptx::tmem_ld_32x32b_x8(s_col + 8 * k, o);
-                                ptx::tmem_ld_wait();
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&o[j], less2);
-                                    o[j] = *(const uint32_t*)&v;
-                                }
-                                ptx::tmem_st_32x32b_x8(s_col + 8 * k, o);
+                            // O has to be at rest: the sums of the half before the last are done (these scores were issued behind them), those of the last are waited for
+                            if (i > 0) {
+                                if (!wait(o_step(t), (halves - 1) & 1)) break;
+                                ptx::tc_fence_after_sync();
                             }
 #pragma unroll 1
                             for (int k = 0; i > 0 && k < D / 8; ++k) {
@@ -329,44 +339,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                 for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * less);
                                 ptx::tmem_st_32x32b_x8(o_col + 8 * k, o);
                             }
-                        };
-#pragma unroll 1
-                        for (int q = 0; q < kTok / 64; ++q) {
-                            float x[64];
-                            ptx::tmem_ld_32x32b_x32(s_col + 64 * q, *(uint32_t(*)[32])x);
-                            ptx::tmem_ld_32x32b_x32(s_col + 64 * q + 32, *(uint32_t(*)[32])(x + 32));
-                            ptx::tmem_ld_wait();
-                            if (!whole) {
+                        }
+                        const float minus = m == -INFINITY ? 0.0f : -m;
 #pragma unroll
-                                for (int j = 0; j < 64; ++j)
-                                    if (j < from - 64 * q || j > to - 64 * q) x[j] = -INFINITY;
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t y[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const float2 e = __ffma2_rn(make_float2(x[32 * k + 2 * j], x[32 * k + 2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
+                                const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                                l[j % 2] = __fadd2_rn(l[j % 2], w);
+                                y[j] = pack(w.x, w.y);
                             }
-                            float tops[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) tops[j] = x[16 * j];
-#pragma unroll
-                            for (int j = 1; j < 16; ++j)
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], x[16 * k + j]);
-                            keep_up(q, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * P.scale_log2);      // (the scale is positive)
-                            const float minus = m == -INFINITY ? 0.0f : -m;
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                uint32_t y[16];
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    const float2 e = __ffma2_rn(make_float2(x[32 * k + 2 * j], x[32 * k + 2 * j + 1]), make_float2(P.scale_log2, P.scale_log2), make_float2(minus, minus));
-                                    const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                                    l[j % 2] = __fadd2_rn(l[j % 2], w);
-                                    y[j] = pack(w.x, w.y);
-                                }
-                                ptx::tmem_st_32x32b_x16(s_col + 32 * q + 16 * k, y);          // over columns that have been read
-                            }
+                            ptx::tmem_st_32x32b_x16(col + 16 * k, y);            // over columns that have been read
                         }
                         ptx::tmem_st_wait();
                         ptx::tc_fence_before_sync();
                         __syncwarp();
-                        ptx::mbar_arrive_if(p_full(t), lane == 0);
+                        ptx::mbar_arrive_if(p_full(t, half), lane == 0);
+                        ++halves;
                     }
                     const float sum = (l[0].x + l[0].y) + (l[1].x + l[1].y);
                     if (!wait(o_full(t), o_phase)) break;
@@ -523,50 +514,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             if (left_out != 0xFFFFFFFFu) report(B, kStatusBadPage, left_out);
         } else if (warp == kIssuer) {
             // ------------------------------------------------------------ the products
-            constexpr uint32_t kIdescS = ptx::make_idesc_bf16_f32(kTile, kTok, 0), kIdescO = ptx::make_idesc_bf16_f32(kTile, D, 1);
+            constexpr uint32_t kIdescS = ptx::make_idesc_bf16_f32(kTile, 64, 0), kIdescO = ptx::make_idesc_bf16_f32(kTile, D, 1), kHalf = 64 * 128 / 16;
             const uint32_t issue = ptx::elect_one();
-            uint32_t stage = 0, phase = 0, q_phase = 0, p_phase[2] = {0, 0};
-            auto scores = [&](uint32_t t) {
-                const uint32_t a = ptx::smem_desc_lo(q_smem + t * kTileBytes, 16), b = ptx::smem_desc_lo(k_smem + stage * kTileBytes, 16);
+            uint32_t k_count = 0, v_count = 0, q_phase = 0, p_phase[2] = {0, 0};        // chunks of K and V so far; stages and phases follow from them
+            auto scores = [&](uint32_t t, uint32_t half) {
+                const uint32_t a = ptx::smem_desc_lo(q_smem + t * kTileBytes, 16), b = ptx::smem_desc_lo(k_smem + (k_count & 1) * kTileBytes, 16) + half * kHalf;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t at = (k / 4) * (kPanel / 16) + (k % 4) * 2;
-                    ptx::umma_bf16_ss_if(issue, tmem + kS + t * kTok, a + at, b + at, kIdescS, k > 0);
+                    ptx::umma_bf16_ss_if(issue, tmem + kS + t * kTok + half * 64, a + at, b + at, kIdescS, k > 0);
                 }
-                ptx::umma_commit_if(issue, s_full(t));
+                ptx::umma_commit_if(issue, s_full(t, half));
             };
-            auto sums = [&](uint32_t t, uint32_t v_stage, bool more) {
-                const uint32_t b = ptx::smem_desc_lo(v_smem + v_stage * kTileBytes, kPanel);
+            auto sums = [&](uint32_t t, uint32_t half, bool more) {
+                const uint32_t b = ptx::smem_desc_lo(v_smem + (v_count & 1) * kTileBytes, kPanel) + half * kHalf;
 #pragma unroll
-                for (int k = 0; k < kTok / 16; ++k) ptx::umma_bf16_ts_mn_if(issue, tmem + kO + t * D, tmem + kS + t * kTok + k * 8, b + k * 128, kIdescO, k > 0 || more);
+                for (int k = 0; k < 4; ++k)
+                    ptx::umma_bf16_ts_mn_if(issue, tmem + kO + t * D, tmem + kS + t * kTok + half * 64 + k * 8, b + k * 128, kIdescO, k > 0 || more);
+                ptx::umma_commit_if(issue, o_step(t));
             };
             for (; ok && walk.n; walk.next(P)) {
                 const uint32_t n = walk.n, total = (uint32_t)it.s.rows * P.group;
                 const uint32_t tiles = it.tile * kRows + kTile < total ? 2 : 1;
-                if (!wait(q_full, q_phase)) break;
+                if (!wait(q_full, q_phase) || !wait(k_full(k_count & 1), (k_count >> 1) & 1)) break;
                 q_phase ^= 1;
-                for (uint32_t i = 0; i <= n && ok; ++i) {   // scores of chunk i, sums of chunk i - 1
-                    const uint32_t before = stage ^ 1, before_phase = phase ^ (stage == 0);
-                    if (i < n && !wait(k_full(stage), phase)) break;
-                    if (i > 0 && !wait(v_full(before), before_phase)) break;
-                    ptx::tc_fence_after_sync();
-                    for (uint32_t t = 0; t < tiles && ok; ++t) {
-                        if (i > 0) {
-                            if (!wait(p_full(t), p_phase[t])) break;
-                            p_phase[t] ^= 1;
-                            ptx::tc_fence_after_sync();
-                            sums(t, before, i > 1);
-                            if (i == n) ptx::umma_commit_if(issue, o_full(t));
-                        }
-                        if (i < n) scores(t);
+                ptx::tc_fence_after_sync();
+                for (uint32_t half = 0; half < 2; ++half)
+                    for (uint32_t t = 0; t < tiles; ++t) scores(t, half);
+                ptx::umma_commit_if(issue, k_empty(k_count & 1));
+                ++k_count;
+                if (n == 1) ptx::umma_commit_if(issue, q_empty);
+                for (uint32_t i = 0; i < 2 * n && ok; ++i) {   // sums of half i, then scores of half i + 2 in the same columns
+                    const uint32_t half = i & 1, c = i / 2;
+                    const bool more = c + 1 < n;
+                    if (half == 0) {
+                        if (!wait(v_full(v_count & 1), (v_count >> 1) & 1)) break;
+                        if (more && !wait(k_full(k_count & 1), (k_count >> 1) & 1)) break;
                     }
-                    if (!ok) break;
-                    if (i > 0) ptx::umma_commit_if(issue, v_empty(before));
-                    if (i < n) {
-                        ptx::umma_commit_if(issue, k_empty(stage));
-                        if (i + 1 == n) ptx::umma_commit_if(issue, q_empty);
-                        stage ^= 1;
-                        phase ^= stage == 0;
+                    for (uint32_t t = 0; t < tiles && ok; ++t) {
+                        if (!wait(p_full(t, half), p_phase[t])) break;
+                        p_phase[t] ^= half;
+                        ptx::tc_fence_after_sync();
+                        sums(t, half, i > 0);
+                        if (i + 1 == 2 * n) ptx::umma_commit_if(issue, o_full(t));
+                        if (more) scores(t, half);
+                    }
+                    if (!ok || half == 0) continue;
+                    ptx::umma_commit_if(issue, v_empty(v_count & 1));
+                    ++v_count;
+                    if (more) {
+                        ptx::umma_commit_if(issue, k_empty(k_count & 1));
+                        ++k_count;
+                        if (c + 2 == n) ptx::umma_commit_if(issue, q_empty);
                     }
                 }
             }
