@@ -22,7 +22,7 @@ constexpr int kTok = 128, kRows = 256, kTile = 128;
 constexpr int kDequantWarps = 4;
 constexpr int kThreads = (12 + kDequantWarps) * 32;
 constexpr uint32_t kIssuer = 8 + kDequantWarps;           // the warp that issues the products
-constexpr uint32_t kItemUnits = 2;                        // an item's queries, results and idle times in chunks' time (10600 of 4400 clocks, measured on a prompt of 8192 tokens)
+constexpr uint32_t kItemUnits = 3;                        // an item's queries, results and idle times in chunks' time (10600 of 3800 clocks, measured on a prompt of 8192 tokens)
 constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed what a row's weights are taken against
 
 template <int D> constexpr uint32_t tile_bytes() { return kTile * D * 2; }
@@ -616,8 +616,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 }
 
 // Joins the parts of the items whose chunks several CTAs of the launch before worked on.  Block (c, z): the item that the boundary before CTA c cuts, if c is the first one
-// to cut it; z: a slice of its rows.  A thread has a row and an eighth of its numbers.
-constexpr int kJoinRows = 32, kJoinThreads = kJoinRows * 8;
+// to cut it; z: a slice of its rows.  A thread has a row and a quarter of its numbers.
+constexpr int kJoinRows = 64, kJoinThreads = kJoinRows * 4;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) kv4_prompt_join_kernel(const __grid_constant__ Params G) {
     const Attention& P = G.P;
@@ -631,14 +631,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_prompt_join_kernel(const __g
     if (at <= chunk0 || start_of(c - 1, cut.units, runs) > chunk0) return;      // all chunks lie in this run, or an earlier boundary cuts them
     if (cut.tile * kRows + z * kJoinRows >= cut.total) return;
     const uint32_t r = z * kJoinRows + threadIdx.x % kJoinRows, part = threadIdx.x / kJoinRows, row = cut.tile * kRows + r;
-    constexpr int kEach = D / 8;
+    constexpr int kEach = D / 4;
     auto record = [&](uint32_t i) { return G.records + (uint64_t)(2 * i + (i == c - 1 ? 1 : 0)) * record_floats<D>() + r; };
     float top = -INFINITY, l = 0.0f, sum[kEach] = {};
     uint32_t parts_end = c;                                // the run behind the last one with a part
     while (parts_end < runs && start_of(parts_end, cut.units, runs) < behind) ++parts_end;
     for (uint32_t i = c - 1; i < parts_end; ++i) top = fmaxf(top, record(i)[D * kRows]);
     const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll 2
+#pragma unroll 1
     for (uint32_t i = c - 1; i < parts_end; ++i) {
         const float* rec = record(i);
         const float w = exp2_fast(rec[D * kRows] - base);
