@@ -52,14 +52,16 @@ __device__ __forceinline__ Sequence sequence(const Batch& B, uint32_t b) {
     return s;
 }
 
-// The sequence that row r belongs to; false where it belongs to none.
+// The sequence that row r belongs to; false where it belongs to none.  By a whole warp, with the same answer in every lane: 33 parts are told apart with one load.
 __device__ __forceinline__ bool sequence_of_row(const Batch& B, uint32_t r, uint32_t* index, Sequence* s) {
     uint32_t b;
     if (B.row_start) {
         uint32_t lo = 0, hi = B.n_seqs;              // the last b with row_start[b] <= r (any index in range where the array is not ascending)
         while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if ((int64_t)B.row_start[mid] <= (int64_t)r) lo = mid; else hi = mid;
+            const uint32_t step = (hi - lo + 31) / 32, at = lo + (threadIdx.x & 31) * step;
+            const uint32_t below = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && (int64_t)B.row_start[at] <= (int64_t)r));
+            lo += below ? (below - 1) * step : 0;
+            hi = min(hi, lo + step);
         }
         b = lo;
     } else {

@@ -65,21 +65,33 @@ struct Append {
     uint32_t end0, end1;                    // first pair of the second and of the third axis
     uint32_t n_axes;
     bool interleaved;
+    uint32_t per_warp;                      // heads of a row that one warp takes
 };
 
+// Eight numbers as they lie in memory, and as f32: apart, so that a load is not waited for where it is issued.
+template <bool F32> struct Eight { uint4 w[F32 ? 2 : 1]; };
 template <bool F32>
-__device__ __forceinline__ void load8(float (&x)[8], const void* base, uint64_t at) {
+__device__ __forceinline__ Eight<F32> load8(const void* base, uint64_t at) {
+    Eight<F32> x;
+    const uint4* p = (const uint4*)((const char*)base + at * (F32 ? 4 : 2));
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) x.w[i] = p[i];
+    return x;
+}
+template <bool F32>
+__device__ __forceinline__ void unpack8(float (&y)[8], const Eight<F32>& x) {
     if constexpr (F32) {
-        const float4* p = (const float4*)((const float*)base + at);
-        const float4 a = p[0], b = p[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            y[4 * i] = __uint_as_float(x.w[i].x); y[4 * i + 1] = __uint_as_float(x.w[i].y);
+            y[4 * i + 2] = __uint_as_float(x.w[i].z); y[4 * i + 3] = __uint_as_float(x.w[i].w);
+        }
     } else {
-        const uint4 w = *(const uint4*)((const __nv_bfloat16*)base + at);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t u[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(u[i] << 16);
-            x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+            y[2 * i] = __uint_as_float(u[i] << 16);
+            y[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
         }
     }
 }
@@ -91,19 +103,43 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
     return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
 }
 
-// A group of D / 8 lanes takes one head of one row, eight numbers a lane: it turns them, and either rounds them to bf16 (queries) or finds the row's
-// range and cuts it to four bits, a 32-bit word of codes a lane.
+// The step of a row: the smallest bf16 not below range / 15, the quotient rounded to f32.  15 b is exact for a bf16 b, and where it is not the range the two are at least a unit
+// in the last place of the range apart, which is more than half a unit of the quotient: the rounded quotient is above b exactly where the range is above 15 b.  So a product
+// with 1 / 15 finds the place to within a neighbour, and exact comparisons the step.
+__device__ __forceinline__ float step_of(float range) {
+    const int up = __float_as_int(-bf16_down(-(range * (1.0f / 15.0f))));
+    float step = __int_as_float(up);
+    const float below = __int_as_float(up - 0x10000);
+    if (up >= 0x10000 && fmaf(-15.0f, below, range) <= 0.0f) step = below;
+    if (fmaf(-15.0f, step, range) > 0.0f) step = __int_as_float(up + 0x10000);
+    return step < 1.17549435e-38f ? 0.0f : step;
+}
+// rint(d / step), the quotient rounded to f32, for 0 <= d <= 15.5 step and a bf16 step with `inverse` near 1 / step.  d - c step is exact (a multiple of d's last place, and no
+// larger than d), and where it is not half a step it differs from it by more than the quotient's rounding: comparisons with half a step say where the quotient lies, and ties go to the even code.
+__device__ __forceinline__ uint32_t code_of(float d, float step, float inverse) {
+    const float near = fmaf(d, inverse, 12582912.0f);      // 1.5 * 2^23: the whole number in the low bits
+    uint32_t c = __float_as_uint(near) & 31;
+    const float rest = fmaf(-(near - 12582912.0f), step, d), half = 0.5f * step;
+    const bool odd = c & 1;
+    if (rest > half || (rest == half && odd)) ++c;
+    if (rest < -half || (rest == -half && odd)) --c;
+    return min(c, 15u);
+}
+
+// A warp takes a row, or `per_warp` of its heads where rows are few: sequence, token, page, positions and the lane's cosines and sines are found once for all of them.  A head is
+// D / 8 lanes wide, eight numbers a lane, so that a warp works on several at a time and asks for kAhead times as many before it needs them.  A lane turns its numbers, and
+// either rounds them to bf16 (queries) or finds the row's range with its group and cuts them to four bits, a 32-bit word of codes a lane.  HBM bound: 8192 rows of 32 query
+// and 8 key/value heads of 128, bf16, three axes, are 157 MB.
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Append P) {
-    constexpr uint32_t kLanes = D / 8;
+    constexpr uint32_t kLanes = D / 8, kAtOnce = 32 / kLanes, kAhead = 4;
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     const Batch& B = P.B;
-    const uint32_t heads = P.n_q_heads + 2 * B.n_kv_heads;
-    const uint64_t unit = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
-    const uint32_t e = threadIdx.x % kLanes;
-    const uint32_t group_mask = (uint32_t)((1ull << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes);
-    const uint32_t r = (uint32_t)(unit / heads), h = (uint32_t)(unit % heads);
+    const uint32_t heads = P.n_q_heads + 2 * B.n_kv_heads, parts = (heads + P.per_warp - 1) / P.per_warp;
+    const uint64_t unit = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x % 32, e = lane % kLanes, sub = lane / kLanes;
+    const uint32_t r = (uint32_t)(unit / parts), h0 = (uint32_t)(unit % parts) * P.per_warp, h1 = min(heads, h0 + P.per_warp);
     if (r >= B.n_rows) return;
     uint32_t b;
     Sequence s;
@@ -111,135 +147,208 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
     const int token = s.len - s.rows + ((int)r - s.first_row);
     if (token < 0) return;
 
-    // the row's positions
-    int pos[3] = {token, token, token};
+    // the row's positions, and the turns of the lane's numbers: (a, b) of pair i are numbers i and i + rot_dim / 2, or 2 i and 2 i + 1 of the lane itself
+    float2 turn[8] = {};
+    bool turns = false, second = false;
+    uint32_t from = lane;                                  // the lane that has the other numbers of the pairs
     if (P.rope) {
+        int pos[3] = {token, token, token};
         if (P.positions)
             for (uint32_t a = 0; a < P.n_axes; ++a) pos[a] = P.positions[(uint64_t)a * B.n_rows + r];
         bool bad = false;
         for (uint32_t a = 0; a < P.n_axes; ++a) bad |= (uint32_t)pos[a] >= P.n_positions;
-        if (bad) {
-            if (e == 0) report(B, kStatusBadPosition, r);
+        if (bad) {                                         // the row is left out as a whole, its values too
+            if (lane == 0) report(B, kStatusBadPosition, r);
             return;
         }
-    }
-    float x[8];
-    const bool is_q = h < P.n_q_heads, is_k = !is_q && h < P.n_q_heads + B.n_kv_heads;
-    const uint32_t head = is_q ? h : is_k ? h - P.n_q_heads : h - P.n_q_heads - B.n_kv_heads;
-    if (is_q) load8<F32>(x, P.q, r * P.q_stride + head * D + 8 * e);
-    else if (is_k) load8<F32>(x, P.k, r * P.k_stride + head * D + 8 * e);
-    else load8<F32>(x, P.v, r * P.v_stride + head * D + 8 * e);
-
-    if ((is_q || is_k) && P.rope) {
-        const uint32_t pairs = P.rot_dim / 2;
-        auto cs = [&](uint32_t pair) {
-            const int p = pair < P.end0 ? pos[0] : pair < P.end1 ? pos[1] : pos[2];
-            return P.rope[(uint64_t)p * pairs + pair];
-        };
-        if (P.interleaved) {
-            if (e < P.rot_dim / 8) {
+        const uint32_t pairs = P.rot_dim / 2, away = P.rot_dim / 16;       // `away`: lanes between the two numbers of a pair
+        turns = e < 2 * away;
+        second = !P.interleaved && turns && e >= away;
+        if (!P.interleaved && turns) from = second ? lane - away : lane + away;
+        const uint32_t first_pair = P.interleaved ? 4 * e : 8 * (second ? e - away : e);
+        if (turns && h0 < P.n_q_heads + B.n_kv_heads) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 t = cs(e * 4 + i);
-                    const float u = x[2 * i], w = x[2 * i + 1];
-                    x[2 * i] = __fsub_rn(__fmul_rn(u, t.x), __fmul_rn(w, t.y));
-                    x[2 * i + 1] = __fadd_rn(__fmul_rn(w, t.x), __fmul_rn(u, t.y));
+            for (int i = 0; i < 8; i += 2) {
+                if (P.interleaved && i >= 4) break;
+                const uint32_t pair = first_pair + i;
+                if (P.n_axes == 1) {                       // (two pairs lie on one 16-byte boundary)
+                    const float4 t = *(const float4*)(P.rope + (uint64_t)pos[0] * pairs + pair);
+                    turn[i] = make_float2(t.x, t.y);
+                    turn[i + 1] = make_float2(t.z, t.w);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int p = pair + j < P.end0 ? pos[0] : pair + j < P.end1 ? pos[1] : pos[2];
+                        turn[i + j] = P.rope[(uint64_t)p * pairs + pair + j];
+                    }
                 }
+            }
+        }
+    }
+    // (first and second number of a pair differ in the sign of the sine's term alone)
+    if (!P.interleaved && !second) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) turn[i].y = -turn[i].y;
+    }
+    auto rotate = [&](float (&y)[8]) {
+        if (P.interleaved) {
+            if (!turns) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = y[2 * i], w = y[2 * i + 1];
+                y[2 * i] = __fsub_rn(__fmul_rn(u, turn[i].x), __fmul_rn(w, turn[i].y));
+                y[2 * i + 1] = __fadd_rn(__fmul_rn(w, turn[i].x), __fmul_rn(u, turn[i].y));
             }
         } else {
-            const uint32_t away = P.rot_dim / 16;          // lanes between the two numbers of a pair
-            const bool first = e < away, second = !first && e < 2 * away;
-            const uint32_t from = threadIdx.x % 32 - e + (first ? e + away : second ? e - away : e);
-            float other[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(group_mask, x[i], from);
-            if (first || second) {
+            for (int i = 0; i < 8; ++i) {
+                const float other = __shfl_sync(0xFFFFFFFFu, y[i], from), z = __fadd_rn(__fmul_rn(y[i], turn[i].x), __fmul_rn(other, turn[i].y));
+                if (turns) y[i] = z;
+            }
+        }
+    };
+
+    // queries
+    const uint32_t q1 = min(h1, P.n_q_heads);
+    if (h0 < q1) {
+        const uint64_t in = r * P.q_stride + (h0 + sub) * D + 8 * e;
+        __nv_bfloat16* out = P.q_out + r * P.q_out_stride + (h0 + sub) * D + 8 * e;
+        for (uint32_t h = 0; h < q1 - h0; h += kAhead * kAtOnce) {
+            Eight<F32> x[kAhead];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 t = cs((first ? e : e - away) * 8 + i);
-                    x[i] = first ? __fsub_rn(__fmul_rn(x[i], t.x), __fmul_rn(other[i], t.y)) : __fadd_rn(__fmul_rn(x[i], t.x), __fmul_rn(other[i], t.y));
-                }
+            for (uint32_t a = 0; a < kAhead; ++a)
+                if (h + a * kAtOnce + sub < q1 - h0) x[a] = load8<F32>(P.q, in + (h + a * kAtOnce) * D);
+#pragma unroll
+            for (uint32_t a = 0; a < kAhead; ++a) {
+                if (h + a * kAtOnce >= q1 - h0) break;
+                float y[8];
+                unpack8<F32>(y, x[a]);
+                if (P.rope) rotate(y);
+                if (h + a * kAtOnce + sub < q1 - h0) *(uint4*)(out + (h + a * kAtOnce) * D) = pack8(y);
             }
         }
     }
-    if (is_q) {
-        *(uint4*)(P.q_out + r * P.q_out_stride + head * D + 8 * e) = pack8(x);
-        return;
-    }
-    // the range
-    float mn = x[0], mx = x[0];
-    bool bad = false;
+    // keys, then values
+    const uint32_t k0 = max(h0, P.n_q_heads) - P.n_q_heads, k1 = h1 - P.n_q_heads;
+    if (h1 <= P.n_q_heads || k0 >= k1) return;
+    uint8_t* block = block_of<D>(B, b, (uint32_t)token >> B.page_log2, 0);
+    if (!block) return;
+    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1), block_bytes = (D + 8) << B.page_log2;
+    const uint32_t group = (uint32_t)((1ull << kLanes) - 1) << (sub * kLanes);
+    for (uint32_t h = k0; h < k1; h += kAhead * kAtOnce) {
+        Eight<F32> x[kAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        mn = fminf(mn, x[i]);
-        mx = fmaxf(mx, x[i]);
-        bad |= !(fabsf(x[i]) < __int_as_float(0x7F800000));
-    }
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            const uint32_t at = h + a * kAtOnce + sub;
+            const bool is_k = at < B.n_kv_heads;
+            if (at < k1) x[a] = load8<F32>(is_k ? P.k : P.v, is_k ? r * P.k_stride + at * D + 8 * e : r * P.v_stride + (at - B.n_kv_heads) * D + 8 * e);
+        }
 #pragma unroll
-    for (uint32_t d = 1; d < kLanes; d *= 2) {
-        mn = fminf(mn, __shfl_xor_sync(group_mask, mn, d));
-        mx = fmaxf(mx, __shfl_xor_sync(group_mask, mx, d));
-    }
-    bad = (__ballot_sync(group_mask, bad) & group_mask) != 0;
-    const float low = bf16_down(mn), range = __fsub_rn(mx, low);
-    bad |= !(range < __int_as_float(0x7F800000));
-    float step = -bf16_down(-__fdiv_rn(range, 15.0f));
-    if (step < 1.17549435e-38f) step = 0.0f;
-    uint32_t codes = 0;
-    if (!bad && step > 0.0f) {
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            if (h + a * kAtOnce >= k1) break;
+            const uint32_t at = h + a * kAtOnce + sub;
+            const bool is_k = at < B.n_kv_heads;
+            float y[8];
+            unpack8<F32>(y, x[a]);
+            if (P.rope && h + a * kAtOnce < B.n_kv_heads) {
+                float z[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], low), step)), 0.0f), 15.0f);
-            codes |= (uint32_t)c << code_shift(i);
+                for (int i = 0; i < 8; ++i) z[i] = y[i];
+                rotate(z);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = is_k ? z[i] : y[i];
+            }
+            // the range
+            float mn = y[0], mx = y[0];
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                mn = fminf(mn, y[i]);
+                mx = fmaxf(mx, y[i]);
+                bad |= !(fabsf(y[i]) < __int_as_float(0x7F800000));
+            }
+#pragma unroll
+            for (uint32_t d = 1; d < kLanes; d *= 2) {
+                mn = fminf(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, d));
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+            }
+            bad = (__ballot_sync(0xFFFFFFFFu, bad) & group) != 0;
+            const float low = bf16_down(mn), range = __fsub_rn(mx, low);
+            bad |= !(range < __int_as_float(0x7F800000));
+            const float step = step_of(range);
+            uint32_t codes = 0;
+            if (!bad && step > 0.0f) {
+                float inverse;
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(step));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) codes |= code_of(__fsub_rn(y[i], low), step, inverse) << code_shift(i);
+            }
+            if (at < k1) {
+                const uint32_t which = is_k ? 0 : 1;
+                uint8_t* to = block + (uint64_t)(is_k ? at : at - B.n_kv_heads) * block_bytes;
+                *(uint32_t*)(to + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e) = codes;
+                if (e == 0)
+                    *(uint32_t*)(to + params_at<D>(B.page_log2, which) + 4 * slot) = bad ? 0x7FC07FC0u : (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
+            }
         }
     }
-    uint8_t* block = block_of<D>(B, b, (uint32_t)token >> B.page_log2, head);
-    if (!block) return;
-    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1), which = is_k ? 0 : 1;
-    *(uint32_t*)(block + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e) = codes;
-    if (e == 0)
-        *(uint32_t*)(block + params_at<D>(B.page_log2, which) + 4 * slot) =
-            bad ? 0x7FC07FC0u : (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
 }
 
 struct Dequant {
     Batch B;
     __nv_bfloat16 *k_out, *v_out;
     uint64_t k_stride, v_stride;
+    uint32_t per_warp;
 };
 
-// A group of D / 8 lanes reads one head of one row of the keys or of the values, a word of eight codes a lane.
+// A warp takes a row, or `per_warp` of its 2 n_kv_heads rows of keys and values: a word of eight codes a lane, D / 8 lanes to a row, kAhead loads under way.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_dequant_kernel(const __grid_constant__ Dequant P) {
-    constexpr uint32_t kLanes = D / 8;
+    constexpr uint32_t kLanes = D / 8, kAtOnce = 32 / kLanes, kAhead = 4;
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     const Batch& B = P.B;
-    const uint64_t unit = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
-    const uint32_t e = threadIdx.x % kLanes;
-    const uint32_t r = (uint32_t)(unit / (2 * B.n_kv_heads)), h = (uint32_t)(unit % (2 * B.n_kv_heads));
+    const uint32_t first = P.k_out ? 0 : B.n_kv_heads, heads = P.v_out ? 2 * B.n_kv_heads : B.n_kv_heads;      // keys, then values: those that are asked for
+    const uint32_t parts = (heads - first + P.per_warp - 1) / P.per_warp;
+    const uint64_t unit = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x % 32, e = lane % kLanes, sub = lane / kLanes;
+    const uint32_t r = (uint32_t)(unit / parts), h0 = first + (uint32_t)(unit % parts) * P.per_warp, h1 = min(heads, h0 + P.per_warp);
     if (r >= B.n_rows) return;
-    const uint32_t which = h < B.n_kv_heads ? 0 : 1, head = which ? h - B.n_kv_heads : h;
-    __nv_bfloat16* out = which ? P.v_out : P.k_out;
-    if (!out) return;
     uint32_t b;
     Sequence s;
     if (!sequence_of_row(B, r, &b, &s)) return;
     const int token = s.len - s.rows + ((int)r - s.first_row);
-    uint4* to = (uint4*)(out + r * (which ? P.v_stride : P.k_stride) + head * D + 8 * e);
-    if (token < 0) {
-        *to = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    const uint8_t* block = block_of<D>(B, b, (uint32_t)token >> B.page_log2, head);
-    if (!block) return;
-    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1);
-    const uint32_t w = *(const uint32_t*)(block + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e);
-    const uint32_t p = *(const uint32_t*)(block + params_at<D>(B.page_log2, which) + 4 * slot);
-    float x[8];
+    const uint8_t* block = token < 0 ? nullptr : block_of<D>(B, b, (uint32_t)token >> B.page_log2, 0);
+    if (token >= 0 && !block) return;
+    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1), block_bytes = (D + 8) << B.page_log2;
+    for (uint32_t h = h0; h < h1; h += kAhead * kAtOnce) {
+        uint32_t w[kAhead], p[kAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(__fmul_rn((float)((w >> code_shift(i)) & 15), param_step(p)), param_low(p));
-    *to = pack8(x);
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            const uint32_t at = h + a * kAtOnce + sub, which = at < B.n_kv_heads ? 0 : 1, head = which ? at - B.n_kv_heads : at;
+            w[a] = p[a] = 0;
+            if (at < h1 && block) {
+                const uint8_t* of = block + (uint64_t)head * block_bytes;
+                w[a] = *(const uint32_t*)(of + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e);
+                p[a] = *(const uint32_t*)(of + params_at<D>(B.page_log2, which) + 4 * slot);
+            }
+        }
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            const uint32_t at = h + a * kAtOnce + sub, which = at < B.n_kv_heads ? 0 : 1, head = which ? at - B.n_kv_heads : at;
+            if (at >= h1) continue;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(__fmul_rn((float)((w[a] >> code_shift(i)) & 15), param_step(p[a])), param_low(p[a]));
+            *(uint4*)((which ? P.v_out : P.k_out) + r * (which ? P.v_stride : P.k_stride) + head * D + 8 * e) = pack8(x);
+        }
+    }
+}
+
+// Head rows for one warp: all of a row's where there are warps enough without it (a few for each of the 48 or so places of an SM), else fewer.
+uint32_t heads_per_warp(uint32_t rows, uint32_t heads, uint32_t at_once, uint32_t sms) {
+    const uint64_t want = (uint64_t)rows * heads / (64ull * sms);
+    return (uint32_t)std::min<uint64_t>(heads, std::max<uint64_t>(at_once, want / at_once * at_once));
 }
 
 }  // namespace
@@ -320,8 +429,9 @@ int t0_kv4_append(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_append
     if ((rc = check_rt(rt)) != T0_OK) return rc;
     P.B.status = rt->d_status + 1;
     DeviceGuard guard(rt->device);
-    const uint64_t threads = (uint64_t)batch->n_rows * (a.n_q_heads + 2 * batch->n_kv_heads) * (D / 8);
-    const uint64_t grid = (threads + 255) / 256;
+    const uint32_t heads = a.n_q_heads + 2 * batch->n_kv_heads;
+    P.per_warp = heads_per_warp(batch->n_rows, heads, 256 / D, (uint32_t)rt->sm_count);
+    const uint64_t grid = ((uint64_t)batch->n_rows * ceil_div(heads, P.per_warp) + 7) / 8;
     if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "too many rows and heads for one launch");
     auto go = [&](auto kernel) { return gemm::launch_pdl(kernel, (uint32_t)grid, 256, 0, rt->stream, P); };
     const cudaError_t e = D == 64 ? (a.in_f32 ? go(kv4_append_kernel<64, true>) : go(kv4_append_kernel<64, false>))
@@ -350,7 +460,9 @@ int t0_kv4_dequant(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_dequa
     if ((rc = check_rt(rt)) != T0_OK) return rc;
     P.B.status = rt->d_status + 1;
     DeviceGuard guard(rt->device);
-    const uint64_t grid = ((uint64_t)batch->n_rows * 2 * batch->n_kv_heads * (D / 8) + 255) / 256;
+    const uint32_t heads = (a.k_out && a.v_out ? 2 : 1) * batch->n_kv_heads;
+    P.per_warp = heads_per_warp(batch->n_rows, heads, 256 / D, (uint32_t)rt->sm_count);
+    const uint64_t grid = ((uint64_t)batch->n_rows * ceil_div(heads, P.per_warp) + 7) / 8;
     if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "too many rows and heads for one launch");
     const cudaError_t e = D == 64 ? gemm::launch_pdl(kv4_dequant_kernel<64>, (uint32_t)grid, 256, 0, rt->stream, P)
                                   : gemm::launch_pdl(kv4_dequant_kernel<128>, (uint32_t)grid, 256, 0, rt->stream, P);
