@@ -114,25 +114,45 @@ __device__ __forceinline__ float step_of(float range) {
     if (fmaf(-15.0f, step, range) > 0.0f) step = __int_as_float(up + 0x10000);
     return step < 1.17549435e-38f ? 0.0f : step;
 }
-// rint(d / step), the quotient rounded to f32, for 0 <= d <= 15.5 step and a bf16 step with `inverse` near 1 / step.  d - c step is exact (a multiple of d's last place, and no
-// larger than d), and where it is not half a step it differs from it by more than the quotient's rounding: comparisons with half a step say where the quotient lies, and ties go to the even code.
-__device__ __forceinline__ uint32_t code_of(float d, float step, float inverse) {
-    const float near = fmaf(d, inverse, 12582912.0f);      // 1.5 * 2^23: the whole number in the low bits
-    uint32_t c = __float_as_uint(near) & 31;
-    const float rest = fmaf(-(near - 12582912.0f), step, d), half = 0.5f * step;
-    const bool odd = c & 1;
-    if (rest > half || (rest == half && odd)) ++c;
-    if (rest < -half || (rest == -half && odd)) --c;
-    return min(c, 15u);
+// The codes of eight numbers, packed: rint((x - low) / step), the quotient rounded to f32, for a bf16 step with `inverse` near 1 / step.  With d = x - low and c near d / step,
+// d - c step is exact (a multiple of d's last place, and no larger than d); where it is not half a step it differs from half a step by more than the quotient's rounding.  So c
+// is the code where that rest is below half a step; where it is not (ties are common in rows of bf16), the comparison says which neighbour is, and a tie goes to the even one.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, float step, float inverse) {
+    const float half = 0.5f * step;
+    float near[8], rest[8], worst = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float d = __fsub_rn(x[i], low);
+        near[i] = fmaf(d, inverse, 12582912.0f);           // 1.5 * 2^23: the whole number in the low bits
+        rest[i] = fmaf(-(near[i] - 12582912.0f), step, d);
+        worst = fmaxf(worst, fabsf(rest[i]));
+    }
+    if (worst >= half) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool odd = __float_as_uint(near[i]) & 1;
+            if (rest[i] > half || (rest[i] == half && odd)) near[i] += 1.0f;
+            if (rest[i] < -half || (rest[i] == -half && odd)) near[i] -= 1.0f;
+            near[i] = fminf(near[i], 12582912.0f + 15.0f);
+        }
+    }
+    uint32_t codes = 0, bias = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        codes += __float_as_uint(near[i]) << code_shift(i);
+        bias += 0x4B400000u << code_shift(i);
+    }
+    return codes - bias;
 }
 
 // A warp takes a row, or `per_warp` of its heads where rows are few: sequence, token, page, positions and the lane's cosines and sines are found once for all of them.  A head is
-// D / 8 lanes wide, eight numbers a lane, so that a warp works on several at a time and asks for kAhead times as many before it needs them.  A lane turns its numbers, and
-// either rounds them to bf16 (queries) or finds the row's range with its group and cuts them to four bits, a 32-bit word of codes a lane.  HBM bound: 8192 rows of 32 query
-// and 8 key/value heads of 128, bf16, three axes, are 157 MB.
+// D / 8 lanes wide, eight numbers a lane, so that a warp works on several at a time and asks for the next ones before it needs them.  A lane turns its numbers, and
+// either rounds them to bf16 (queries) or finds the row's range with its group and cuts them to four bits, a 32-bit word of codes a lane.  8192 rows of 32 query and
+// 8 key/value heads of 128, bf16, three axes, are 157 MB (24 us); it takes 57 us, bound by its instructions (about 4400 a row, half of them the range and the codes) at the 24 warps
+// an SM holds: 3 blocks of 80 registers and two loads ahead measured 71 us with the read-out, 4 blocks 68 to 76, four loads ahead 70 (and 13 instead of 10 us at 256 rows).
 template <int D, bool F32>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Append P) {
-    constexpr uint32_t kLanes = D / 8, kAtOnce = 32 / kLanes, kAhead = 4;
+__global__ void __launch_bounds__(256, 3) kv4_append_kernel(const __grid_constant__ Append P) {
+    constexpr uint32_t kLanes = D / 8, kAtOnce = 32 / kLanes, kAhead = 2;
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     const Batch& B = P.B;
@@ -146,6 +166,17 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
     if (!sequence_of_row(B, r, &b, &s)) return;
     const int token = s.len - s.rows + ((int)r - s.first_row);
     if (token < 0) return;
+
+    // the first loads, before the chain of lookups that the turns need; each is followed by the next one to take its place
+    constexpr uint32_t kSize = F32 ? 4 : 2;
+    const char* const q_in = (const char*)P.q + (r * P.q_stride + 8 * e) * kSize;
+    const char* const k_in = (const char*)P.k + (r * P.k_stride + 8 * e) * kSize - (uint64_t)P.n_q_heads * (D * kSize);
+    const char* const v_in = (const char*)P.v + (r * P.v_stride + 8 * e) * kSize - (uint64_t)(P.n_q_heads + B.n_kv_heads) * (D * kSize);
+    auto load = [&](uint32_t h) { return load8<F32>(h < P.n_q_heads ? q_in : h < P.n_q_heads + B.n_kv_heads ? k_in : v_in, h * D); };
+    Eight<F32> x[kAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a)
+        if (h0 + a * kAtOnce + sub < h1) x[a] = load(h0 + a * kAtOnce + sub);
 
     // the row's positions, and the turns of the lane's numbers: (a, b) of pair i are numbers i and i + rot_dim / 2, or 2 i and 2 i + 1 of the lane itself
     float2 turn[8] = {};
@@ -190,6 +221,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
 #pragma unroll
         for (int i = 0; i < 8; ++i) turn[i].y = -turn[i].y;
     }
+    const bool whole_turn = P.rot_dim == D;                // (the same for the whole launch: no choice lane by lane)
     auto rotate = [&](float (&y)[8]) {
         if (P.interleaved) {
             if (!turns) return;
@@ -200,79 +232,60 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
                 y[2 * i + 1] = __fadd_rn(__fmul_rn(w, turn[i].x), __fmul_rn(u, turn[i].y));
             }
         } else {
+            // two at a time: products and sum are rounded one by one all the same
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float other = __shfl_sync(0xFFFFFFFFu, y[i], from), z = __fadd_rn(__fmul_rn(y[i], turn[i].x), __fmul_rn(other, turn[i].y));
-                if (turns) y[i] = z;
+            for (int i = 0; i < 8; i += 2) {
+                const float2 other = make_float2(__shfl_sync(0xFFFFFFFFu, y[i], from), __shfl_sync(0xFFFFFFFFu, y[i + 1], from));
+                const float2 z = __fadd2_rn(__fmul2_rn(make_float2(y[i], y[i + 1]), make_float2(turn[i].x, turn[i + 1].x)), __fmul2_rn(other, make_float2(turn[i].y, turn[i + 1].y)));
+                if (whole_turn || turns) {
+                    y[i] = z.x;
+                    y[i + 1] = z.y;
+                }
             }
         }
     };
 
-    // queries
-    const uint32_t q1 = min(h1, P.n_q_heads);
-    if (h0 < q1) {
-        const uint64_t in = r * P.q_stride + (h0 + sub) * D + 8 * e;
-        __nv_bfloat16* out = P.q_out + r * P.q_out_stride + (h0 + sub) * D + 8 * e;
-        for (uint32_t h = 0; h < q1 - h0; h += kAhead * kAtOnce) {
-            Eight<F32> x[kAhead];
-#pragma unroll
-            for (uint32_t a = 0; a < kAhead; ++a)
-                if (h + a * kAtOnce + sub < q1 - h0) x[a] = load8<F32>(P.q, in + (h + a * kAtOnce) * D);
-#pragma unroll
-            for (uint32_t a = 0; a < kAhead; ++a) {
-                if (h + a * kAtOnce >= q1 - h0) break;
-                float y[8];
-                unpack8<F32>(y, x[a]);
-                if (P.rope) rotate(y);
-                if (h + a * kAtOnce + sub < q1 - h0) *(uint4*)(out + (h + a * kAtOnce) * D) = pack8(y);
-            }
-        }
-    }
-    // keys, then values
-    const uint32_t k0 = max(h0, P.n_q_heads) - P.n_q_heads, k1 = h1 - P.n_q_heads;
-    if (h1 <= P.n_q_heads || k0 >= k1) return;
-    uint8_t* block = block_of<D>(B, b, (uint32_t)token >> B.page_log2, 0);
-    if (!block) return;
+    uint8_t* block = h1 > P.n_q_heads ? block_of<D>(B, b, (uint32_t)token >> B.page_log2, 0) : nullptr;
     const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1), block_bytes = (D + 8) << B.page_log2;
-    const uint32_t group = (uint32_t)((1ull << kLanes) - 1) << (sub * kLanes);
-    for (uint32_t h = k0; h < k1; h += kAhead * kAtOnce) {
-        Eight<F32> x[kAhead];
+    const uint32_t group = (uint32_t)((1ull << kLanes) - 1) << (sub * kLanes), keys_end = P.n_q_heads + B.n_kv_heads;
+    __nv_bfloat16* out = P.q_out + r * P.q_out_stride + 8 * e;
+    for (uint32_t h = h0; h < h1; h += kAhead * kAtOnce) {
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
-            const uint32_t at = h + a * kAtOnce + sub;
-            const bool is_k = at < B.n_kv_heads;
-            if (at < k1) x[a] = load8<F32>(is_k ? P.k : P.v, is_k ? r * P.k_stride + at * D + 8 * e : r * P.v_stride + (at - B.n_kv_heads) * D + 8 * e);
-        }
-#pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a) {
-            if (h + a * kAtOnce >= k1) break;
-            const uint32_t at = h + a * kAtOnce + sub;
-            const bool is_k = at < B.n_kv_heads;
+            const uint32_t from_h = h + a * kAtOnce, to_h = from_h + kAtOnce, at = from_h + sub;     // the heads that the warp has now, and this lane's
+            if (from_h >= h1) break;
             float y[8];
             unpack8<F32>(y, x[a]);
-            if (P.rope && h + a * kAtOnce < B.n_kv_heads) {
+            if (at + kAhead * kAtOnce < h1) x[a] = load(at + kAhead * kAtOnce);
+            if (P.rope && to_h <= keys_end) {
+                rotate(y);
+            } else if (P.rope && from_h < keys_end) {          // keys and values at once
                 float z[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z[i] = y[i];
                 rotate(z);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = is_k ? z[i] : y[i];
+                for (int i = 0; i < 8; ++i) y[i] = at < keys_end ? z[i] : y[i];
             }
-            // the range
-            float mn = y[0], mx = y[0];
-            bool bad = false;
+            if (from_h < P.n_q_heads) {
+                if (at < min(h1, P.n_q_heads)) *(uint4*)(out + at * D) = pack8(y);
+                if (to_h <= P.n_q_heads) continue;
+            }
+            if (!block) continue;
+            // the range; zero times an infinity or a NaN shows it
+            float mn = y[0], mx = y[0], zero = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 mn = fminf(mn, y[i]);
                 mx = fmaxf(mx, y[i]);
-                bad |= !(fabsf(y[i]) < __int_as_float(0x7F800000));
+                zero = fmaf(y[i], 0.0f, zero);
             }
 #pragma unroll
             for (uint32_t d = 1; d < kLanes; d *= 2) {
                 mn = fminf(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, d));
                 mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
             }
-            bad = (__ballot_sync(0xFFFFFFFFu, bad) & group) != 0;
+            bool bad = (__ballot_sync(0xFFFFFFFFu, !(zero == 0.0f)) & group) != 0;
             const float low = bf16_down(mn), range = __fsub_rn(mx, low);
             bad |= !(range < __int_as_float(0x7F800000));
             const float step = step_of(range);
@@ -280,12 +293,11 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
             if (!bad && step > 0.0f) {
                 float inverse;
                 asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(step));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) codes |= code_of(__fsub_rn(y[i], low), step, inverse) << code_shift(i);
+                codes = codes_of(y, low, step, inverse);
             }
-            if (at < k1) {
-                const uint32_t which = is_k ? 0 : 1;
-                uint8_t* to = block + (uint64_t)(is_k ? at : at - B.n_kv_heads) * block_bytes;
+            if (at >= P.n_q_heads && at < h1) {
+                const uint32_t which = at < keys_end ? 0 : 1;
+                uint8_t* to = block + (uint64_t)(at - (which ? keys_end : P.n_q_heads)) * block_bytes;
                 *(uint32_t*)(to + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e) = codes;
                 if (e == 0)
                     *(uint32_t*)(to + params_at<D>(B.page_log2, which) + 4 * slot) = bad ? 0x7FC07FC0u : (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
@@ -347,8 +359,9 @@ __global__ void __launch_bounds__(256) kv4_dequant_kernel(const __grid_constant_
 
 // Head rows for one warp: all of a row's where there are warps enough without it (a few for each of the 48 or so places of an SM), else fewer.
 uint32_t heads_per_warp(uint32_t rows, uint32_t heads, uint32_t at_once, uint32_t sms) {
-    const uint64_t want = (uint64_t)rows * heads / (64ull * sms);
-    return (uint32_t)std::min<uint64_t>(heads, std::max<uint64_t>(at_once, want / at_once * at_once));
+    const uint64_t want = std::max<uint64_t>((uint64_t)rows * heads / (64ull * sms), 1);
+    const uint32_t parts = (uint32_t)((heads + want - 1) / want), each = ceil_div(heads, parts);
+    return ceil_div(each, at_once) * at_once;
 }
 
 }  // namespace
