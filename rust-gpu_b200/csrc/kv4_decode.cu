@@ -135,6 +135,73 @@ __device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, ui
     return it;
 }
 
+// The parts of one item, in order: records of the CTA's warps (record `from`, then the first ones of the warps behind), or of CTAs (the second one of the first, then the first ones).
+struct Parts {
+    const float* const* here;        // null: records of CTAs
+    int from;
+    const float* of_ctas;            // ... the second record of the first CTA
+    uint32_t floats;                 // ... of a record
+    uint32_t n;
+    __device__ __forceinline__ const float* operator[](uint32_t i) const {
+        if (here) return here[i == 0 ? from : 2 * (from / 2 + (int)i)];
+        return of_ctas + (i == 0 ? 0 : (int64_t)(2 * i - 1) * floats);
+    }
+};
+
+// Adds the parts of an item up, by one warp: maximum and sum for this lane's column (lane % kCols), and four numbers of every 128 in `total`.  `weight`: a row for each part.
+template <int D, int NT>
+__device__ __forceinline__ void add_parts(const Parts& parts, float (*weight)[8 * NT], float* top, float* sum, float4 (&total)[8 * NT * D / 128]) {
+    constexpr int kCols = 8 * NT, kPieces = kCols * D / 128;
+    constexpr uint32_t kEach = 32 / kCols;
+    const uint32_t lane = threadIdx.x % 32, col = lane % kCols;
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t i = lane / kCols; i < parts.n; i += kEach) m = fmaxf(m, parts[i][kCols * D + col]);
+#pragma unroll
+    for (uint32_t d = kCols; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    const float base = m == -INFINITY ? 0.0f : m;
+    for (uint32_t i = lane / kCols; i < parts.n; i += kEach) {
+        const float* r = parts[i] + kCols * D + col;
+        const float w = exp2_fast(r[0] - base);
+        l += w * r[kCols];
+        weight[i][col] = w;
+    }
+#pragma unroll
+    for (uint32_t d = kCols; d < 32; d *= 2) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
+    __syncwarp();
+    *top = m;
+    *sum = l;
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) total[j] = make_float4(0, 0, 0, 0);
+#pragma unroll 2
+    for (uint32_t i = 0; i < parts.n; ++i) {
+        const float4* r = (const float4*)parts[i] + lane;
+        float4 x[kPieces];
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) x[j] = r[32 * j];
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const float f = weight[i][(128 * j + 4 * lane) / D];
+            total[j].x = fmaf(f, x[j].x, total[j].x); total[j].y = fmaf(f, x[j].y, total[j].y);
+            total[j].z = fmaf(f, x[j].z, total[j].z); total[j].w = fmaf(f, x[j].w, total[j].w);
+        }
+    }
+    __syncwarp();
+}
+
+template <int D, int NT>
+__device__ __forceinline__ void finish(const Attention& P, const Item& it, const float4 (&total)[8 * NT * D / 128], float sum) {
+    const uint32_t lane = threadIdx.x % 32;
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < 8 * NT * D / 128; ++j) {
+        const uint32_t e = 128 * j + 4 * lane, c = e / D;
+        const float f = __shfl_sync(0xFFFFFFFFu, inverse, c);
+        if (c >= (uint32_t)it.s.rows * P.group) continue;
+        __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
+        *(uint2*)y = make_uint2(pack(total[j].x * f, total[j].y * f), pack(total[j].z * f, total[j].w * f));
+    }
+}
+
 template <int D, int NT>
 struct Params {
     Attention P;
@@ -152,11 +219,9 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Plan plan;
     __shared__ __align__(8) uint64_t bars[kWarps * kStages];
-    __shared__ int abort_flag, rec_there[2 * kWarps], rec_open[2 * kWarps], is_last[2];
-    __shared__ uint32_t parts_from[2], parts_of[2];
-    __shared__ Item edge_item[2];                           // the items that the CTA may have begun in, and may end in
-    __shared__ float2 part_ml[kMaxParts][kCols];          // joining: maximum and sum of each part, then its weight
-    __shared__ float scale_of[kCols];
+    __shared__ int abort_flag, rec_there[2 * kWarps], rec_open[2 * kWarps];
+    __shared__ Item first_item, last_item[kWarps];         // the item that the CTA begins in, and those that the warps' runs end in
+    __shared__ float weight_here[3 * kWarps][kCols], weight_of[2][kMaxParts][kCols];       // joining: of the parts in the CTA, and of CTAs' parts
     __shared__ const float* rec_at[2 * kWarps];
     const Attention& P = G.P;
     const Batch& B = P.B;
@@ -460,7 +525,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             }
         };
 
-        if (warp == 0 && lane == 0) edge_item[0] = it;
+        if (warp == 0 && lane == 0) first_item = it;
         uint32_t u = begin, phase = 0;
         while (u < end) {
             if (u != begin) it = item_of<kThreads>(P, plan, u);
@@ -482,7 +547,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             if (!ok) break;
             end_item(opens, u < item_end, u == end);
         }
-        if (warp == here - 1 && lane == 0) edge_item[1] = it;
+        if (lane == 0) last_item[warp] = it;
         if (!ok) {                                         // copies in flight end before the CTA does
             for (int s = 0; s < kStages; ++s) {
                 volatile int never = 0;
@@ -495,170 +560,43 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     if (abort_flag) return;
 
     // ---- joining.  A record a warp begins in (index 2 w) continues what the warp before has as the record it ends in (2 w + 1), or, where the warp lies in the item as a
-    // whole, as its own 2 w.  So a run of parts of one item is the record 2 a + 1, then 2 (a + 1), 2 (a + 2), ... to the one that is not open.  Runs with both ends in the
-    // CTA are finished by the warp they begin in, all at the same time; at most two are open, at the CTA's begin and at its end: they become records of the CTA.
-    auto index_of = [&](int from, uint32_t i) { return i == 0 ? from : 2 * (from / 2 + (int)i); };
-    auto parts = [&](int from, bool* closed) {              // of the run that begins at record `from`
-        uint32_t n = 1;
-        *closed = rec_open[from] == 0;
-        for (uint32_t w = from / 2 + 1; !*closed && w < here; ++w, ++n) *closed = rec_open[2 * w] == 0;
-        return n;
-    };
-    auto store = [&](const Item& it, uint32_t e, float4 sum, float f) {
-        const uint32_t c = e / D;
-        __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
-        *(uint2*)y = make_uint2(pack(sum.x * f, sum.y * f), pack(sum.z * f, sum.w * f));
-    };
-    bool closed = false;
-    if (active && rec_there[2 * warp + 1]) {
-        const int from = 2 * warp + 1;
-        const uint32_t n = parts(from, &closed);
-        if (closed) {
-            const Item it = item_of<kThreads>(P, plan, start_of(me + 1) - 1);
-            // weights: a lane to a column, the parts dealt to the lanes of a column
-            constexpr uint32_t kEach = 32 / kCols;
-            const uint32_t c = lane % kCols;
-            float top = -INFINITY, sum = 0.0f;
-            for (uint32_t i = lane / kCols; i < n; i += kEach) top = fmaxf(top, rec_at[index_of(from, i)][kCols * D + c]);
-#pragma unroll
-            for (uint32_t d = kCols; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-            const float base = top == -INFINITY ? 0.0f : top;
-            for (uint32_t i = lane / kCols; i < n; i += kEach) {
-                const float* r = rec_at[index_of(from, i)] + kCols * D + c;
-                const float w = exp2_fast(r[0] - base);
-                sum += w * r[kCols];
-                part_ml[index_of(from, i)][c].x = w;
-            }
-#pragma unroll
-            for (uint32_t d = kCols; d < 32; d *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-            __syncwarp();
-            // every lane takes four numbers of every column, all columns of a part at once
-            constexpr int kPieces = kCols * D / 128;
-            float4 total[kPieces];
-#pragma unroll
-            for (int j = 0; j < kPieces; ++j) total[j] = make_float4(0, 0, 0, 0);
-            for (uint32_t i = 0; i < n; ++i) {
-                const float4* r = (const float4*)rec_at[index_of(from, i)] + lane;
-                float4 x[kPieces];
-#pragma unroll
-                for (int j = 0; j < kPieces; ++j) x[j] = r[32 * j];
-#pragma unroll
-                for (int j = 0; j < kPieces; ++j) {
-                    const float w = part_ml[index_of(from, i)][(128 * j + 4 * lane) / D].x;
-                    total[j].x = fmaf(w, x[j].x, total[j].x); total[j].y = fmaf(w, x[j].y, total[j].y);
-                    total[j].z = fmaf(w, x[j].z, total[j].z); total[j].w = fmaf(w, x[j].w, total[j].w);
-                }
-            }
-            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const uint32_t cols = (uint32_t)it.s.rows * P.group;
-#pragma unroll
-            for (int j = 0; j < kPieces; ++j) {
-                const uint32_t e = 128 * j + 4 * lane;
-                const float f = __shfl_sync(0xFFFFFFFFu, inverse, e / D);
-                if (e / D < cols) store(it, e, total[j], f);
-            }
-        }
-    }
-    // the open runs: the one that record 0 begins, and the one that the last record belongs to
-    int open_from[2] = {-1, -1};
-    uint32_t open_parts[2] = {0, 0};
-    bool ends;
-    if (rec_there[0]) {
-        open_from[0] = 0;
-        open_parts[0] = parts(0, &ends);
-    }
-    const int tail = 2 * (here - 1) + 1;
-    if (rec_there[tail]) {
-        open_from[1] = tail;
-        open_parts[1] = 1;
-    } else if (rec_there[tail - 1] && rec_open[tail - 1]) {
-        int w = here - 1;
-        while (w > 0 && !rec_there[2 * w + 1]) --w;
-        if (rec_there[2 * w + 1]) {                     // (else it is the run of record 0)
-            open_from[1] = 2 * w + 1;
-            open_parts[1] = here - w;
-        }
-    }
-    if (open_from[0] < 0 && open_from[1] < 0) return;
+    // whole, as its own 2 w.  So a run of parts of one item is the record 2 a + 1 (or 0), then 2 (a + 1), 2 (a + 2), ... to the one that is not open.  Every run is one warp's,
+    // all at the same time.  At most two are open, at the CTA's begin and at its end: they become records of the CTA, and the CTA that arrives last finishes the item.
     float* const cta_records = G.records + (uint64_t)gridDim.x * kWarps * kRecord;
-    // the weights of `n` parts, a warp to a column; with `finish` the inverse of the whole sum
-    auto weigh = [&](uint32_t n, auto record, bool finish, float* to) {
-        for (uint32_t e = threadIdx.x; e < n * kCols; e += kThreads) {
-            const float* r = record(e / kCols) + kCols * D + e % kCols;
-            part_ml[e / kCols][e % kCols] = make_float2(r[0], r[kCols]);
-        }
-        __syncthreads();
-        for (uint32_t c = warp; c < kCols; c += kWarps) {
-            float top = -INFINITY, sum = 0.0f;
-            for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, part_ml[i][c].x);
+    auto join = [&](int from, const Item& it) {              // the run that begins with record `from`
+        Parts parts = {rec_at, from, nullptr, 0, 1};
+        bool open = rec_open[from] != 0;
+        for (uint32_t w = from / 2 + 1; open && w < here; ++w, ++parts.n) open = rec_open[2 * w] != 0;
+        float top, sum;
+        float4 total[kCols * D / 128];
+        add_parts<D, NT>(parts, weight_here + from, &top, &sum, total);
+        const uint32_t k = from & 1;                          // 0: begun before the CTA's run, 1: in it
+        if (k == 0 || open) {
+            float* to = cta_records + (uint64_t)(2 * blockIdx.x + k) * kRecord;
 #pragma unroll
-            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-            const float base = top == -INFINITY ? 0.0f : top;
-            for (uint32_t i = lane; i < n; i += 32) {
-                const float w = exp2_fast(part_ml[i][c].x - base);
-                sum += w * part_ml[i][c].y;
-                part_ml[i][c].x = w;
+            for (int j = 0; j < kCols * D / 128; ++j) ((float4*)to)[32 * j + lane] = total[j];
+            if (lane < kCols) {
+                to[kCols * D + lane] = top;
+                to[kCols * D + kCols + lane] = sum;
             }
-#pragma unroll
-            for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-            if (lane == 0) {
-                scale_of[c] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (!finish) {
-                    to[kCols * D + c] = top;
-                    to[kCols * D + kCols + c] = sum;
-                }
-            }
-        }
-        __syncthreads();
-    };
-    auto add_up = [&](uint32_t n, auto record, uint32_t e) {
-        float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-        for (uint32_t i = 0; i < n; ++i) {
-            const float w = part_ml[i][e / D].x;
-            const float4 x = *(const float4*)(record(i) + e);
-            sum.x = fmaf(w, x.x, sum.x); sum.y = fmaf(w, x.y, sum.y); sum.z = fmaf(w, x.z, sum.z); sum.w = fmaf(w, x.w, sum.w);
-        }
-        return sum;
-    };
-    for (int k = 0; k < 2; ++k) {
-        if (open_from[k] < 0) continue;
-        float* to = cta_records + (uint64_t)(2 * blockIdx.x + k) * kRecord;
-        if (open_parts[k] == 1) {
-            const float* from = rec_at[open_from[k]];
-            for (uint32_t e = threadIdx.x * 2; e < kRecord; e += kThreads * 2) *(float2*)(to + e) = *(const float2*)(from + e);
-            continue;
-        }
-        auto record = [&](uint32_t i) { return rec_at[index_of(open_from[k], i)]; };
-        __syncthreads();                                    // (the table of weights may be in use)
-        weigh(open_parts[k], record, false, to);
-        for (uint32_t e = threadIdx.x * 4; e < kCols * D; e += kThreads * 4) *(float4*)(to + e) = add_up(open_parts[k], record, e);
-    }
-    // the CTA that arrives last finishes the item
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const int k = threadIdx.x;
-        is_last[k] = 0;
-        if (open_from[k] >= 0) {
-            const Item& it = edge_item[k];
-            const uint32_t first_cta = worker_of(it.first) / per_cta, last_cta = worker_of(it.first + it.chunks - 1) / per_cta;
-            parts_from[k] = first_cta;
-            parts_of[k] = last_cta - first_cta + 1;
-            is_last[k] = atomicAdd(G.counters + first_cta, 1) == (int)(last_cta - first_cta);
-            if (is_last[k]) G.counters[first_cta] = 0;
+            const uint32_t first_cta = worker_of(it.first) / per_cta, n = worker_of(it.first + it.chunks - 1) / per_cta - first_cta + 1;
             __threadfence();
+            __syncwarp();
+            uint32_t before = 0;
+            if (lane == 0) before = (uint32_t)atomicAdd(G.counters + first_cta, 1);
+            if (__shfl_sync(0xFFFFFFFFu, before, 0) != n - 1) return;
+            if (lane == 0) G.counters[first_cta] = 0;
+            __threadfence();
+            parts = Parts{nullptr, 0, cta_records + (uint64_t)(2 * first_cta + 1) * kRecord, kRecord, n};
+            add_parts<D, NT>(parts, weight_of[k], &top, &sum, total);
         }
-    }
-    __syncthreads();
-    for (int k = 0; k < 2; ++k) {
-        if (!is_last[k]) continue;
-        const Item it = edge_item[k];
-        const uint32_t from = parts_from[k], n = parts_of[k];
-        auto part = [&](uint32_t i) { return cta_records + (uint64_t)(2 * (from + i) + (i == 0 ? 1 : 0)) * kRecord; };
-        weigh(n, part, true, nullptr);
-        for (uint32_t e = threadIdx.x * 4; e < (uint32_t)it.s.rows * P.group * D; e += kThreads * 4) store(it, e, add_up(n, part, e), scale_of[e / D]);
-        __syncthreads();
+        finish<D, NT>(P, it, total, sum);
+    };
+    if (warp < here && rec_there[2 * warp + 1]) join(2 * warp + 1, last_item[warp]);
+    if (rec_there[0]) {
+        // the run of record 0 goes to a warp that has none, the first warp if they all do
+        const uint32_t idle = __ballot_sync(0xFFFFFFFFu, lane < kWarps && (lane >= here || !rec_there[2 * min(lane, (uint32_t)kWarps - 1) + 1]));
+        if (warp == (idle ? (uint32_t)__ffs(idle) - 1 : 0u)) join(0, first_item);
     }
 }
 
