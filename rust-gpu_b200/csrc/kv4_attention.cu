@@ -16,7 +16,7 @@ extern "C" {
 
 size_t t0_kv4_scratch_bytes(const t0_runtime* rt) {
     const uint32_t sms = rt ? (uint32_t)rt->sm_count : 0;
-    return rt ? kv4_counter_bytes() + std::max(kv4::decode_scratch_bytes(sms), kv4::prompt_scratch_bytes(sms)) : 0;
+    return rt ? kv4_counter_bytes() + kv4::decode_scratch_bytes(sms) + kv4::prompt_scratch_bytes(sms) : 0;
 }
 
 int t0_kv4_attention(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_attention_args* args) {

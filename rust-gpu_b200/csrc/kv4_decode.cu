@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kTok = 64;                                  // tokens of a chunk
 constexpr int kStages = 2;
+constexpr uint32_t kManyParts = 4;                        // CTAs' parts that one warp joins; more are shared by a CTA's warps
 constexpr uint32_t kMaxParts = kMaxCtas;                  // parts of one item: at most one for each CTA
 
 template <int D> constexpr int stage_bytes() { return kTok * (D + 8); }
@@ -148,10 +149,10 @@ struct Parts {
     }
 };
 
-// Adds the parts of an item up, by one warp: maximum and sum for this lane's column (lane % kCols), and four numbers of every 128 in `total`.  `weight`: a row for each part.
+// Maximum and sum of the parts of an item, by one warp, for this lane's column (lane % kCols), and each part's weight: a row of `weight` for each.
 template <int D, int NT>
-__device__ __forceinline__ void add_parts(const Parts& parts, float (*weight)[8 * NT], float* top, float* sum, float4 (&total)[8 * NT * D / 128]) {
-    constexpr int kCols = 8 * NT, kPieces = kCols * D / 128;
+__device__ __forceinline__ void weigh_parts(const Parts& parts, float (*weight)[8 * NT], float* top, float* sum) {
+    constexpr int kCols = 8 * NT;
     constexpr uint32_t kEach = 32 / kCols;
     const uint32_t lane = threadIdx.x % 32, col = lane % kCols;
     float m = -INFINITY, l = 0.0f;
@@ -170,6 +171,14 @@ __device__ __forceinline__ void add_parts(const Parts& parts, float (*weight)[8 
     __syncwarp();
     *top = m;
     *sum = l;
+}
+
+// The parts of an item added up by one warp: four numbers of every 128 for a lane.
+template <int D, int NT>
+__device__ __forceinline__ void add_parts(const Parts& parts, float (*weight)[8 * NT], float* top, float* sum, float4 (&total)[8 * NT * D / 128]) {
+    constexpr int kPieces = 8 * NT * D / 128;
+    const uint32_t lane = threadIdx.x % 32;
+    weigh_parts<D, NT>(parts, weight, top, sum);
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) total[j] = make_float4(0, 0, 0, 0);
 #pragma unroll 2
@@ -188,17 +197,22 @@ __device__ __forceinline__ void add_parts(const Parts& parts, float (*weight)[8 
     __syncwarp();
 }
 
+// numbers e .. e + 3 of an item's result; columns that are no row's are passed over
+template <int D>
+__device__ __forceinline__ void store(const Attention& P, const Item& it, uint32_t e, float4 x, float f) {
+    const uint32_t c = e / D;
+    if (c >= (uint32_t)it.s.rows * P.group) return;
+    __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
+    *(uint2*)y = make_uint2(pack(x.x * f, x.y * f), pack(x.z * f, x.w * f));
+}
 template <int D, int NT>
 __device__ __forceinline__ void finish(const Attention& P, const Item& it, const float4 (&total)[8 * NT * D / 128], float sum) {
     const uint32_t lane = threadIdx.x % 32;
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int j = 0; j < 8 * NT * D / 128; ++j) {
-        const uint32_t e = 128 * j + 4 * lane, c = e / D;
-        const float f = __shfl_sync(0xFFFFFFFFu, inverse, c);
-        if (c >= (uint32_t)it.s.rows * P.group) continue;
-        __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
-        *(uint2*)y = make_uint2(pack(total[j].x * f, total[j].y * f), pack(total[j].z * f, total[j].w * f));
+        const uint32_t e = 128 * j + 4 * lane;
+        store<D>(P, it, e, total[j], __shfl_sync(0xFFFFFFFFu, inverse, e / D));
     }
 }
 
@@ -220,6 +234,8 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     __shared__ Plan plan;
     __shared__ __align__(8) uint64_t bars[kWarps * kStages];
     __shared__ int abort_flag, rec_there[2 * kWarps], rec_open[2 * kWarps];
+    __shared__ uint32_t many_parts[2], many_from[2];
+    __shared__ Item many_item[2];
     __shared__ Item first_item, last_item[kWarps];         // the item that the CTA begins in, and those that the warps' runs end in
     __shared__ float weight_here[3 * kWarps][kCols], weight_of[2][kMaxParts][kCols];       // joining: of the parts in the CTA, and of CTAs' parts
     __shared__ const float* rec_at[2 * kWarps];
@@ -229,13 +245,13 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
     const uint32_t ring = ptx::smem_u32(smem) + warp * kStages * stage_bytes<D>();
     const uint8_t* ring_ptr = smem + warp * kStages * stage_bytes<D>();
     const uint32_t bar = ptx::smem_u32(bars) + warp * kStages * 8;
-    if (threadIdx.x == 0) abort_flag = 0;
+    if (threadIdx.x == 0) abort_flag = many_parts[0] = many_parts[1] = 0;
     if (lane == 0) {
         for (int i = 0; i < kStages; ++i) ptx::mbar_init(bar + 8 * i, 1);
         ptx::fence_barrier_init();
     }
     ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
+    ptx::grid_launch_dependents();                         // (only now: kv4_prompt_kernel counts on it)
     const uint32_t units = make_plan<kThreads>(P, plan);
     if (units == 0) return;
     // how many warps of a CTA work: all, or fewer where that spreads the chunks over more SMs
@@ -587,6 +603,14 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             if (__shfl_sync(0xFFFFFFFFu, before, 0) != n - 1) return;
             if (lane == 0) G.counters[first_cta] = 0;
             __threadfence();
+            if (n > kManyParts) {                           // a long item: the CTA's warps share it, below
+                if (lane == 0) {
+                    many_parts[k] = n;
+                    many_from[k] = first_cta;
+                    many_item[k] = it;
+                }
+                return;
+            }
             parts = Parts{nullptr, 0, cta_records + (uint64_t)(2 * first_cta + 1) * kRecord, kRecord, n};
             add_parts<D, NT>(parts, weight_of[k], &top, &sum, total);
         }
@@ -597,6 +621,27 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
         // the run of record 0 goes to a warp that has none, the first warp if they all do
         const uint32_t idle = __ballot_sync(0xFFFFFFFFu, lane < kWarps && (lane >= here || !rec_there[2 * min(lane, (uint32_t)kWarps - 1) + 1]));
         if (warp == (idle ? (uint32_t)__ffs(idle) - 1 : 0u)) join(0, first_item);
+    }
+    __syncthreads();
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t n = many_parts[k];
+        if (n == 0) continue;
+        // every warp weighs all parts for itself, and adds up the 128 numbers of a record that are its own
+        const Parts parts = {nullptr, 0, cta_records + (uint64_t)(2 * many_from[k] + 1) * kRecord, kRecord, n};
+        float top, sum;
+        weigh_parts<D, NT>(parts, weight_of[k], &top, &sum);
+        __syncthreads();                                    // (the same weights from every warp)
+        const Item it = many_item[k];
+        for (uint32_t e = 128 * warp + 4 * lane; e < kCols * D; e += 128 * kWarps) {
+            float4 total = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+            for (uint32_t i = 0; i < n; ++i) {
+                const float4 x = *(const float4*)(parts[i] + e);
+                const float f = weight_of[k][i][e / D];
+                total.x = fmaf(f, x.x, total.x); total.y = fmaf(f, x.y, total.y); total.z = fmaf(f, x.z, total.z); total.w = fmaf(f, x.w, total.w);
+            }
+            store<D>(P, it, e, total, __shfl_sync(0xFFFFFFFFu, sum == 0.0f ? 0.0f : 1.0f / sum, e / D));
+        }
     }
 }
 
@@ -623,9 +668,10 @@ int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
 
 }  // namespace
 
+// a multiple of 128
 size_t decode_scratch_bytes(uint32_t sms) {
     const size_t n = std::min(sms, kMaxCtas);
-    auto one = [&](size_t warps, size_t record) { return (n * warps + 2 * n) * record * sizeof(float); };
+    auto one = [&](size_t warps, size_t record) { return ((n * warps + 2 * n) * record * sizeof(float) + 127) / 128 * 128; };
     return std::max(std::max(one(warps<128, 1>(), record_floats<128, 1>()), one(warps<128, 2>(), record_floats<128, 2>())),
                     std::max(one(warps<64, 1>(), record_floats<64, 1>()), one(warps<64, 2>(), record_floats<64, 2>())));
 }

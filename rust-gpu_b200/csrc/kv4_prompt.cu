@@ -184,6 +184,7 @@ struct Params {
     Attention P;
     float* records;                  // two for each CTA: of the item it begins in, of the item it ends in
     Cut* cuts;                       // one for each CTA
+    bool beside_decode;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -261,7 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     ptx::tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_holder, 0);
     ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
+    // Behind kv4_decode in one call there is nothing of that kernel to wait for: it lets this one begin only after what came before both is done, and writes other rows
+    // and other scratch.  The wait is then made up for at the end, so that this kernel is never done before that one.
+    if (!G.beside_decode) ptx::grid_dependency_wait();
 
     const uint32_t per_head = make_plan(P, plan), units = per_head * B.n_kv_heads, runs = min(gridDim.x, units);
     const uint32_t begin = blockIdx.x < runs ? start_of(blockIdx.x, units, runs) : 0, end = blockIdx.x < runs ? start_of(blockIdx.x + 1, units, runs) : 0;
@@ -613,6 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc(tmem, kTmem);
     }
+    if (G.beside_decode) ptx::grid_dependency_wait();
 }
 
 // Joins the parts of the items whose chunks several CTAs of the launch before worked on.  Block (c, z): the item that the boundary before CTA c cuts, if c is the first one
@@ -671,7 +675,8 @@ int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
     }
     Params g;
     g.P = p;
-    g.cuts = (Cut*)(p.scratch + kv4_counter_bytes());
+    g.cuts = (Cut*)(p.scratch + kv4_counter_bytes() + decode_scratch_bytes(sms));
+    g.beside_decode = p.few != 0;
     g.records = (float*)(g.cuts + kMaxCtas);
     const uint32_t ctas = std::min(sms, kMaxCtas);
     cudaError_t e = gemm::launch_pdl(kv4_prompt_kernel<D>, ctas, kThreads, smem, stream, g);
