@@ -232,11 +232,11 @@ __global__ void __launch_bounds__(256, 3) kv4_append_kernel(const __grid_constan
                 y[2 * i + 1] = __fadd_rn(__fmul_rn(w, turn[i].x), __fmul_rn(u, turn[i].y));
             }
         } else {
-            // two at a time: products and sum are rounded one by one all the same
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
+            for (int i = 0; i < 8; i += 2) {                       // (products and sums of pairs in one instruction would be contracted)
                 const float2 other = make_float2(__shfl_sync(0xFFFFFFFFu, y[i], from), __shfl_sync(0xFFFFFFFFu, y[i + 1], from));
-                const float2 z = __fadd2_rn(__fmul2_rn(make_float2(y[i], y[i + 1]), make_float2(turn[i].x, turn[i + 1].x)), __fmul2_rn(other, make_float2(turn[i].y, turn[i + 1].y)));
+                const float2 z = make_float2(__fadd_rn(__fmul_rn(y[i], turn[i].x), __fmul_rn(other.x, turn[i].y)),
+                                             __fadd_rn(__fmul_rn(y[i + 1], turn[i + 1].x), __fmul_rn(other.y, turn[i + 1].y)));
                 if (whole_turn || turns) {
                     y[i] = z.x;
                     y[i + 1] = z.y;

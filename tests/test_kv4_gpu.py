@@ -141,6 +141,30 @@ def test_append_holds_the_rows_and_rotates_the_queries(t0, rt, dev, lens, rows, 
         assert np.array_equal(buf.read(total * stride * 2, np.uint16).reshape(total, stride), want)
 
 
+@pytest.mark.parametrize("f32, interleaved", [(False, False), (True, False), (False, True)])
+def test_a_long_append_is_exact(t0, rt, dev, f32, interleaved):
+    # six million numbers: an operation that is not rounded by itself, or a quotient off by its last place, shows in some of them
+    rng = np.random.default_rng(77)
+    heads, dim, page, n = 8, 128, 64, 1024
+    cache = ref.Cache(rng, [n], heads, dim, page, spare=0, extra_columns=0)
+    pool = dev.up(np.zeros((cache.n_pages, heads, page * (dim + 8)), np.uint8))
+    b = make_batch(t0, dev, cache, pool, [n], uniform=True)
+    x = (rng.standard_normal((n, 6 * heads, dim)) * 2).astype(np.float32)
+    if not f32:
+        x = ref.bf16_round(x)
+    data, table, q_out = dev.up(x if f32 else ref.bf16_bits(x)), rope_table(rng, n, dim // 2), dev.up(np.zeros((n, 4 * heads, dim), np.uint16))
+    at, size, wide = data.gpu_addr(), (4 if f32 else 2), 6 * heads * dim
+    rt.kv4_append(b, rt.kv4_append_args(at + 4 * heads * dim * size, at + 5 * heads * dim * size, k_stride=wide, v_stride=wide, in_f32=f32, q=at, q_stride=wide,
+                                        q_out=q_out.gpu_addr(), n_q_heads=4 * heads, rope=dev.up(table).gpu_addr(), n_positions=n, rot_dim=dim, interleaved=interleaved))
+    rt.synchronize()
+    turned = ref.rotate(x[:, :5 * heads], table, interleaved)
+    assert np.array_equal(q_out.read(n * 4 * heads * dim * 2, np.uint16), ref.bf16_bits(turned[:, :4 * heads]).ravel())
+    k, x = turned[:, 4 * heads:], x[:, 4 * heads:]
+    want = ref.block_bytes(*(a.reshape(-1, page, heads, dim).transpose(0, 2, 1, 3) for a in (k, x[:, heads:])))
+    got = pool.read(want.size).reshape(want.shape[0], heads, -1)[cache.table[0]]
+    assert np.array_equal(got, want)
+
+
 def test_rows_that_four_bits_have_trouble_with(t0, rt, dev):
     # infinities, NaNs, ranges that overflow or vanish, constants, ties: the bytes are the restatement's, and what is read back its values
     rng = np.random.default_rng(5)
