@@ -577,7 +577,8 @@ long t0_gptq_to_b200(const uint8_t* packed, const float* scales, const int32_t* 
  * sequence are neither read nor written.  page_table, seq_lens and row_start are read on the device when the call runs, so a recorded call may be
  * replayed with other values in them.  What they hold is checked there: a sequence with a negative length, more tokens than its row of
  * the table has places, rows outside n_rows or more than max_rows of them is left out; a page outside the cache is neither read nor written
- * (what the sequence's rows get is then of no use, other sequences' are as ever); in either case the next
+ * (what the sequence's rows get is then of no use, other sequences' are as ever; where sequences'
+ * rows overlap, sequences of more than one row may get nothing); in either case the next
  * synchronising call returns T0_ERR_BOUNDS (the runtime is not poisoned).  Sequences may share pages that they only read; a token's place
  * must not be another's whose row is in the same append. */
 typedef struct t0_kv4_batch {
@@ -624,7 +625,7 @@ int t0_kv4_dequant(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_dequa
 /* Attention of the rows over their sequences' cached tokens: row at token p sees the tokens j <= p, with window > 0 those with
  * j > p - window, and y = sum_j softmax_j(scale * q . k_j) v_j for each of its n_q_heads heads (a multiple of n_kv_heads, at most 64 to a
  * key/value head; head h reads key/value head h / (n_q_heads / n_kv_heads)).  q and y are bf16 rows, 16-byte aligned, strides multiples of 8 (0 = dense);
- * y may be q itself.  scale is positive and finite.  A row without a token, or that sees none, becomes zeros.  Sums and softmax statistics are f32.
+ * y may be q itself.  scale is positive, and scale * log2(e) finite.  A row without a token, or that sees none, becomes zeros.  Sums and softmax statistics are f32.
  * The rows' own tokens are read from the cache like any other: call t0_kv4_append first.  The work is cut by what the device finds in the batch, not by host
  * values, so a recorded call stays balanced when its lengths change; sums are added in an order that depends on the batch alone, so a call repeats bit for bit. */
 typedef struct t0_kv4_attention_args {

@@ -31,7 +31,7 @@ int t0_kv4_attention(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_att
     if (!a.q || !a.y) return fail(T0_ERR_INVALID, "null device pointer");
     if (a.n_q_heads == 0 || a.n_q_heads % batch->n_kv_heads || a.n_q_heads / batch->n_kv_heads > 64)
         return fail(T0_ERR_INVALID, "n_q_heads=%u must be a multiple of n_kv_heads=%u, at most 64 times it", a.n_q_heads, batch->n_kv_heads);
-    if (!(a.scale > 0.0f) || std::isinf(a.scale)) return fail(T0_ERR_INVALID, "scale=%g must be positive and finite", (double)a.scale);
+    if (!(a.scale > 0.0f) || std::isinf(a.scale * 1.44269504f)) return fail(T0_ERR_INVALID, "scale=%g must be positive and finite, in powers of two too", (double)a.scale);
     if (a.window > 0x7FFFFFFFu) return fail(T0_ERR_INVALID, "window=%u", a.window);
     if ((rc = check_rows("q", a.q, &a.q_stride, width, 2)) != T0_OK) return rc;
     if ((rc = check_rows("y", a.y, &a.y_stride, width, 2)) != T0_OK) return rc;

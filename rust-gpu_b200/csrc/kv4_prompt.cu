@@ -114,9 +114,13 @@ __device__ __forceinline__ Item tile_at(const Attention& P, const Plan& plan, ui
 __device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
     const uint32_t n = P.B.n_seqs, each = (n + kThreads - 1) / kThreads, tid = threadIdx.x;
     if (tid == 0) plan.seqs_each = each;
+    // Sequences whose rows do not overlap have no more tiles than this, 2^23 at most, and the host saw to it that their units fit into 32 bits.  Where row_start is not
+    // ascending (which sequence() reports) there may be more: then none is taken.
+    const uint32_t most = (uint32_t)((uint64_t)P.B.n_rows * P.group / kRows) + n;
     uint32_t mine = 0;
-    for (uint32_t b = tid * each; b < min(n, (tid + 1) * each); ++b) mine += tiles_of(P, sequence(P.B, b));
+    for (uint32_t b = tid * each; b < min(n, (tid + 1) * each); ++b) mine = min(mine + tiles_of(P, sequence(P.B, b)), most + 1);
     const uint32_t tiles = scan(mine, plan.warp_sum, plan.tiles);
+    if (tiles > most) return 0;
     const uint32_t tiles_each = (tiles + kThreads - 1) / kThreads;
     if (tid == 0) plan.tiles_each = tiles_each;
     mine = 0;

@@ -128,7 +128,7 @@ def test_dequant_calls_in_order(t0):
 
 @pytest.mark.parametrize("change, text", [
     (dict(q=0), "null"), (dict(y=0), "null"), (dict(n_q_heads=0), "n_q_heads"), (dict(n_q_heads=3), "multiple"), (dict(n_q_heads=130), "64 times"),
-    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=3e38), "scale"),
     (dict(window=1 << 31), "window"), (dict(q=0x10004), "q: rows"), (dict(y_stride=260), "y: rows"), (dict(q_stride=248), "q: a stride"), (dict(y=0x10100), "overlaps"),
     (dict(y=0x10000, y_stride=264), "overlaps"),
 ])
@@ -137,6 +137,18 @@ def test_attention_refusals(t0, change, text):
     args = t0.GpuRuntime.kv4_attention_args(kw.pop("q", 0x10000), kw.pop("y", 0x20000), **kw)
     code, message = refused(t0, "t0_kv4_attention", batch(t0), args)
     assert code == "INVALID" and text in message, message
+
+
+@pytest.mark.parametrize("change", [
+    dict(n_seqs=1 << 18, n_rows=1 << 18, table_stride=1 << 16, page_size=16),                        # units of few rows: 2^18 x 2^14 x 2
+    dict(n_seqs=1, n_rows=1 << 24, max_rows=1 << 24, table_stride=1 << 16, page_size=16, row_start=0x4000),   # of many: 2^17 tiles x 2^13 x 2
+])
+def test_attention_too_long_for_one_call(t0, change):
+    args = t0.GpuRuntime.kv4_attention_args(0x10000, 1 << 44, n_q_heads=4, scale=0.125)
+    code, message = refused(t0, "t0_kv4_attention", batch(t0, **change), args)
+    assert code == "UNSUPPORTED" and "too much for one call" in message, message
+    change.update(table_stride=64)
+    assert refused(t0, "t0_kv4_attention", batch(t0, **change), args)[1] == "null runtime"
 
 
 def test_the_reference_holds_what_it_is_given(t0):

@@ -431,6 +431,29 @@ def test_bad_device_arrays_are_left_out_and_reported(t0, own, rows, what, text):
     dev.free()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sequences_with_the_same_rows_are_reported_and_do_no_harm(t0, own, dim):
+    # row_start goes down again and again: the sequences have three times the rows that there are.  What y holds is of no use; the next call's is.
+    dev = Device(own)
+    rng = np.random.default_rng(6)
+    cache = ref.Cache(rng, [600] * 6, 2, dim, 16)
+    q = ref.bf16_bits(rng.standard_normal((600, 8, dim)).astype(np.float32))
+    pool, table, lens, qb = dev.up(cache.pool(0)), dev.up(cache.table), dev.up(np.array(cache.lens, np.int32)), dev.up(q)
+    out = []
+    for start in ([0, 100, 200, 300, 400, 500, 600], [0, 600, 0, 600, 0, 600, 600], [0, 100, 200, 300, 400, 500, 600]):
+        y = dev.up(np.full(q.shape, 0xABCD, np.uint16))
+        b = own.kv4_batch(pool.gpu_addr(), table.gpu_addr(), lens.gpu_addr(), n_pages=cache.n_pages, page_size=16, n_kv_heads=2, head_dim=dim, n_seqs=6,
+                          table_stride=cache.stride, n_rows=600, max_rows=600, row_start=dev.up(np.array(start, np.int32)).gpu_addr())
+        own.kv4_attention(b, own.kv4_attention_args(qb.gpu_addr(), y.gpu_addr(), n_q_heads=8, scale=0.1))
+        if start[2] == 0:
+            bounds_error(t0, own, "sequence")
+        else:
+            own.synchronize()
+        out.append(y.read(q.nbytes, np.uint16))
+    assert np.array_equal(out[0], out[2]) and not np.any(out[0] == 0xABCD)
+    dev.free()
+
+
 def test_positions_outside_the_rope_table(t0, own):
     dev = Device(own)
     rng = np.random.default_rng(2)
