@@ -111,12 +111,9 @@ __device__ __forceinline__ Item tile_at(const Attention& P, const Plan& plan, ui
     return it;
 }
 // returns the units of one head
-__device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
+__device__ __forceinline__ uint32_t make_plan(const Attention& P, uint32_t most, Plan& plan) {
     const uint32_t n = P.B.n_seqs, each = (n + kThreads - 1) / kThreads, tid = threadIdx.x;
     if (tid == 0) plan.seqs_each = each;
-    // Sequences whose rows do not overlap have no more tiles than this, 2^23 at most, and the host saw to it that their units fit into 32 bits.  Where row_start is not
-    // ascending (which sequence() reports) there may be more: then none is taken.
-    const uint32_t most = (uint32_t)((uint64_t)P.B.n_rows * P.group / kRows) + n;
     uint32_t mine = 0;
     for (uint32_t b = tid * each; b < min(n, (tid + 1) * each); ++b) mine = min(mine + tiles_of(P, sequence(P.B, b)), most + 1);
     const uint32_t tiles = scan(mine, plan.warp_sum, plan.tiles);
@@ -188,6 +185,9 @@ struct Params {
     Attention P;
     float* records;                  // two for each CTA: of the item it begins in, of the item it ends in
     Cut* cuts;                       // one for each CTA
+    // Sequences whose rows do not overlap have no more tiles than this (2^23 at most), and their units fit into 32 bits.  Where row_start is not ascending, which
+    // sequence() reports, there may be more: then none is taken.
+    uint32_t most_tiles;
     bool beside_decode;
 };
 
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     // and other scratch.  The wait is then made up for at the end, so that this kernel is never done before that one.
     if (!G.beside_decode) ptx::grid_dependency_wait();
 
-    const uint32_t per_head = make_plan(P, plan), units = per_head * B.n_kv_heads, runs = min(gridDim.x, units);
+    const uint32_t per_head = make_plan(P, G.most_tiles, plan), units = per_head * B.n_kv_heads, runs = min(gridDim.x, units);
     const uint32_t begin = blockIdx.x < runs ? start_of(blockIdx.x, units, runs) : 0, end = blockIdx.x < runs ? start_of(blockIdx.x + 1, units, runs) : 0;
     bool ok = true;
     auto wait = [&](uint32_t b, uint32_t parity) {
@@ -681,6 +681,7 @@ int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
     g.P = p;
     g.cuts = (Cut*)(p.scratch + kv4_counter_bytes() + decode_scratch_bytes(sms));
     g.beside_decode = p.few != 0;
+    g.most_tiles = (uint32_t)((uint64_t)p.B.n_rows * p.group / kRows) + p.B.n_seqs;
     g.records = (float*)(g.cuts + kMaxCtas);
     const uint32_t ctas = std::min(sms, kMaxCtas);
     cudaError_t e = gemm::launch_pdl(kv4_prompt_kernel<D>, ctas, kThreads, smem, stream, g);
