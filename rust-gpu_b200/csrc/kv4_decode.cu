@@ -6,7 +6,9 @@
 // logical operation.  Steps and lows stay outside of the products:
 //   score_j = a_j (q . (128 + c_j)) + b_j sum(q),   a_j = step_j, b_j = low_j - 128 step_j    (f32)
 //   o       = sum_j (p_j step_j) (c_j - 8) + sum_j p_j (low_j + 8 step_j)
-// where p_j step_j is rounded to bf16 (one rounding for each token and row, off by at most 2^-9 of its weight either way; the second sum stays f32).
+// where p_j step_j is rounded to bf16 (one rounding for each token and row, which a sum feels by at most 2^-8 of eight steps of the token's weight; the second sum stays f32).
+// (The codes are centred before the product: 128 + c there, and 136 p_j step_j off the second sum, is 2.5 % faster, but the product's own sums then grow so far beyond their
+// difference that an average of 4096 random values was off by 7e-3 in place of 2e-3.)
 // A code is never an infinity or a NaN, so a token that a row must not see can be cut off by its factors alone, whatever its parameters are.
 //
 // The work is the list of all (sequence, key/value head) items' chunks of 64 tokens, cut into equal contiguous runs, one for each warp: whatever the lengths, every warp
@@ -20,6 +22,7 @@ namespace {
 
 constexpr int kTok = 64;                                  // tokens of a chunk
 constexpr int kStages = 2;
+constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed what its row's weights are taken against
 constexpr uint32_t kManyParts = 4;                        // CTAs' parts that one warp joins; more are shared by a CTA's warps
 constexpr uint32_t kMaxParts = kMaxCtas;                  // parts of one item: at most one for each CTA
 
@@ -397,12 +400,12 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                     }
                 }
             }
-            // running maximum
+            // the maximum that weights are taken against moves where a lane finds it left behind
             float2 top[NT];
             bool moved = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                top[n] = make_float2(m[n][0], m[n][1]);
+                top[n] = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
                 for (int i = 0; i < kTok / 16; ++i)
 #pragma unroll
@@ -410,16 +413,17 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                         top[n].x = fmaxf(top[n].x, x[n][i][r].x);
                         top[n].y = fmaxf(top[n].y, x[n][i][r].y);
                     }
-#pragma unroll
-                for (int d = 4; d < 32; d *= 2) {
-                    top[n].x = fmaxf(top[n].x, __shfl_xor_sync(0xFFFFFFFFu, top[n].x, d));
-                    top[n].y = fmaxf(top[n].y, __shfl_xor_sync(0xFFFFFFFFu, top[n].y, d));
-                }
-                moved |= top[n].x > m[n][0] || top[n].y > m[n][1];
+                moved |= top[n].x > m[n][0] + kLag || top[n].y > m[n][1] + kLag;
             }
             if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) {
+                        top[n].x = fmaxf(top[n].x, __shfl_xor_sync(0xFFFFFFFFu, top[n].x, d));
+                        top[n].y = fmaxf(top[n].y, __shfl_xor_sync(0xFFFFFFFFu, top[n].y, d));
+                    }
+                    top[n] = make_float2(fmaxf(top[n].x, m[n][0]), fmaxf(top[n].y, m[n][1]));
                     const float2 less = make_float2(m[n][0] == top[n].x ? 1.0f : exp2_fast(m[n][0] - top[n].x), m[n][1] == top[n].y ? 1.0f : exp2_fast(m[n][1] - top[n].y));
                     m[n][0] = top[n].x;
                     m[n][1] = top[n].y;
