@@ -330,10 +330,11 @@ __device__ __forceinline__ void values_of(float (&x)[8], uint32_t w, float step,
 }
 
 // A warp takes a row, or `per_warp` of its 2 n_kv_heads rows of keys and values: a word of eight codes a lane, D / 8 lanes to a row, kAhead loads under way.
-// Bound by memory, mostly by what it writes: 16 sequences of 2200 tokens on average, 8 heads of 128, take 39 us at 4.7 TB/s (28 us at the rate of a plain copy); the codes through
-// integer conversions, a quarter of the other instructions' rate, 42 us; 5 blocks an SM 40, two loads ahead 39 to 40, eight 43.
+// 16 sequences of 2200 tokens on average, 8 heads of 128, are 183 MB and take 38 us at 4.8 TB/s (28 us at the rate of a plain copy): memory and the issue of instructions (77 % of
+// the cycles) are both close.  With the codes through integer conversions, at a quarter of the other instructions' rate, it took 42 us; with every place worked out anew
+// 39; 6 blocks an SM spill (42), two loads ahead and 7 blocks take 38 too, eight ahead 43.
 template <int D>
-__global__ void __launch_bounds__(256, 6) kv4_dequant_kernel(const __grid_constant__ Dequant P) {
+__global__ void __launch_bounds__(256, 5) kv4_dequant_kernel(const __grid_constant__ Dequant P) {
     constexpr uint32_t kLanes = D / 8, kAtOnce = 32 / kLanes, kAhead = 4;
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
@@ -350,26 +351,29 @@ __global__ void __launch_bounds__(256, 6) kv4_dequant_kernel(const __grid_consta
     const int token = s.len - s.rows + ((int)r - s.first_row);
     const uint8_t* block = token < 0 ? nullptr : block_of<D>(B, b, (uint32_t)token >> B.page_log2, 0);
     if (token >= 0 && !block) return;
-    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1), block_bytes = (D + 8) << B.page_log2;
-    for (uint32_t h = h0; h < h1; h += kAhead * kAtOnce) {
+    const uint32_t slot = (uint32_t)token & ((1u << B.page_log2) - 1), block_bytes = (D + 8) << B.page_log2, H = B.n_kv_heads;
+    // a value's places, less what its number among the heads is too large by
+    const uint32_t k_codes = slot * (D / 2) + 4 * e, v_codes = codes_at<D>(B.page_log2, 1) + k_codes - H * block_bytes;
+    const uint32_t k_params = params_at<D>(B.page_log2, 0) + 4 * slot, v_params = params_at<D>(B.page_log2, 1) + 4 * slot - H * block_bytes;
+    __nv_bfloat16 *const k_out = P.k_out + r * P.k_stride + 8 * e, *const v_out = P.v_out + r * P.v_stride + 8 * e;
+    for (uint32_t h = h0 + sub; h < h1; h += kAhead * kAtOnce) {
         uint32_t w[kAhead], p[kAhead];
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
-            const uint32_t at = h + a * kAtOnce + sub, which = at < B.n_kv_heads ? 0 : 1, head = which ? at - B.n_kv_heads : at;
+            const uint32_t at = h + a * kAtOnce;
             w[a] = p[a] = 0;
             if (at < h1 && block) {
-                const uint8_t* of = block + (uint64_t)head * block_bytes;
-                w[a] = *(const uint32_t*)(of + codes_at<D>(B.page_log2, which) + slot * (D / 2) + 4 * e);
-                p[a] = *(const uint32_t*)(of + params_at<D>(B.page_log2, which) + 4 * slot);
+                w[a] = *(const uint32_t*)(block + (at * block_bytes + (at < H ? k_codes : v_codes)));
+                p[a] = *(const uint32_t*)(block + (at * block_bytes + (at < H ? k_params : v_params)));
             }
         }
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
-            const uint32_t at = h + a * kAtOnce + sub, which = at < B.n_kv_heads ? 0 : 1, head = which ? at - B.n_kv_heads : at;
-            if (at >= h1) continue;
+            const uint32_t at = h + a * kAtOnce;
+            if (at >= h1) break;
             float x[8];
             values_of(x, w[a], param_step(p[a]), param_low(p[a]));
-            *(uint4*)((which ? P.v_out : P.k_out) + r * (which ? P.v_stride : P.k_stride) + head * D + 8 * e) = pack8(x);
+            *(uint4*)(at < H ? k_out + at * D : v_out + (at - H) * D) = pack8(x);
         }
     }
 }
