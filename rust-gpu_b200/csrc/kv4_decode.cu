@@ -14,6 +14,12 @@
 // The work is the list of all (sequence, key/value head) items' chunks of 64 tokens, cut into equal contiguous runs, one for each warp: whatever the lengths, every warp
 // reads as much as the next.  A warp has its own two buffers, filled by bulk copies (the blocks of a chunk are contiguous pieces of the pages), and its own running
 // maximum and sums.  Items that end up in several warps are joined, first inside the CTA, then between CTAs by the one that arrives last, always in order.
+//
+// 128 sequences of 5100 tokens on average, 8 key/value heads of 128 and 8 rows each (713 MB), take 161 to 168 us, 4.3 TB/s (109 us at the rate of a plain copy): three warps a
+// scheduler with 168 registers, the ALU busy for 62 % of the cycles and an instruction issued in 57 %, most of them taking codes apart.  One row on 131072 tokens (143 MB)
+// takes 44 us: 5 until a warp has its first chunk, 24 of chunks, 5 for two joins.  32 sequences' five rows in a window of 1000, 16 heads of 64 (36 MB): 25 us, 5 before, 8 of
+// chunks (3 or 4 a warp), 4 of joins, and the launch.  8, 10 or 11 warps and chunks of 32 tokens were slower; codes by way of fp16 (half the shifts) 3 % faster for keys, but values'
+// weights leave its range.
 #include "kv4_attention.cuh"
 
 namespace t0 {

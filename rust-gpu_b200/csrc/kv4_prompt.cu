@@ -7,11 +7,20 @@
 // back), so the sums stay far inside f32 and O is rarely touched.
 //   warps 0-3, 4-7  softmax of tile 0 and 1, and their results     warps 8-11   codes -> bf16, K and V into rings of two stages
 //   warp 12         issues the products                            warps 13-15  queries of the next item into shared memory
-// Keys and values are rounded to bf16 here (step * code + low, once), which a score feels by at most 2^-8 of sum |q k|.  A value row that is NaN is put in as zeros and
+// Keys, values and weights are rounded to bf16 for the products (step * code + low, once; the sums of weights are of unrounded ones): a score feels that by at most 2^-8 of
+// sum |q k|, a result by 2^-8 of sum p |v| for each of weights and values.  Results of random numbers are off by 4.4e-3 of their size, 1.7e-3 of which is their own rounding.
+// Keys and queries in fp16, kept in range by powers of two for each chunk and row, brought that to 2.8e-3 and took 4 to 18 % longer: the powers have to be agreed on by
+// all warps that make a chunk's keys before the first is stored.  A value row that is NaN is put in as zeros and
 // its key as NaN: a row that sees the token becomes NaN through its score, a row that must not see it has weight 0, and 0 x 0 adds nothing.
 //
 // The units of work are all items' chunks, and kItemUnits for what an item costs beside them, in equal contiguous runs, one for each CTA.  Items whose chunks end up in
 // several CTAs leave parts (O, m, l) that a second kernel joins.
+//
+// 8192 tokens on themselves, 32 query and 8 key/value heads of 128, take 595 us, 925 TFLOP/s of what the mask leaves; 2048 behind 8192 others 330 us.  A chunk takes a CTA 3700
+// clocks, of which the products need 2048 and the powers of two 2048 (a scheduler makes four a clock): the softmax warps work for 2800 of them and wait for the rest.  Over
+// more than a few launches the clock falls from 1965 to 1725 MHz at the board's 1000 W (534 us before that), so that less work in one unit saves little: no scores in one
+// product a chunk (610 us), maxima of three numbers (600), a quarter of the powers by a polynomial (605) nor eight warps for the codes were faster; without the codes'
+// work altogether 544.
 #include "kv4_attention.cuh"
 
 namespace t0 {
@@ -623,7 +632,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     if (G.beside_decode) ptx::grid_dependency_wait();
 }
 
-// Joins the parts of the items whose chunks several CTAs of the launch before worked on.  Block (c, z): the item that the boundary before CTA c cuts, if c is the first one
+// Joins the parts of the items whose chunks several CTAs of the launch before worked on: sum_i 2^(m_i - m) O_i over sum_i 2^(m_i - m) l_i, in order.  Bound by latency and by
+// the reads of the parts (133 KB each, 39 MB at most, from L2): 17 us for all 148 CTAs' by itself, from cold.  Block (c, z): the item that the boundary before CTA c cuts, if c is the first one
 // to cut it; z: a slice of its rows.  A thread has a row and a quarter of its numbers.
 constexpr int kJoinRows = 64, kJoinThreads = kJoinRows * 4;
 template <int D>
