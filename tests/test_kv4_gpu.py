@@ -454,6 +454,43 @@ def test_sequences_with_the_same_rows_are_reported_and_do_no_harm(t0, own, dim):
     dev.free()
 
 
+@pytest.mark.parametrize("dim, page", [(128, 64), (64, 16)])
+def test_pages_beyond_four_gigabytes(t0, own, dim, page):
+    # the same calls on a small cache and on one whose pages lie at both ends of 4.8 GB: the same rows, bit for bit
+    dev = Device(own)
+    rng = np.random.default_rng(12)
+    heads, lens = 8, [200, 65]
+    cache = ref.Cache(rng, lens, heads, dim, page)
+    each = t0.kv4_page_bytes(page, heads, dim)
+    n_pages = 4_800_000_000 // each
+    far = np.where((cache.table >= 0) & (cache.table % 3 > 0), cache.table + n_pages - cache.n_pages, cache.table).astype(np.int32)
+    big = own.alloc(n_pages * each)
+    dev.bufs.append(big)
+    x = ref.bf16_bits(rng.standard_normal((sum(lens), 2 * heads, dim)).astype(np.float32))
+    rows_in, lens_buf, got = dev.up(x), dev.up(np.array(lens, np.int32)), []
+    for pages, count, table in ((dev.up(np.zeros(cache.n_pages * each, np.uint8)), cache.n_pages, cache.table), (big, n_pages, far)):
+        table_buf, out = dev.up(table), []
+
+        def batch(rows):
+            start = dev.up(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+            return own.kv4_batch(pages.gpu_addr(), table_buf.gpu_addr(), lens_buf.gpu_addr(), n_pages=count, page_size=page, n_kv_heads=heads, head_dim=dim, n_seqs=2,
+                                 table_stride=cache.stride, n_rows=sum(rows), max_rows=max(rows), row_start=start.gpu_addr())
+
+        wide = 2 * heads * dim
+        own.kv4_append(batch(lens), own.kv4_append_args(rows_in.gpu_addr(), rows_in.gpu_addr() + wide, k_stride=wide, v_stride=wide))
+        k, v = (dev.up(np.zeros((sum(lens), heads, dim), np.uint16)) for _ in range(2))
+        own.kv4_dequant(batch(lens), own.kv4_dequant_args(k.gpu_addr(), v.gpu_addr()))
+        for rows in ([1, 1], [40, 30]):
+            y = dev.up(np.zeros((sum(rows), 2 * heads, dim), np.uint16))
+            own.kv4_attention(batch(rows), own.kv4_attention_args(rows_in.gpu_addr(), y.gpu_addr(), n_q_heads=2 * heads, scale=0.1))
+            out.append((y, sum(rows) * wide))
+        own.synchronize()
+        got.append([b.read(2 * n, np.uint16) for b, n in out + [(k, sum(lens) * wide // 2), (v, sum(lens) * wide // 2)]])
+    for a, b in zip(*got):
+        assert a.any() and np.array_equal(a, b)
+    dev.free()
+
+
 def test_positions_outside_the_rope_table(t0, own):
     dev = Device(own)
     rng = np.random.default_rng(2)
