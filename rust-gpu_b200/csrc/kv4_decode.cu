@@ -15,9 +15,9 @@
 // reads as much as the next.  A warp has its own two buffers, filled by bulk copies (the blocks of a chunk are contiguous pieces of the pages), and its own running
 // maximum and sums.  Items that end up in several warps are joined, first inside the CTA, then between CTAs by the one that arrives last, always in order.
 //
-// 128 sequences of 5100 tokens on average, 8 key/value heads of 128 and 8 rows each (713 MB), take 161 to 168 us, 4.3 TB/s (109 us at the rate of a plain copy): three warps a
+// 128 sequences of 5100 tokens on average, 8 key/value heads of 128 and 8 rows each (713 MB), take 156 to 167 us, 4.4 TB/s (109 us at the rate of a plain copy): three warps a
 // scheduler with 168 registers, the ALU busy for 62 % of the cycles and an instruction issued in 57 %, most of them taking codes apart.  One row on 131072 tokens (143 MB)
-// takes 44 us: 5 until a warp has its first chunk, 24 of chunks, 5 for two joins.  32 sequences' five rows in a window of 1000, 16 heads of 64 (36 MB): 25 us, 5 before, 8 of
+// takes 44 us: 5 until a warp has its first chunk, 24 of chunks, 5 for two joins.  32 sequences' five rows in a window of 1000, 16 heads of 64 (36 MB): 23.6 us, 4 before, 8 of
 // chunks (3 or 4 a warp), 4 of joins, and the launch.  8, 10 or 11 warps and chunks of 32 tokens were slower; codes by way of fp16 (half the shifts) 3 % faster for keys, but values'
 // weights leave its range.
 #include "kv4_attention.cuh"
@@ -108,8 +108,7 @@ __device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
     }
     if ((tid & 31) == 31) plan.warp_sum[tid / 32] = upto;
     __syncthreads();
-    uint32_t before = 0;
-    for (uint32_t w = 0; w < tid / 32; ++w) before += plan.warp_sum[w];
+    const uint32_t before = __reduce_add_sync(0xFFFFFFFFu, (tid & 31) < tid / 32 ? plan.warp_sum[tid & 31] : 0);
     plan.prefix[tid + 1] = before + upto;
     if (tid == 0) {
         plan.prefix[0] = 0;
@@ -119,15 +118,16 @@ __device__ __forceinline__ uint32_t make_plan(const Attention& P, Plan& plan) {
     return plan.prefix[kThreads] * P.B.n_kv_heads;           // (less than 2^31: checked on the host)
 }
 
-// The item that unit u belongs to (u < all units).
+// The item that unit u belongs to (u < all units).  By a whole warp, for one u: two votes in place of nine dependent steps took 0.5 us off the smallest call (8.0 us) and
+// 1.4 off one whose warps have three or four chunks each (25.0).
 template <int kThreads>
 __device__ __forceinline__ Item item_of(const Attention& P, const Plan& plan, uint32_t u) {
     const uint32_t H = P.B.n_kv_heads;
-    uint32_t lo = 0, hi = kThreads;                       // the last thread whose prefix does not exceed u
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (plan.prefix[mid] * H <= u) lo = mid; else hi = mid;
-    }
+    constexpr uint32_t kStep = kThreads / 32;             // the last thread whose prefix does not exceed u: the step of 32, then the place in it
+    static_assert(kStep <= 32 && kThreads % 32 == 0);
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = (__popc(__ballot_sync(0xFFFFFFFFu, plan.prefix[lane * kStep] * H <= u)) - 1) * kStep;
+    lo += __popc(__ballot_sync(0xFFFFFFFFu, lane < kStep && plan.prefix[lo + min(lane, kStep - 1)] * H <= u)) - 1;
     Item it;
     it.b = lo * plan.per_thread;
     uint32_t at = plan.prefix[lo] * H;
