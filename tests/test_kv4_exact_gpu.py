@@ -1,0 +1,58 @@
+"""Attention over the four-bit cache on the GPU, held to the roundings that each kernel makes (tests/kv4_bounds.py; tests/test_kv4_bounds.py shows that results which lost a part, took a
+neighbour's place or have a mask off by one are over these bounds).  The numbers at the far ends of the types are here too."""
+import numpy as np
+import pytest
+
+import kv4_bounds as kb
+import kv4_reference as ref
+from test_kv4_gpu import Device, bounds_error, dev, make_batch, own, rope_table  # noqa: F401  (fixtures)
+from test_recorded_launches_gpu import Driver
+
+pytestmark = pytest.mark.gpu
+
+
+def cache_of(rng, k, v, page, copies=1):
+    """A cache of one sequence with these keys and values, `copies` of it on the same pages."""
+    cache = ref.Cache(rng, [k.shape[0]], k.shape[1], k.shape[2], page)
+    cache.k, cache.v = [k], [v]
+    pool = cache.pool()
+    cache.lens, cache.table = cache.lens * copies, np.repeat(cache.table, copies, 0)
+    return cache, pool
+
+
+def attend(t0, dev, b, q, scale, window=0):  # noqa: F811
+    """q [rows, heads, dim] -> y, f64."""
+    rt = dev.rt
+    bits = ref.bf16_bits(q.astype(np.float32))
+    qb, y = dev.up(bits), dev.up(np.full(bits.shape, 0xABCD, np.uint16))
+    rt.kv4_attention(b, rt.kv4_attention_args(qb.gpu_addr(), y.gpu_addr(), n_q_heads=q.shape[1], scale=scale, window=window))
+    rt.synchronize()
+    return ref.from_bits(y.read(bits.nbytes, np.uint16)).reshape(q.shape).astype(np.float64)
+
+
+def held_to(t0, dev, k, v, page, q, scale, window=0, whole_q=True):  # noqa: F811
+    n, rows = k.shape[0], q.shape[0]
+    cache, pool = cache_of(np.random.default_rng(n), k, v, page)
+    got = attend(t0, dev, make_batch(t0, dev, cache, dev.up(pool), [rows], uniform=True), q, scale, window)
+    e = kb.Exact(q, k, v, np.arange(n - rows, n), np.float64(np.float32(scale)), window, whole_q)
+    over = e.over(got)
+    assert over.max() <= 0, f"row {np.argmax(over)} is {over.max()} over its bound"
+
+
+@pytest.mark.parametrize("case", kb.LONG)
+def test_every_run_of_a_long_sequence_counts(t0, rt, dev, case):  # noqa: F811
+    k, v, _, qs, scale = kb.long_case(*case)
+    for q in qs:
+        held_to(t0, dev, k, v, case[5], q, scale)
+
+
+@pytest.mark.parametrize("case", kb.EDGES)
+def test_rows_see_what_the_mask_leaves_and_no_more(t0, rt, dev, case):  # noqa: F811
+    k, v, q, scale = kb.edge_case(*case)
+    held_to(t0, dev, k, v, case[5], q, scale, case[6])
+
+
+@pytest.mark.parametrize("case", kb.RANDOM)
+def test_random_scores(t0, rt, dev, case):  # noqa: F811
+    k, v, q, scale = kb.random_case(*case)
+    held_to(t0, dev, k, v, case[5], q, scale, whole_q=False)
