@@ -28,7 +28,8 @@ namespace {
 
 constexpr int kTok = 64;                                  // tokens of a chunk
 constexpr int kStages = 2;
-constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed what its row's weights are taken against
+constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed its row's maximum so far; weights are 2^(score - maximum - kLag),
+                                                          // so that none is above one: a weight times a step near the end of f32's range is no infinity
 constexpr uint32_t kManyParts = 4;                        // CTAs' parts that one warp joins; more are shared by a CTA's warps
 constexpr uint32_t kMaxParts = kMaxCtas;                  // parts of one item: at most one for each CTA
 
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                     }
                 }
             }
-            // the maximum that weights are taken against moves where a lane finds it left behind
+            // the maximum moves where a lane finds it left behind
             float2 top[NT];
             bool moved = false;
 #pragma unroll
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
             uint32_t pf[NT][kTok / 16][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float2 minus = make_float2(m[n][0] == -INFINITY ? 0.0f : -m[n][0], m[n][1] == -INFINITY ? 0.0f : -m[n][1]);
+                const float2 minus = make_float2(m[n][0] == -INFINITY ? 0.0f : -m[n][0] - kLag, m[n][1] == -INFINITY ? 0.0f : -m[n][1] - kLag);
 #pragma unroll
                 for (int i = 0; i < kTok / 16; ++i)
 #pragma unroll

@@ -3,8 +3,8 @@
 // An item is 256 rows (pairs of token and query head of one key/value head, two tiles of 128) against the chunks of 128 tokens that any of them sees.  Per chunk
 //   S = Q K^T (shared memory x shared memory -> tensor memory),  P = 2^(S - m) (one thread a row),  O += P V (P in tensor memory, over S's own columns)
 // half a chunk at a time: the 512 columns of tensor memory are O of both tiles and, for each, S of two halves, so that the scores of one half are there when the softmax
-// warps are done with the other.  The maximum a row's weights are taken against only moves when it is left behind by more than 2^8 (then O is read, scaled and written
-// back), so the sums stay far inside f32 and O is rarely touched.
+// warps are done with the other.  The maximum only moves when it is left behind by more than 2^8 (then O is read, scaled and written back), so that O is rarely touched; weights are taken
+// against 2^8 times the maximum, so that none is above one and a sum of them and of values leaves f32 only where a sum against the true maximum could.
 //   warps 0-3, 4-7  softmax of tile 0 and 1, and their results     warps 8-11   codes -> bf16, K and V into rings of two stages
 //   warp 12         issues the products                            warps 13-15  queries of the next item into shared memory
 // Keys, values and weights are rounded to bf16 for the products (step * code + low, once; the sums of weights are of unrounded ones): a score feels that by at most 2^-8 of
@@ -32,7 +32,7 @@ constexpr int kDequantWarps = 4;
 constexpr int kThreads = (12 + kDequantWarps) * 32;
 constexpr uint32_t kIssuer = 8 + kDequantWarps;           // the warp that issues the products
 constexpr uint32_t kItemUnits = 3;                        // an item's queries, results and idle times in chunks' time (10600 of 3800 clocks, measured on a prompt of 8192 tokens)
-constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed what a row's weights are taken against
+constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed its row's maximum so far; weights are 2^(score - maximum - kLag)
 
 template <int D> constexpr uint32_t tile_bytes() { return kTile * D * 2; }
 template <int D> constexpr uint32_t smem_bytes() { return 6 * tile_bytes<D>() + 1024 + 512; }
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                                 ptx::tmem_st_32x32b_x8(o_col + 8 * k, o);
                             }
                         }
-                        const float minus = m == -INFINITY ? 0.0f : -m;
+                        const float minus = m == -INFINITY ? 0.0f : -m - kLag;
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             uint32_t y[16];

@@ -56,3 +56,22 @@ def test_rows_see_what_the_mask_leaves_and_no_more(t0, rt, dev, case):  # noqa: 
 def test_random_scores(t0, rt, dev, case):  # noqa: F811
     k, v, q, scale = kb.random_case(*case)
     held_to(t0, dev, k, v, case[5], q, scale, whole_q=False)
+
+
+@pytest.mark.parametrize("rows, copies", [(1, 2000), (2, 1), (20, 1), (20, 40)])
+@pytest.mark.parametrize("size", [3e38, 1e36])
+def test_values_near_the_end_of_the_range(t0, rt, dev, rows, copies, size):  # noqa: F811
+    # the token with such values comes behind others and has 2^6.5 times their weights: less than what moves the maximum that weights are taken against.  (Many copies: several chunks of the
+    # sequence are one warp's work.)
+    rng = np.random.default_rng(22)
+    n, dim, at = 200, 64, 150 if rows <= 16 else 100
+    k, v = np.zeros((n, 1, dim), np.float32), rng.standard_normal((n, 1, dim)).astype(np.float32)
+    k[at, 0, 0] = 4.5
+    v[at, 0] = np.where(rng.integers(0, 2, dim), 0.49, -0.49) * size
+    q = np.zeros((rows, 1, dim))
+    q[:, :, 0] = 1.0
+    cache, pool = cache_of(rng, k, v, 16, copies)
+    got = attend(t0, dev, make_batch(t0, dev, cache, dev.up(pool), [rows] * copies, uniform=True), np.tile(q, (copies, 1, 1)), 1.0)
+    e = kb.Exact(q, k, v, np.arange(n - rows, n), 1.0, 0, True)
+    for y in got.reshape(copies, rows, 1, dim):
+        assert e.over(y).max() <= 0
