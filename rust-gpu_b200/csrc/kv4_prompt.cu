@@ -11,7 +11,8 @@
 // sum |q k|, a result by 2^-8 of sum p |v| for each of weights and values.  Results of random numbers are off by 4.4e-3 of their size, 1.7e-3 of which is their own rounding.
 // Keys and queries in fp16, kept in range by powers of two for each chunk and row, brought that to 2.8e-3 and took 4 to 18 % longer: the powers have to be agreed on by
 // all warps that make a chunk's keys before the first is stored.  A value row that is NaN is put in as zeros and
-// its key as NaN: a row that sees the token becomes NaN through its score, a row that must not see it has weight 0, and 0 x 0 adds nothing.
+// its key as NaN: a row that sees the token becomes NaN through its score, a row that must not see it has weight 0, and 0 x 0 adds nothing.  For the same reason a value
+// whose rounding to bf16 would be an infinity is bf16's largest number here.
 //
 // The units of work are all items' chunks, and kItemUnits for what an item costs beside them, in equal contiguous runs, one for each CTA.  Items whose chunks end up in
 // several CTAs leave parts (O, m, l) that a second kernel joins.
@@ -214,6 +215,16 @@ __device__ __forceinline__ uint32_t value_of(uint32_t w, int i, uint32_t k128, _
     const __nv_bfloat162 k = __nv_bfloat162(__ushort_as_bfloat16(0x4300), __ushort_as_bfloat16(0x4300));
     const __nv_bfloat162 v = __hfma2(__hsub2(*(const __nv_bfloat162*)&x, k), step, low);
     return *(const uint32_t*)&v;
+}
+// infinities (of finite parameters, so positive ones) made bf16's largest number; a NaN stays one
+__device__ __forceinline__ uint32_t bounded(uint32_t x) {
+    const __nv_bfloat162 v = __hmin2_nan(*(const __nv_bfloat162*)&x, __nv_bfloat162(__ushort_as_bfloat16(0x7F7F), __ushort_as_bfloat16(0x7F7F)));
+    return *(const uint32_t*)&v;
+}
+// Whether the largest value that a row's parameters allow, 15 step + low, leaves bf16 where the parameters are finite.
+__device__ __forceinline__ bool leaves_bf16(uint32_t params) {
+    const __nv_bfloat16 top = __hfma(__ushort_as_bfloat16(0x4170), __ushort_as_bfloat16((uint16_t)params), __ushort_as_bfloat16((uint16_t)(params >> 16)));
+    return __bfloat16_as_ushort(top) == 0x7F80;
 }
 __device__ __forceinline__ __nv_bfloat162 twice(uint32_t bits16) {
     const uint32_t x = bits16 * 0x10001u;
@@ -482,16 +493,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                 }
             };
             auto store = [&](int which, uint32_t base, const uint32_t (&params)[kEach]) {
+                auto put = [&](auto with_bound) {
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    const __nv_bfloat162 step = twice(params[i] & 0xFFFFu), low = twice(params[i] >> 16);
+                    for (int i = 0; i < kEach; ++i) {
+                        const __nv_bfloat162 step = twice(params[i] & 0xFFFFu), low = twice(params[i] >> 16);
 #pragma unroll
-                    for (int j = 0; j < kWords; ++j) {
-                        const uint32_t w = swapped ? raw[which][i][(j ^ 2) % kWords] : raw[which][i][j];
-                        const uint32_t v0 = value_of(w, 0, k128, step, low), v1 = value_of(w, 1, k128, step, low), v2 = value_of(w, 2, k128, step, low), v3 = value_of(w, 3, k128, step, low);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + unit_off[j] + i * (kRowStep * 128)), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
+                        for (int j = 0; j < kWords; ++j) {
+                            const uint32_t w = swapped ? raw[which][i][(j ^ 2) % kWords] : raw[which][i][j];
+                            uint32_t v[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                v[k] = value_of(w, k, k128, step, low);
+                                if constexpr (decltype(with_bound)::value) v[k] = bounded(v[k]);
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + unit_off[j] + i * (kRowStep * 128)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                        }
                     }
-                }
+                };
+                bool far = false;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) far |= leaves_bf16(params[i]);
+                if (__any_sync(0xFFFFFFFFu, far)) put(std::true_type{});
+                else put(std::false_type{});
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
             };

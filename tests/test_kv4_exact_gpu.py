@@ -75,3 +75,27 @@ def test_values_near_the_end_of_the_range(t0, rt, dev, rows, copies, size):  # n
     e = kb.Exact(q, k, v, np.arange(n - rows, n), 1.0, 0, True)
     for y in got.reshape(copies, rows, 1, dim):
         assert e.over(y).max() <= 0
+
+
+@pytest.mark.parametrize("dim, page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_a_number_beyond_bf16_stays_out_of_rows_that_do_not_see_it(t0, rt, dev, dim, page, what):  # noqa: F811
+    # step 2.28e37, low -1.73e36: the top code's value, 3.397e38, is a number in f32 and rounds to an infinity in bf16.  Nothing of it may reach rows before the token; rows that see it get
+    # their share, and a token of the same chunk that is NaN stays one.
+    rng = np.random.default_rng(21)
+    n, rows, at, bad = 150, 60, 120, 140
+    k, v = (rng.standard_normal((n, 1, dim)).astype(np.float32) for _ in range(2))
+    x = k if what == "k" else v
+    x[at] = 0.0
+    x[at, 0, :2] = 3.376e38, -1.72e36
+    assert np.isinf(kb.bf16_once(ref.held(x[at]))).any() and np.isfinite(ref.held(x[at])).all()
+    q = ref.bf16_round(rng.standard_normal((rows, 4, dim)).astype(np.float32)).astype(np.float64)
+    if what == "k":
+        q = np.copysign(2.0**-124, q)                                       # scores of the size of one at that token, of nothing at the others
+    spoilt = x.copy()
+    spoilt[bad, 0, 3] = np.nan
+    cache, pool = cache_of(rng, spoilt if what == "k" else k, spoilt if what == "v" else v, page)
+    got = attend(t0, dev, make_batch(t0, dev, cache, dev.up(pool), [rows], uniform=True), q, 0.125)
+    tokens = np.arange(n - rows, n)
+    e = kb.Exact(q, k, v, tokens, 0.125, 0, True)
+    assert e.over(got)[tokens < bad].max() <= 0 and np.isnan(got[tokens >= bad]).all()
