@@ -492,29 +492,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     }
                 }
             };
-            auto store = [&](int which, uint32_t base, const uint32_t (&params)[kEach]) {
-                auto put = [&](auto with_bound) {
+            auto store = [&](int which, uint32_t base, const uint32_t (&params)[kEach], bool far) {
 #pragma unroll
-                    for (int i = 0; i < kEach; ++i) {
-                        const __nv_bfloat162 step = twice(params[i] & 0xFFFFu), low = twice(params[i] >> 16);
+                for (int i = 0; i < kEach; ++i) {
+                    const __nv_bfloat162 step = twice(params[i] & 0xFFFFu), low = twice(params[i] >> 16);
 #pragma unroll
-                        for (int j = 0; j < kWords; ++j) {
-                            const uint32_t w = swapped ? raw[which][i][(j ^ 2) % kWords] : raw[which][i][j];
-                            uint32_t v[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                v[k] = value_of(w, k, k128, step, low);
-                                if constexpr (decltype(with_bound)::value) v[k] = bounded(v[k]);
-                            }
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + unit_off[j] + i * (kRowStep * 128)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-                        }
+                    for (int j = 0; j < kWords; ++j) {
+                        const uint32_t w = swapped ? raw[which][i][(j ^ 2) % kWords] : raw[which][i][j];
+                        const uint32_t v0 = value_of(w, 0, k128, step, low), v1 = value_of(w, 1, k128, step, low), v2 = value_of(w, 2, k128, step, low), v3 = value_of(w, 3, k128, step, low);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + unit_off[j] + i * (kRowStep * 128)), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
                     }
-                };
-                bool far = false;
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) far |= leaves_bf16(params[i]);
-                if (__any_sync(0xFFFFFFFFu, far)) put(std::true_type{});
-                else put(std::false_type{});
+                }
+                if (far) {                                  // hardly ever: over this thread's units once more, in a loop (bounds in the lines above, in a second copy of them, took 3 % of a mixed batch)
+#pragma unroll 1
+                    for (uint32_t n = 0; n < kEach * kWords; ++n) {
+                        const uint32_t unit = part * kWords + n % kWords, at = base + unit / 8 * kPanel + (tid / 4 + n / kWords * kRowStep) * 128 + ((unit % 8 ^ (tid / 4 & 7)) << 4);
+                        uint32_t v0, v1, v2, v3;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v0), "=r"(v1), "=r"(v2), "=r"(v3) : "r"(at) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(bounded(v0)), "r"(bounded(v1)), "r"(bounded(v2)), "r"(bounded(v3)) : "memory");
+                    }
+                }
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
             };
@@ -529,19 +526,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             while (ok && at_hand) {
                 // parameters of this chunk; those of a NaN value go into its key
                 uint32_t kq[kEach], vq[kEach];
+                bool far = false;
 #pragma unroll
                 for (int i = 0; i < kEach; ++i) {
                     const bool bad = (vp[i] & 0x7F800000u) == 0x7F800000u || (vp[i] & 0x7F80u) == 0x7F80u;
                     kq[i] = !there[i] ? 0u : bad ? 0x7FC07FC0u : kp[i];
                     vq[i] = !there[i] || bad ? 0u : vp[i];
+                    far |= leaves_bf16(kq[i]) || leaves_bf16(vq[i]);
                 }
+                far = __any_sync(0xFFFFFFFFu, far);
                 if (!wait(k_empty(stage), phase ^ 1)) break;
-                store(0, k_smem + stage * kTileBytes, kq);
+                store(0, k_smem + stage * kTileBytes, kq, far);
                 ptx::mbar_arrive_if(k_full(stage), lane == 0);
                 at_hand = more;
                 if (more) load(0);
                 if (!wait(v_empty(stage), phase ^ 1)) break;
-                store(1, v_smem + stage * kTileBytes, vq);
+                store(1, v_smem + stage * kTileBytes, vq, far);
                 ptx::mbar_arrive_if(v_full(stage), lane == 0);
                 if (more) {
                     load(1);
