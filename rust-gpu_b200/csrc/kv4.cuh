@@ -103,5 +103,18 @@ __device__ __forceinline__ constexpr int code_shift(int e) { return 4 * ((e >> 1
 __device__ __forceinline__ float param_step(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float param_low(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 
+// step * code + low, rounded once, of nibbles i and i + 4: 128 + code in a bf16, less 128, times step plus low
+__device__ __forceinline__ uint32_t value_of(uint32_t w, int i, uint32_t k128, __nv_bfloat162 step, __nv_bfloat162 low) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(k128));
+    const __nv_bfloat162 k = __nv_bfloat162(__ushort_as_bfloat16(0x4300), __ushort_as_bfloat16(0x4300));
+    const __nv_bfloat162 v = __hfma2(__hsub2(*(const __nv_bfloat162*)&x, k), step, low);
+    return *(const uint32_t*)&v;
+}
+__device__ __forceinline__ __nv_bfloat162 twice(uint32_t bits16) {
+    const uint32_t x = bits16 * 0x10001u;
+    return *(const __nv_bfloat162*)&x;
+}
+
 }  // namespace kv4
 }  // namespace t0

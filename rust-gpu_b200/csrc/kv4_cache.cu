@@ -313,26 +313,10 @@ struct Dequant {
     uint32_t per_warp;
 };
 
-// The eight numbers of a word of codes.  A nibble at bit k of the mantissa of 2^(23 - k) adds the code to it, exactly, and taking the power away leaves the code: no nibble of
-// the lower five has to be shifted, and none is converted.  step * code has twelve bits at most, so that it is exact too and the sum rounded once.
-__device__ __forceinline__ void values_of(float (&x)[8], uint32_t w, float step, float low) {
-    const uint32_t high = w >> 12;
-    auto place = [](int i) { return code_shift(i) < 20 ? code_shift(i) : code_shift(i) - 12; };
-    auto power = [&](int i) { return (uint32_t)(150 - place(i)) << 23; };
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const uint32_t a = ((code_shift(i) < 20 ? w : high) & (15u << place(i))) | power(i), b = ((code_shift(i + 1) < 20 ? w : high) & (15u << place(i + 1))) | power(i + 1);
-        const float2 code = __fadd2_rn(make_float2(__uint_as_float(a), __uint_as_float(b)), make_float2(-__uint_as_float(power(i)), -__uint_as_float(power(i + 1))));
-        const float2 y = __ffma2_rn(code, make_float2(step, step), make_float2(low, low));
-        x[i] = y.x;
-        x[i + 1] = y.y;
-    }
-}
-
 // A warp takes a row, or `per_warp` of its 2 n_kv_heads rows of keys and values: a word of eight codes a lane, D / 8 lanes to a row, kAhead loads under way.
-// 16 sequences of 2200 tokens on average, 8 heads of 128, are 183 MB and take 38 us at 4.8 TB/s (28 us at the rate of a plain copy): memory and the issue of instructions (77 % of
-// the cycles) are both close.  With the codes through integer conversions, at a quarter of the other instructions' rate, it took 42 us; with every place worked out anew
-// 39; 6 blocks an SM spill (42), two loads ahead and 7 blocks take 38 too, eight ahead 43.
+// A value is step * code + low rounded to bf16 in one step (value_of): a sum in f32 first, rounded again for the result, was a bf16 number off wherever f32 loses what decides a tie, and
+// longer: 16 sequences of 2200 tokens on average, 8 heads of 128, are 183 MB and take 35.3 us at 5.2 TB/s (28 us at the rate of a plain copy), 38.2 in that form.  With every place worked
+// out anew for a head it was 0.5 us more.
 template <int D>
 __global__ void __launch_bounds__(256, 5) kv4_dequant_kernel(const __grid_constant__ Dequant P) {
     constexpr uint32_t kLanes = D / 8, kAtOnce = 32 / kLanes, kAhead = 4;
@@ -356,6 +340,8 @@ __global__ void __launch_bounds__(256, 5) kv4_dequant_kernel(const __grid_consta
     const uint32_t k_codes = slot * (D / 2) + 4 * e, v_codes = codes_at<D>(B.page_log2, 1) + k_codes - H * block_bytes;
     const uint32_t k_params = params_at<D>(B.page_log2, 0) + 4 * slot, v_params = params_at<D>(B.page_log2, 1) + 4 * slot - H * block_bytes;
     __nv_bfloat16 *const k_out = P.k_out + r * P.k_stride + 8 * e, *const v_out = P.v_out + r * P.v_stride + 8 * e;
+    uint32_t k128;
+    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(k128));
     for (uint32_t h = h0 + sub; h < h1; h += kAhead * kAtOnce) {
         uint32_t w[kAhead], p[kAhead];
 #pragma unroll
@@ -371,9 +357,9 @@ __global__ void __launch_bounds__(256, 5) kv4_dequant_kernel(const __grid_consta
         for (uint32_t a = 0; a < kAhead; ++a) {
             const uint32_t at = h + a * kAtOnce;
             if (at >= h1) break;
-            float x[8];
-            values_of(x, w[a], param_step(p[a]), param_low(p[a]));
-            *(uint4*)(at < H ? k_out + at * D : v_out + (at - H) * D) = pack8(x);
+            const __nv_bfloat162 step = twice(p[a] & 0xFFFFu), low = twice(p[a] >> 16);
+            *(uint4*)(at < H ? k_out + at * D : v_out + (at - H) * D) =
+                make_uint4(value_of(w[a], 0, k128, step, low), value_of(w[a], 1, k128, step, low), value_of(w[a], 2, k128, step, low), value_of(w[a], 3, k128, step, low));
         }
     }
 }

@@ -208,14 +208,6 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&p;
 }
-// step * code + low, rounded once, of nibbles i and i + 4: 128 + code in a bf16, less 128, times step plus low
-__device__ __forceinline__ uint32_t value_of(uint32_t w, int i, uint32_t k128, __nv_bfloat162 step, __nv_bfloat162 low) {
-    uint32_t x;
-    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(k128));
-    const __nv_bfloat162 k = __nv_bfloat162(__ushort_as_bfloat16(0x4300), __ushort_as_bfloat16(0x4300));
-    const __nv_bfloat162 v = __hfma2(__hsub2(*(const __nv_bfloat162*)&x, k), step, low);
-    return *(const uint32_t*)&v;
-}
 // infinities (of finite parameters, so positive ones) made bf16's largest number; a NaN stays one
 __device__ __forceinline__ uint32_t bounded(uint32_t x) {
     const __nv_bfloat162 v = __hmin2_nan(*(const __nv_bfloat162*)&x, __nv_bfloat162(__ushort_as_bfloat16(0x7F7F), __ushort_as_bfloat16(0x7F7F)));
@@ -226,11 +218,6 @@ __device__ __forceinline__ bool leaves_bf16(uint32_t params) {
     const __nv_bfloat16 top = __hfma(__ushort_as_bfloat16(0x4170), __ushort_as_bfloat16((uint16_t)params), __ushort_as_bfloat16((uint16_t)(params >> 16)));
     return __bfloat16_as_ushort(top) == 0x7F80;
 }
-__device__ __forceinline__ __nv_bfloat162 twice(uint32_t bits16) {
-    const uint32_t x = bits16 * 0x10001u;
-    return *(const __nv_bfloat162*)&x;
-}
-
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_constant__ Params G) {
     constexpr uint32_t kTileBytes = tile_bytes<D>(), kPanel = kTile * 128, kTmem = 512;

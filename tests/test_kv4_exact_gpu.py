@@ -99,3 +99,22 @@ def test_a_number_beyond_bf16_stays_out_of_rows_that_do_not_see_it(t0, rt, dev, 
     tokens = np.arange(n - rows, n)
     e = kb.Exact(q, k, v, tokens, 0.125, 0, True)
     assert e.over(got)[tokens < bad].max() <= 0 and np.isnan(got[tokens >= bad]).all()
+
+
+def test_the_read_out_rounds_once(t0, rt, dev):  # noqa: F811
+    # rows whose least number is next to zero: step * code + low lies beside the middle of two bf16 numbers, by less than an f32 shows
+    rng = np.random.default_rng(23)
+    n, dim, page = 4096, 64, 64
+    x = np.abs(rng.standard_normal((n, 1, dim))).astype(np.float32) * 10
+    x[:, 0, 0] = 2.0**-rng.integers(18, 40, n)
+    x = ref.bf16_round(x)
+    x[0, 0, 0], x[0, 0, 1], x[0, 0, 2:] = 2.0**-30, 15.234375, 5.078125
+    cache, pool = cache_of(rng, x, x[::-1].copy(), page)
+    b = make_batch(t0, dev, cache, dev.up(pool), [n], uniform=True)
+    out = [dev.up(np.zeros((n, dim), np.uint16)) for _ in range(2)]
+    rt.kv4_dequant(b, rt.kv4_dequant_args(*(o.gpu_addr() for o in out)))
+    rt.synchronize()
+    want = kb.bf16_once(ref.held(x)[:, 0])
+    assert want[0, 5] == 5.09375 and (want != ref.bf16_round(ref.held(x)[:, 0].astype(np.float32))).sum() > 1000
+    for o, w in zip(out, (want, want[::-1])):
+        assert np.array_equal(ref.from_bits(o.read(2 * n * dim, np.uint16)).reshape(n, dim), w)
