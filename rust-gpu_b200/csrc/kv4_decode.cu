@@ -215,10 +215,16 @@ __device__ __forceinline__ void store(const Attention& P, const Item& it, uint32
     __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + e % D;
     *(uint2*)y = make_uint2(pack(x.x * f, x.y * f), pack(x.z * f, x.w * f));
 }
+// What this lane's column (lane % kCols) is multiplied with.  A row with a token sees that token at least, so a sum of zero there has scores of minus infinity alone and makes the row NaN;
+// a row without one is zeros.
+template <int kCols>
+__device__ __forceinline__ float inverse_of(const Attention& P, const Item& it, float sum) {
+    return threadIdx.x % kCols < max(it.s.rows - it.s.len, 0) * P.group ? 0.0f : 1.0f / sum;
+}
 template <int D, int NT>
 __device__ __forceinline__ void finish(const Attention& P, const Item& it, const float4 (&total)[8 * NT * D / 128], float sum) {
     const uint32_t lane = threadIdx.x % 32;
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inverse = inverse_of<8 * NT>(P, it, sum);
 #pragma unroll
     for (int j = 0; j < 8 * NT * D / 128; ++j) {
         const uint32_t e = 128 * j + 4 * lane;
@@ -518,7 +524,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                         const uint32_t c = 8 * n + 2 * t + k;
                         if (c >= cols) continue;
                         __nv_bfloat16* to = P.y + (uint64_t)(it.s.first_row + c / P.group) * P.y_stride + (it.head * P.group + c % P.group) * D + g * (D / 8);
-                        const float inverse = sum[n][k] == 0.0f ? 0.0f : 1.0f / sum[n][k];
+                        const float inverse = p_row[n][k] < 0 ? 0.0f : 1.0f / sum[n][k];         // (as inverse_of)
                         uint32_t out[D / 16];
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) out[i] = pack((o[n][i][k] + rest[n][k]) * inverse, (o[n][i][2 + k] + rest[n][k]) * inverse);
@@ -643,6 +649,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
         weigh_parts<D, NT>(parts, weight_of[k], &top, &sum);
         __syncthreads();                                    // (the same weights from every warp)
         const Item it = many_item[k];
+        const float inverse = inverse_of<kCols>(P, it, sum);
         for (uint32_t e = 128 * warp + 4 * lane; e < kCols * D; e += 128 * kWarps) {
             float4 total = make_float4(0, 0, 0, 0);
 #pragma unroll 8
@@ -651,7 +658,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
                 const float f = weight_of[k][i][e / D];
                 total.x = fmaf(f, x.x, total.x); total.y = fmaf(f, x.y, total.y); total.z = fmaf(f, x.z, total.z); total.w = fmaf(f, x.w, total.w);
             }
-            store<D>(P, it, e, total, __shfl_sync(0xFFFFFFFFu, sum == 0.0f ? 0.0f : 1.0f / sum, e / D));
+            store<D>(P, it, e, total, __shfl_sync(0xFFFFFFFFu, inverse, e / D));
         }
     }
 }

@@ -188,7 +188,7 @@ struct Cut {
     uint32_t tile, head;
     int first_row;
     uint32_t total;                  // rows x group of the sequence
-    uint32_t _pad;
+    int first_token;                 // of its first row
 };
 
 struct Params {
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         Walk walk(P, plan, per_head, begin, end);
         const Item& it = walk.it;
         if (threadIdx.x == 0)
-            G.cuts[blockIdx.x] = Cut{units, walk.first, (uint32_t)(it.c1 - it.c0), it.tile, it.head, it.s.first_row, (uint32_t)it.s.rows * P.group, 0};
+            G.cuts[blockIdx.x] = Cut{units, walk.first, (uint32_t)(it.c1 - it.c0), it.tile, it.head, it.s.first_row, (uint32_t)it.s.rows * P.group, it.s.len - it.s.rows};
 
         if (warp < 8) {
             // ------------------------------------------------------------ softmax: a thread has a row
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
                     o_phase ^= 1;
                     ptx::tc_fence_after_sync();
                     if (opens && closes) {
-                        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        const float inverse = p < 0 ? 0.0f : 1.0f / sum;         // a row with a token sees that: scores of minus infinity alone make it NaN
                         __nv_bfloat16* y = P.y + (uint64_t)(it.s.first_row + last / (int)P.group) * P.y_stride + (it.head * P.group + last % P.group) * D;
 #pragma unroll
                         for (int q = 0; q < D / 32; ++q) {
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_prompt_join_kernel(const __g
         for (int j = 0; j < kEach; ++j) sum[j] = fmaf(w, rec[(part * kEach + j) * kRows], sum[j]);
     }
     if (row >= cut.total) return;
-    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inverse = row < max(-cut.first_token, 0) * P.group ? 0.0f : 1.0f / l;
     __nv_bfloat16* y = P.y + (uint64_t)(cut.first_row + row / P.group) * P.y_stride + (cut.head * P.group + row % P.group) * D + part * kEach;
 #pragma unroll
     for (int j = 0; j < kEach / 8; ++j) {

@@ -118,3 +118,19 @@ def test_the_read_out_rounds_once(t0, rt, dev):  # noqa: F811
     assert want[0, 5] == 5.09375 and (want != ref.bf16_round(ref.held(x)[:, 0].astype(np.float32))).sum() > 1000
     for o, w in zip(out, (want, want[::-1])):
         assert np.array_equal(ref.from_bits(o.read(2 * n * dim, np.uint16)).reshape(n, dim), w)
+
+
+@pytest.mark.parametrize("n, rows, group", [(40, 1, 1), (3000, 1, 4), (3000, 4, 4), (100, 30, 4), (5000, 30, 4), (5000, 20, 1)])
+def test_scores_that_are_all_minus_infinity_give_nan(t0, rt, dev, n, rows, group):  # noqa: F811
+    # what the formula gives, and no zeros, which stand for rows without tokens
+    rng = np.random.default_rng(24)
+    dim = 128
+    k = 100 + rng.uniform(0, 0.1, (n, 1, dim)).astype(np.float32)
+    q = np.zeros((rows, group, dim))
+    q[:, 0, 5] = -np.inf
+    cache, pool = cache_of(rng, k, rng.standard_normal((n, 1, dim)).astype(np.float32), 64)
+    got = attend(t0, dev, make_batch(t0, dev, cache, dev.up(pool), [rows], uniform=True), q, 1.0)
+    assert np.isnan(got[:, 0]).all() and np.isfinite(got[:, 1:]).all()
+    short, pool = cache_of(rng, k[:3], k[:3], 64)                           # three tokens: rows before the first are zeros, whatever the queries are
+    got = attend(t0, dev, make_batch(t0, dev, short, dev.up(pool), [rows], uniform=True), q, 1.0)
+    assert np.all(got[:max(rows - 3, 0)] == 0) and np.isnan(got[max(rows - 3, 0):, 0]).all()
