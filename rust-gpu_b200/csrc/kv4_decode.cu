@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(warps<D, NT>() * 32, 1) kv4_decode_kernel(cons
         ptx::fence_barrier_init();
     }
     ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();                         // (only now: kv4_prompt_kernel counts on it)
+    ptx::grid_launch_dependents();
     const uint32_t units = make_plan<kThreads>(P, plan);
     if (units == 0) return;
     // how many warps of a CTA work: all, or fewer where that spreads the chunks over more SMs

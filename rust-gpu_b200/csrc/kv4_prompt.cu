@@ -198,7 +198,6 @@ struct Params {
     // Sequences whose rows do not overlap have no more tiles than this (2^23 at most), and their units fit into 32 bits.  Where row_start is not ascending, which
     // sequence() reports, there may be more: then none is taken.
     uint32_t most_tiles;
-    bool beside_decode;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -273,9 +272,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     ptx::tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_holder, 0);
     ptx::grid_launch_dependents();
-    // Behind kv4_decode in one call there is nothing of that kernel to wait for: it lets this one begin only after what came before both is done, and writes other rows
-    // and other scratch.  The wait is then made up for at the end, so that this kernel is never done before that one.
-    if (!G.beside_decode) ptx::grid_dependency_wait();
+    // Behind kv4_decode in one call too, whose rows and scratch are others: without this wait nothing says that what an append before both wrote is visible here.  (Beginning beside that
+    // kernel, and waiting at the end, took 218.2 us in place of 220.8 for a batch of 24 sequences of both kinds; with a word that it releases and this one acquires, 221.7.)
+    ptx::grid_dependency_wait();
 
     const uint32_t per_head = make_plan(P, G.most_tiles, plan), units = per_head * B.n_kv_heads, runs = min(gridDim.x, units);
     const uint32_t begin = blockIdx.x < runs ? start_of(blockIdx.x, units, runs) : 0, end = blockIdx.x < runs ? start_of(blockIdx.x + 1, units, runs) : 0;
@@ -639,7 +638,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc(tmem, kTmem);
     }
-    if (G.beside_decode) ptx::grid_dependency_wait();
 }
 
 // Joins the parts of the items whose chunks several CTAs of the launch before worked on: sum_i 2^(m_i - m) O_i over sum_i 2^(m_i - m) l_i, in order.  Bound by latency and by
@@ -700,7 +698,6 @@ int launch(const Attention& p, uint32_t sms, cudaStream_t stream) {
     Params g;
     g.P = p;
     g.cuts = (Cut*)(p.scratch + kv4_counter_bytes() + decode_scratch_bytes(sms));
-    g.beside_decode = p.few != 0;
     g.most_tiles = (uint32_t)((uint64_t)p.B.n_rows * p.group / kRows) + p.B.n_seqs;
     g.records = (float*)(g.cuts + kMaxCtas);
     const uint32_t ctas = std::min(sms, kMaxCtas);

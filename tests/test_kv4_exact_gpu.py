@@ -134,3 +134,57 @@ def test_scores_that_are_all_minus_infinity_give_nan(t0, rt, dev, n, rows, group
     short, pool = cache_of(rng, k[:3], k[:3], 64)                           # three tokens: rows before the first are zeros, whatever the queries are
     got = attend(t0, dev, make_batch(t0, dev, short, dev.up(pool), [rows], uniform=True), q, 1.0)
     assert np.all(got[:max(rows - 3, 0)] == 0) and np.isnan(got[max(rows - 3, 0):, 0]).all()
+
+
+@pytest.mark.parametrize("dim, page", [(128, 64), (64, 16)])
+def test_a_recorded_batch_of_both_kinds_reads_what_the_append_before_it_wrote(t0, own, dim, page):  # noqa: F811
+    # append and attention recorded together, single tokens and chunks of prompts in one batch: each replay has other rows, pages, lengths and places of the rows, and is compared with
+    # the same calls with a wait between them
+    driver, dev = Driver(), Device(own)  # noqa: F811
+    rng = np.random.default_rng(31)
+    heads, group, seqs, places = 2, 4, 12, 900
+    hq, total, most = heads * group, 600, 300
+    wide = (hq + 2 * heads) * dim
+    columns = -(-places // page)
+    n_pages = seqs * columns
+    bytes_of = n_pages * t0.kv4_page_bytes(page, heads, dim)
+    first = np.zeros(bytes_of, np.uint8)
+    pools, ys, qs = ([dev.up(np.zeros(shape, kind)) for _ in range(2)] for shape, kind in (((bytes_of,), np.uint8), ((total, hq, dim), np.uint16), ((total, hq, dim), np.uint16)))
+    table, lens, start = dev.up(np.zeros((seqs, columns), np.int32)), dev.up(np.zeros(seqs, np.int32)), dev.up(np.zeros(seqs + 1, np.int32))
+    data, rope = dev.up(np.zeros((total, hq + 2 * heads, dim), np.uint16)), dev.up(rope_table(rng, places, dim // 2))
+
+    def calls(i, between):
+        b = own.kv4_batch(pools[i].gpu_addr(), table.gpu_addr(), lens.gpu_addr(), n_pages=n_pages, page_size=page, n_kv_heads=heads, head_dim=dim, n_seqs=seqs,
+                          table_stride=columns, n_rows=total, max_rows=most, row_start=start.gpu_addr())
+        at = data.gpu_addr()
+        own.kv4_append(b, own.kv4_append_args(at + hq * dim * 2, at + (hq + heads) * dim * 2, k_stride=wide, v_stride=wide, q=at, q_stride=wide, q_out=qs[i].gpu_addr(),
+                                              n_q_heads=hq, rope=rope.gpu_addr(), n_positions=places, rot_dim=dim))
+        between()
+        own.kv4_attention(b, own.kv4_attention_args(qs[i].gpu_addr(), ys[i].gpu_addr(), n_q_heads=hq, scale=dim**-0.5))
+
+    own.reserve_scratch("kv4", own.kv4_scratch_bytes())
+    own.synchronize()
+    with driver.record(own) as made:
+        calls(0, lambda: None)
+    for turn in range(24):
+        rows = np.ones(seqs, int)
+        for s in rng.permutation(seqs)[:3]:
+            rows[s] = rng.integers(5, most if turn % 2 else 60)
+        rows[rng.integers(0, seqs)] = 0
+        rows = np.where(np.cumsum(rows) > total, 0, rows)
+        lens.write(np.array([rng.integers(max(r, 1), places + 1) for r in rows], np.int32))
+        start.write(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+        table.write(rng.permutation(n_pages).reshape(seqs, columns).astype(np.int32))
+        data.write(ref.bf16_bits(rng.standard_normal((total, hq + 2 * heads, dim)).astype(np.float32)))
+        for p in pools:                                                     # what lies before the rows: zeros, the same in both
+            p.write(first)
+        own.synchronize()
+        driver.replay(made[0], own.stream())
+        own.synchronize()
+        calls(1, own.synchronize)
+        own.synchronize()
+        got = [y.read(total * hq * dim * 2, np.uint16).reshape(total, -1) for y in ys]
+        assert got[0][:rows.sum()].any(1).all() and np.array_equal(*got), turn
+        assert np.array_equal(*(p.read(bytes_of) for p in pools)), turn
+    driver.drop(ex=made[0])
+    dev.free()
