@@ -224,6 +224,7 @@ def _calls(s):
     t0 = importlib.import_module("rust-gpu_b200")
     if _runtime is None:
         _runtime = t0.GpuRuntime(0)
+    torch.cuda.current_stream().synchronize()    # the runtime's stream does not wait for torch's, on which the inputs were made (nor torch's for results: readers wait for the device)
     rt, case = _runtime, s["case"]
     heads, dim, group = case["heads"], case["dim"], case["group"]
     batch = rt.kv4_batch(s["pool"].data_ptr(), s["table"].data_ptr(), s["lens"].data_ptr(), n_pages=s["pool"].shape[0], page_size=case["page"],
