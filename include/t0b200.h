@@ -580,7 +580,7 @@ long t0_gptq_to_b200(const uint8_t* packed, const float* scales, const int32_t* 
  * (what the sequence's rows get is then of no use, other sequences' are as ever; where sequences'
  * rows overlap, sequences of more than one row may get nothing); in either case the next
  * synchronising call returns T0_ERR_BOUNDS (the runtime is not poisoned).  Sequences may share pages that they only read; a token's place
- * must not be another's whose row is in the same append. */
+ * must not be another's whose row is in the same append.  Rows that a call writes (q_out, k_out, v_out, y) must not lie in the cache: refused. */
 typedef struct t0_kv4_batch {
     uint64_t pages;          /* the cache; 16-byte aligned */
     uint64_t page_table;     /* i32 [n_seqs][table_stride] */

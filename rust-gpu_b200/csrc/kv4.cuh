@@ -25,6 +25,8 @@ int check_batch(const t0_kv4_batch* b, Batch* out);
 int check_rows(const char* name, uint64_t base, uint32_t* stride, uint32_t width, uint32_t bytes);
 // Whether rows [a, a + a_bytes), a_stride apart, and rows of b touch; all in bytes, `rows` rows each.
 bool rows_touch(uint64_t a, uint64_t a_bytes, uint64_t a_stride, uint64_t b, uint64_t b_bytes, uint64_t b_stride, uint64_t rows);
+// T0_ERR_INVALID where rows that a call writes lie in the cache (all in bytes).
+int check_outside(const char* name, const t0_kv4_batch* b, uint64_t base, uint64_t bytes, uint64_t stride);
 
 // ------------------------------------------------------------------ device side
 struct Sequence {

@@ -38,6 +38,7 @@ int t0_kv4_attention(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_att
     const bool in_place = a.y == a.q && (a.y_stride == a.q_stride || batch->n_rows == 1);
     if (!in_place && rows_touch(a.q, 2ull * width, 2ull * a.q_stride, a.y, 2ull * width, 2ull * a.y_stride, batch->n_rows))
         return fail(T0_ERR_INVALID, "y overlaps q (it may be q itself)");
+    if ((rc = check_outside("y", batch, a.y, 2ull * width, 2ull * a.y_stride)) != T0_OK) return rc;
     // the kernels count the chunks (64 tokens for few rows, 128 against 256 rows for many) that a batch of this shape may hold, for every head, in 32 bits
     const uint64_t places = (uint64_t)batch->table_stride * batch->page_size;
     if ((uint64_t)batch->n_seqs * (places / 64 + 1) * batch->n_kv_heads >= 1ull << 31 ||

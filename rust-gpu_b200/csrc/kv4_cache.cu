@@ -52,6 +52,12 @@ bool rows_touch(uint64_t a, uint64_t a_bytes, uint64_t a_stride, uint64_t b, uin
     return d < a_bytes || d + b_bytes > a_stride;
 }
 
+int check_outside(const char* name, const t0_kv4_batch* b, uint64_t base, uint64_t bytes, uint64_t stride) {
+    const uint64_t cache = b->n_pages * (uint64_t)t0_kv4_page_bytes(b->page_size, b->n_kv_heads, b->head_dim), end = base + (b->n_rows - 1) * stride + bytes;
+    if (base < b->pages + cache && b->pages < end) return fail(T0_ERR_INVALID, "%s overlaps the cache", name);
+    return T0_OK;
+}
+
 namespace {
 
 struct Append {
@@ -419,6 +425,7 @@ int t0_kv4_append(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_append
             rows_touch(a.q_out, out_bytes, out_stride, a.k, kv_bytes, (uint64_t)a.k_stride * size, n) ||
             rows_touch(a.q_out, out_bytes, out_stride, a.v, kv_bytes, (uint64_t)a.v_stride * size, n))
             return fail(T0_ERR_INVALID, "q_out overlaps q, k or v (it may be q itself where q is bf16)");
+        if ((rc = check_outside("q_out", batch, a.q_out, out_bytes, out_stride)) != T0_OK) return rc;
     }
     if (a.rope) {
         if ((a.rope & 15) || (a.positions & 3)) return fail(T0_ERR_INVALID, "the rope table must be 16-byte aligned, positions 4-byte");
@@ -475,6 +482,8 @@ int t0_kv4_dequant(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_dequa
     if (a.v_out && (rc = check_rows("v_out", a.v_out, &a.v_out_stride, width, 2)) != T0_OK) return rc;
     if (a.k_out && a.v_out && rows_touch(a.k_out, 2ull * width, 2ull * a.k_out_stride, a.v_out, 2ull * width, 2ull * a.v_out_stride, batch->n_rows))
         return fail(T0_ERR_INVALID, "k_out and v_out overlap");
+    if (a.k_out && (rc = check_outside("k_out", batch, a.k_out, 2ull * width, 2ull * a.k_out_stride)) != T0_OK) return rc;
+    if (a.v_out && (rc = check_outside("v_out", batch, a.v_out, 2ull * width, 2ull * a.v_out_stride)) != T0_OK) return rc;
     P.k_out = (__nv_bfloat16*)a.k_out; P.v_out = (__nv_bfloat16*)a.v_out;
     P.k_stride = a.k_out_stride; P.v_stride = a.v_out_stride;
     if ((rc = check_rt(rt)) != T0_OK) return rc;
