@@ -625,7 +625,12 @@ int t0_kv4_dequant(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_dequa
 /* Attention of the rows over their sequences' cached tokens: row at token p sees the tokens j <= p, with window > 0 those with
  * j > p - window, and y = sum_j softmax_j(scale * q . k_j) v_j for each of its n_q_heads heads (a multiple of n_kv_heads, at most 64 to a
  * key/value head; head h reads key/value head h / (n_q_heads / n_kv_heads)).  q and y are bf16 rows, 16-byte aligned, strides multiples of 8 (0 = dense);
- * y may be q itself.  scale is positive, and scale * log2(e) finite.  A row without a token, or that sees none, becomes zeros.  Sums and softmax statistics are f32.
+ * y may be q itself.  scale is positive, and scale * log2(e) finite.  A row without a token becomes zeros; one whose scores
+ * are all minus infinity is NaN, and so is a row that sees a token held as NaN; what a row does not see leaves no trace in it.  Sums and softmax statistics are f32.
+ * What is rounded to bf16 on the way (y itself aside) depends on the sequence's rows times query heads to a key/value head: up to 16, each weight times its value's step; keys and values are
+ * as the cache has them.  Above 16, or with more than 16 heads to one, each weight, each key and each value (step * code + low, once; at most bf16's largest number).  The same row may so differ in
+ * its last places with the rows it comes with: results of random numbers are off by 2.4e-3 of their size in the first form and 4.4e-3 in the second, 1.7e-3 of which is y's own rounding.
+ * Ranges: with up to 16, the sizes of a query's numbers may sum to 2^120; values that are all below 2^-106 in size lose places.
  * The rows' own tokens are read from the cache like any other: call t0_kv4_append first.  The work is cut by what the device finds in the batch, not by host
  * values, so a recorded call stays balanced when its lengths change; sums are added in an order that depends on the batch alone, so a call repeats bit for bit. */
 typedef struct t0_kv4_attention_args {

@@ -21,7 +21,9 @@ struct Attention {
     uint8_t* scratch;
 };
 
-constexpr uint32_t kFewColumns = 16;                     // rows x group that kv4_decode takes
+// rows x group that kv4_decode takes: what its registers hold (two column tiles of eight).  131072 tokens of 8 heads of 128 (143 MB), and 32 times 4096: 44 and 43 us up to 8 columns, 55 up to 16
+// there; 133 and 120 from 17 to 64 in kv4_prompt, which makes 128 rows of any number.
+constexpr uint32_t kFewColumns = 16;
 constexpr uint32_t kMaxCtas = 160;                       // of a persistent launch, one for each SM: arrival counters, parts of one item
 
 size_t decode_scratch_bytes(uint32_t sms);               // behind the counters

@@ -154,8 +154,9 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, flo
 // A warp takes a row, or `per_warp` of its heads where rows are few: sequence, token, page, positions and the lane's cosines and sines are found once for all of them.  A head is
 // D / 8 lanes wide, eight numbers a lane, so that a warp works on several at a time and asks for the next ones before it needs them.  A lane turns its numbers, and
 // either rounds them to bf16 (queries) or finds the row's range with its group and cuts them to four bits, a 32-bit word of codes a lane.  8192 rows of 32 query and
-// 8 key/value heads of 128, bf16, three axes, are 157 MB (24 us); it takes 57 us, bound by its instructions (about 4400 a row, half of them the range and the codes) at the 24 warps
-// an SM holds: 3 blocks of 80 registers and two loads ahead measured 71 us with the read-out, 4 blocks 68 to 76, four loads ahead 70 (and 13 instead of 10 us at 256 rows).
+// 8 key/value heads of 128, bf16, three axes, are 181 MB (27.6 us); it takes 59.5 us, bound by its instructions (about 4400 a row, half of them the range and the codes) at the 24 warps
+// an SM holds: 3 blocks of 80 registers and two loads ahead measured 71 us with the read-out behind it (now 67.4), 4 blocks 68 to 76, four loads ahead 70 (and 13 instead of 10 us at 256 rows).
+// f32 rows with one axis take 64 us, 256 single tokens 7.0 and one 3.6.
 template <int D, bool F32>
 __global__ void __launch_bounds__(256, 3) kv4_append_kernel(const __grid_constant__ Append P) {
     constexpr uint32_t kLanes = D / 8, kAtOnce = 32 / kLanes, kAhead = 2;

@@ -5,7 +5,7 @@
 // the A operands of both: a nibble in the mantissa of a bf16 128 is 128 + code, so the codes of two neighbours become a register of the operand with a shift and a
 // logical operation.  Steps and lows stay outside of the products:
 //   score_j = a_j (q . (128 + c_j)) + b_j sum(q),   a_j = step_j, b_j = low_j - 128 step_j    (f32)
-//   o       = sum_j (p_j step_j) (c_j - 8) + sum_j p_j (low_j + 8 step_j)
+//   o       = sum_j (p_j step_j) (c_j - 8) + sum_j p_j (low_j + 8 step_j),   no p_j above 1
 // where p_j step_j is rounded to bf16 (one rounding for each token and row, which a sum feels by at most 2^-8 of eight steps of the token's weight; the second sum stays f32).
 // (The codes are centred before the product: 128 + c there, and 136 p_j step_j off the second sum, is 2.5 % faster, but the product's own sums then grow so far beyond their
 // difference that an average of 4096 random values was off by 7e-3 in place of 2e-3.)
@@ -15,9 +15,9 @@
 // reads as much as the next.  A warp has its own two buffers, filled by bulk copies (the blocks of a chunk are contiguous pieces of the pages), and its own running
 // maximum and sums.  Items that end up in several warps are joined, first inside the CTA, then between CTAs by the one that arrives last, always in order.
 //
-// 128 sequences of 5100 tokens on average, 8 key/value heads of 128 and 8 rows each (713 MB), take 156 to 167 us, 4.4 TB/s (109 us at the rate of a plain copy): 130 in chunks
+// 128 sequences of 5100 tokens on average, 8 key/value heads of 128 and 8 rows each (713 MB), take 156 to 167 us, 4.3 to 4.6 TB/s (109 us at the rate of a plain copy): 130 in chunks
 // (5.5 TB/s), which the warps leave 10 us apart, 5 before, 5 of joins.  With three warps a scheduler of 168 registers the ALU is busy for 62 % of the cycles and an instruction issued
-// in 57 %, most of them taking codes apart.  One row on 131072 tokens (143 MB) takes 44 us: 7 until a warp has its first chunk, 26 of chunks, 4 of joins, and the launch.  32 sequences' five rows in a window of 1000, 16 heads of 64 (36 MB): 23.6 us, 4 before, 8 of
+// in 57 %, most of them taking codes apart.  One row on 131072 tokens (143 MB) takes 44 us: 7 until a warp has its first chunk, 26 of chunks, 4 of joins, and the launch.  32 sequences' five rows in a window of 1000, 16 heads of 64 (36 MB): 23.7 us, 4 before, 8 of
 // chunks (3 or 4 a warp), 4 of joins, and the launch.  8, 10 or 11 warps and chunks of 32 tokens were slower; codes by way of fp16 (half the shifts) 3 % faster for keys, but values'
 // weights leave its range.
 #include "kv4_attention.cuh"

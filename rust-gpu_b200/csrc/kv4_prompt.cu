@@ -17,7 +17,7 @@
 // The units of work are all items' chunks, and kItemUnits for what an item costs beside them, in equal contiguous runs, one for each CTA.  Items whose chunks end up in
 // several CTAs leave parts (O, m, l) that a second kernel joins.
 //
-// 8192 tokens on themselves, 32 query and 8 key/value heads of 128, take 595 us, 925 TFLOP/s of what the mask leaves; 2048 behind 8192 others 330 us.  A chunk takes a CTA 3700
+// 8192 tokens on themselves, 32 query and 8 key/value heads of 128, take 595 us, 925 TFLOP/s of what the mask leaves (heads of 64: 438 us, before the clock falls); 2048 behind 8192 others 328 us.  A chunk takes a CTA 3700
 // clocks, of which the products need 2048 and the powers of two 2048 (a scheduler makes four a clock): the softmax warps work for 2800 of them and wait for the rest.  Over
 // more than a few launches the clock falls from 1965 to 1725 MHz at the board's 1000 W (534 us before that), so that less work in one unit saves little: no scores in one
 // product a chunk (610 us), maxima of three numbers (600), a quarter of the powers by a polynomial (605) nor eight warps for the codes were faster; without the codes'
@@ -32,7 +32,8 @@ constexpr int kTok = 128, kRows = 256, kTile = 128;
 constexpr int kDequantWarps = 4;
 constexpr int kThreads = (12 + kDequantWarps) * 32;
 constexpr uint32_t kIssuer = 8 + kDequantWarps;           // the warp that issues the products
-constexpr uint32_t kItemUnits = 3;                        // an item's queries, results and idle times in chunks' time (10600 of 3800 clocks, measured on a prompt of 8192 tokens)
+constexpr uint32_t kItemUnits = 3;                        // an item's queries, results and idle times in chunks' time (10600 of 3800 clocks, measured on a prompt of 8192 tokens with heads
+                                                          // of 128; with heads of 64, a mixed batch of 24 sequences took 217 us, 222 with 1 here)
 constexpr float kLag = 8.0f;                              // powers of two by which a score may exceed its row's maximum so far; weights are 2^(score - maximum - kLag)
 
 template <int D> constexpr uint32_t tile_bytes() { return kTile * D * 2; }
