@@ -643,6 +643,86 @@ typedef struct t0_kv4_attention_args {
 int t0_kv4_attention(t0_runtime* rt, const t0_kv4_batch* batch, const t0_kv4_attention_args* args);
 size_t t0_kv4_scratch_bytes(const t0_runtime* rt);
 
+/* ------------------------------------------------------- products in eight bits */
+/* Activations and weights held as eight-bit integers with a scale for each row (no counterpart in the reference, whose INT4 weights meet bf16 or f32 activations,
+ * src/t0/quant_kernels.rs:53-171): what a decoder layer needs to run its products on the tensor cores' integer rate and to read a weight as one byte.
+ * The entries of a step: t0_q8_rmsnorm (adds the residual, leaves codes), t0_q8_gemm (q, k, v: f32 or bf16 rows, what t0_kv4_append takes), t0_q8_quant (the rows that
+ * t0_kv4_attention writes), t0_q8_gemm (output projection), t0_q8_rmsnorm, t0_q8_gated (bf16 rows), t0_q8_quant, t0_q8_gemm (down projection).
+ *
+ * An array of rows in eight bits: i8 codes, `stride` bytes from one row to the next (a multiple of 16, at least the row's length; 0 = the length rounded up to 16), 16-byte aligned,
+ * and f32 scales, one a row.  Code c stands for c * scale.  A row x of f32 numbers is held as
+ *   a = max |x|,  scale = a / 127,  code = rint(x * (127 / a))  (halves to even), every operation rounded to f32;
+ *   a < 2^-119: scale 0 and codes 0;  an infinity or a NaN in the row: scale NaN and codes 0, so that all that is computed from the row is NaN.
+ * An array holds rows * stride bytes; those between a row's length and its stride are never written, and what they hold changes no result.
+ * All calls run on the runtime's stream, allocate nothing and may be recorded.  Rows that a call writes must not lie where it reads, but for the places named below: refused. */
+
+/* Rows of f32 (x_f32) or bf16 numbers into eight bits: activations, or a weight matrix [n][k] with a scale for each of its channels.  x: 16-byte aligned, x_stride in
+ * numbers, a multiple of 8 (f32: 4), 0 = dense.  dim 1 .. 32768. */
+typedef struct t0_q8_quant_args {
+    uint64_t x;
+    uint64_t q, scales;      /* i8 [n_rows][q_stride], f32 [n_rows] */
+    uint32_t n_rows, dim;
+    uint32_t x_stride, q_stride;
+    uint8_t x_f32;
+    uint8_t _pad[7];
+} t0_q8_quant_args;
+int t0_q8_quant(t0_runtime* rt, const t0_q8_quant_args* args);
+/* The way back: y = code * scale, rounded once, f32 (out_f32) or bf16 rows; y 16-byte aligned, y_stride a multiple of 8 (f32: 4), 0 = dense.  (With t0_gemm_launch on
+ * what it writes, eight-bit weights meet bf16 activations.)  dim 1 .. 131071. */
+typedef struct t0_q8_dequant_args {
+    uint64_t q, scales;
+    uint64_t y;
+    uint32_t n_rows, dim;
+    uint32_t q_stride, y_stride;
+    uint8_t out_f32;
+    uint8_t _pad[7];
+} t0_q8_dequant_args;
+int t0_q8_dequant(t0_runtime* rt, const t0_q8_dequant_args* args);
+/* Root-mean-square norm of rows, with the residual's addition before it and eight bits after it:
+ *   h = x + residual, rounded to the residual's type, written to residual_out (residual = 0: h = x);
+ *   y = (h * r) * weight with r = 1 / sqrt(sum h^2 / dim + eps): the sum and r in f64, r rounded to f32 once, both products rounded to f32;
+ *   y into eight bits (q, scales) as above, or rounded to bf16 rows (y), or both.
+ * x f32 (x_f32) or bf16, residual and residual_out f32 (residual_f32) or bf16, weight [dim] f32 (weight_f32) or bf16; all 16-byte aligned, strides in numbers as in t0_q8_quant.
+ * residual_out may be residual itself or, of one type, x itself (strides equal); 0 = the sum is not kept.  dim 1 .. 32768; eps finite and not negative. */
+typedef struct t0_q8_rmsnorm_args {
+    uint64_t x, residual, residual_out, weight;
+    uint64_t q, scales;      /* or 0 */
+    uint64_t y;              /* bf16, or 0 */
+    uint32_t n_rows, dim;
+    uint32_t x_stride, residual_stride, residual_out_stride, q_stride, y_stride;
+    float eps;
+    uint8_t x_f32, residual_f32, weight_f32;
+    uint8_t _pad[5];
+} t0_q8_rmsnorm_args;
+int t0_q8_rmsnorm(t0_runtime* rt, const t0_q8_rmsnorm_args* args);
+/* y[i][j] = (sum_e a[i][e] w[j][e]) * a_scales[i] * w_scales[j] + bias[j], a: [m][k] and w: [n][k] in eight bits.  The sum is exact (k 1 .. 131071; a code may be -128);
+ * it, the two products in this order and the bias's addition are rounded to f32 each, then to bf16 where out_bf16: the same bits however many rows come together.  y: aligned to its
+ * numbers, y_stride in numbers (0 = n, any from n on); bias f32 [n] or 0. */
+typedef struct t0_q8_gemm_args {
+    uint64_t a, a_scales;
+    uint64_t w, w_scales;
+    uint64_t bias;
+    uint64_t y;
+    uint32_t m, n, k;
+    uint32_t a_stride, w_stride, y_stride;
+    uint8_t out_bf16;
+    uint8_t _pad[7];
+} t0_q8_gemm_args;
+int t0_q8_gemm(t0_runtime* rt, const t0_q8_gemm_args* args);
+/* The gated pair of products of a feed-forward block in one kernel: y = act(g) * u with g = a gate^T and u = a up^T as t0_q8_gemm gives them in f32 (gate and up: [n][k] each, one w_stride),
+ * act of {T0_TEPI_RELU, T0_TEPI_SILU, T0_TEPI_GELU}, their meaning that of the epilogues: x sigmoid(x), x sigmoid(1.702 x).  y as in t0_q8_gemm. */
+typedef struct t0_q8_gated_args {
+    uint64_t a, a_scales;
+    uint64_t gate, gate_scales;
+    uint64_t up, up_scales;
+    uint64_t y;
+    uint32_t m, n, k;
+    uint32_t a_stride, w_stride, y_stride;
+    uint8_t out_bf16, activation;
+    uint8_t _pad[6];
+} t0_q8_gated_args;
+int t0_q8_gated(t0_runtime* rt, const t0_q8_gated_args* args);
+
 /* ------------------------------------------------------- multi-GPU sharding */
 /* The reference is single-GPU (its MultiGpuManager bounces through host memory, src/universal/runtime/multi_gpu.rs:64-159);
  * this section has no Rust counterpart to bind.  A large GEMM shards by N-column blocks: GPU r computes

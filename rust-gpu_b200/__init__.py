@@ -303,6 +303,37 @@ def kv4_page_bytes(page_size: int, n_kv_heads: int, head_dim: int) -> int:
     return int(lib().t0_kv4_page_bytes(page_size, n_kv_heads, head_dim))
 
 
+class Q8QuantArgs(C.Structure):
+    """``t0_q8_quant_args``."""
+    _fields_ = [(f, C.c_uint64) for f in ("x", "q", "scales")] + [(f, C.c_uint32) for f in ("n_rows", "dim", "x_stride", "q_stride")] + [
+        ("x_f32", C.c_uint8), ("_pad", C.c_uint8 * 7)]
+
+
+class Q8DequantArgs(C.Structure):
+    """``t0_q8_dequant_args``."""
+    _fields_ = [(f, C.c_uint64) for f in ("q", "scales", "y")] + [(f, C.c_uint32) for f in ("n_rows", "dim", "q_stride", "y_stride")] + [
+        ("out_f32", C.c_uint8), ("_pad", C.c_uint8 * 7)]
+
+
+class Q8RmsnormArgs(C.Structure):
+    """``t0_q8_rmsnorm_args``."""
+    _fields_ = [(f, C.c_uint64) for f in ("x", "residual", "residual_out", "weight", "q", "scales", "y")] + [
+        (f, C.c_uint32) for f in ("n_rows", "dim", "x_stride", "residual_stride", "residual_out_stride", "q_stride", "y_stride")] + [
+        ("eps", C.c_float), ("x_f32", C.c_uint8), ("residual_f32", C.c_uint8), ("weight_f32", C.c_uint8), ("_pad", C.c_uint8 * 5)]
+
+
+class Q8GemmArgs(C.Structure):
+    """``t0_q8_gemm_args``."""
+    _fields_ = [(f, C.c_uint64) for f in ("a", "a_scales", "w", "w_scales", "bias", "y")] + [
+        (f, C.c_uint32) for f in ("m", "n", "k", "a_stride", "w_stride", "y_stride")] + [("out_bf16", C.c_uint8), ("_pad", C.c_uint8 * 7)]
+
+
+class Q8GatedArgs(C.Structure):
+    """``t0_q8_gated_args``."""
+    _fields_ = [(f, C.c_uint64) for f in ("a", "a_scales", "gate", "gate_scales", "up", "up_scales", "y")] + [
+        (f, C.c_uint32) for f in ("m", "n", "k", "a_stride", "w_stride", "y_stride")] + [("out_bf16", C.c_uint8), ("activation", C.c_uint8), ("_pad", C.c_uint8 * 6)]
+
+
 class Int4WmmaConfig(C.Structure):
     """``Int4WmmaConfig`` (quant_kernels.rs:316-336): the INT4 tile record and its two constructors."""
     _fields_ = [("tile_m", C.c_uint32), ("tile_n", C.c_uint32), ("tile_k", C.c_uint32)]
@@ -864,6 +895,52 @@ class GpuRuntime:
     def kv4_scratch_bytes(self) -> int:
         return int(lib().t0_kv4_scratch_bytes(self._h))
 
+    @staticmethod
+    def q8_quant_args(x: int, q: int, scales: int, *, n_rows: int, dim: int, x_f32: bool = False, x_stride: int = 0, q_stride: int = 0) -> Q8QuantArgs:
+        return Q8QuantArgs(x, q, scales, n_rows, dim, x_stride, q_stride, int(x_f32))
+
+    @staticmethod
+    def q8_dequant_args(q: int, scales: int, y: int, *, n_rows: int, dim: int, out_f32: bool = False, q_stride: int = 0, y_stride: int = 0) -> Q8DequantArgs:
+        return Q8DequantArgs(q, scales, y, n_rows, dim, q_stride, y_stride, int(out_f32))
+
+    @staticmethod
+    def q8_rmsnorm_args(x: int, weight: int, *, n_rows: int, dim: int, eps: float, q: int = 0, scales: int = 0, y: int = 0, residual: int = 0,
+                        residual_out: int = 0, x_f32: bool = False, residual_f32: bool = False, weight_f32: bool = False, x_stride: int = 0,
+                        residual_stride: int = 0, residual_out_stride: int = 0, q_stride: int = 0, y_stride: int = 0) -> Q8RmsnormArgs:
+        return Q8RmsnormArgs(x, residual, residual_out, weight, q, scales, y, n_rows, dim, x_stride, residual_stride, residual_out_stride, q_stride, y_stride,
+                             eps, int(x_f32), int(residual_f32), int(weight_f32))
+
+    @staticmethod
+    def q8_gemm_args(a: int, a_scales: int, w: int, w_scales: int, y: int, *, m: int, n: int, k: int, bias: int = 0, out_bf16: bool = False, a_stride: int = 0,
+                     w_stride: int = 0, y_stride: int = 0) -> Q8GemmArgs:
+        return Q8GemmArgs(a, a_scales, w, w_scales, bias, y, m, n, k, a_stride, w_stride, y_stride, int(out_bf16))
+
+    @staticmethod
+    def q8_gated_args(a: int, a_scales: int, gate: int, gate_scales: int, up: int, up_scales: int, y: int, *, m: int, n: int, k: int, activation: str = "silu",
+                      out_bf16: bool = True, a_stride: int = 0, w_stride: int = 0, y_stride: int = 0) -> Q8GatedArgs:
+        """``activation``: "silu", "gelu" or "relu", as in the epilogues of a TileGemm."""
+        return Q8GatedArgs(a, a_scales, gate, gate_scales, up, up_scales, y, m, n, k, a_stride, w_stride, y_stride, int(out_bf16), TEPI[activation])
+
+    def q8_quant(self, args: Q8QuantArgs) -> None:
+        """``t0_q8_quant``: rows into eight bits, a scale for each."""
+        _check(lib().t0_q8_quant(self._h, C.byref(args)))
+
+    def q8_dequant(self, args: Q8DequantArgs) -> None:
+        """``t0_q8_dequant``: rows in eight bits back to f32 or bf16."""
+        _check(lib().t0_q8_dequant(self._h, C.byref(args)))
+
+    def q8_rmsnorm(self, args: Q8RmsnormArgs) -> None:
+        """``t0_q8_rmsnorm``: residual addition, root-mean-square norm, rows in eight bits and/or bf16."""
+        _check(lib().t0_q8_rmsnorm(self._h, C.byref(args)))
+
+    def q8_gemm(self, args: Q8GemmArgs) -> None:
+        """``t0_q8_gemm``: product of rows in eight bits with weights in eight bits."""
+        _check(lib().t0_q8_gemm(self._h, C.byref(args)))
+
+    def q8_gated(self, args: Q8GatedArgs) -> None:
+        """``t0_q8_gated``: act(a gate^T) * (a up^T) in one kernel."""
+        _check(lib().t0_q8_gated(self._h, C.byref(args)))
+
     def fill_uniform_bf16(self, dst: int, n: int, seed: int, first_index: int = 0) -> None:
         _check(lib().t0_fill_uniform_bf16(self._h, dst, n, seed, first_index))
 
@@ -1186,6 +1263,11 @@ def _declare(L: C.CDLL) -> None:
     sig("t0_kv4_dequant", i32, vp, C.POINTER(Kv4Batch), C.POINTER(Kv4DequantArgs))
     sig("t0_kv4_attention", i32, vp, C.POINTER(Kv4Batch), C.POINTER(Kv4AttentionArgs))
     sig("t0_kv4_scratch_bytes", sz, vp)
+    sig("t0_q8_quant", i32, vp, C.POINTER(Q8QuantArgs))
+    sig("t0_q8_dequant", i32, vp, C.POINTER(Q8DequantArgs))
+    sig("t0_q8_rmsnorm", i32, vp, C.POINTER(Q8RmsnormArgs))
+    sig("t0_q8_gemm", i32, vp, C.POINTER(Q8GemmArgs))
+    sig("t0_q8_gated", i32, vp, C.POINTER(Q8GatedArgs))
     sig("t0_gptq_parse", i32, vp, sz, u32p, u32p, u32p, C.POINTER(sz), C.POINTER(sz), C.POINTER(sz))
     sig("t0_gptq_gpu_buffer_size", sz, u32, u32, u32)
     sig("t0_gptq_to_b200", C.c_long, vp, vp, vp, u32, u32, u32, vp, vp, vp)

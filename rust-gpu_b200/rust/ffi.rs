@@ -237,6 +237,98 @@ pub struct t0_kv4_attention_args {
     pub _pad: u32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_q8_quant_args {
+    pub x: u64,
+    pub q: u64,
+    pub scales: u64,
+    pub n_rows: u32,
+    pub dim: u32,
+    pub x_stride: u32,
+    pub q_stride: u32,
+    pub x_f32: u8,
+    pub _pad: [u8; 7],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_q8_dequant_args {
+    pub q: u64,
+    pub scales: u64,
+    pub y: u64,
+    pub n_rows: u32,
+    pub dim: u32,
+    pub q_stride: u32,
+    pub y_stride: u32,
+    pub out_f32: u8,
+    pub _pad: [u8; 7],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_q8_rmsnorm_args {
+    pub x: u64,
+    pub residual: u64,
+    pub residual_out: u64,
+    pub weight: u64,
+    pub q: u64,
+    pub scales: u64,
+    pub y: u64,
+    pub n_rows: u32,
+    pub dim: u32,
+    pub x_stride: u32,
+    pub residual_stride: u32,
+    pub residual_out_stride: u32,
+    pub q_stride: u32,
+    pub y_stride: u32,
+    pub eps: f32,
+    pub x_f32: u8,
+    pub residual_f32: u8,
+    pub weight_f32: u8,
+    pub _pad: [u8; 5],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_q8_gemm_args {
+    pub a: u64,
+    pub a_scales: u64,
+    pub w: u64,
+    pub w_scales: u64,
+    pub bias: u64,
+    pub y: u64,
+    pub m: u32,
+    pub n: u32,
+    pub k: u32,
+    pub a_stride: u32,
+    pub w_stride: u32,
+    pub y_stride: u32,
+    pub out_bf16: u8,
+    pub _pad: [u8; 7],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct t0_q8_gated_args {
+    pub a: u64,
+    pub a_scales: u64,
+    pub gate: u64,
+    pub gate_scales: u64,
+    pub up: u64,
+    pub up_scales: u64,
+    pub y: u64,
+    pub m: u32,
+    pub n: u32,
+    pub k: u32,
+    pub a_stride: u32,
+    pub w_stride: u32,
+    pub y_stride: u32,
+    pub out_bf16: u8,
+    pub activation: u8,
+    pub _pad: [u8; 6],
+}
+
 extern "C" {
     pub fn t0_last_error() -> *const c_char;
     pub fn t0_version() -> c_int;
@@ -397,6 +489,11 @@ extern "C" {
     pub fn t0_kv4_dequant(rt: *mut t0_runtime, batch: *const t0_kv4_batch, args: *const t0_kv4_dequant_args) -> c_int;
     pub fn t0_kv4_attention(rt: *mut t0_runtime, batch: *const t0_kv4_batch, args: *const t0_kv4_attention_args) -> c_int;
     pub fn t0_kv4_scratch_bytes(rt: *const t0_runtime) -> usize;
+    pub fn t0_q8_quant(rt: *mut t0_runtime, args: *const t0_q8_quant_args) -> c_int;
+    pub fn t0_q8_dequant(rt: *mut t0_runtime, args: *const t0_q8_dequant_args) -> c_int;
+    pub fn t0_q8_rmsnorm(rt: *mut t0_runtime, args: *const t0_q8_rmsnorm_args) -> c_int;
+    pub fn t0_q8_gemm(rt: *mut t0_runtime, args: *const t0_q8_gemm_args) -> c_int;
+    pub fn t0_q8_gated(rt: *mut t0_runtime, args: *const t0_q8_gated_args) -> c_int;
     pub fn t0_shard_columns(n: u32, n_gpus: u32, rank: u32, first_col: *mut u32, n_cols: *mut u32) -> c_int;
     pub fn t0_mg_new(n_gpus: c_int, out: *mut *mut t0_mg) -> c_int;
     pub fn t0_mg_free(mg: *mut t0_mg);
