@@ -431,12 +431,46 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtens
         : "memory");
 }
 
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap* map, uint32_t leader_bar, int32_t c0, int32_t c1) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_dst), "l"((uint64_t)map), "r"(leader_bar), "r"(c0), "r"(c1)
+                 : "memory");
+}
+// The product of eight-bit integers with i32 sums (kind::i8): one step is 32 deep, 32 bytes of a row, so operands lie in shared memory as those of bf16 do.
+__device__ __forceinline__ void umma_i8_ss_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_i8_ss_if(uint32_t issue, uint32_t tmem_d, uint32_t desc_a_lo, uint32_t desc_b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        ".reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %5};\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, p;\n\t"
+        "}"
+        ::"r"(tmem_d), "r"(desc_a_lo), "r"(desc_b_lo), "r"(idesc), "r"(accumulate), "n"((1024 >> 4) | (1 << 14) | (2 << 29)), "r"(issue)
+        : "memory");
+}
+
 // Tiled TMA store of one box from shared to global memory (bulk async-group completion).  Rows and columns of the box
 // that lie outside the tensor are not written.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t smem_src, int32_t c0, int32_t c1, int32_t c2) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                  ::"l"((uint64_t)map), "r"(smem_src), "r"(c0), "r"(c1), "r"(c2)
                  : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int32_t c0, int32_t c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"((uint64_t)map), "r"(smem_src), "r"(c0), "r"(c1) : "memory");
 }
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // the shared-memory source of every committed store has been read (the buffer may be overwritten)
@@ -467,6 +501,15 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16_f32(uint32_t m, uint32_t 
          | (1u << 10)           // B format bf16
          | (a_mn_major << 15)   // A major
          | (b_mn_major << 16)   // B major
+         | ((n >> 3) << 17)
+         | ((m >> 4) << 24);
+}
+
+// Instruction descriptor for kind::i8: signed A and B, both K-major, i32 accumulation, M x N tile.
+__host__ __device__ constexpr uint32_t make_idesc_i8_s32(uint32_t m, uint32_t n) {
+    return (2u << 4)            // D format i32
+         | (1u << 7)            // A format signed
+         | (1u << 10)           // B format signed
          | ((n >> 3) << 17)
          | ((m >> 4) << 24);
 }

@@ -3,6 +3,8 @@
 
 #include <cuda_bf16.h>
 
+#include <cuda.h>
+
 #include "kv4.cuh"
 
 namespace t0 {
@@ -29,6 +31,12 @@ struct Product {
 int check_codes(const char* name, uint64_t codes, uint64_t scales, uint32_t* stride, uint32_t length);
 // Whether rows of `a` and rows of `b` touch, all in bytes.
 bool touch(uint64_t a, uint64_t a_bytes, uint64_t a_stride, uint64_t a_rows, uint64_t b, uint64_t b_bytes, uint64_t b_stride, uint64_t b_rows);
+
+// The kernels: what each is for stands with it.
+int launch_pair(t0_runtime* rt, const Product& P, bool gated);
+
+// Box of 128 codes of `box_rows` rows, 128-byte swizzle; codes from `length` on and rows from `rows` on are read as zero.
+int make_map_codes(CUtensorMap* map, const int8_t* codes, uint64_t stride, uint32_t rows, uint32_t length, uint32_t box_rows);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ float sigmoid(float x) {

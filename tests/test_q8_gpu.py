@@ -233,7 +233,7 @@ def test_products_bit_for_bit(t0, rt, dev, m, n, k):
     a_stride, w_stride = up16(k) + (0 if dense else 32), up16(k) + (0 if dense else 16)
     a, a_scales, ab, asb = rows8(rng, dev, m, k, a_stride, True)
     w, w_scales, wb, wsb = rows8(rng, dev, n, k, w_stride, True)
-    y_stride, shift = (n, 0) if dense else (n + 5, 3)
+    y_stride, shift = (n, 0) if dense else [(n + 5, 3), (up16(n) + 16, 8)][k % 2]     # the second: rows on 16-byte boundaries
     y, at = out_rows(dev, m, n, y_stride, bf16, shift)
     bias = (rng.standard_normal(n) * 1000).astype(np.float32) if with_bias else None
     rt.q8_gemm(rt.q8_gemm_args(ab.gpu_addr(), asb.gpu_addr(), wb.gpu_addr(), wsb.gpu_addr(), at, m=m, n=n, k=k, bias=dev.up(bias).gpu_addr() if with_bias else 0, out_bf16=bf16,
@@ -278,7 +278,7 @@ def test_gated_products(t0, rt, dev, m, n, k):
     a_scales[0] *= 300                                                    # gates far into both ends of the sigmoid
     asb = dev.up(a_scales)
     (g, g_scales, gb, gsb), (u, u_scales, ub, usb) = weights
-    y_stride, shift = (n, 0) if dense else (n + 3, 5)
+    y_stride, shift = (n, 0) if dense else [(n + 3, 5), (up16(n), 0)][k % 2]
     y, at = out_rows(dev, m, n, y_stride, bf16, shift)
     rt.q8_gated(rt.q8_gated_args(ab.gpu_addr(), asb.gpu_addr(), gb.gpu_addr(), gsb.gpu_addr(), ub.gpu_addr(), usb.gpu_addr(), at, m=m, n=n, k=k, activation=act, out_bf16=bf16,
                                  a_stride=stride, w_stride=stride, y_stride=y_stride))
