@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256) q8_gemm_kernel(const Product P) {
 }
 
 int launch(t0_runtime* rt, const Product& P, bool gated) {
-    if (P.m > 128) return launch_pair(rt, P, gated);
+    return P.m > 256 ? launch_pair(rt, P, gated) : launch_stream(rt, P, gated);
     const uint64_t grid = (uint64_t)ceil_div(P.m, kTile) * ceil_div(P.n, kTile);
     if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "m=%u, n=%u: too much for one launch", P.m, P.n);
     const DeviceGuard guard(rt->device);

@@ -1,0 +1,271 @@
+// Products of few rows in eight bits, plain or gated: the weights are streamed once, tcgen05.mma kind::i8 with the WEIGHTS as its 128 rows and the tokens as its columns.
+//
+// What bounds these products is the weights' way from memory.  A tile is `rows` rows of the weights (up to 128, as many as give every SM the same share: the tensor core works on
+// 128 whatever is in them) by `tokens` rows of A (a multiple of 16, up to 256; 128 for the gated pair, whose two matrices take a tile each), and a CTA takes a tile, or a part of its
+// k blocks where the tiles of whole sums would be too few: the parts' CTAs form a cluster, park their sums in shared memory and share the adding out by tokens (whole numbers: the
+// order is of no matter).  A lane of tensor memory is one row of the weights, so a store instruction writes 32 neighbouring numbers of one row of y whatever its alignment.
+#include "gemm_common.cuh"
+#include "q8.cuh"
+#include "runtime_internal.h"
+
+namespace t0 {
+namespace q8 {
+namespace {
+
+constexpr uint32_t kThreads = 192;                   // producer, UMMA issuer, four epilogue warps
+constexpr uint32_t kBlock = 128;                     // codes a stage is deep
+constexpr uint32_t kRing = 192 * 1024;               // shared memory for stages
+constexpr uint32_t kMaxStages = 32;
+constexpr uint32_t kSlack = 16384;                   // the tensor core reads 128 rows from where a tile of fewer begins
+constexpr uint32_t kSmem = 1024 + kRing + kSlack + 1024;
+
+struct StreamParams {
+    Product P;
+    uint32_t rows, tokens;                           // of a tile
+    uint32_t tiles_n, tiles_m, parts;
+    uint32_t k_blocks, stages;
+    uint32_t w_bytes, stage_bytes;                   // one matrix's rows of a stage (whole kilobytes), all of a stage
+    uint32_t tmem_cols, drop_load;
+    int* status;
+    uint64_t wait_limit_ns;
+};
+
+// The rows of the weights from n0 on that are lanes of a warp, and what they are multiplied with.
+struct Column {
+    uint32_t n;
+    bool in;
+    float scale, scale2, bias;
+};
+template <bool kGated>
+__device__ __forceinline__ Column column_of(const StreamParams& p, uint32_t n0, uint32_t lane_row) {
+    Column c;
+    c.n = n0 + lane_row;
+    c.in = lane_row < p.rows && c.n < p.P.n;
+    c.scale = c.in ? p.P.w_scales[0][c.n] : 0.0f;
+    c.scale2 = kGated && c.in ? p.P.w_scales[1][c.n] : 0.0f;
+    c.bias = !kGated && c.in && p.P.bias ? p.P.bias[c.n] : 0.0f;
+    return c;
+}
+template <bool kGated>
+__device__ __forceinline__ void put(const StreamParams& p, const Column& c, uint32_t token, int32_t sum, int32_t sum2, float a_scale) {
+    float v = scaled(sum, a_scale, c.scale);
+    if constexpr (kGated) v = __fmul_rn(activate(v, p.P.act), scaled(sum2, a_scale, c.scale2));
+    else if (p.P.bias) v = __fadd_rn(v, c.bias);
+    if (!c.in) return;
+    const uint64_t at = token * p.P.y_stride + c.n;
+    if (p.P.out_bf16) ((__nv_bfloat16*)p.P.y)[at] = __float2bfloat16_rn(v);
+    else ((float*)p.P.y)[at] = v;
+}
+
+template <bool kGated>
+__global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
+                                                             const StreamParams p) {
+    constexpr uint32_t kW = kGated ? 2 : 1;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = (uint64_t*)(smem + kRing + kSlack);
+    uint64_t* full_bar = bars;
+    uint64_t* empty_bar = bars + kMaxStages;
+    uint64_t* done_bar = bars + 2 * kMaxStages;
+    uint32_t* tmem_holder = (uint32_t*)(bars + 2 * kMaxStages + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
+    const Product& P = p.P;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t part = blockIdx.x % p.parts, tile = blockIdx.x / p.parts, n0 = tile / p.tiles_m * p.rows, m0 = tile % p.tiles_m * p.tokens;
+    const uint32_t kb0 = (uint32_t)((uint64_t)p.k_blocks * part / p.parts), kb1 = (uint32_t)((uint64_t)p.k_blocks * (part + 1) / p.parts);
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.stages; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
+        }
+        ptx::mbar_init(ptx::smem_u32(done_bar), 1);
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+        ptx::tma_prefetch_desc(&map_a);
+        ptx::tma_prefetch_desc(&map_w);
+        if (kGated) ptx::tma_prefetch_desc(&map_w2);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(ptx::smem_u32(tmem_holder), p.tmem_cols);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_holder;
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+
+    if (warp == 0) {
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            if (!ptx::mbar_wait_warp(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.wait_limit_ns)) {
+                if (lane == 0) atomicCAS(p.status, 0, kStatusProducerTimeout | (int)(tile & 0xFFFFFF));
+                break;
+            }
+            const uint32_t issue = ptx::elect_one() && !(p.drop_load && blockIdx.x == 0 && kb == 0);       // (self-test of the failure path)
+            const uint32_t fb = ptx::smem_u32(&full_bar[stage]), to = ptx::smem_u32(smem) + stage * p.stage_bytes;
+            ptx::mbar_arrive_expect_tx_if(issue, fb, (kW * p.rows + p.tokens) * kBlock);
+            ptx::tma_load_2d_if(issue, to, &map_w, fb, (int32_t)(kb * kBlock), (int32_t)n0);
+            if (kGated) ptx::tma_load_2d_if(issue, to + p.w_bytes, &map_w2, fb, (int32_t)(kb * kBlock), (int32_t)n0);
+            ptx::tma_load_2d_if(issue, to + kW * p.w_bytes, &map_a, fb, (int32_t)(kb * kBlock), (int32_t)m0);
+            if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = ptx::make_idesc_i8_s32(128, p.tokens);
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            if (!ptx::mbar_wait_warp(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.wait_limit_ns)) {
+                if (lane == 0) atomicCAS(p.status, 0, kStatusMmaTimeout | (int)(tile & 0xFFFFFF));
+                ok = false;
+                break;
+            }
+            ptx::tc_fence_after_sync();
+            const uint32_t issue = ptx::elect_one();
+            const uint32_t w_lo = ptx::smem_desc_lo(ptx::smem_u32(smem) + stage * p.stage_bytes, 16), a_lo = w_lo + ((kW * p.w_bytes) >> 4);
+#pragma unroll
+            for (uint32_t e = 0; e < kBlock / 32; ++e) {
+                ptx::umma_i8_ss_if(issue, tmem_base, w_lo + 2 * e, a_lo + 2 * e, idesc, kb != kb0 || e != 0 ? 1u : 0u);
+                if (kGated) ptx::umma_i8_ss_if(issue, tmem_base + p.tokens, w_lo + (p.w_bytes >> 4) + 2 * e, a_lo + 2 * e, idesc, kb != kb0 || e != 0 ? 1u : 0u);
+            }
+            ptx::umma_commit_if(issue, ptx::smem_u32(&empty_bar[stage]));
+            if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) ptx::umma_commit_if(ptx::elect_one(), ptx::smem_u32(done_bar));
+    } else {
+        const uint32_t quarter = warp & 3;
+        const bool some = quarter * 32 < p.rows && n0 + quarter * 32 < P.n;          // of this warp's rows
+        const Column c = column_of<kGated>(p, n0, quarter * 32 + lane);
+        if (!ptx::mbar_wait_warp(ptx::smem_u32(done_bar), 0, abort_flag, p.wait_limit_ns)) {
+            if (lane == 0) atomicCAS(p.status, 0, kStatusEpilogueTimeout | (int)(tile & 0xFFFFFF));
+        } else if (some) {
+            ptx::tc_fence_after_sync();
+            const uint32_t tmem = tmem_base + ((quarter * 32) << 16), tokens = min(p.tokens, P.m - m0);
+            const uint32_t parked = ptx::smem_u32(smem) + (quarter * 32 + lane) * 4;
+#pragma unroll 1
+            for (uint32_t t = 0; t < tokens; t += 16) {
+                uint32_t r[16], r2[kGated ? 16 : 1];
+                ptx::tmem_ld_32x32b_x16(tmem + t, r);
+                if constexpr (kGated) ptx::tmem_ld_32x32b_x16(tmem + p.tokens + t, r2);
+                ptx::tmem_ld_wait();
+                if (p.parts == 1) {
+                    const float mine = t + (lane & 15) < tokens ? P.a_scales[m0 + t + (lane & 15)] : 0.0f;
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; ++j) {
+                        const float a_scale = __shfl_sync(0xFFFFFFFFu, mine, j);
+                        if (t + j < tokens) put<kGated>(p, c, m0 + t + j, (int)r[j], kGated ? (int)r2[kGated ? j : 0] : 0, a_scale);
+                    }
+                } else {
+                    // over the ring, which is idle: all copies have landed and all products read them
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; ++j) {
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(parked + (t + j) * 512), "r"(r[j]) : "memory");
+                        if constexpr (kGated) asm volatile("st.shared.b32 [%0], %1;" ::"r"(parked + (p.tokens + t + j) * 512), "r"(r2[j]) : "memory");
+                    }
+                }
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- the parts' sums
+    __syncwarp();
+    if (*abort_flag) {
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+    ptx::tc_fence_before_sync();
+    if (p.parts > 1) {
+        ptx::cluster_sync_all();
+        const uint32_t tokens = min(p.tokens, P.m - m0), quarters = (min(p.rows, P.n - n0) + 31) / 32;
+        uint32_t last = 0xFFFFFFFFu;
+        Column c = {};
+        if (!*abort_flag) {
+            for (uint32_t i = warp; i < quarters * 6; i += 6) {                       // a warp for a quarter's tokens, every sixth of this part's
+                const uint32_t quarter = i / 6;
+                if (quarter != last) c = column_of<kGated>(p, n0, quarter * 32 + lane), last = quarter;
+                const uint32_t at = ptx::smem_u32(smem) + (quarter * 32 + lane) * 4;
+                for (uint32_t t = part + warp * p.parts; t < tokens; t += 6 * p.parts) {
+                    int32_t sum = 0, sum2 = 0;
+                    for (uint32_t s = 0; s < p.parts; ++s) {
+                        sum += ptx::ld_cluster_i32(ptx::mapa(at + t * 512, s));
+                        if (kGated) sum2 += ptx::ld_cluster_i32(ptx::mapa(at + (p.tokens + t) * 512, s));
+                    }
+                    put<kGated>(p, c, m0 + t, sum, sum2, P.a_scales[m0 + t]);
+                }
+            }
+        }
+        ptx::cluster_sync_all();                       // a CTA's shared memory stays until all have read it
+    } else {
+        __syncthreads();
+    }
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem_base, p.tmem_cols);
+    }
+}
+
+// How a product is cut: rows of the weights and tokens to a tile, parts of K.
+struct Cut { uint32_t rows, tokens, parts; };
+
+Cut choose(const Product& P, bool gated, uint32_t sms) {
+    Cut c;
+    const uint32_t most = gated ? 128 : 256, tiles_m = ceil_div(P.m, most);
+    c.tokens = (ceil_div(P.m, tiles_m) + 15) & ~15u;
+    c.parts = 1;
+    while (c.parts < 8 && ceil_div(P.k, kBlock) >= 4 * (c.parts + 1) && (uint64_t)P.n * tiles_m * (c.parts + 1) <= 128ull * sms) ++c.parts;
+    c.rows = std::min(128u, std::max(8u, ceil_div(P.n, std::max(1u, sms / tiles_m / c.parts))));
+    return c;
+}
+
+template <bool kGated>
+int launch_instance(t0_runtime* rt, const Product& P) {
+    auto kern = q8_stream_kernel<kGated>;
+    static std::atomic<bool> ready[64];
+    const int dev = rt->device;
+    if (dev < 0 || dev >= 64) return fail(T0_ERR_INVALID, "device ordinal out of range");
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+        if (e != cudaSuccess) return fail(T0_ERR_CUDA, "cudaFuncSetAttribute(smem=%u): %s", kSmem, cudaGetErrorString(e));
+        ready[dev].store(true, std::memory_order_release);
+    }
+    const Cut cut = choose(P, kGated, (uint32_t)rt->sm_count);
+    StreamParams p;
+    memset((void*)&p, 0, sizeof p);
+    p.P = P;
+    p.rows = cut.rows; p.tokens = cut.tokens; p.parts = cut.parts;
+    p.tiles_n = ceil_div(P.n, p.rows); p.tiles_m = ceil_div(P.m, p.tokens);
+    p.k_blocks = ceil_div(P.k, kBlock);
+    p.w_bytes = ((p.rows + 7) & ~7u) * kBlock;
+    p.stage_bytes = (kGated ? 2 : 1) * p.w_bytes + p.tokens * kBlock;
+    p.stages = std::min(std::min(kMaxStages, kRing / p.stage_bytes), std::max(1u, ceil_div(p.k_blocks, p.parts)));
+    p.tmem_cols = 32;
+    while (p.tmem_cols < (kGated ? 2 : 1) * p.tokens) p.tmem_cols *= 2;
+    p.status = rt->d_status;
+    const uint64_t limit = rt->wait_limit_ns.load(std::memory_order_relaxed);
+    p.wait_limit_ns = limit ? limit : ptx::kWaitLimitNs;
+    p.drop_load = rt->drop_next_load.exchange(0) != 0;
+    const uint64_t grid = (uint64_t)p.tiles_n * p.tiles_m * p.parts;
+    if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "m=%u, n=%u: too much for one launch", P.m, P.n);
+    CUtensorMap ma, mw, mw2;
+    int rc = make_map_codes(&ma, P.a, P.a_stride, P.m, P.k, p.tokens);
+    if (rc == T0_OK) rc = make_map_codes(&mw, P.w[0], P.w_stride, P.n, P.k, p.rows);
+    mw2 = mw;
+    if (rc == T0_OK && kGated) rc = make_map_codes(&mw2, P.w[1], P.w_stride, P.n, P.k, p.rows);
+    if (rc != T0_OK) return rc;
+    const cudaError_t e = gemm::launch_pdl_clusters(kern, (uint32_t)grid, p.parts, kThreads, kSmem, rt->stream, ma, mw, mw2, p);
+    if (e != cudaSuccess) return fail(T0_ERR_CUDA, "launch of the eight-bit product failed: %s", cudaGetErrorString(e));
+    rt->launches.fetch_add(1);
+    return T0_OK;
+}
+
+}  // namespace
+
+int launch_stream(t0_runtime* rt, const Product& P, bool gated) {
+    const DeviceGuard guard(rt->device);
+    return gated ? launch_instance<true>(rt, P) : launch_instance<false>(rt, P);
+}
+
+}  // namespace q8
+}  // namespace t0
