@@ -170,6 +170,12 @@ __device__ __forceinline__ void tma_load_2d_if(uint32_t issue, uint32_t smem_dst
         ::"r"(smem_dst), "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(issue)
         : "memory");
 }
+// The box on its way into L2, where `issue` holds.
+__device__ __forceinline__ void tma_prefetch_2d_if(uint32_t issue, const CUtensorMap* map, int32_t c0, int32_t c1) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\t@q cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];\n\t}"
+                 ::"l"((uint64_t)map), "r"(c0), "r"(c1), "r"(issue)
+                 : "memory");
+}
 // Untiled bulk copy global -> shared (both addresses 16-byte aligned, size a multiple of 16), completion bytes on `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"

@@ -12,20 +12,21 @@ namespace t0 {
 namespace q8 {
 namespace {
 
-constexpr uint32_t kThreads = 192;                   // producer, UMMA issuer, four epilogue warps
+constexpr uint32_t kMostWarps = 2 + 16;             // producer, UMMA issuer, one to four epilogue warps for each quarter of the rows
 constexpr uint32_t kBlock = 128;                     // codes a stage is deep
-constexpr uint32_t kRing = 192 * 1024;               // shared memory for stages
 constexpr uint32_t kMaxStages = 32;
-constexpr uint32_t kSlack = 16384;                   // the tensor core reads 128 rows from where a tile of fewer begins
-constexpr uint32_t kSmem = 1024 + kRing + kSlack + 1024;
+constexpr uint32_t kTile = 128 * kBlock;             // bytes that the tensor core reads from where a tile of the weights begins, however many rows it has
+constexpr uint32_t kMostRing = 192 * 1024;           // shared memory for stages
+constexpr uint32_t kMostSmem = 1024 + kMostRing + kTile + 1024;
 
 struct StreamParams {
     Product P;
     uint32_t rows, tokens;                           // of a tile
     uint32_t tiles_n, tiles_m, parts;
-    uint32_t k_blocks, stages;
+    uint32_t k_blocks, stages, ring;                 // the ring in bytes, with what the last tile is short of 128 rows
     uint32_t w_bytes, stage_bytes;                   // one matrix's rows of a stage (whole kilobytes), all of a stage
     uint32_t tmem_cols, drop_load;
+    uint32_t ahead;                                  // blocks of a part that are asked into L2 before the launch waits for the one before it
     int* status;
     uint64_t wait_limit_ns;
 };
@@ -46,24 +47,41 @@ __device__ __forceinline__ Column column_of(const StreamParams& p, uint32_t n0, 
     c.bias = !kGated && c.in && p.P.bias ? p.P.bias[c.n] : 0.0f;
     return c;
 }
-template <bool kGated>
-__device__ __forceinline__ void put(const StreamParams& p, const Column& c, uint32_t token, int32_t sum, int32_t sum2, float a_scale) {
-    float v = scaled(sum, a_scale, c.scale);
-    if constexpr (kGated) v = __fmul_rn(activate(v, p.P.act), scaled(sum2, a_scale, c.scale2));
-    else if (p.P.bias) v = __fadd_rn(v, c.bias);
+// kCount sums of this lane's column, of kCount tokens, to what y has there.
+template <bool kGated, int kCount>
+__device__ __forceinline__ void finish(const StreamParams& p, const Column& c, const int32_t (&sum)[kCount], const int32_t (&sum2)[kGated ? kCount : 1], const float (&a_scale)[kCount],
+                                       float (&v)[kCount]) {
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) v[j] = scaled(sum[j], a_scale[j], c.scale);
+    if constexpr (kGated) {
+        if (p.P.act == T0_TEPI_RELU) {
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
+        } else {
+            const float turn = p.P.act == T0_TEPI_GELU ? 1.702f : 1.0f;
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) v[j] *= sigmoid(v[j] * turn);
+        }
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = __fmul_rn(v[j], scaled(sum2[j], a_scale[j], c.scale2));
+    } else if (p.P.bias) {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = __fadd_rn(v[j], c.bias);
+    }
+}
+__device__ __forceinline__ void put(const StreamParams& p, const Column& c, uint64_t at, float v) {
     if (!c.in) return;
-    const uint64_t at = token * p.P.y_stride + c.n;
     if (p.P.out_bf16) ((__nv_bfloat16*)p.P.y)[at] = __float2bfloat16_rn(v);
     else ((float*)p.P.y)[at] = v;
 }
 
 template <bool kGated>
-__global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
+__global__ void __launch_bounds__(32 * kMostWarps) q8_stream_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
                                                              const StreamParams p) {
     constexpr uint32_t kW = kGated ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = (uint64_t*)(smem + kRing + kSlack);
+    uint64_t* bars = (uint64_t*)(smem + p.ring);
     uint64_t* full_bar = bars;
     uint64_t* empty_bar = bars + kMaxStages;
     uint64_t* done_bar = bars + 2 * kMaxStages;
@@ -73,6 +91,8 @@ __global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_consta
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t part = blockIdx.x % p.parts, tile = blockIdx.x / p.parts, n0 = tile / p.tiles_m * p.rows, m0 = tile % p.tiles_m * p.tokens;
     const uint32_t kb0 = (uint32_t)((uint64_t)p.k_blocks * part / p.parts), kb1 = (uint32_t)((uint64_t)p.k_blocks * (part + 1) / p.parts);
+    // Every CTA begins at another block of its part: all read the same rows of A, and in step they would ask the same few lines of L2 at the same time.
+    const uint32_t first = kb0 + (uint32_t)((uint64_t)tile * 2654435761ull % (kb1 - kb0));
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < p.stages; ++s) {
@@ -96,16 +116,24 @@ __global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_consta
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_holder;
     ptx::grid_launch_dependents();
+    if (warp == 0) {
+        // What the launch before this one leaves idle of the memory's time: the first stages' weights on their way into L2 (a hint: whatever that launch still writes, L2 has it).
+        const uint32_t issue = ptx::elect_one(), ahead = min(p.ahead, kb1 - kb0);
+        for (uint32_t i = 0, kb = first; i < ahead; ++i, kb = kb + 1 == kb1 ? kb0 : kb + 1) {
+            ptx::tma_prefetch_2d_if(issue, &map_w, (int32_t)(kb * kBlock), (int32_t)n0);
+            if (kGated) ptx::tma_prefetch_2d_if(issue, &map_w2, (int32_t)(kb * kBlock), (int32_t)n0);
+        }
+    }
     ptx::grid_dependency_wait();
 
     if (warp == 0) {
         uint32_t stage = 0, phase = 0;
-        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+        for (uint32_t i = kb0, kb = first; i < kb1; ++i, kb = kb + 1 == kb1 ? kb0 : kb + 1) {
             if (!ptx::mbar_wait_warp(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.wait_limit_ns)) {
                 if (lane == 0) atomicCAS(p.status, 0, kStatusProducerTimeout | (int)(tile & 0xFFFFFF));
                 break;
             }
-            const uint32_t issue = ptx::elect_one() && !(p.drop_load && blockIdx.x == 0 && kb == 0);       // (self-test of the failure path)
+            const uint32_t issue = ptx::elect_one() && !(p.drop_load && blockIdx.x == 0 && i == 0);       // (self-test of the failure path)
             const uint32_t fb = ptx::smem_u32(&full_bar[stage]), to = ptx::smem_u32(smem) + stage * p.stage_bytes;
             ptx::mbar_arrive_expect_tx_if(issue, fb, (kW * p.rows + p.tokens) * kBlock);
             ptx::tma_load_2d_if(issue, to, &map_w, fb, (int32_t)(kb * kBlock), (int32_t)n0);
@@ -136,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_consta
         }
         if (ok) ptx::umma_commit_if(ptx::elect_one(), ptx::smem_u32(done_bar));
     } else {
-        const uint32_t quarter = warp & 3;
+        const uint32_t quarter = warp & 3, turn = (warp - 2) >> 2, turns = (blockDim.x / 32 - 2) >> 2;
         const bool some = quarter * 32 < p.rows && n0 + quarter * 32 < P.n;          // of this warp's rows
         const Column c = column_of<kGated>(p, n0, quarter * 32 + lane);
         if (!ptx::mbar_wait_warp(ptx::smem_u32(done_bar), 0, abort_flag, p.wait_limit_ns)) {
@@ -146,17 +174,25 @@ __global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_consta
             const uint32_t tmem = tmem_base + ((quarter * 32) << 16), tokens = min(p.tokens, P.m - m0);
             const uint32_t parked = ptx::smem_u32(smem) + (quarter * 32 + lane) * 4;
 #pragma unroll 1
-            for (uint32_t t = 0; t < tokens; t += 16) {
+            for (uint32_t t = turn * 16; t < tokens; t += 16 * turns) {
                 uint32_t r[16], r2[kGated ? 16 : 1];
                 ptx::tmem_ld_32x32b_x16(tmem + t, r);
                 if constexpr (kGated) ptx::tmem_ld_32x32b_x16(tmem + p.tokens + t, r2);
                 ptx::tmem_ld_wait();
                 if (p.parts == 1) {
                     const float mine = t + (lane & 15) < tokens ? P.a_scales[m0 + t + (lane & 15)] : 0.0f;
+                    float a_scale[16], v[16];
 #pragma unroll
-                    for (uint32_t j = 0; j < 16; ++j) {
-                        const float a_scale = __shfl_sync(0xFFFFFFFFu, mine, j);
-                        if (t + j < tokens) put<kGated>(p, c, m0 + t + j, (int)r[j], kGated ? (int)r2[kGated ? j : 0] : 0, a_scale);
+                    for (uint32_t j = 0; j < 16; ++j) a_scale[j] = __shfl_sync(0xFFFFFFFFu, mine, j);
+                    finish<kGated, 16>(p, c, (const int32_t(&)[16])r, (const int32_t(&)[kGated ? 16 : 1])r2, a_scale, v);
+                    const uint64_t at = (uint64_t)(m0 + t) * P.y_stride + c.n;
+                    if (t + 16 <= tokens) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j) put(p, c, at + j * P.y_stride, v[j]);
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j)
+                            if (t + j < tokens) put(p, c, at + j * P.y_stride, v[j]);
                     }
                 } else {
                     // over the ring, which is idle: all copies have landed and all products read them
@@ -179,21 +215,30 @@ __global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_consta
     if (p.parts > 1) {
         ptx::cluster_sync_all();
         const uint32_t tokens = min(p.tokens, P.m - m0), quarters = (min(p.rows, P.n - n0) + 31) / 32;
-        uint32_t last = 0xFFFFFFFFu;
-        Column c = {};
         if (!*abort_flag) {
-            for (uint32_t i = warp; i < quarters * 6; i += 6) {                       // a warp for a quarter's tokens, every sixth of this part's
-                const uint32_t quarter = i / 6;
-                if (quarter != last) c = column_of<kGated>(p, n0, quarter * 32 + lane), last = quarter;
-                const uint32_t at = ptx::smem_u32(smem) + (quarter * 32 + lane) * 4;
-                for (uint32_t t = part + warp * p.parts; t < tokens; t += 6 * p.parts) {
-                    int32_t sum = 0, sum2 = 0;
-                    for (uint32_t s = 0; s < p.parts; ++s) {
-                        sum += ptx::ld_cluster_i32(ptx::mapa(at + t * 512, s));
-                        if (kGated) sum2 += ptx::ld_cluster_i32(ptx::mapa(at + (p.tokens + t) * 512, s));
+            // a warp takes a quarter of the rows and every so many of this part's tokens, four at a time with all their loads in flight
+            const uint32_t quarter = warp % quarters, each = p.parts * ((blockDim.x / 32 - quarter + quarters - 1) / quarters);
+            const Column c = column_of<kGated>(p, n0, quarter * 32 + lane);
+            const uint32_t at = ptx::smem_u32(smem) + (quarter * 32 + lane) * 4;
+            for (uint32_t t = part + warp / quarters * p.parts; t < tokens; t += 4 * each) {
+                int32_t sum[4] = {}, sum2[kGated ? 4 : 1] = {};
+                float a_scale[4], v[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) a_scale[j] = t + j * each < tokens ? P.a_scales[m0 + t + j * each] : 0.0f;
+#pragma unroll 2
+                for (uint32_t s = 0; s < p.parts; ++s) {
+                    const uint32_t from = ptx::mapa(at, s);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t tt = min(t + j * each, tokens - 1);
+                        sum[j] += ptx::ld_cluster_i32(from + tt * 512);
+                        if constexpr (kGated) sum2[j] += ptx::ld_cluster_i32(from + (p.tokens + tt) * 512);
                     }
-                    put<kGated>(p, c, m0 + t, sum, sum2, P.a_scales[m0 + t]);
                 }
+                finish<kGated, 4>(p, c, sum, sum2, a_scale, v);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    if (t + j * each < tokens) put(p, c, (uint64_t)(m0 + t + j * each) * P.y_stride + c.n, v[j]);
             }
         }
         ptx::cluster_sync_all();                       // a CTA's shared memory stays until all have read it
@@ -207,7 +252,7 @@ __global__ void __launch_bounds__(kThreads) q8_stream_kernel(const __grid_consta
 }
 
 // How a product is cut: rows of the weights and tokens to a tile, parts of K.
-struct Cut { uint32_t rows, tokens, parts; };
+struct Cut { uint32_t rows, tokens, parts, ring, warps; };
 
 Cut choose(const Product& P, bool gated, uint32_t sms) {
     Cut c;
@@ -216,6 +261,8 @@ Cut choose(const Product& P, bool gated, uint32_t sms) {
     c.parts = 1;
     while (c.parts < 8 && ceil_div(P.k, kBlock) >= 4 * (c.parts + 1) && (uint64_t)P.n * tiles_m * (c.parts + 1) <= 128ull * sms) ++c.parts;
     c.rows = std::min(128u, std::max(8u, ceil_div(P.n, std::max(1u, sms / tiles_m / c.parts))));
+    c.ring = kMostRing;
+    c.warps = c.tokens <= 16 ? 4 : c.tokens <= 64 ? 8 : 16;
     return c;
 }
 
@@ -226,8 +273,8 @@ int launch_instance(t0_runtime* rt, const Product& P) {
     const int dev = rt->device;
     if (dev < 0 || dev >= 64) return fail(T0_ERR_INVALID, "device ordinal out of range");
     if (!ready[dev].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-        if (e != cudaSuccess) return fail(T0_ERR_CUDA, "cudaFuncSetAttribute(smem=%u): %s", kSmem, cudaGetErrorString(e));
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem);
+        if (e != cudaSuccess) return fail(T0_ERR_CUDA, "cudaFuncSetAttribute(smem=%u): %s", kMostSmem, cudaGetErrorString(e));
         ready[dev].store(true, std::memory_order_release);
     }
     const Cut cut = choose(P, kGated, (uint32_t)rt->sm_count);
@@ -239,7 +286,10 @@ int launch_instance(t0_runtime* rt, const Product& P) {
     p.k_blocks = ceil_div(P.k, kBlock);
     p.w_bytes = ((p.rows + 7) & ~7u) * kBlock;
     p.stage_bytes = (kGated ? 2 : 1) * p.w_bytes + p.tokens * kBlock;
-    p.stages = std::min(std::min(kMaxStages, kRing / p.stage_bytes), std::max(1u, ceil_div(p.k_blocks, p.parts)));
+    p.stages = std::min(kMaxStages, cut.ring / p.stage_bytes);
+    p.ring = p.stages * p.stage_bytes + (p.w_bytes + p.tokens * kBlock < kTile ? kTile - p.w_bytes - p.tokens * kBlock : 0);
+    if (p.parts > 1) p.ring = std::max(p.ring, (kGated ? 2 : 1) * p.tokens * 512);
+    p.ahead = std::min(p.stages, 8u);
     p.tmem_cols = 32;
     while (p.tmem_cols < (kGated ? 2 : 1) * p.tokens) p.tmem_cols *= 2;
     p.status = rt->d_status;
@@ -254,7 +304,7 @@ int launch_instance(t0_runtime* rt, const Product& P) {
     mw2 = mw;
     if (rc == T0_OK && kGated) rc = make_map_codes(&mw2, P.w[1], P.w_stride, P.n, P.k, p.rows);
     if (rc != T0_OK) return rc;
-    const cudaError_t e = gemm::launch_pdl_clusters(kern, (uint32_t)grid, p.parts, kThreads, kSmem, rt->stream, ma, mw, mw2, p);
+    const cudaError_t e = gemm::launch_pdl_clusters(kern, (uint32_t)grid, p.parts, 32 * (2 + cut.warps), 1024 + p.ring + 1024, rt->stream, ma, mw, mw2, p);
     if (e != cudaSuccess) return fail(T0_ERR_CUDA, "launch of the eight-bit product failed: %s", cudaGetErrorString(e));
     rt->launches.fetch_add(1);
     return T0_OK;
