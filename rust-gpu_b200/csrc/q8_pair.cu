@@ -4,6 +4,7 @@
 // the tensor pipe, as a stage of 64 bf16 is, and moves as many bytes: the roles are those of the bf16 pair kernel, and so is the order of the tiles.
 // The gated pair of products takes 128 rows of each matrix as the two halves of B: the even CTA loads the gate's, the odd one the other's, and the sums of one output stand in one
 // lane of tensor memory, 128 columns apart.  The tile gives 256 x 128 outputs, and neither product leaves the SM.
+// A last round that would leave half of the pairs idle is taken in half tiles.
 #include "gemm_common.cuh"
 #include "q8.cuh"
 #include "runtime_internal.h"
@@ -26,7 +27,7 @@ int make_map_codes(CUtensorMap* map, const int8_t* codes, uint64_t stride, uint3
 
 namespace {
 
-constexpr uint32_t kThreads = 192;                   // producer, UMMA issuer, four epilogue warps
+constexpr uint32_t kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;   // producer, UMMA issuer, two epilogue warps for each quarter of the rows
 constexpr uint32_t kHalf = 128;                      // rows of A, and of B, that one CTA loads
 constexpr uint32_t kBlock = 128;                     // codes a stage is deep
 constexpr uint32_t kOperandBytes = kHalf * kBlock, kStageBytes = 2 * kOperandBytes;
@@ -36,29 +37,30 @@ constexpr uint32_t kRaster = 8;                      // column tiles that are wa
 struct PairParams {
     Product P;
     uint32_t tiles_m, tiles_n, k_blocks;
+    uint32_t whole;                                  // tiles that are taken whole; those after them are taken in two halves of their columns
     uint32_t tma_store, drop_load;
     int* status;
     uint64_t wait_limit_ns;
 };
 
-struct Tile { uint32_t m, n; };
-__device__ __forceinline__ Tile tile_of(uint32_t w, const PairParams& p) {
+struct Tile { uint32_t m, n, half; bool halved; };
+__device__ __forceinline__ Tile tile_of(uint32_t i, const PairParams& p) {
+    const bool halved = i >= p.whole;
+    const uint32_t w = halved ? p.whole + (i - p.whole) / 2 : i, half = halved ? (i - p.whole) & 1u : 0u;
     const uint32_t group = w / (kRaster * p.tiles_m), first = group * kRaster, wide = min(kRaster, p.tiles_n - first), r = w - group * kRaster * p.tiles_m;
-    return {r / wide, first + r % wide};
+    return {r / wide, first + r % wide, half, halved};
 }
 
-constexpr uint32_t smem_bytes() { return 1024 + kStages * kStageBytes + 8 * gemm::kEpiStageBytes + 4 * 256 + 256; }
+constexpr uint32_t smem_bytes() { return kStages * kStageBytes + kEpilogueWarps * (gemm::kEpiStageBytes + 256) + 256; }
 
-// 32 rows x 32 columns on their way to y, this lane's row `row0 + lane`: through `stage` (two 4 KiB blocks of this warp, 16-byte slots turned by the row) and out as one tiled TMA
-// store a block (f32: a chunk, bf16: an even chunk and the odd one after it) where y's rows begin and end on 16-byte boundaries, else row by row.  n_stores counts the warp's
-// committed stores: block i & 1 is written again only when every store but the latest has been read.
-__device__ __forceinline__ void put_chunk(const PairParams& p, const CUtensorMap* map_y, const float (&v)[32], uint32_t row0, uint32_t col0, uint32_t c, uint32_t lane, uint32_t stage,
-                                          uint32_t& n_stores) {
+// 32 rows x 32 columns on their way to y, this lane's row `row0 + lane`: through `stage` (a 4 KiB block of this warp, 16-byte slots turned by the row) and out as one tiled TMA
+// store a block (f32: a chunk; bf16: the two chunks of 64 columns, `half` of it) where y's rows begin and end on 16-byte boundaries, else row by row.
+__device__ __forceinline__ void put_chunk(const PairParams& p, const CUtensorMap* map_y, const float (&v)[32], uint32_t row0, uint32_t col0, uint32_t which, uint32_t lane, uint32_t stage) {
     const Product& P = p.P;
     if (p.tma_store) {
-        const uint32_t sb = stage + (n_stores & 1u) * gemm::kEpiStageBytes, half = P.out_bf16 ? c & 1u : 0u;
+        const uint32_t sb = stage, half = P.out_bf16 ? which : 0u;
         if (half == 0) {
-            if (lane == 0) ptx::bulk_wait_group_read_but_one();
+            if (lane == 0) ptx::bulk_wait_group_read_all();
             __syncwarp();
         }
         if (P.out_bf16) {
@@ -72,7 +74,7 @@ __device__ __forceinline__ void put_chunk(const PairParams& p, const CUtensorMap
                 }
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sb + (lane * 8 + ((half * 4 + j) ^ (lane & 7))) * 16), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
             }
-            if (half == 0 && col0 + 32 < P.n) return;          // the odd chunk completes the block
+            if (half == 0 && col0 + 32 < P.n) return;          // the second chunk completes the block
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 8; ++j)
@@ -84,7 +86,6 @@ __device__ __forceinline__ void put_chunk(const PairParams& p, const CUtensorMap
             ptx::tma_store_2d(map_y, sb, (int32_t)(col0 - half * 32), (int32_t)row0);
             ptx::bulk_commit_group();
         }
-        ++n_stores;
         return;
     }
 #pragma unroll
@@ -115,17 +116,17 @@ __device__ __forceinline__ float4 spread4(uint32_t at, uint32_t j) {
 
 template <bool kGated>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_y,
+q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
+               const __grid_constant__ CUtensorMap map_w_half, const __grid_constant__ CUtensorMap map_w2_half, const __grid_constant__ CUtensorMap map_y,
                const PairParams p) {
     constexpr uint32_t kWide = kGated ? 128 : 256;               // columns of y a tile has
-    constexpr uint32_t kIdesc = ptx::make_idesc_i8_s32(256, 256);
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    constexpr uint32_t kIdesc = ptx::make_idesc_i8_s32(256, 256), kIdescHalf = ptx::make_idesc_i8_s32(256, 128);
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* a_tiles = smem;
     uint8_t* b_tiles = smem + kStages * kOperandBytes;
-    uint8_t* epi_stage = smem + kStages * kStageBytes;           // 4 warps x 2 blocks
-    uint8_t* epi_cols = epi_stage + 8 * gemm::kEpiStageBytes;    // 4 warps x 2 x 32 numbers
-    uint64_t* bars = (uint64_t*)(epi_cols + 4 * 256);
+    uint8_t* epi_stage = smem + kStages * kStageBytes;           // a block for each epilogue warp
+    uint8_t* epi_cols = epi_stage + kEpilogueWarps * gemm::kEpiStageBytes;       // 2 x 32 numbers likewise
+    uint64_t* bars = (uint64_t*)(epi_cols + kEpilogueWarps * 256);
     uint64_t* full_bar = bars;                                   // used in the even CTA only
     uint64_t* empty_bar = bars + kStages;
     uint64_t* tmem_full_bar = bars + 2 * kStages;
@@ -134,7 +135,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
     const Product& P = p.P;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta_rank = ptx::cluster_ctarank(), pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-    const uint32_t total = p.tiles_m * p.tiles_n;
+    const uint32_t total = p.whole + 2 * (p.tiles_m * p.tiles_n - p.whole);
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
@@ -143,7 +144,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         for (uint32_t b = 0; b < 2; ++b) {
             ptx::mbar_init(ptx::smem_u32(&tmem_full_bar[b]), 1);
-            ptx::mbar_init(ptx::smem_u32(&tmem_empty_bar[b]), 8);
+            ptx::mbar_init(ptx::smem_u32(&tmem_empty_bar[b]), 2 * kEpilogueWarps);
         }
         *abort_flag = 0;
         ptx::fence_barrier_init();
@@ -167,11 +168,12 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (warp == 0) {
         // ------------------------------------------------------------ copies (both CTAs): this CTA's rows of A, its half of B
         const CUtensorMap* const my_w = kGated && cta_rank ? &map_w2 : &map_w;
+        const CUtensorMap* const my_w_half = kGated && cta_rank ? &map_w2_half : &map_w_half;
         uint32_t stage = 0, phase = 0;
         bool ok = true;
         for (uint32_t w = pair_id; ok && w < total; w += n_pairs) {
             const Tile t = tile_of(w, p);
-            const int32_t row = (int32_t)(t.m * 256 + cta_rank * kHalf), col = (int32_t)(t.n * kWide + (kGated ? 0 : cta_rank * kHalf));
+            const int32_t row = (int32_t)(t.m * 256 + cta_rank * kHalf), col = (int32_t)(t.n * kWide + t.half * (kWide / 2) + (kGated ? 0 : cta_rank * (t.halved ? kHalf / 2 : kHalf)));
             for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
                 if (!ptx::mbar_wait_warp(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.wait_limit_ns)) {
                     if (lane == 0) atomicCAS(p.status, 0, kStatusProducerTimeout | (int)(w & 0xFFFFFF));
@@ -180,10 +182,10 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 }
                 if (!(p.drop_load && pair_id == 0 && w == 0 && kb == 0) && ptx::elect_one()) {    // (self-test of the failure path: neither CTA of pair 0 fills its first stage)
                     const uint32_t fb_local = ptx::smem_u32(&full_bar[stage]);
-                    if (cta_rank == 0) ptx::mbar_arrive_expect_tx(fb_local, 2 * kStageBytes);
+                    if (cta_rank == 0) ptx::mbar_arrive_expect_tx(fb_local, t.halved ? 2 * (kOperandBytes + kOperandBytes / 2) : 2 * kStageBytes);
                     const uint32_t fb = ptx::mapa(fb_local, 0);
                     ptx::tma_load_2d_pair(ptx::smem_u32(a_tiles + stage * kOperandBytes), &map_a, fb, (int32_t)(kb * kBlock), row);
-                    ptx::tma_load_2d_pair(ptx::smem_u32(b_tiles + stage * kOperandBytes), my_w, fb, (int32_t)(kb * kBlock), col);
+                    ptx::tma_load_2d_pair(ptx::smem_u32(b_tiles + stage * kOperandBytes), t.halved ? my_w_half : my_w, fb, (int32_t)(kb * kBlock), col);
                 }
                 __syncwarp();
                 if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -201,7 +203,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     break;
                 }
                 ptx::tc_fence_after_sync();
-                const uint32_t tmem_d = tmem_base + buf * 256;
+                const uint32_t tmem_d = tmem_base + buf * 256, idesc = w >= p.whole ? kIdescHalf : kIdesc;
                 for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
                     if (!ptx::mbar_wait_warp(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.wait_limit_ns)) {
                         if (lane == 0) atomicCAS(p.status, 0, kStatusMmaTimeout | 0x800000 | (int)(w & 0x7FFFFF));
@@ -213,7 +215,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         const uint32_t a_addr = ptx::smem_u32(a_tiles + stage * kOperandBytes), b_addr = ptx::smem_u32(b_tiles + stage * kOperandBytes);
 #pragma unroll
                         for (uint32_t e = 0; e < kBlock / 32; ++e)
-                            ptx::umma_i8_ss_pair(tmem_d, ptx::make_smem_desc(a_addr + e * 32, 16, 1024), ptx::make_smem_desc(b_addr + e * 32, 16, 1024), kIdesc, kb != 0 || e != 0 ? 1u : 0u);
+                            ptx::umma_i8_ss_pair(tmem_d, ptx::make_smem_desc(a_addr + e * 32, 16, 1024), ptx::make_smem_desc(b_addr + e * 32, 16, 1024), idesc, kb != 0 || e != 0 ? 1u : 0u);
                         const uint32_t eb = ptx::smem_u32(&empty_bar[stage]);
                         ptx::umma_commit_pair(eb);
                         ptx::umma_commit_pair(ptx::mapa(eb, 1));
@@ -230,9 +232,9 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
         }
     } else {
-        // ------------------------------------------------------------ sums to y (warps 2 .. 5, both CTAs)
-        const uint32_t quarter = warp & 3, stage = ptx::smem_u32(epi_stage) + quarter * 2 * gemm::kEpiStageBytes, cols = ptx::smem_u32(epi_cols) + quarter * 256;
-        uint32_t iter = 0, n_stores = 0;
+        // ------------------------------------------------------------ sums to y (both CTAs): a quarter's two warps take its columns in turns of 64
+        const uint32_t quarter = warp & 3, turn = (warp - 2) >> 2, stage = ptx::smem_u32(epi_stage) + (warp - 2) * gemm::kEpiStageBytes, cols = ptx::smem_u32(epi_cols) + (warp - 2) * 256;
+        uint32_t iter = 0;
         for (uint32_t w = pair_id; w < total; w += n_pairs, ++iter) {
             const Tile t = tile_of(w, p);
             const uint32_t buf = iter & 1, acc_phase = (iter >> 1) & 1;
@@ -244,10 +246,12 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
             ptx::tc_fence_after_sync();
             __syncwarp();
-            const uint32_t tmem = tmem_base + ((quarter * 32) << 16) + buf * 256;
+            const uint32_t tmem = tmem_base + ((quarter * 32) << 16) + buf * 256, wide = t.halved ? kWide / 2 : kWide;
 #pragma unroll 1
-            for (uint32_t c = 0; c < kWide / 32; ++c) {
-                const uint32_t col0 = t.n * kWide + c * 32;
+            for (uint32_t i = 0;; ++i) {
+                const uint32_t c = (i >> 1) * 4 + turn * 2 + (i & 1);
+                if (c * 32 >= wide) break;
+                const uint32_t col0 = t.n * kWide + t.half * (kWide / 2) + c * 32;
                 if (col0 >= P.n || row0 >= P.m) break;
                 const bool in = col0 + lane < P.n;
                 spread(cols, in ? P.w_scales[0][col0 + lane] : 0.0f, lane);
@@ -255,7 +259,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 else if (P.bias) spread(cols + 128, in ? P.bias[col0 + lane] : 0.0f, lane);
                 uint32_t r[32], r2[kGated ? 32 : 1];
                 ptx::tmem_ld_32x32b_x32(tmem + c * 32, r);
-                if constexpr (kGated) ptx::tmem_ld_32x32b_x32(tmem + 128 + c * 32, r2);
+                if constexpr (kGated) ptx::tmem_ld_32x32b_x32(tmem + wide + c * 32, r2);
                 ptx::tmem_ld_wait();
                 __syncwarp();
                 float v[32];
@@ -287,7 +291,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         v[4 * j] = __fadd_rn(v[4 * j], s.x); v[4 * j + 1] = __fadd_rn(v[4 * j + 1], s.y); v[4 * j + 2] = __fadd_rn(v[4 * j + 2], s.z); v[4 * j + 3] = __fadd_rn(v[4 * j + 3], s.w);
                     }
                 }
-                put_chunk(p, &map_y, v, row0, col0, c, lane, stage, n_stores);
+                put_chunk(p, &map_y, v, row0, col0, c & 1, lane, stage);
                 __syncwarp();                                    // the next chunk's numbers take the place of this one's
             }
             ptx::tc_fence_before_sync();
@@ -356,15 +360,23 @@ int launch_instance(t0_runtime* rt, const Product& P) {
     p.k_blocks = ceil_div(P.k, kBlock);
     const uint64_t total = (uint64_t)p.tiles_m * p.tiles_n;
     if (total > 0x7FFFFFFFull / kRaster) return fail(T0_ERR_UNSUPPORTED, "m=%u, n=%u: too much for one launch", P.m, P.n);
+    // the last round of tiles, where it would leave half of the pairs idle or more: in halves, on twice as many
+    const uint32_t rest = (uint32_t)(total % (uint64_t)pairs);
+    p.whole = (uint32_t)total - (2 * rest <= (uint32_t)pairs ? rest : 0);
+    const uint64_t items = p.whole + 2 * (total - p.whole);
     p.status = rt->d_status;
     const uint64_t limit = rt->wait_limit_ns.load(std::memory_order_relaxed);
     p.wait_limit_ns = limit ? limit : ptx::kWaitLimitNs;
     p.drop_load = rt->drop_next_load.exchange(0) != 0;
-    CUtensorMap ma, mw, mw2, my;
+    CUtensorMap ma, mw, mw2, mwh, mw2h, my;
     int rc = make_map_codes(&ma, P.a, P.a_stride, P.m, P.k, kHalf);
     if (rc == T0_OK) rc = make_map_codes(&mw, P.w[0], P.w_stride, P.n, P.k, kHalf);
-    mw2 = mw;
+    mw2 = mwh = mw2h = mw;
     if (rc == T0_OK && kGated) rc = make_map_codes(&mw2, P.w[1], P.w_stride, P.n, P.k, kHalf);
+    if (p.whole < total) {
+        if (rc == T0_OK) rc = make_map_codes(&mwh, P.w[0], P.w_stride, P.n, P.k, kHalf / 2);
+        if (rc == T0_OK && kGated) rc = make_map_codes(&mw2h, P.w[1], P.w_stride, P.n, P.k, kHalf / 2);
+    }
     if (rc != T0_OK) return rc;
     my = ma;
     // a TMA store writes whole 16 bytes: rows have to begin and end on such boundaries
@@ -373,7 +385,7 @@ int launch_instance(t0_runtime* rt, const Product& P) {
         if ((rc = make_map_y(&my, P)) != T0_OK) return rc;
         p.tma_store = 1;
     }
-    const cudaError_t e = gemm::launch_pdl(kern, 2 * (uint32_t)std::min<uint64_t>(total, (uint64_t)pairs), kThreads, smem_bytes(), rt->stream, ma, mw, mw2, my, p);
+    const cudaError_t e = gemm::launch_pdl(kern, 2 * (uint32_t)std::min<uint64_t>(items, (uint64_t)pairs), kThreads, smem_bytes(), rt->stream, ma, mw, mw2, mwh, mw2h, my, p);
     if (e != cudaSuccess) return fail(T0_ERR_CUDA, "launch of the eight-bit product failed: %s", cudaGetErrorString(e));
     rt->launches.fetch_add(1);
     return T0_OK;
