@@ -34,7 +34,10 @@ bool touch(uint64_t a, uint64_t a_bytes, uint64_t a_stride, uint64_t a_rows, uin
 
 // The kernels: what each is for stands with it.
 int launch_pair(t0_runtime* rt, const Product& P, bool gated);
-int launch_stream(t0_runtime* rt, const Product& P, bool gated);
+// How the stream kernel cuts a product: rows of the weights and tokens to a tile, parts of K; parts = 0: pairs take it.
+struct Cut { uint32_t rows, tokens, parts; };
+constexpr uint32_t kMostTokens = 256;      // of a tile, both products' together
+int launch_stream(t0_runtime* rt, const Product& P, bool gated, const Cut& cut);
 
 // Box of 128 codes of `box_rows` rows, 128-byte swizzle; codes from `length` on and rows from `rows` on are read as zero.
 int make_map_codes(CUtensorMap* map, const int8_t* codes, uint64_t stride, uint32_t rows, uint32_t length, uint32_t box_rows);

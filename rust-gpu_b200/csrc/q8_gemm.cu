@@ -1,4 +1,6 @@
-// Products of rows in eight bits with weights in eight bits: the entries, and a kernel that takes every shape.
+// Products of rows in eight bits with weights in eight bits: the entries, and which kernel takes what.
+#include <cmath>
+
 #include "gemm_common.cuh"
 #include "q8.cuh"
 #include "runtime_internal.h"
@@ -7,67 +9,52 @@ namespace t0 {
 namespace q8 {
 namespace {
 
-constexpr uint32_t kTile = 64, kStep = 64;
-
-// Four codes of a row from `e` on, as a word; those from k on are zero.
-__device__ __forceinline__ uint32_t word_at(const int8_t* row, uint32_t e, uint32_t k) {
-    if (e >= k) return 0;
-    const uint32_t w = *(const uint32_t*)(row + e);            // strides are multiples of 16: the word is the row's
-    return k - e >= 4 ? w : w & ((1u << (8 * (k - e))) - 1);
+// Which kernel takes a product, and how it is cut: by a fit of both kernels' times over 130 shapes (1 .. 1024 rows, n 1024 .. 14336, k 1000 .. 11008, plain and gated; 1000 cuts), all
+// in nanoseconds and bytes per nanosecond.  What it chooses takes 2 % longer than the best cut on average, and 21 % at most.  Both sides, plain, us on pairs / streamed: 128 x 4096 x 4096
+// 12.4 / 9.3, 256 x 4096 x 4096 12.8 / 13.2, 512 x 4096 x 4096 13.0 / 16.2, 400 x 1024 x 4096 11.8 / 9.7, 1024 x 11008 x 4096 35.5 / 50.1.
+//   streamed, a round of tiles: k blocks times the slowest of { issuing a block's copies and products, the weights' way from memory (a little slower with few CTAs), all operands' way
+//     from L2, the products, one SM's way from L2 }, then the epilogue by its tokens, and the adding of parts;
+//   pairs, a round: k blocks times { the products, the weights' way from memory }, and the epilogue; the last round may be one of half tiles.
+float stream_time(const Product& P, uint32_t g, uint32_t tiles_m, const Cut& c, uint32_t clusters) {
+    const uint32_t tiles = ceil_div(P.n, c.rows) * tiles_m, rounds = ceil_div(tiles, clusters), blocks = ceil_div(ceil_div(P.k, 128), c.parts);
+    const float ctas = (float)std::min(tiles, clusters) * c.parts, w = g * c.rows * 128.0f, a = c.tokens * 128.0f;
+    float block = g == 1 ? 141.0f : 231.0f;
+    block = std::max(block, ctas * w / tiles_m / 6670.0f / std::sqrt(std::sqrt(std::min(1.0f, ctas / 140.0f))));
+    block = std::max(block, std::max(ctas * (w + a) / 14900.0f, (w + a) / 144.0f));
+    block = std::max(block, 1.14f * g * c.tokens);
+    const float parts = c.parts > 1 ? 640.0f + 4.9f * g * c.tokens + 278.0f * (c.parts - 2) : 0.0f;
+    return 1900.0f + rounds * (blocks * block + 1040.0f + 15.5f * g * c.tokens + parts + (c.rows % 32 ? 200.0f : 0.0f));
+}
+float pair_time(const Product& P, uint32_t g, uint32_t pairs) {
+    const uint64_t tiles_n = ceil_div(P.n, 256 / g), tiles = ceil_div(P.m, 256) * tiles_n, rest = tiles % pairs, halved = 2 * rest <= pairs ? rest : 0;
+    const float blocks = (float)ceil_div(P.k, 128), rounds = (float)((tiles - halved + pairs - 1) / pairs);
+    const float whole = std::max(315.0f, std::min<uint64_t>(std::min<uint64_t>(tiles, pairs), tiles_n) * 32768 / 7300.0f), half = std::max(210.0f, std::min(halved, tiles_n) * 32768 / 7300.0f);
+    return 6020.0f + rounds * (blocks * whole + 2270.0f) + (halved ? blocks * half + 190.0f : 0.0f);
 }
 
-// 64 x 64 numbers a block, 16 a thread.
-template <bool kGated>
-__global__ void __launch_bounds__(256) q8_gemm_kernel(const Product P) {
-    constexpr int kW = kGated ? 2 : 1;
-    __shared__ uint32_t as[kTile][kStep / 4 + 1], ws[kW][kTile][kStep / 4 + 1];
-    ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
-    const uint64_t tiles_n = (P.n + kTile - 1) / kTile;
-    const uint64_t m0 = blockIdx.x / tiles_n * kTile, n0 = blockIdx.x % tiles_n * kTile;
-    const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    int32_t sum[kW][4][4] = {};
-    for (uint32_t k0 = 0; k0 < P.k; k0 += kStep) {
-        for (uint32_t i = threadIdx.x; i < kTile * kStep / 4; i += 256) {
-            const uint32_t r = i / (kStep / 4), c = i % (kStep / 4);
-            as[r][c] = m0 + r < P.m ? word_at(P.a + (m0 + r) * P.a_stride, k0 + 4 * c, P.k) : 0;
-#pragma unroll
-            for (int h = 0; h < kW; ++h) ws[h][r][c] = n0 + r < P.n ? word_at(P.w[h] + (n0 + r) * P.w_stride, k0 + 4 * c, P.k) : 0;
+Cut choose(const Product& P, bool gated, uint32_t sms) {
+    const uint32_t g = gated ? 2 : 1, tiles_m = ceil_div(P.m, kMostTokens / g);
+    Cut best = {0, 0, 0};
+    if (tiles_m > 8) return best;                                          // streamed, the weights would be read nine times
+    const uint32_t* at_once = gemm_clusters_at_once();
+    float least = pair_time(P, g, std::max(1u, sms / 2));
+    for (uint32_t parts = 1; parts <= 4 && parts <= ceil_div(P.k, 128); ++parts) {
+        const uint32_t clusters = std::max(1u, parts == 1 ? sms : at_once[parts]);
+        const uint32_t even = ceil_div(P.n, std::max(1u, clusters / tiles_m));   // rows that make one round of everything
+        for (const uint32_t rows : {even, 64u, 128u}) {
+            if (rows > 128) continue;
+            const Cut c = {std::max(8u, rows), (ceil_div(P.m, tiles_m) + 15) & ~15u, parts};
+            const float t = stream_time(P, g, tiles_m, c, clusters);
+            if (t < least) least = t, best = c;
         }
-        __syncthreads();
-        for (uint32_t c = 0; c < kStep / 4; ++c)
-#pragma unroll
-            for (int h = 0; h < kW; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum[h][i][j] = __dp4a((int)as[ty + 16 * i][c], (int)ws[h][tx + 16 * j][c], sum[h][i][j]);
-        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint64_t r = m0 + ty + 16 * i, c = n0 + tx + 16 * j;
-            if (r >= P.m || c >= P.n) continue;
-            float v = scaled(sum[0][i][j], P.a_scales[r], P.w_scales[0][c]);
-            if constexpr (kGated) v = __fmul_rn(activate(v, P.act), scaled(sum[kW - 1][i][j], P.a_scales[r], P.w_scales[1][c]));
-            else if (P.bias) v = __fadd_rn(v, P.bias[c]);
-            if (P.out_bf16) ((__nv_bfloat16*)P.y)[r * P.y_stride + c] = __float2bfloat16_rn(v);
-            else ((float*)P.y)[r * P.y_stride + c] = v;
-        }
+    return best;
 }
 
 int launch(t0_runtime* rt, const Product& P, bool gated) {
-    return P.m > 256 ? launch_pair(rt, P, gated) : launch_stream(rt, P, gated);
-    const uint64_t grid = (uint64_t)ceil_div(P.m, kTile) * ceil_div(P.n, kTile);
-    if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "m=%u, n=%u: too much for one launch", P.m, P.n);
     const DeviceGuard guard(rt->device);
-    const cudaError_t e = gated ? gemm::launch_pdl(q8_gemm_kernel<true>, (uint32_t)grid, 256, 0, rt->stream, P)
-                                : gemm::launch_pdl(q8_gemm_kernel<false>, (uint32_t)grid, 256, 0, rt->stream, P);
-    if (e != cudaSuccess) return fail(T0_ERR_CUDA, "launch of the eight-bit product failed: %s", cudaGetErrorString(e));
-    rt->launches.fetch_add(1);
-    return T0_OK;
+    const Cut cut = choose(P, gated, (uint32_t)rt->sm_count);
+    return cut.parts ? launch_stream(rt, P, gated, cut) : launch_pair(rt, P, gated);
 }
 
 // What both entries check; fills `P` but for the second matrix, the bias and the activation.

@@ -251,23 +251,8 @@ __global__ void __launch_bounds__(32 * kMostWarps) q8_stream_kernel(const __grid
     }
 }
 
-// How a product is cut: rows of the weights and tokens to a tile, parts of K.
-struct Cut { uint32_t rows, tokens, parts, ring, warps; };
-
-Cut choose(const Product& P, bool gated, uint32_t sms) {
-    Cut c;
-    const uint32_t most = gated ? 128 : 256, tiles_m = ceil_div(P.m, most);
-    c.tokens = (ceil_div(P.m, tiles_m) + 15) & ~15u;
-    c.parts = 1;
-    while (c.parts < 8 && ceil_div(P.k, kBlock) >= 4 * (c.parts + 1) && (uint64_t)P.n * tiles_m * (c.parts + 1) <= 128ull * sms) ++c.parts;
-    c.rows = std::min(128u, std::max(8u, ceil_div(P.n, std::max(1u, sms / tiles_m / c.parts))));
-    c.ring = kMostRing;
-    c.warps = c.tokens <= 16 ? 4 : c.tokens <= 64 ? 8 : 16;
-    return c;
-}
-
 template <bool kGated>
-int launch_instance(t0_runtime* rt, const Product& P) {
+int launch_instance(t0_runtime* rt, const Product& P, const Cut& cut) {
     auto kern = q8_stream_kernel<kGated>;
     static std::atomic<bool> ready[64];
     const int dev = rt->device;
@@ -277,7 +262,6 @@ int launch_instance(t0_runtime* rt, const Product& P) {
         if (e != cudaSuccess) return fail(T0_ERR_CUDA, "cudaFuncSetAttribute(smem=%u): %s", kMostSmem, cudaGetErrorString(e));
         ready[dev].store(true, std::memory_order_release);
     }
-    const Cut cut = choose(P, kGated, (uint32_t)rt->sm_count);
     StreamParams p;
     memset((void*)&p, 0, sizeof p);
     p.P = P;
@@ -286,7 +270,7 @@ int launch_instance(t0_runtime* rt, const Product& P) {
     p.k_blocks = ceil_div(P.k, kBlock);
     p.w_bytes = ((p.rows + 7) & ~7u) * kBlock;
     p.stage_bytes = (kGated ? 2 : 1) * p.w_bytes + p.tokens * kBlock;
-    p.stages = std::min(kMaxStages, cut.ring / p.stage_bytes);
+    p.stages = std::min(kMaxStages, kMostRing / p.stage_bytes);
     p.ring = p.stages * p.stage_bytes + (p.w_bytes + p.tokens * kBlock < kTile ? kTile - p.w_bytes - p.tokens * kBlock : 0);
     if (p.parts > 1) p.ring = std::max(p.ring, (kGated ? 2 : 1) * p.tokens * 512);
     p.ahead = std::min(p.stages, 8u);
@@ -298,13 +282,15 @@ int launch_instance(t0_runtime* rt, const Product& P) {
     p.drop_load = rt->drop_next_load.exchange(0) != 0;
     const uint64_t grid = (uint64_t)p.tiles_n * p.tiles_m * p.parts;
     if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "m=%u, n=%u: too much for one launch", P.m, P.n);
+    // epilogue warps: one to four turns of 16 tokens (1 x 11008 x 4096 with 4 / 8 / 16: 10.1 / 10.2 / 10.5 us; gated 100 x 14336 x 4096 with 8 / 16: 25.4 / 23.8)
+    const uint32_t warps = p.tokens <= 16 ? 4 : p.tokens <= 64 ? 8 : 16;
     CUtensorMap ma, mw, mw2;
     int rc = make_map_codes(&ma, P.a, P.a_stride, P.m, P.k, p.tokens);
     if (rc == T0_OK) rc = make_map_codes(&mw, P.w[0], P.w_stride, P.n, P.k, p.rows);
     mw2 = mw;
     if (rc == T0_OK && kGated) rc = make_map_codes(&mw2, P.w[1], P.w_stride, P.n, P.k, p.rows);
     if (rc != T0_OK) return rc;
-    const cudaError_t e = gemm::launch_pdl_clusters(kern, (uint32_t)grid, p.parts, 32 * (2 + cut.warps), 1024 + p.ring + 1024, rt->stream, ma, mw, mw2, p);
+    const cudaError_t e = gemm::launch_pdl_clusters(kern, (uint32_t)grid, p.parts, 32 * (2 + warps), 1024 + p.ring + 1024, rt->stream, ma, mw, mw2, p);
     if (e != cudaSuccess) return fail(T0_ERR_CUDA, "launch of the eight-bit product failed: %s", cudaGetErrorString(e));
     rt->launches.fetch_add(1);
     return T0_OK;
@@ -312,9 +298,9 @@ int launch_instance(t0_runtime* rt, const Product& P) {
 
 }  // namespace
 
-int launch_stream(t0_runtime* rt, const Product& P, bool gated) {
+int launch_stream(t0_runtime* rt, const Product& P, bool gated, const Cut& cut) {
     const DeviceGuard guard(rt->device);
-    return gated ? launch_instance<true>(rt, P) : launch_instance<false>(rt, P);
+    return gated ? launch_instance<true>(rt, P, cut) : launch_instance<false>(rt, P, cut);
 }
 
 }  // namespace q8
