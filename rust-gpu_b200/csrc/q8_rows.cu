@@ -29,6 +29,8 @@ bool touch(uint64_t a, uint64_t a_bytes, uint64_t a_stride, uint64_t a_rows, uin
 
 namespace {
 
+constexpr uint32_t kMostSlots = 16;
+
 struct Rows {
     const void *x, *residual, *weight;
     void* residual_out;
@@ -37,166 +39,333 @@ struct Rows {
     __nv_bfloat16* y;
     uint64_t x_stride, residual_stride, residual_out_stride, q_stride, y_stride;
     uint32_t n_rows, dim;
+    uint32_t slots, slot_bytes, residual_at;           // the ring: rows, bytes a row, where in it the residual begins
+    int* status;
+    uint64_t wait_limit_ns;
     double inv_dim, eps;
     bool x_f32, residual_f32, weight_f32;
 };
 
-// Eight numbers from `at` on, as f32; those from `end` on are zero.
-__device__ __forceinline__ void load8(float (&v)[8], const void* base, uint64_t at, uint32_t have, bool f32) {
+// Two f32 in one register pair: the adders and multipliers take both at once, each rounded by itself.
+__device__ __forceinline__ uint64_t pair_of(float2 a) {
+    uint64_t x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+    return x;
+}
+__device__ __forceinline__ float2 two_of(uint64_t x) {
+    float2 a;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+    return a;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
+    return two_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
+    return two_of(d);
+}
+// The largest of a and of two sizes; NaN where one is.
+__device__ __forceinline__ float most_of(float a, float2 b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b.x)), "f"(fabsf(b.y)));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float2 a) {
+    const __nv_bfloat162 p = __float22bfloat162_rn(a);
+    return *(const uint32_t*)&p;
+}
+__device__ __forceinline__ float2 unpack_bf16(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)); }
+
+// Eight numbers from element `at` of a row on; of the last ones of the row only `have`, the others zero.
+template <bool kF32>
+__device__ __forceinline__ void load8(float2 (&v)[4], const void* row, uint32_t at, uint32_t have) {
     if (have >= 8) {
-        if (f32) {
-            const float4 a = ((const float4*)((const float*)base + at))[0], b = ((const float4*)((const float*)base + at))[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        const uint4* p = (const uint4*)((const char*)row + at * (kF32 ? 4 : 2));
+        const uint4 a = p[0];
+        if constexpr (kF32) {
+            const uint4 b = p[1];
+            v[0] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y)); v[1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+            v[2] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y)); v[3] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
         } else {
-            const uint4 w = *(const uint4*)((const uint16_t*)base + at);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u); }
+            v[0] = unpack_bf16(a.x); v[1] = unpack_bf16(a.y); v[2] = unpack_bf16(a.z); v[3] = unpack_bf16(a.w);
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i] = i >= (int)have ? 0.0f : f32 ? ((const float*)base)[at + i] : __uint_as_float((uint32_t)((const uint16_t*)base)[at + i] << 16);
+    for (int i = 0; i < 8; ++i) {
+        const float f = i >= (int)have ? 0.0f : kF32 ? ((const float*)row)[at + i] : __uint_as_float((uint32_t)((const uint16_t*)row)[at + i] << 16);
+        if (i & 1) v[i >> 1].y = f;
+        else v[i >> 1].x = f;
+    }
 }
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
-    return *(const uint32_t*)&p;
+// ... from shared memory, whole.
+template <bool kF32>
+__device__ __forceinline__ void lds8(float2 (&v)[4], uint32_t at) {
+    uint32_t a[4], b[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(at) : "memory");
+    if constexpr (kF32) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(at + 16) : "memory");
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v[i] = make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+            v[2 + i] = make_float2(__uint_as_float(b[2 * i]), __uint_as_float(b[2 * i + 1]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = unpack_bf16(a[i]);
+    }
 }
-__device__ __forceinline__ void store8(void* base, uint64_t at, uint32_t have, bool f32, const float (&v)[8]) {
+template <bool kF32>
+__device__ __forceinline__ void store8(void* row, uint32_t at, uint32_t have, const float2 (&v)[4]) {
     if (have >= 8) {
-        if (f32) {
-            float4* p = (float4*)((float*)base + at);
-            p[0] = make_float4(v[0], v[1], v[2], v[3]);
-            p[1] = make_float4(v[4], v[5], v[6], v[7]);
+        uint4* p = (uint4*)((char*)row + at * (kF32 ? 4 : 2));
+        if constexpr (kF32) {
+            p[0] = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+            p[1] = make_uint4(__float_as_uint(v[2].x), __float_as_uint(v[2].y), __float_as_uint(v[3].x), __float_as_uint(v[3].y));
         } else {
-            *(uint4*)((uint16_t*)base + at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+            p[0] = make_uint4(pack_bf16(v[0]), pack_bf16(v[1]), pack_bf16(v[2]), pack_bf16(v[3]));
         }
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (i < (int)have) {
-            if (f32) ((float*)base)[at + i] = v[i];
-            else ((__nv_bfloat16*)base)[at + i] = __float2bfloat16_rn(v[i]);
+            const float f = i & 1 ? v[i >> 1].y : v[i >> 1].x;
+            if constexpr (kF32) ((float*)row)[at + i] = f;
+            else ((__nv_bfloat16*)row)[at + i] = __float2bfloat16_rn(f);
         }
 }
+// Four whole numbers of at most 127 in size, halves rounded to even, as bytes: 1.5 * 2^23 is added, which leaves the number in the low bits of the sum (the conversion instruction
+// has an eighth of the adder's rate).  One at a time: the assembler makes one operation of a product and a sum of pairs, which loses the product's rounding and with it the ties.
+__device__ __forceinline__ uint32_t bytes_of(float2 a, float2 b) {
+    const float k = 12582912.0f;
+    const uint32_t x = __float_as_uint(__fadd_rn(a.x, k)), y = __float_as_uint(__fadd_rn(a.y, k)), z = __float_as_uint(__fadd_rn(b.x, k)), w = __float_as_uint(__fadd_rn(b.y, k));
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
 
-// kThreads threads a row, eight numbers a chunk, kChunks chunks a thread; rows of one warp share a block.
-template <int kThreads, int kChunks, bool kNorm>
-__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) q8_rows_kernel(const Rows P) {
-    constexpr int kWarps = kThreads / 32;
-    __shared__ double sums[kNorm && kWarps > 1 ? kWarps : 1];
-    __shared__ uint32_t tops[kWarps > 1 ? kWarps : 1];
-    const uint32_t t = kWarps == 1 ? threadIdx.x & 31 : threadIdx.x, warp = t >> 5;
-    const uint64_t row = kWarps == 1 ? (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+enum { kNone = 0, kBf16 = 1, kF32 = 2 };               // the residual's type
+
+// Rows of up to kThreads * kChunks * 8 numbers, kThreads threads each (four rows to a block where a warp has a row).
+//   kRing = false: a row a group of threads, loaded straight into registers: the shortest way for few rows.
+//   kRing = true: groups walk over the rows, and copies bring the next ones into a ring in shared memory (P.slots rows), so that memory works while a row is reduced; a slot is filled again
+//     as soon as all threads have taken its numbers into registers.
+template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes, bool kRing>
+__global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads) q8_rows_kernel(const Rows P) {
+    constexpr int kWarps = kThreads / 32, kGroups = kThreads == 32 ? 4 : 1;
+    constexpr bool kEarly = kNorm && !kRing && kChunks <= 2;       // the weight is asked for with the row, where registers allow
+    constexpr uint32_t kXSize = kX32 ? 4 : 2, kRSize = kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0;
+    __shared__ double sums[2][kWarps];
+    __shared__ uint32_t tops[2][kWarps];
+    __shared__ uint64_t full[kGroups][kMostSlots];
+    __shared__ int abort_flag;
+    extern __shared__ __align__(16) uint8_t ring[];
+    const uint32_t t = threadIdx.x % kThreads, group = threadIdx.x / kThreads, warp = t >> 5;
+    const uint64_t groups = (uint64_t)gridDim.x * kGroups, first = (uint64_t)blockIdx.x * kGroups + group;
+    const uint32_t whole = P.dim & ~7u;                            // what the copies bring: whole chunks
+    const uint32_t mine = ptx::smem_u32(ring) + group * P.slots * P.slot_bytes;
     ptx::grid_launch_dependents();
-    ptx::grid_dependency_wait();
-    if (row >= P.n_rows) return;                       // whole warps, and only where a block has no barriers
-    float v[kChunks][8];
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const uint32_t e = (c * kThreads + t) * 8;
-        load8(v[c], P.x, row * P.x_stride + e, e < P.dim ? P.dim - e : 0, P.x_f32);
+    if constexpr (kRing) {
+        if (t == 0) {
+            for (uint32_t s = 0; s < P.slots; ++s) ptx::mbar_init(ptx::smem_u32(&full[group][s]), 1);
+            ptx::fence_barrier_init();
+            ptx::fence_proxy_async_smem();
+            abort_flag = 0;
+        }
+        __syncthreads();
     }
-    if constexpr (kNorm) {
-        if (P.residual) {
-            float u[kChunks][8];
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const uint32_t e = (c * kThreads + t) * 8;
-                load8(u[c], P.residual, row * P.residual_stride + e, e < P.dim ? P.dim - e : 0, P.residual_f32);
-            }
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const uint32_t e = (c * kThreads + t) * 8;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[c][i] = __fadd_rn(v[c][i], u[c][i]);
-                    if (!P.residual_f32) v[c][i] = __bfloat162float(__float2bfloat16_rn(v[c][i]));
-                }
-                if (P.residual_out && e < P.dim) store8(P.residual_out, row * P.residual_out_stride + e, P.dim - e, P.residual_f32, v[c]);
-            }
+    ptx::grid_dependency_wait();
+    const auto fill = [&](uint64_t row, uint32_t slot) {
+        const uint32_t bar = ptx::smem_u32(&full[group][slot]), to = mine + slot * P.slot_bytes;
+        ptx::mbar_arrive_expect_tx(bar, whole * (kXSize + kRSize));
+        if (whole) ptx::bulk_load(to, (const char*)P.x + row * P.x_stride * kXSize, whole * kXSize, bar);
+        if (kRes && whole) ptx::bulk_load(to + P.residual_at, (const char*)P.residual + row * P.residual_stride * kRSize, whole * kRSize, bar);
+    };
+    if constexpr (kRing) {
+        if (t == 0)
+            for (uint32_t s = 0; s < P.slots; ++s)
+                if (first + s * groups < P.n_rows) fill(first + s * groups, s);
+    }
+    uint32_t slot = 0, phase = 0, turn = 0;
+    for (uint64_t row = first; row < P.n_rows; row += groups, turn ^= 1) {
+        if constexpr (kRing) {
+            if (!ptx::mbar_wait_warp(ptx::smem_u32(&full[group][slot]), phase, &abort_flag, P.wait_limit_ns) && (t & 31) == 0) atomicCAS(P.status, 0, kStatusProducerTimeout | (int)(row & 0xFFFFFF));
         }
-        double sum = 0;                                // squares of f32 are exact in f64
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fma((double)v[c][i], (double)v[c][i], sum);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-        if constexpr (kWarps > 1) {
-            if ((t & 31) == 0) sums[warp] = sum;
-            __syncthreads();
-            sum = 0;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) sum += sums[w];
-        }
-        const float r = (float)rsqrt(fma(sum, P.inv_dim, P.eps));
+        const uint32_t in_ring = mine + slot * P.slot_bytes;
+        const char* const x_row = (const char*)P.x + row * P.x_stride * kXSize;
+        float2 v[kChunks][4], w[kEarly ? kChunks : 1][4];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-            const uint32_t e = (c * kThreads + t) * 8;
-            if (e >= P.dim) continue;
-            float w[8];
-            load8(w, P.weight, e, P.dim - e, P.weight_f32);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[c][i] = __fmul_rn(__fmul_rn(v[c][i], r), w[i]);
-            if (P.dim - e < 8) {                       // what lies behind the row stays zero, whatever r is
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[c][i] = i < (int)(P.dim - e) ? v[c][i] : 0.0f;
+            const uint32_t e = (c * kThreads + t) * 8, have = e < P.dim ? P.dim - e : 0;
+            if (kRing && have >= 8) lds8<kX32>(v[c], in_ring + e * kXSize);
+            else load8<kX32>(v[c], x_row, e, have);
+            if constexpr (kEarly) {
+                if (P.weight_f32) load8<true>(w[c], P.weight, e, have);
+                else load8<false>(w[c], P.weight, e, have);
             }
-            if (P.y) store8(P.y, row * P.y_stride + e, P.dim - e, false, v[c]);
         }
-        if (!P.q) return;
-    }
-    // the largest of the row: the bits of sizes are in their order, infinities and NaNs above all numbers
-    uint32_t top = 0;
+        if constexpr (kRes != kNone) {
+            const char* const r_row = (const char*)P.residual + row * P.residual_stride * kRSize;
+            char* const o_row = (char*)P.residual_out + row * P.residual_out_stride * kRSize;
+            float2 u[kRing ? 1 : kChunks][4];                      // loads from memory are all asked for before one is waited for
+            if constexpr (!kRing) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
+                for (int c = 0; c < kChunks; ++c) {
+                    const uint32_t e = (c * kThreads + t) * 8;
+                    load8<kRes == kF32>(u[c], r_row, e, e < P.dim ? P.dim - e : 0);
+                }
+            }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[c][i]) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if constexpr (kWarps > 1) {
-        if ((t & 31) == 0) tops[warp] = top;
-        __syncthreads();
-        top = 0;
+            for (int c = 0; c < kChunks; ++c) {
+                const uint32_t e = (c * kThreads + t) * 8, have = e < P.dim ? P.dim - e : 0;
+                if constexpr (kRing) {
+                    if (have >= 8) lds8<kRes == kF32>(u[0], in_ring + P.residual_at + e * kRSize);
+                    else load8<kRes == kF32>(u[0], r_row, e, have);
+                }
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
-    }
-    const float most = __uint_as_float(top);
-    const bool held = most >= 0x1p-119f && top < 0x7F800000u;
-    const float inverse = held ? __fdiv_rn(127.0f, most) : 0.0f;
-    if (t == 0) P.scales[row] = held ? __fdiv_rn(most, 127.0f) : top < 0x7F800000u ? 0.0f : __uint_as_float(0x7FFFFFFFu);
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const uint32_t e = (c * kThreads + t) * 8;
-        if (e >= P.dim) continue;
-        uint32_t w[2] = {0, 0};
-        if (held) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)__float2int_rn(__fmul_rn(v[c][i], inverse)) & 0xFFu) << (8 * (i & 3));
+                for (int i = 0; i < 4; ++i) {
+                    v[c][i] = add2(v[c][i], u[kRing ? 0 : c][i]);
+                    if constexpr (kRes == kBf16) v[c][i] = unpack_bf16(pack_bf16(v[c][i]));
+                }
+                if (P.residual_out && have) store8<kRes == kF32>(o_row, e, have, v[c]);
+            }
         }
-        int8_t* q = P.q + row * P.q_stride + e;
-        if (P.dim - e >= 8) {
-            *(uint2*)q = make_uint2(w[0], w[1]);
+        if constexpr (kNorm) {
+            double part[4] = {0, 0, 0, 0};                         // squares of f32 are exact in f64
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const double a = v[c][i].x, b = v[c][i].y;
+                    part[(i & 1) * 2] = fma(a, a, part[(i & 1) * 2]);
+                    part[(i & 1) * 2 + 1] = fma(b, b, part[(i & 1) * 2 + 1]);
+                }
+            double sum = (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+            if constexpr (kWarps > 1) {
+                if ((t & 31) == 0) sums[turn][warp] = sum;
+                __syncthreads();
+                sum = 0;
+#pragma unroll
+                for (int i = 0; i < kWarps; ++i) sum += sums[turn][i];
+            }
+            const float r = (float)rsqrt(fma(sum, P.inv_dim, P.eps));
+            const float2 r2 = make_float2(r, r);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const uint32_t e = (c * kThreads + t) * 8, have = e < P.dim ? P.dim - e : 0;
+                float2 f[4];
+                if constexpr (!kEarly) {
+                    if (P.weight_f32) load8<true>(f, P.weight, e, have);
+                    else load8<false>(f, P.weight, e, have);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[c][i] = mul2(mul2(v[c][i], r2), kEarly ? w[c][i] : f[i]);
+                if (have < 8) {                                    // what lies behind the row stays zero, whatever r is
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[c][i] = make_float2(2 * i < (int)have ? v[c][i].x : 0.0f, 2 * i + 1 < (int)have ? v[c][i].y : 0.0f);
+                }
+                if (P.y && have) store8<false>(P.y + row * P.y_stride, e, have, v[c]);
+            }
+        }
+        if (!kNorm || P.q) {
+            float most = 0;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = most_of(most, v[c][i]);
+            // the bits of sizes are in their order, infinities and NaNs above all numbers
+            uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most) & 0x7FFFFFFFu);
+            if constexpr (kWarps > 1) {
+                if ((t & 31) == 0) tops[turn][warp] = top;
+                __syncthreads();
+                top = 0;
+#pragma unroll
+                for (int i = 0; i < kWarps; ++i) top = max(top, tops[turn][i]);
+            }
+            most = __uint_as_float(top);
+            const bool held = most >= 0x1p-119f && top < 0x7F800000u;
+            const float inverse = held ? __fdiv_rn(127.0f, most) : 0.0f;
+            const float2 inverse2 = make_float2(inverse, inverse);
+            if (t == 0) P.scales[row] = held ? __fdiv_rn(most, 127.0f) : top < 0x7F800000u ? 0.0f : __uint_as_float(0x7FFFFFFFu);
+            int8_t* const q_row = P.q + row * P.q_stride;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const uint32_t e = (c * kThreads + t) * 8;
+                if (e >= P.dim) continue;
+                uint2 b = make_uint2(bytes_of(mul2(v[c][0], inverse2), mul2(v[c][1], inverse2)), bytes_of(mul2(v[c][2], inverse2), mul2(v[c][3], inverse2)));
+                if (!held) b = make_uint2(0, 0);                   // (products of infinities and NaNs)
+                if (P.dim - e >= 8) {
+                    *(uint2*)(q_row + e) = b;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < (int)(P.dim - e)) q_row[e + i] = (int8_t)((i < 4 ? b.x : b.y) >> (8 * (i & 3)));
+                }
+            }
+        }
+        if constexpr (kRing) {
+            // all threads have met since they took the slot's numbers (a warp that has a row to itself meets here)
+            if constexpr (kWarps == 1) __syncwarp();
+            if (t == 0 && row + P.slots * groups < P.n_rows) fill(row + P.slots * groups, slot);
+            if (++slot == P.slots) slot = 0, phase ^= 1;
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < (int)(P.dim - e)) q[i] = (int8_t)(w[i >> 2] >> (8 * (i & 3)));
+            break;
         }
     }
+    if constexpr (kRing) {
+        if (*(volatile int*)&abort_flag)                           // copies that were given up on may still be on their way
+            for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+}
+
+template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes>
+cudaError_t launch_instance(t0_runtime* rt, Rows& P) {
+    constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1, kRoom = 200u << 10;
+    const uint64_t blocks = ((uint64_t)P.n_rows + kGroups - 1) / kGroups;
+    // Few rows, one after the other on an SM: straight into registers.
+    if (blocks <= 2ull * rt->sm_count) return gemm::launch_pdl(q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, false>, (uint32_t)blocks, kGroups * kThreads, 0, rt->stream, P);
+    P.residual_at = ((P.dim & ~7u) * (kX32 ? 4 : 2) + 127) & ~127u;
+    P.slot_bytes = P.residual_at + (((P.dim & ~7u) * (kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0) + 127) & ~127u);
+    const uint32_t row_bytes = std::max(1u, kGroups * P.slot_bytes);
+    const uint32_t at_once = std::max(1u, std::min(kThreads == 32 ? 8u : 1024u / kThreads, kRoom / (2 * row_bytes)));       // blocks an SM
+    P.slots = std::min(kMostSlots, std::max(1u, kRoom / at_once / row_bytes));
+    auto kern = q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, true>;
+    static std::atomic<bool> ready[64];
+    if (rt->device < 0 || rt->device >= 64) return cudaErrorInvalidDevice;
+    if (!ready[rt->device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10);
+        if (e != cudaSuccess) return e;
+        ready[rt->device].store(true, std::memory_order_release);
+    }
+    return gemm::launch_pdl(kern, (uint32_t)std::min<uint64_t>(blocks, (uint64_t)at_once * rt->sm_count), kGroups * kThreads, P.slots * row_bytes, rt->stream, P);
+}
+
+template <bool kNorm, bool kX32, int kRes>
+cudaError_t launch_by_dim(t0_runtime* rt, Rows& P) {
+    return P.dim <= 512 ? launch_instance<32, 2, kNorm, kX32, kRes>(rt, P) : P.dim <= 1024 ? launch_instance<32, 4, kNorm, kX32, kRes>(rt, P)
+         : P.dim <= 2048 ? launch_instance<128, 2, kNorm, kX32, kRes>(rt, P) : P.dim <= 4096 ? launch_instance<256, 2, kNorm, kX32, kRes>(rt, P)
+         : P.dim <= 8192 ? launch_instance<256, 4, kNorm, kX32, kRes>(rt, P) : P.dim <= 16384 ? launch_instance<512, 4, kNorm, kX32, kRes>(rt, P)
+                         : launch_instance<1024, 4, kNorm, kX32, kRes>(rt, P);
 }
 
 template <bool kNorm>
-int launch_rows(t0_runtime* rt, const Rows& P) {
+int launch_rows(t0_runtime* rt, Rows& P) {
     const DeviceGuard guard(rt->device);
-    // the fewest threads that hold the row in two chunks (registers for four rows or more an SM); above 8192, and in single warps, in four
-    const auto go = [&](auto kernel, uint32_t threads) {
-        return gemm::launch_pdl(kernel, threads == 32 ? (uint32_t)(((uint64_t)P.n_rows + 7) / 8) : P.n_rows, threads == 32 ? 256u : threads, 0, rt->stream, P);
-    };
-    const cudaError_t e = P.dim <= 1024 ? go(q8_rows_kernel<32, 4, kNorm>, 32) : P.dim <= 2048 ? go(q8_rows_kernel<128, 2, kNorm>, 128)
-                        : P.dim <= 4096 ? go(q8_rows_kernel<256, 2, kNorm>, 256) : P.dim <= 8192 ? go(q8_rows_kernel<512, 2, kNorm>, 512)
-                        : P.dim <= 16384 ? go(q8_rows_kernel<512, 4, kNorm>, 512) : go(q8_rows_kernel<1024, 4, kNorm>, 1024);
+    P.status = rt->d_status;
+    const uint64_t limit = rt->wait_limit_ns.load(std::memory_order_relaxed);
+    P.wait_limit_ns = limit ? limit : ptx::kWaitLimitNs;
+    cudaError_t e;
+    if constexpr (kNorm) {
+        const int res = !P.residual ? kNone : P.residual_f32 ? kF32 : kBf16;
+        e = P.x_f32 ? (res == kNone ? launch_by_dim<true, true, kNone>(rt, P) : res == kF32 ? launch_by_dim<true, true, kF32>(rt, P) : launch_by_dim<true, true, kBf16>(rt, P))
+                    : (res == kNone ? launch_by_dim<true, false, kNone>(rt, P) : res == kF32 ? launch_by_dim<true, false, kF32>(rt, P) : launch_by_dim<true, false, kBf16>(rt, P));
+    } else {
+        e = P.x_f32 ? launch_by_dim<false, true, kNone>(rt, P) : launch_by_dim<false, false, kNone>(rt, P);
+    }
     if (e != cudaSuccess) return fail(T0_ERR_CUDA, "launch of the rows in eight bits failed: %s", cudaGetErrorString(e));
     rt->launches.fetch_add(1);
     return T0_OK;
@@ -230,12 +399,19 @@ __global__ void __launch_bounds__(256) q8_dequant_kernel(const Back P) {
         for (int i = 0; i < 16; ++i)
             if (i < (int)have) w[i >> 2] |= (uint32_t)(uint8_t)q[i] << (8 * (i & 3));
     }
+    const float2 scale2 = make_float2(scale, scale), k = make_float2(-8388736.0f, -8388736.0f);
+    char* const y_row = (char*)P.y + row * P.y_stride * (P.out_f32 ? 4 : 2);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        float v[8];
+        float2 v[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn((float)(int8_t)(w[2 * h + (i >> 2)] >> (8 * (i & 3))), scale);
-        if (have > (uint32_t)(8 * h)) store8(P.y, row * P.y_stride + e + 8 * h, have - 8 * h, P.out_f32, v);
+        for (int i = 0; i < 4; ++i) {                  // code + 128 in the low bits of 2^23, less 2^23 + 128: exact, and not the conversion's eighth of the adder's rate
+            const uint32_t u = w[2 * h + (i >> 1)] ^ 0x80808080u;
+            v[i] = mul2(add2(make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + 2 * (i & 1))), __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7541 + 2 * (i & 1)))), k), scale2);
+        }
+        if (have <= (uint32_t)(8 * h)) break;
+        if (P.out_f32) store8<true>(y_row, e + 8 * h, have - 8 * h, v);
+        else store8<false>(y_row, e + 8 * h, have - 8 * h, v);
     }
 }
 
@@ -311,6 +487,7 @@ int t0_q8_rmsnorm(t0_runtime* rt, const t0_q8_rmsnorm_args* args) {
     }
     if ((rc = check_rt(rt)) != T0_OK) return rc;
     Rows P;
+    memset(&P, 0, sizeof P);
     P.x = (const void*)a.x; P.residual = (const void*)a.residual; P.weight = (const void*)a.weight; P.residual_out = (void*)a.residual_out;
     P.q = (int8_t*)a.q; P.scales = (float*)a.scales; P.y = (__nv_bfloat16*)a.y;
     P.x_stride = a.x_stride; P.residual_stride = a.residual_stride; P.residual_out_stride = a.residual_out_stride; P.q_stride = a.q_stride; P.y_stride = a.y_stride;

@@ -107,6 +107,20 @@ def test_quant_and_dequant(t0, rt, dev, rows, dim, f32):
             assert same_bf16(np.where(nan, 0, got), np.where(nan, 0, bits)) and ((got[nan] & 0x7FFF) > 0x7F80).all()
 
 
+@pytest.mark.parametrize("f32", [True, False])
+def test_a_long_quant_is_exact(t0, rt, dev, f32):
+    # four million numbers: an operation that is not rounded by itself shows in some of them (codes half way between two)
+    rng = np.random.default_rng(78)
+    rows, dim = 1024, 4096
+    x = rng.standard_normal((rows, dim)).astype(np.float32)
+    x = x if f32 else ref.bf16_round(x)
+    q, scales = dev.up(np.zeros((rows, dim), np.int8)), dev.up(np.zeros(rows, np.float32))
+    rt.q8_quant(rt.q8_quant_args(dev.up(x if f32 else ref.bf16_bits(x)).gpu_addr(), q.gpu_addr(), scales.gpu_addr(), n_rows=rows, dim=dim, x_f32=f32))
+    rt.synchronize()
+    codes, want = ref.hold(x)
+    assert np.array_equal(q.read(rows * dim, np.int8).reshape(rows, dim), codes) and same(scales.read(4 * rows, np.float32), want)
+
+
 def test_dequant_of_long_rows(t0, rt, dev):
     rng = np.random.default_rng(3)
     codes, scales = rng.integers(-128, 128, (2, 131071)).astype(np.int8), np.array([0.5, -3e-3], np.float32)
