@@ -146,6 +146,16 @@ __device__ __forceinline__ uint32_t bytes_of(float2 a, float2 b) {
     return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
 }
 
+// 1 / sqrt(m) to f64's last places: the hardware's f32 estimate (2^-22) and one cubic step, 1 - m r^2 = e, r (1 + e / 2 + 3 e^2 / 8); outside of f32's range the library's function.
+__device__ __forceinline__ double inverse_root(double m) {
+    const float f = (float)m;
+    if (!(f > 1e-30f && f < 1e30f)) return rsqrt(m);
+    float r0;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(f));
+    const double r = r0, e = fma(-m * r, r, 1.0);
+    return fma(r * e, fma(e, 0.375, 0.5), r);
+}
+
 enum { kNone = 0, kBf16 = 1, kF32 = 2 };               // the residual's type
 
 // Rows of up to kThreads * kChunks * 8 numbers, kThreads threads each (four rows to a block where a warp has a row).
@@ -248,11 +258,12 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads) q8_rows_kerne
             if constexpr (kWarps > 1) {
                 if ((t & 31) == 0) sums[turn][warp] = sum;
                 __syncthreads();
-                sum = 0;
+                double s[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < kWarps; ++i) sum += sums[turn][i];
+                for (int i = 0; i < kWarps; ++i) s[i & 3] += sums[turn][i];
+                sum = (s[0] + s[1]) + (s[2] + s[3]);
             }
-            const float r = (float)rsqrt(fma(sum, P.inv_dim, P.eps));
+            const float r = (float)inverse_root(fma(sum, P.inv_dim, P.eps));
             const float2 r2 = make_float2(r, r);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
@@ -322,16 +333,19 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads) q8_rows_kerne
     }
 }
 
+// A row a group of threads, straight into registers.
 template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes>
-cudaError_t launch_instance(t0_runtime* rt, Rows& P) {
-    constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1, kRoom = 200u << 10;
-    const uint64_t blocks = ((uint64_t)P.n_rows + kGroups - 1) / kGroups;
-    // Few rows, one after the other on an SM: straight into registers.
-    if (blocks <= 2ull * rt->sm_count) return gemm::launch_pdl(q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, false>, (uint32_t)blocks, kGroups * kThreads, 0, rt->stream, P);
+cudaError_t launch_few(t0_runtime* rt, const Rows& P) {
+    constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1;
+    return gemm::launch_pdl(q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, false>, (P.n_rows + kGroups - 1) / kGroups, kGroups * kThreads, 0, rt->stream, P);
+}
+template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes>
+cudaError_t launch_many(t0_runtime* rt, Rows& P) {
+    constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1, kRoom = 200u << 10, kAtOnce = std::max(1, (kNorm ? 1536 : 1024) / (int)(kGroups * kThreads));
     P.residual_at = ((P.dim & ~7u) * (kX32 ? 4 : 2) + 127) & ~127u;
     P.slot_bytes = P.residual_at + (((P.dim & ~7u) * (kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0) + 127) & ~127u);
     const uint32_t row_bytes = std::max(1u, kGroups * P.slot_bytes);
-    const uint32_t at_once = std::max(1u, std::min(kThreads == 32 ? 8u : 1024u / kThreads, kRoom / (2 * row_bytes)));       // blocks an SM
+    const uint32_t at_once = std::max(1u, std::min(kAtOnce, kRoom / (2 * row_bytes)));       // blocks an SM
     P.slots = std::min(kMostSlots, std::max(1u, kRoom / at_once / row_bytes));
     auto kern = q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, true>;
     static std::atomic<bool> ready[64];
@@ -341,15 +355,21 @@ cudaError_t launch_instance(t0_runtime* rt, Rows& P) {
         if (e != cudaSuccess) return e;
         ready[rt->device].store(true, std::memory_order_release);
     }
+    const uint64_t blocks = ((uint64_t)P.n_rows + kGroups - 1) / kGroups;
     return gemm::launch_pdl(kern, (uint32_t)std::min<uint64_t>(blocks, (uint64_t)at_once * rt->sm_count), kGroups * kThreads, P.slots * row_bytes, rt->stream, P);
 }
 
+// Up to two rows an SM: as many threads a row as have a chunk each, for the shortest chain (one row of 4096 through the norm: 2.9 us with 256 threads and two chunks). More: fewer threads a row,
+// several rows an SM at the same time.
 template <bool kNorm, bool kX32, int kRes>
 cudaError_t launch_by_dim(t0_runtime* rt, Rows& P) {
-    return P.dim <= 512 ? launch_instance<32, 2, kNorm, kX32, kRes>(rt, P) : P.dim <= 1024 ? launch_instance<32, 4, kNorm, kX32, kRes>(rt, P)
-         : P.dim <= 2048 ? launch_instance<128, 2, kNorm, kX32, kRes>(rt, P) : P.dim <= 4096 ? launch_instance<256, 2, kNorm, kX32, kRes>(rt, P)
-         : P.dim <= 8192 ? launch_instance<256, 4, kNorm, kX32, kRes>(rt, P) : P.dim <= 16384 ? launch_instance<512, 4, kNorm, kX32, kRes>(rt, P)
-                         : launch_instance<1024, 4, kNorm, kX32, kRes>(rt, P);
+    const uint32_t d = P.dim;
+    if (P.n_rows <= 2u * rt->sm_count)
+        return d <= 1024 ? launch_few<128, 1, kNorm, kX32, kRes>(rt, P) : d <= 4096 ? launch_few<512, 1, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_few<1024, 1, kNorm, kX32, kRes>(rt, P)
+             : d <= 16384 ? launch_few<1024, 2, kNorm, kX32, kRes>(rt, P) : launch_few<1024, 4, kNorm, kX32, kRes>(rt, P);
+    return d <= 512 ? launch_many<32, 2, kNorm, kX32, kRes>(rt, P) : d <= 1024 ? launch_many<32, 4, kNorm, kX32, kRes>(rt, P) : d <= 2048 ? launch_many<128, 2, kNorm, kX32, kRes>(rt, P)
+         : d <= 4096 ? launch_many<256, 2, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P)
+         : d <= 16384 ? launch_many<kNorm ? 1024 : 512, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);
 }
 
 template <bool kNorm>
@@ -376,42 +396,46 @@ struct Back {
     const float* scales;
     void* y;
     uint64_t q_stride, y_stride;
-    uint32_t dim, parts;                               // blocks a row
-    bool out_f32;
+    uint64_t chunks;                                   // of all rows
+    uint32_t dim, per_row, magic;                      // chunks a row; 2^32 / per_row, rounded up
 };
 
-// Sixteen codes a thread, 4096 a block.
+// Eight codes a chunk, so that a warp's stores stand side by side, and four chunks a thread, asked for together: 1024 chunks a block, whatever rows they are of.
+template <bool kOutF32>
 __global__ void __launch_bounds__(256) q8_dequant_kernel(const Back P) {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
-    const uint64_t row = blockIdx.x / P.parts;
-    const uint32_t e = ((blockIdx.x % P.parts) * 256 + threadIdx.x) * 16;
-    if (e >= P.dim) return;
-    const float scale = P.scales[row];
-    const int8_t* q = P.q + row * P.q_stride + e;
-    uint32_t w[4] = {0, 0, 0, 0};
-    const uint32_t have = P.dim - e;
-    if (have >= 16) {
-        const uint4 u = *(const uint4*)q;
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else {
+    const uint64_t first = (uint64_t)blockIdx.x * 1024, row0 = first / P.per_row;
+    const uint32_t skip = (uint32_t)(first - row0 * P.per_row);
+    uint2 w[4];
+    float scale[4];
+    uint64_t row[4];
+    uint32_t at[4], have[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < (int)have) w[i >> 2] |= (uint32_t)(uint8_t)q[i] << (8 * (i & 3));
+    for (int c = 0; c < 4; ++c) {
+        // the row of a chunk: x < per_row + 1024, for which the product with the rounded inverse is exact
+        const uint32_t x = skip + c * 256 + threadIdx.x, r = P.per_row == 1 ? x : __umulhi(x, P.magic);
+        row[c] = row0 + r;
+        at[c] = (x - r * P.per_row) * 8;
+        have[c] = first + c * 256 + threadIdx.x < P.chunks ? P.dim - at[c] : 0;
+        w[c] = make_uint2(0, 0);
+        scale[c] = 0.0f;
+        if (!have[c]) continue;
+        w[c] = *(const uint2*)(P.q + row[c] * P.q_stride + at[c]);     // (a row's last chunk with what lies behind it, up to the stride)
+        scale[c] = P.scales[row[c]];
     }
-    const float2 scale2 = make_float2(scale, scale), k = make_float2(-8388736.0f, -8388736.0f);
-    char* const y_row = (char*)P.y + row * P.y_stride * (P.out_f32 ? 4 : 2);
+    const float2 k = make_float2(-8388736.0f, -8388736.0f);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int c = 0; c < 4; ++c) {
+        if (!have[c]) break;
+        const float2 scale2 = make_float2(scale[c], scale[c]);
         float2 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                  // code + 128 in the low bits of 2^23, less 2^23 + 128: exact, and not the conversion's eighth of the adder's rate
-            const uint32_t u = w[2 * h + (i >> 1)] ^ 0x80808080u;
+            const uint32_t u = (i < 2 ? w[c].x : w[c].y) ^ 0x80808080u;
             v[i] = mul2(add2(make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + 2 * (i & 1))), __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7541 + 2 * (i & 1)))), k), scale2);
         }
-        if (have <= (uint32_t)(8 * h)) break;
-        if (P.out_f32) store8<true>(y_row, e + 8 * h, have - 8 * h, v);
-        else store8<false>(y_row, e + 8 * h, have - 8 * h, v);
+        store8<kOutF32>((char*)P.y + row[c] * P.y_stride * (kOutF32 ? 4 : 2), at[c], have[c], v);
     }
 }
 
@@ -512,11 +536,13 @@ int t0_q8_dequant(t0_runtime* rt, const t0_q8_dequant_args* args) {
     if ((rc = check_rt(rt)) != T0_OK) return rc;
     Back P;
     P.q = (const int8_t*)a.q; P.scales = (const float*)a.scales; P.y = (void*)a.y;
-    P.q_stride = a.q_stride; P.y_stride = a.y_stride; P.dim = a.dim; P.parts = ceil_div(a.dim, 4096); P.out_f32 = a.out_f32 != 0;
-    const uint64_t grid = n * P.parts;
+    P.q_stride = a.q_stride; P.y_stride = a.y_stride; P.dim = a.dim; P.per_row = ceil_div(a.dim, 8);
+    P.magic = (uint32_t)(((1ull << 32) + P.per_row - 1) / P.per_row);
+    P.chunks = n * P.per_row;
+    const uint64_t grid = (P.chunks + 1023) / 1024;
     if (grid > 0x7FFFFFFFull) return fail(T0_ERR_UNSUPPORTED, "too many rows for one launch");
     const DeviceGuard guard(rt->device);
-    const cudaError_t e = gemm::launch_pdl(q8_dequant_kernel, (uint32_t)grid, 256, 0, rt->stream, P);
+    const cudaError_t e = a.out_f32 ? gemm::launch_pdl(q8_dequant_kernel<true>, (uint32_t)grid, 256, 0, rt->stream, P) : gemm::launch_pdl(q8_dequant_kernel<false>, (uint32_t)grid, 256, 0, rt->stream, P);
     if (e != cudaSuccess) return fail(T0_ERR_CUDA, "launch of the read-out failed: %s", cudaGetErrorString(e));
     rt->launches.fetch_add(1);
     return T0_OK;
