@@ -43,21 +43,39 @@ int launch_stream(t0_runtime* rt, const Product& P, bool gated, const Cut& cut);
 int make_map_codes(CUtensorMap* map, const int8_t* codes, uint64_t stride, uint32_t rows, uint32_t length, uint32_t box_rows);
 
 #ifdef __CUDACC__
-__device__ __forceinline__ float sigmoid(float x) {
-    // 1 / (1 + 2^(-x log2 e)): the hardware's power of two and reciprocal, and one step of Newton's method for the quotient; on d / 4, so that neither d nor the result leaves the
-    // normal range before d overflows, from where on the result is zero.
+// Two f32 in one register pair: the adders and multipliers take both at once, each rounded by itself.
+__device__ __forceinline__ uint64_t pair_of(float2 a) {
+    uint64_t x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+    return x;
+}
+__device__ __forceinline__ float2 two_of(uint64_t x) {
+    float2 a;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+    return a;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
+    return two_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
+    return two_of(d);
+}
+// x / (1 + 2^(slope x)): the hardware's power of two and reciprocal, each within 2^-22 of its value; x times zero where the power overflows.  slope is minus log2(e), times 1.702 for gelu.
+__device__ __forceinline__ float gate_of(float x, float slope) {
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504088896340736f));
-    const float d = __fmaf_rn(e, 0.25f, 0.25f);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    r = __fmaf_rn(r, __fmaf_rn(-d, r, 1.0f), r) * 0.25f;
-    return d <= 0x1p126f ? r : d != d ? d : 0.0f;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * slope));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+    return x * r;
 }
-__device__ __forceinline__ float activate(float x, uint32_t act) {
-    return act == T0_TEPI_RELU ? (x < 0.0f ? 0.0f : x) : x * sigmoid(act == T0_TEPI_GELU ? x * 1.702f : x);
+__device__ __forceinline__ float slope_of(uint32_t act) { return act == T0_TEPI_GELU ? -1.702f * 1.44269504088896340736f : -1.44269504088896340736f; }
+// exact sums as y has them, but for the bias: three roundings
+__device__ __forceinline__ float2 scaled(int32_t sum0, int32_t sum1, float2 a_scale, float2 w_scale) {
+    return mul2(mul2(make_float2(__int2float_rn(sum0), __int2float_rn(sum1)), a_scale), w_scale);
 }
-// the exact sum as y has it, but for the bias: three roundings
-__device__ __forceinline__ float scaled(int32_t sum, float a_scale, float w_scale) { return __fmul_rn(__fmul_rn(__int2float_rn(sum), a_scale), w_scale); }
 #endif
 
 }  // namespace q8

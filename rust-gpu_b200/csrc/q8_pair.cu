@@ -263,26 +263,28 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 ptx::tmem_ld_wait();
                 __syncwarp();
                 float v[32];
+                const float2 a2 = make_float2(a_scale, a_scale);
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j) {
                     const float4 s = spread4(cols, j);
-                    v[4 * j] = scaled((int)r[4 * j], a_scale, s.x); v[4 * j + 1] = scaled((int)r[4 * j + 1], a_scale, s.y);
-                    v[4 * j + 2] = scaled((int)r[4 * j + 2], a_scale, s.z); v[4 * j + 3] = scaled((int)r[4 * j + 3], a_scale, s.w);
+                    const float2 x = scaled((int)r[4 * j], (int)r[4 * j + 1], a2, make_float2(s.x, s.y)), y = scaled((int)r[4 * j + 2], (int)r[4 * j + 3], a2, make_float2(s.z, s.w));
+                    v[4 * j] = x.x, v[4 * j + 1] = x.y, v[4 * j + 2] = y.x, v[4 * j + 3] = y.y;
                 }
                 if constexpr (kGated) {
                     if (P.act == T0_TEPI_RELU) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 32; ++j) v[j] = activate(v[j], T0_TEPI_RELU);
+                        for (uint32_t j = 0; j < 32; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
                     } else {
-                        const float turn = P.act == T0_TEPI_GELU ? 1.702f : 1.0f;
+                        const float slope = slope_of(P.act);
 #pragma unroll
-                        for (uint32_t j = 0; j < 32; ++j) v[j] *= sigmoid(v[j] * turn);
+                        for (uint32_t j = 0; j < 32; ++j) v[j] = gate_of(v[j], slope);
                     }
 #pragma unroll
                     for (uint32_t j = 0; j < 8; ++j) {
                         const float4 s = spread4(cols + 128, j);
-                        v[4 * j] = __fmul_rn(v[4 * j], scaled((int)r2[4 * j], a_scale, s.x)); v[4 * j + 1] = __fmul_rn(v[4 * j + 1], scaled((int)r2[4 * j + 1], a_scale, s.y));
-                        v[4 * j + 2] = __fmul_rn(v[4 * j + 2], scaled((int)r2[4 * j + 2], a_scale, s.z)); v[4 * j + 3] = __fmul_rn(v[4 * j + 3], scaled((int)r2[4 * j + 3], a_scale, s.w));
+                        const float2 x = mul2(make_float2(v[4 * j], v[4 * j + 1]), scaled((int)r2[4 * j], (int)r2[4 * j + 1], a2, make_float2(s.x, s.y)));
+                        const float2 y = mul2(make_float2(v[4 * j + 2], v[4 * j + 3]), scaled((int)r2[4 * j + 2], (int)r2[4 * j + 3], a2, make_float2(s.z, s.w)));
+                        v[4 * j] = x.x, v[4 * j + 1] = x.y, v[4 * j + 2] = y.x, v[4 * j + 3] = y.y;
                     }
                 } else if (P.bias) {
 #pragma unroll

@@ -46,27 +46,6 @@ struct Rows {
     bool x_f32, residual_f32, weight_f32;
 };
 
-// Two f32 in one register pair: the adders and multipliers take both at once, each rounded by itself.
-__device__ __forceinline__ uint64_t pair_of(float2 a) {
-    uint64_t x;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
-    return x;
-}
-__device__ __forceinline__ float2 two_of(uint64_t x) {
-    float2 a;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
-    return a;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
-    return two_of(d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
-    return two_of(d);
-}
 // The largest of a and of two sizes; NaN where one is.
 __device__ __forceinline__ float most_of(float a, float2 b) {
     float d;

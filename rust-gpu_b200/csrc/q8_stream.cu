@@ -51,19 +51,26 @@ __device__ __forceinline__ Column column_of(const StreamParams& p, uint32_t n0, 
 template <bool kGated, int kCount>
 __device__ __forceinline__ void finish(const StreamParams& p, const Column& c, const int32_t (&sum)[kCount], const int32_t (&sum2)[kGated ? kCount : 1], const float (&a_scale)[kCount],
                                        float (&v)[kCount]) {
+    const float2 w = make_float2(c.scale, c.scale), w2 = make_float2(c.scale2, c.scale2);
 #pragma unroll
-    for (int j = 0; j < kCount; ++j) v[j] = scaled(sum[j], a_scale[j], c.scale);
+    for (int j = 0; j < kCount; j += 2) {
+        const float2 x = scaled(sum[j], sum[j + 1], make_float2(a_scale[j], a_scale[j + 1]), w);
+        v[j] = x.x, v[j + 1] = x.y;
+    }
     if constexpr (kGated) {
         if (p.P.act == T0_TEPI_RELU) {
 #pragma unroll
             for (int j = 0; j < kCount; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
         } else {
-            const float turn = p.P.act == T0_TEPI_GELU ? 1.702f : 1.0f;
+            const float slope = slope_of(p.P.act);
 #pragma unroll
-            for (int j = 0; j < kCount; ++j) v[j] *= sigmoid(v[j] * turn);
+            for (int j = 0; j < kCount; ++j) v[j] = gate_of(v[j], slope);
         }
 #pragma unroll
-        for (int j = 0; j < kCount; ++j) v[j] = __fmul_rn(v[j], scaled(sum2[j], a_scale[j], c.scale2));
+        for (int j = 0; j < kCount; j += 2) {
+            const float2 x = mul2(make_float2(v[j], v[j + 1]), scaled(sum2[j], sum2[j + 1], make_float2(a_scale[j], a_scale[j + 1]), w2));
+            v[j] = x.x, v[j + 1] = x.y;
+        }
     } else if (p.P.bias) {
 #pragma unroll
         for (int j = 0; j < kCount; ++j) v[j] = __fadd_rn(v[j], c.bias);
