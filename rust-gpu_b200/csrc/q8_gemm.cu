@@ -9,27 +9,27 @@ namespace t0 {
 namespace q8 {
 namespace {
 
-// Which kernel takes a product, and how it is cut: by a fit of both kernels' times over 130 shapes (1 .. 1024 rows, n 1024 .. 14336, k 1000 .. 11008, plain and gated; 1000 cuts), all
-// in nanoseconds and bytes per nanosecond.  What it chooses takes 2 % longer than the best cut on average, and 21 % at most.  Both sides, plain, us on pairs / streamed: 128 x 4096 x 4096
-// 12.4 / 9.3, 256 x 4096 x 4096 12.8 / 13.2, 512 x 4096 x 4096 13.0 / 16.2, 400 x 1024 x 4096 11.8 / 9.7, 1024 x 11008 x 4096 35.5 / 50.1.
-//   streamed, a round of tiles: k blocks times the slowest of { issuing a block's copies and products, the weights' way from memory (a little slower with few CTAs), all operands' way
-//     from L2, the products, one SM's way from L2 }, then the epilogue by its tokens, and the adding of parts;
-//   pairs, a round: k blocks times { the products, the weights' way from memory }, and the epilogue; the last round may be one of half tiles.
+// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 176 shapes (1 .. 1500 rows, n 256 .. 16384,
+// k 256 .. 14336, plain and gated; 20 cuts each): 1.5 % over each shape's best on average, 21 % at most.  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
+// 128 x 4096 x 4096 12.4 / 9.3, 256 x 4096 x 4096 12.8 / 13.2, 512 x 4096 x 4096 13.0 / 16.2, 400 x 1024 x 4096 11.8 / 9.7, 1024 x 11008 x 4096 35.5 / 50.1.
+//   streamed, a round of tiles: k blocks times the slowest of { issuing a block's copies and products, the weights' way from memory (slower with few CTAs), all operands' way from L2, the
+//     products, one SM's way from L2 }, then the epilogue by its tokens, and the adding of parts;
+//   pairs, a round: k blocks times the slower of { the products, the weights' way from memory }, and the epilogue; the last round may be one of half tiles.
 float stream_time(const Product& P, uint32_t g, uint32_t tiles_m, const Cut& c, uint32_t clusters) {
     const uint32_t tiles = ceil_div(P.n, c.rows) * tiles_m, rounds = ceil_div(tiles, clusters), blocks = ceil_div(ceil_div(P.k, 128), c.parts);
     const float ctas = (float)std::min(tiles, clusters) * c.parts, w = g * c.rows * 128.0f, a = c.tokens * 128.0f;
-    float block = g == 1 ? 141.0f : 231.0f;
-    block = std::max(block, ctas * w / tiles_m / 6670.0f / std::sqrt(std::sqrt(std::min(1.0f, ctas / 140.0f))));
-    block = std::max(block, std::max(ctas * (w + a) / 14900.0f, (w + a) / 144.0f));
-    block = std::max(block, 1.14f * g * c.tokens);
-    const float parts = c.parts > 1 ? 640.0f + 4.9f * g * c.tokens + 278.0f * (c.parts - 2) : 0.0f;
-    return 1900.0f + rounds * (blocks * block + 1040.0f + 15.5f * g * c.tokens + parts + (c.rows % 32 ? 200.0f : 0.0f));
+    float block = g == 1 ? 192.0f : 230.0f;
+    block = std::max(block, ctas * w / tiles_m / 7930.0f / std::cbrt(std::min(1.0f, ctas / 140.0f)));
+    block = std::max(block, std::max(ctas * (w + a) / 19500.0f, (w + a) / 170.0f));
+    block = std::max(block, 1.42f * g * c.tokens);
+    const float parts = c.parts > 1 ? 1020.0f + 10.3f * g * c.tokens + 166.0f * (c.parts - 2) : 0.0f;
+    return 2910.0f + rounds * (blocks * block + 9.05f * g * c.tokens + parts + (c.rows % 32 ? 638.0f : 0.0f));
 }
 float pair_time(const Product& P, uint32_t g, uint32_t pairs) {
     const uint64_t tiles_n = ceil_div(P.n, 256 / g), tiles = ceil_div(P.m, 256) * tiles_n, rest = tiles % pairs, halved = 2 * rest <= pairs ? rest : 0;
     const float blocks = (float)ceil_div(P.k, 128), rounds = (float)((tiles - halved + pairs - 1) / pairs);
-    const float whole = std::max(315.0f, std::min<uint64_t>(std::min<uint64_t>(tiles, pairs), tiles_n) * 32768 / 7300.0f), half = std::max(210.0f, std::min(halved, tiles_n) * 32768 / 7300.0f);
-    return 6020.0f + rounds * (blocks * whole + 2270.0f) + (halved ? blocks * half + 190.0f : 0.0f);
+    const float whole = std::max(196.0f, std::min<uint64_t>(std::min<uint64_t>(tiles, pairs), tiles_n) * 32768 / 13400.0f), half = std::max(208.0f, std::min(halved, tiles_n) * 32768 / 13400.0f);
+    return 6700.0f + rounds * (blocks * whole + 3480.0f) + (halved ? blocks * half : 0.0f);
 }
 
 Cut choose(const Product& P, bool gated, uint32_t sms) {
@@ -41,7 +41,7 @@ Cut choose(const Product& P, bool gated, uint32_t sms) {
     for (uint32_t parts = 1; parts <= 4 && parts <= ceil_div(P.k, 128); ++parts) {
         const uint32_t clusters = std::max(1u, parts == 1 ? sms : at_once[parts]);
         const uint32_t even = ceil_div(P.n, std::max(1u, clusters / tiles_m));   // rows that make one round of everything
-        for (const uint32_t rows : {even, 64u, 128u}) {
+        for (const uint32_t rows : {even, 32u, 64u, 96u, 128u}) {
             if (rows > 128) continue;
             const Cut c = {std::max(8u, rows), (ceil_div(P.m, tiles_m) + 15) & ~15u, parts};
             const float t = stream_time(P, g, tiles_m, c, clusters);
