@@ -339,15 +339,16 @@ cudaError_t launch_many(t0_runtime* rt, Rows& P) {
 }
 
 // Up to two rows an SM: as many threads a row as have a chunk each, for the shortest chain (one row of 4096 through the norm: 2.9 us with 256 threads and two chunks). More: fewer threads a row,
-// several rows an SM at the same time.
+// several rows an SM at the same time.  With the norm a row has a long chain of sums, which more threads shorten (8192 x 4096, 256 threads and two chunks / 128 and four / 64 and eight:
+// 44.8 / 46.4 / 73.9 us); without it a thread's fixed work counts (8192 x 4096 with 256 / 128: 19.8 / 18.9; 16384 x 2048 with 128 / 64: 23.0 / 18.9).
 template <bool kNorm, bool kX32, int kRes>
 cudaError_t launch_by_dim(t0_runtime* rt, Rows& P) {
     const uint32_t d = P.dim;
     if (P.n_rows <= 2u * rt->sm_count)
         return d <= 1024 ? launch_few<128, 1, kNorm, kX32, kRes>(rt, P) : d <= 4096 ? launch_few<512, 1, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_few<1024, 1, kNorm, kX32, kRes>(rt, P)
              : d <= 16384 ? launch_few<1024, 2, kNorm, kX32, kRes>(rt, P) : launch_few<1024, 4, kNorm, kX32, kRes>(rt, P);
-    return d <= 512 ? launch_many<32, 2, kNorm, kX32, kRes>(rt, P) : d <= 1024 ? launch_many<32, 4, kNorm, kX32, kRes>(rt, P) : d <= 2048 ? launch_many<128, 2, kNorm, kX32, kRes>(rt, P)
-         : d <= 4096 ? launch_many<256, 2, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P)
+    return d <= 512 ? launch_many<32, 2, kNorm, kX32, kRes>(rt, P) : d <= 1024 ? launch_many<32, 4, kNorm, kX32, kRes>(rt, P) : d <= 2048 ? launch_many<kNorm ? 128 : 64, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
+         : d <= 4096 ? launch_many<kNorm ? 256 : 128, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P)
          : d <= 16384 ? launch_many<kNorm ? 1024 : 512, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);
 }
 

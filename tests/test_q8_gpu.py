@@ -496,3 +496,95 @@ def test_a_decoder_layer(t0, rt, dev):
     assert same(ref.from_bits(res.read(2 * n * dim, np.uint16)).reshape(n, dim), h)
     codes, scales = ref.hold(after)
     assert np.array_equal(k8.read(n * up16(dim), np.int8).reshape(n, -1)[:, :dim], codes) and same(k8s.read(4 * n, np.float32), scales)
+
+
+@pytest.mark.parametrize("m, n, k, gated", [(1, 2048, 1024, False), (20, 512, 4096, False), (40, 1024, 4096, True), (600, 2048, 1024, False), (600, 2048, 1024, True)])
+def test_a_wait_that_runs_out_is_reported(t0, m, n, k, gated):
+    # the first copy of the first tile is left out (whole sums, parts over a cluster, pairs): the kernel gives up after the wait limit by itself, and says so
+    rng = np.random.default_rng(m)
+    r = t0.GpuRuntime(0)
+    dev = Device(r)
+    _, _, a, a_s = rows8(rng, dev, m, k, up16(k))
+    _, _, w, w_s = rows8(rng, dev, n, k, up16(k))
+    y = dev.up(np.zeros((m, n), np.float32))
+    at = lambda b: b.gpu_addr()  # noqa: E731
+    call = (lambda: r.q8_gated(r.q8_gated_args(at(a), at(a_s), at(w), at(w_s), at(w), at(w_s), at(y), m=m, n=n, k=k, out_bf16=False))) if gated else (
+        lambda: r.q8_gemm(r.q8_gemm_args(at(a), at(a_s), at(w), at(w_s), at(y), m=m, n=n, k=k)))
+    call()
+    r.synchronize()
+    want = y.read(m * n * 4, np.float32)
+    r.set_wait_limit_ns(3_000_000)
+    r.selftest_drop_one_load()
+    call()
+    with pytest.raises(t0.T0Error) as e:
+        r.synchronize()
+    assert e.value.code == 4 and "wait expired" in str(e.value) and r.is_poisoned()
+    with pytest.raises(t0.T0Error) as e:
+        call()
+    assert e.value.code == 3
+    dev.free()
+    r.close()
+    # another runtime on the device goes on, and gives what the first one gave
+    r = t0.GpuRuntime(0)
+    dev = Device(r)
+    rng = np.random.default_rng(m)
+    _, _, a, a_s = rows8(rng, dev, m, k, up16(k))
+    _, _, w, w_s = rows8(rng, dev, n, k, up16(k))
+    y = dev.up(np.zeros((m, n), np.float32))
+    call()
+    r.synchronize()
+    assert same(y.read(m * n * 4, np.float32), want)
+    dev.free()
+    r.close()
+
+
+FIRST_CALLS = """
+import importlib, sys
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+import numpy as np
+t0 = importlib.import_module("rust-gpu_b200")
+import q8_reference as ref
+from test_q8_gpu import Driver, rows8, same, up16
+from test_kv4_gpu import Device
+rt = t0.GpuRuntime(0)
+dev, rng, d = Device(rt), np.random.default_rng(1), Driver()
+at = lambda b: b.gpu_addr()
+done = []
+with d.record(rt) as graph:
+    pass
+uploads = []
+for m, n, k in ((1, 600, 1024), (24, 256, 4096), (700, 512, 256)):
+    a, w = rows8(rng, dev, m, k, up16(k)), rows8(rng, dev, n, k, up16(k))
+    uploads.append((m, n, k, a, w, dev.up(np.zeros((m, n), np.float32)), dev.up(np.zeros((m, n), np.float32))))
+x = [(rows, dim, rng.standard_normal((rows, dim)).astype(np.float32)) for rows, dim in ((2, 512), (2000, 512))]
+x = [(rows, dim, v, dev.up(v), dev.up(np.zeros((rows, dim), np.int8)), dev.up(np.zeros(rows, np.float32)), dev.up(np.zeros((rows, dim), np.float32)), dev.up(np.ones(dim, np.float32))) for rows, dim, v in x]
+with d.record(rt) as graph:
+    for m, n, k, a, w, y, z in uploads:
+        rt.q8_gemm(rt.q8_gemm_args(at(a[2]), at(a[3]), at(w[2]), at(w[3]), at(y), m=m, n=n, k=k))
+        rt.q8_gated(rt.q8_gated_args(at(a[2]), at(a[3]), at(w[2]), at(w[3]), at(w[2]), at(w[3]), at(z), m=m, n=n, k=k, activation="relu", out_bf16=False))
+    for rows, dim, v, b, q, s, back, one in x:
+        rt.q8_quant(rt.q8_quant_args(at(b), at(q), at(s), n_rows=rows, dim=dim, x_f32=True))
+        rt.q8_dequant(rt.q8_dequant_args(at(q), at(s), at(back), n_rows=rows, dim=dim, out_f32=True))
+        rt.q8_rmsnorm(rt.q8_rmsnorm_args(at(b), at(one), n_rows=rows, dim=dim, eps=1e-5, x_f32=True, weight_f32=True, q=at(q), scales=at(s)))
+d.replay(graph[0], rt.stream())
+rt.synchronize()
+for m, n, k, a, w, y, z in uploads:
+    want = ref.product(a[0], a[1], w[0], w[1])
+    assert same(y.read(m * n * 4, np.float32).reshape(m, n), want)
+    assert same(z.read(m * n * 4, np.float32).reshape(m, n), np.maximum(want, 0) * want)
+for rows, dim, v, b, q, s, back, one in x:
+    codes, scales = ref.hold(v)
+    assert same(back.read(rows * dim * 4, np.float32).reshape(rows, dim), codes.astype(np.float32) * scales[:, None])
+    assert np.array_equal(q.read(rows * dim, np.int8).reshape(rows, dim), ref.hold(ref.rmsnorm(v, np.ones(dim), 1e-5)[0])[0])
+d.drop(graph[0])
+print("recorded")
+"""
+
+
+def test_the_first_calls_of_a_program_may_be_recorded(t0):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=root)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "recorded" in r.stdout, r.stderr[-2000:]
