@@ -236,7 +236,7 @@ PRODUCTS = [
     (1, 1, 1), (1, 8, 16), (1, 4096, 4096), (1, 11008, 512), (2, 33, 31), (3, 130, 129), (5, 1000, 1357), (7, 20001, 256), (8, 128, 128), (9, 148, 640), (15, 4097, 1000), (16, 4096, 2048),
     (17, 300, 384), (31, 2000, 4096), (32, 128, 8192), (33, 512, 511), (64, 4096, 4096), (65, 777, 1025), (100, 1500, 768), (127, 129, 127), (128, 4096, 1024), (129, 640, 2000),
     (200, 3000, 300), (255, 257, 4096), (256, 1024, 1024), (257, 2049, 640), (300, 5000, 129), (512, 512, 4096), (600, 600, 600), (777, 1111, 1357), (1000, 4096, 256), (1024, 1024, 1024),
-    (1500, 2300, 1100), (2048, 4096, 512), (4100, 260, 1024), (300, 20000, 256), (2, 5, 131071),
+    (1500, 2300, 1100), (2048, 4096, 512), (4100, 260, 1024), (300, 20000, 256), (2, 5, 131071), (2100, 1001, 300), (2101, 1003, 300), (2100, 1000, 301), (2500, 999, 127),
 ]
 
 
@@ -277,7 +277,7 @@ def test_sums_at_the_ends_of_32_bits(t0, rt, dev):
 
 
 GATED = [(1, 1, 1), (1, 11008, 4096), (2, 100, 100), (4, 333, 1357), (8, 2048, 512), (15, 4096, 640), (16, 1000, 4096), (17, 700, 300), (40, 5001, 256), (64, 4096, 1024), (100, 1433, 4096),
-         (128, 130, 2000), (129, 2048, 384), (200, 129, 129), (256, 3000, 512), (300, 1111, 1025), (600, 1000, 600), (1024, 2048, 256), (1300, 777, 1357), (2500, 512, 512)]
+         (128, 130, 2000), (129, 2048, 384), (200, 129, 129), (256, 3000, 512), (300, 1111, 1025), (600, 1000, 600), (1024, 2048, 256), (1300, 777, 1357), (2500, 512, 512), (2300, 701, 130), (2301, 705, 131)]
 
 
 @pytest.mark.parametrize("m, n, k", GATED)
