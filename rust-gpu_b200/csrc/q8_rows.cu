@@ -138,7 +138,7 @@ __device__ __forceinline__ double inverse_root(double m) {
 enum { kNone = 0, kBf16 = 1, kF32 = 2 };               // the residual's type
 
 // Rows of up to kThreads * kChunks * 8 numbers, kThreads threads each (four rows to a block where a warp has a row).
-//   kRing = false: a row a group of threads, loaded straight into registers: the shortest way for few rows.
+//   kRing = false: a row a group of threads, loaded straight into registers: the shortest way for few rows, and for short ones.
 //   kRing = true: groups walk over the rows, and copies bring the next ones into a ring in shared memory (P.slots rows), so that memory works while a row is reduced; a slot is filled again
 //     as soon as all threads have taken its numbers into registers.
 template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes, bool kRing>
@@ -338,18 +338,27 @@ cudaError_t launch_many(t0_runtime* rt, Rows& P) {
     return gemm::launch_pdl(kern, (uint32_t)std::min<uint64_t>(blocks, (uint64_t)at_once * rt->sm_count), kGroups * kThreads, P.slots * row_bytes, rt->stream, P);
 }
 
-// Up to two rows an SM: as many threads a row as have a chunk each, for the shortest chain (one row of 4096 through the norm: 2.9 us with 256 threads and two chunks). More: fewer threads a row,
-// several rows an SM at the same time.  With the norm a row has a long chain of sums, which more threads shorten (8192 x 4096, 256 threads and two chunks / 128 and four / 64 and eight:
-// 44.8 / 46.4 / 73.9 us); without it a thread's fixed work counts (8192 x 4096 with 256 / 128: 19.8 / 18.9; 16384 x 2048 with 128 / 64: 23.0 / 18.9).
+// As many rows as have a thread for each chunk of eight at the same time (2048 threads an SM): so many threads a row, for the shortest chain (one row of 4096 through the norm: 2.4 us; with 256
+// threads and two chunks 2.9).  More rows: fewer threads each and the ring.  With the norm a row has a long chain of sums, which more threads shorten (8192 x 4096, 256 threads and two chunks /
+// 128 and four / 64 and eight: 44.8 / 46.4 / 73.9 us); without it a thread's fixed work counts (8192 x 4096 with 256 / 128: 19.8 / 18.9; 16384 x 2048 with 128 / 64: 23.0 / 18.9).
+// Short rows never take the ring, whose copies are too small to be worth their issue: up to 256 numbers a warp a row (30000 x 128 through the norm: 14.5 us, 25.2 with it), with the norm up to
+// 1024 too (5000 x 1024: 10.3, 12.6 with it).
+// Directly / with the ring, us: 600 x 4096 3.5 / 3.9, 1200 x 4096 5.0 / 4.6, 2500 x 1024 3.7 / 3.6, norm of 300 x 512 2.4 / 2.8, of 1200 x 512 4.1 / 3.8.
 template <bool kNorm, bool kX32, int kRes>
 cudaError_t launch_by_dim(t0_runtime* rt, Rows& P) {
     const uint32_t d = P.dim;
-    if (P.n_rows <= 2u * rt->sm_count)
-        return d <= 1024 ? launch_few<128, 1, kNorm, kX32, kRes>(rt, P) : d <= 4096 ? launch_few<512, 1, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_few<1024, 1, kNorm, kX32, kRes>(rt, P)
-             : d <= 16384 ? launch_few<1024, 2, kNorm, kX32, kRes>(rt, P) : launch_few<1024, 4, kNorm, kX32, kRes>(rt, P);
-    return d <= 512 ? launch_many<32, 2, kNorm, kX32, kRes>(rt, P) : d <= 1024 ? launch_many<32, 4, kNorm, kX32, kRes>(rt, P) : d <= 2048 ? launch_many<kNorm ? 128 : 64, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
-         : d <= 4096 ? launch_many<kNorm ? 256 : 128, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P)
-         : d <= 16384 ? launch_many<kNorm ? 1024 : 512, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);
+    if (d <= 256) return launch_few<32, 1, kNorm, kX32, kRes>(rt, P);
+    const uint64_t threads = d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024;
+    if (P.n_rows * threads <= 2048ull * rt->sm_count || (kNorm && d > 512 && d <= 1024))
+        return d <= 512 ? launch_few<64, 1, kNorm, kX32, kRes>(rt, P) : d <= 1024 ? launch_few<128, 1, kNorm, kX32, kRes>(rt, P) : d <= 2048 ? launch_few<256, 1, kNorm, kX32, kRes>(rt, P)
+             : d <= 4096 ? launch_few<512, 1, kNorm, kX32, kRes>(rt, P) : d <= 8192 ? launch_few<1024, 1, kNorm, kX32, kRes>(rt, P) : d <= 16384 ? launch_few<1024, 2, kNorm, kX32, kRes>(rt, P)
+                         : launch_few<1024, 4, kNorm, kX32, kRes>(rt, P);
+    if (d <= 512) return launch_many<32, 2, kNorm, kX32, kRes>(rt, P);
+    if constexpr (!kNorm)
+        if (d <= 1024) return launch_many<32, 4, kNorm, kX32, kRes>(rt, P);
+    return d <= 2048 ? launch_many<kNorm ? 128 : 64, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : d <= 4096 ? launch_many<kNorm ? 256 : 128, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
+         : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P) : d <= 16384 ? launch_many<kNorm ? 1024 : 512, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
+                     : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);
 }
 
 template <bool kNorm>

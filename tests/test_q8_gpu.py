@@ -65,6 +65,9 @@ ROWS = [
     # rows, dim, f32
     (1, 1, True), (1, 7, False), (3, 8, False), (9, 64, True), (17, 100, False), (8, 1023, True), (33, 1024, False), (5, 1025, True), (6, 2048, False), (12, 2049, True),
     (150, 4096, False), (7, 4099, True), (3, 8192, True), (11, 8200, False), (2, 11008, True), (9, 14336, False), (8, 16385, False), (9, 28672, True), (1, 32768, False), (300, 32, True),
+    # enough rows for the ring
+    (4801, 300, False), (4740, 512, True), (2400, 1000, True), (2371, 1024, False), (1201, 1500, False), (1190, 2048, True), (610, 4096, False), (605, 3001, True), (300, 8192, False), (303, 5003, True),
+    (300, 12000, True), (299, 16384, False), (297, 20001, False), (298, 32768, True),
 ]
 
 
@@ -137,6 +140,10 @@ NORMS = [
     (20, 129, True, None, False, "y", ""), (9, 1000, False, "f32", False, "qy", "residual"), (9, 1024, True, "f32", False, "qy", "x"), (5, 2050, False, "bf16", True, "qy", "x"),
     (40, 4096, False, "bf16", False, "qy", ""), (8, 8191, True, "bf16", True, "q", ""), (8, 11008, False, None, False, "q", ""), (3, 16384, True, "f32", False, "y", ""),
     (8, 20001, False, "bf16", False, "qy", "residual"), (2, 32768, True, None, True, "q", ""), (700, 2048, False, "bf16", False, "q", "nothing"),
+    (4800, 500, True, "bf16", False, "qy", "residual"), (4737, 512, True, "f32", True, "q", "x"), (2500, 1021, False, "bf16", False, "q", "residual"), (1200, 2000, True, "f32", False, "qy", "x"),
+    (1187, 2048, False, None, False, "y", ""), (600, 4096, True, "bf16", False, "q", "residual"), (610, 3001, False, "f32", True, "qy", ""), (298, 8192, False, "bf16", False, "q", "residual"),
+    (300, 5000, True, "f32", False, "q", "residual"), (300, 16384, True, "bf16", True, "q", "residual"), (297, 9999, False, None, False, "qy", ""), (297, 32768, False, "bf16", False, "q", "residual"),
+    (298, 17000, True, "f32", False, "y", ""),
 ]
 
 
