@@ -20,7 +20,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 SOURCES = ["host_config.cpp", "cost_model.cpp", "tuner.cpp", "runtime.cu", "gemm_sm100.cu", "gemm_sm100_pair.cu", "gemm_sm100_splitk.cu", "aux_kernels.cu",
            "w4a16.cu", "w4a16_stream.cu", "w4a16_umma.cu", "w4a16_umma_cut.cu", "multi_gpu.cu", "no_alloc.cu", "matmul_f32.cu", "host_pipeline.cu",
-           "kv4_cache.cu", "kv4_attention.cu", "kv4_decode.cu", "kv4_prompt.cu", "q8_rows.cu", "q8_gemm.cu", "q8_pair.cu", "q8_stream.cu"]
+           "kv4_cache.cu", "kv4_attention.cu", "kv4_decode.cu", "kv4_prompt.cu", "q8_rows.cu", "q8_norm.cu", "q8_norm_f32.cu", "q8_gemm.cu", "q8_pair.cu", "q8_stream.cu"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-Wall,-Wno-unused-function", "-Xptxas", "-v", "--expt-relaxed-constexpr"]
