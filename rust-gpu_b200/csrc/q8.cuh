@@ -34,7 +34,7 @@ bool touch(uint64_t a, uint64_t a_bytes, uint64_t a_stride, uint64_t a_rows, uin
 
 // The kernels: what each is for stands with it.
 int launch_pair(t0_runtime* rt, const Product& P, bool gated);
-// How the stream kernel cuts a product: rows of the weights and tokens to a tile, parts of K; parts = 0: pairs take it.
+// How the stream kernel cuts a product: rows of the weights and tokens to a tile, parts of K (four at most); parts = 0: pairs take it.
 struct Cut { uint32_t rows, tokens, parts; };
 constexpr uint32_t kMostTokens = 256;      // of a tile, both products' together
 int launch_stream(t0_runtime* rt, const Product& P, bool gated, const Cut& cut);
