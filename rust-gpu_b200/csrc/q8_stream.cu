@@ -280,11 +280,9 @@ __global__ void __launch_bounds__(32 * kMostWarps) q8_stream_kernel(const __grid
     }
     ptx::tc_fence_before_sync();
     if (p.parts > 1) {
-        // loads in flight against loads of tokens that are not there: 16 x 4096 x 4096 in two parts 7.0 us, 7.3 with eight tokens; 128 rows 9.3, 9.5 with four
-        const uint32_t at = ptx::smem_u32(smem);
-        if (p.tokens <= 32 || (kGated && p.parts > 2)) add_parts<kGated, kMostParts, 2>(p, at, n0, m0, part, abort_flag);
-        else if (p.parts == 2) add_parts<kGated, 2, kGated ? 4 : 8>(p, at, n0, m0, part, abort_flag);
-        else add_parts<kGated, kMostParts, 4>(p, at, n0, m0, part, abort_flag);
+        // two tokens ahead (128 x 4096 x 4096 in four parts with one / two / four: 10.2 / 9.7 / 10.1 us; in two parts with two / four / eight: 9.2 / 9.4 / 9.3)
+        if (p.parts == 2) add_parts<kGated, 2, 2>(p, ptx::smem_u32(smem), n0, m0, part, abort_flag);
+        else add_parts<kGated, kMostParts, 2>(p, ptx::smem_u32(smem), n0, m0, part, abort_flag);
         ptx::cluster_sync_all();                       // a CTA's shared memory stays until all have read it
     } else {
         __syncthreads();
