@@ -9,8 +9,8 @@ namespace t0 {
 namespace q8 {
 namespace {
 
-// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 176 shapes (1 .. 1500 rows, n 256 .. 16384,
-// k 256 .. 14336, plain and gated; 20 cuts each): 1.5 % over each shape's best on average, 21 % at most.  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
+// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 236 shapes (1 .. 1500 rows, n 256 .. 16384,
+// k 256 .. 14336, plain and gated; 20 cuts each): 0.9 % over each shape's best on average, 21 % at most.  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
 // 128 x 4096 x 4096 12.4 / 9.3, 256 x 4096 x 4096 12.8 / 13.2, 512 x 4096 x 4096 13.0 / 16.2, 400 x 1024 x 4096 11.8 / 9.7, 1024 x 11008 x 4096 35.5 / 50.1.
 //   streamed, a round of tiles: k blocks times the slowest of { issuing a block's copies and products, the weights' way from memory (slower with few CTAs), all operands' way from L2, the
 //     products, one SM's way from L2 }, then the epilogue by its tokens, and the adding of parts;
@@ -18,18 +18,20 @@ namespace {
 float stream_time(const Product& P, uint32_t g, uint32_t tiles_m, const Cut& c, uint32_t clusters) {
     const uint32_t tiles = ceil_div(P.n, c.rows) * tiles_m, rounds = ceil_div(tiles, clusters), blocks = ceil_div(ceil_div(P.k, 128), c.parts);
     const float ctas = (float)std::min(tiles, clusters) * c.parts, w = g * c.rows * 128.0f, a = c.tokens * 128.0f;
-    float block = g == 1 ? 192.0f : 230.0f;
-    block = std::max(block, ctas * w / tiles_m / 7930.0f / std::cbrt(std::min(1.0f, ctas / 140.0f)));
-    block = std::max(block, std::max(ctas * (w + a) / 19500.0f, (w + a) / 170.0f));
+    float block = g == 1 ? 206.0f : 417.0f;
+    block = std::max(block, ctas * w / tiles_m / 8620.0f / std::cbrt(std::min(1.0f, ctas / 140.0f)));
+    block = std::max(block, std::max(ctas * (w + a) / 21600.0f, (w + a) / 256.0f));
     block = std::max(block, 1.42f * g * c.tokens);
-    const float parts = c.parts > 1 ? 1020.0f + 10.3f * g * c.tokens + 166.0f * (c.parts - 2) : 0.0f;
-    return 2910.0f + rounds * (blocks * block + 9.05f * g * c.tokens + parts + (c.rows % 32 ? 638.0f : 0.0f));
+    const float parts = c.parts > 1 ? 1190.0f + 11.3f * g * c.tokens + 165.0f * (c.parts - 2) : 0.0f;
+    return 2340.0f + rounds * (blocks * block + 7.29f * g * c.tokens + parts + (c.rows % 32 ? 187.0f : 0.0f));
 }
 float pair_time(const Product& P, uint32_t g, uint32_t pairs) {
     const uint64_t tiles_n = ceil_div(P.n, 256 / g), tiles = ceil_div(P.m, 256) * tiles_n, rest = tiles % pairs, halved = 2 * rest <= pairs ? rest : 0;
     const float blocks = (float)ceil_div(P.k, 128), rounds = (float)((tiles - halved + pairs - 1) / pairs);
-    const float whole = std::max(196.0f, std::min<uint64_t>(std::min<uint64_t>(tiles, pairs), tiles_n) * 32768 / 13400.0f), half = std::max(208.0f, std::min(halved, tiles_n) * 32768 / 13400.0f);
-    return 6700.0f + rounds * (blocks * whole + 3480.0f) + (halved ? blocks * half : 0.0f);
+    const float apart = P.a_stride % 128 || P.w_stride % 128 ? 1.23f : 1.0f;           // a row's 128 bytes lie in two lines
+    const float whole = std::max(134.0f * apart, std::min<uint64_t>(std::min<uint64_t>(tiles, pairs), tiles_n) * 32768 / 12400.0f);
+    const float half = std::max(171.0f * apart, std::min(halved, tiles_n) * 32768 / 12400.0f);
+    return 6930.0f + rounds * (blocks * whole + 3220.0f) + (halved ? blocks * half : 0.0f);
 }
 
 Cut choose(const Product& P, bool gated, uint32_t sms) {
