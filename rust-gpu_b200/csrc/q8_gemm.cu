@@ -9,8 +9,8 @@ namespace t0 {
 namespace q8 {
 namespace {
 
-// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 236 shapes (1 .. 1500 rows, n 256 .. 16384,
-// k 256 .. 14336, plain and gated; 20 cuts each): 0.9 % over each shape's best on average, 21 % at most.  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
+// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 376 shapes (1 .. 1500 rows, n 256 .. 16384,
+// k 256 .. 14336, plain and gated; 20 cuts each): 1.3 % over each shape's best on average, 24 % at most.  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
 // 128 x 4096 x 4096 12.4 / 9.3, 256 x 4096 x 4096 12.8 / 13.2, 512 x 4096 x 4096 13.0 / 16.2, 400 x 1024 x 4096 11.8 / 9.7, 1024 x 11008 x 4096 35.5 / 50.1.
 //   streamed, a round of tiles: k blocks times the slowest of { issuing a block's copies and products, the weights' way from memory (slower with few CTAs), all operands' way from L2, the
 //     products, one SM's way from L2 }, then the epilogue by its tokens, and the adding of parts;
@@ -18,8 +18,8 @@ namespace {
 float stream_time(const Product& P, uint32_t g, uint32_t tiles_m, const Cut& c, uint32_t clusters) {
     const uint32_t tiles = ceil_div(P.n, c.rows) * tiles_m, rounds = ceil_div(tiles, clusters), blocks = ceil_div(ceil_div(P.k, 128), c.parts);
     const float ctas = (float)std::min(tiles, clusters) * c.parts, w = g * c.rows * 128.0f, a = c.tokens * 128.0f;
-    float block = g == 1 ? 206.0f : 417.0f;
-    block = std::max(block, ctas * w / tiles_m / 8620.0f / std::cbrt(std::min(1.0f, ctas / 140.0f)));
+    float block = g * (160.0f + 0.5f * c.tokens);
+    block = std::max(block, ctas * w / tiles_m / 8000.0f / std::sqrt(std::sqrt(std::min(1.0f, ctas / 140.0f))));
     block = std::max(block, std::max(ctas * (w + a) / 21600.0f, (w + a) / 256.0f));
     block = std::max(block, 1.42f * g * c.tokens);
     const float parts = c.parts > 1 ? 1190.0f + 11.3f * g * c.tokens + 165.0f * (c.parts - 2) : 0.0f;
