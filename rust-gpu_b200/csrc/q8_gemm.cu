@@ -9,7 +9,7 @@ namespace t0 {
 namespace q8 {
 namespace {
 
-// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 376 shapes (1 .. 1500 rows, n 256 .. 16384,
+// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 430 shapes (1 .. 2200 rows, n 256 .. 16384,
 // k 256 .. 14336, plain and gated; 20 cuts each): 1.3 % over each shape's best on average, 24 % at most.  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
 // 128 x 4096 x 4096 12.4 / 9.3, 256 x 4096 x 4096 12.8 / 13.2, 512 x 4096 x 4096 13.0 / 16.2, 400 x 1024 x 4096 11.8 / 9.7, 1024 x 11008 x 4096 35.5 / 50.1.
 //   streamed, a round of tiles: k blocks times the slowest of { issuing a block's copies and products, the weights' way from memory (slower with few CTAs), all operands' way from L2, the
@@ -37,7 +37,7 @@ float pair_time(const Product& P, uint32_t g, uint32_t pairs) {
 Cut choose(const Product& P, bool gated, uint32_t sms) {
     const uint32_t g = gated ? 2 : 1, tiles_m = ceil_div(P.m, kMostTokens / g);
     Cut best = {0, 0, 0};
-    if (tiles_m > 8) return best;                                          // streamed, the weights would be read nine times
+    if (tiles_m > 6) return best;                                          // streamed, the weights would be read that often (1985 x 896 x 1740 12.0 us, on pairs 9.5; 1145 x 2304 x 4096 15.4 and 17.1)
     const uint32_t* at_once = gemm_clusters_at_once();
     float least = pair_time(P, g, std::max(1u, sms / 2));
     for (uint32_t parts = 1; parts <= 4 && parts <= ceil_div(P.k, 128); ++parts) {
