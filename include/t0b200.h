@@ -655,7 +655,8 @@ size_t t0_kv4_scratch_bytes(const t0_runtime* rt);
  *   a < 2^-119: scale 0 and codes 0;  an infinity or a NaN in the row: scale NaN and codes 0, so that all that is computed from the row is NaN.
  * An array holds rows * stride bytes; those between a row's length and its stride are never written, and what they hold changes no result.
  * Rows whose stride is a multiple of 128 are read fastest (8108 x 4736 x 7591 on strides of 7600: 268 us, of 7680: 204).
- * All calls run on the runtime's stream, allocate nothing and may be recorded.  Rows that a call writes must not lie where it reads, but for the places named below: refused. */
+ * All calls run on the runtime's stream, allocate nothing and may be recorded.  Rows that a call writes must not lie where it reads, but for the
+ * places named below, nor, where strides differ, between the first and the last row of what it reads: refused. */
 
 /* Rows of f32 (x_f32) or bf16 numbers into eight bits: activations, or a weight matrix [n][k] with a scale for each of its channels.  x: 16-byte aligned, x_stride in
  * numbers, a multiple of 8 (f32: 4), 0 = dense.  dim 1 .. 32768. */

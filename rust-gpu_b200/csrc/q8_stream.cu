@@ -4,6 +4,9 @@
 // 128 whatever is in them) by `tokens` rows of A (a multiple of 16, up to 256; 128 for the gated pair, whose two matrices take a tile each), and a CTA takes a tile, or a part of its
 // k blocks where the tiles of whole sums would be too few: the parts' CTAs form a cluster, park their sums in shared memory and share the adding out by tokens (whole numbers: the
 // order is of no matter).  A lane of tensor memory is one row of the weights, so a store instruction writes 32 neighbouring numbers of one row of y whatever its alignment.
+// 1 x 11008 x 4096 takes 10.0 us: 5.9 from the first block to the last (7.6 TB/s), the rest is launch (2.2), first operands (1.3) and epilogue (0.7).  Gated 100 x 14336 x 4096 takes 23.8: 15.8 for the
+// blocks (7.4 TB/s), 2.2 until the first is there, 2.5 of epilogue.  Shared memory for 192 KB of stages, one CTA an SM: with 96 KB and two CTAs too little is on its way (10.6 and 19.0 us for one
+// token plain and gated, 10.4 and 17.1 so).
 #include "gemm_common.cuh"
 #include "q8.cuh"
 #include "runtime_internal.h"

@@ -455,6 +455,53 @@ def test_many_calls_behind_one_another(t0, rt, dev):
     assert np.array_equal(layer.q.read(20 * 256, np.int8).reshape(20, 256), q) and same(layer.qs.read(80, np.float32), qs)
 
 
+@pytest.mark.parametrize("m, n, k", [(1, 3000, 1024), (24, 512, 2048), (300, 700, 512)])
+def test_weights_made_by_the_call_before(t0, rt, dev, m, n, k):
+    # a product asks for its first weights before the launch before it is over: what that launch writes is what it multiplies
+    rng = np.random.default_rng(n)
+    a, a_scales, ab, asb = rows8(rng, dev, m, k, up16(k))
+    sources = [rng.standard_normal((n, k)).astype(np.float32) for _ in range(3)]
+    bufs = [dev.up(s) for s in sources]
+    q, s = dev.up(np.zeros((n, up16(k)), np.int8)), dev.up(np.zeros(n, np.float32))
+    ys = [dev.up(np.zeros((m, n), np.float32)) for _ in range(24)]
+    for i, y in enumerate(ys):
+        rt.q8_quant(rt.q8_quant_args(bufs[i % 3].gpu_addr(), q.gpu_addr(), s.gpu_addr(), n_rows=n, dim=k, x_f32=True))
+        rt.q8_gemm(rt.q8_gemm_args(ab.gpu_addr(), asb.gpu_addr(), q.gpu_addr(), s.gpu_addr(), y.gpu_addr(), m=m, n=n, k=k))
+    rt.synchronize()
+    want = [ref.product(a, a_scales, *ref.hold(x)) for x in sources]
+    for i, y in enumerate(ys):
+        assert same(y.read(m * n * 4, np.float32).reshape(m, n), want[i % 3]), i
+
+
+def test_two_runtimes_at_once(t0, rt):
+    # products of every kernel on two streams beside one another: clusters of both wait for room, and nothing of one is another's
+    runs = [t0.GpuRuntime(0), t0.GpuRuntime(0)]
+    devs = [Device(r) for r in runs]
+    shapes = [(1, 2048, 1024), (20, 512, 4096), (40, 1024, 2048), (600, 1024, 512)]
+    jobs = []
+    for i, (r, d) in enumerate(zip(runs, devs)):
+        rng = np.random.default_rng(i)
+        for m, n, k in shapes:
+            a, w, u = rows8(rng, d, m, k, up16(k)), rows8(rng, d, n, k, up16(k)), rows8(rng, d, n, k, up16(k))
+            y, z = d.up(np.zeros((m, n), np.float32)), d.up(np.zeros((m, n), np.float32))
+            at = lambda b: b.gpu_addr()  # noqa: E731
+            jobs.append((i, r.q8_gemm, r.q8_gemm_args(at(a[2]), at(a[3]), at(w[2]), at(w[3]), at(y), m=m, n=n, k=k), y, ref.product(a[0], a[1], w[0], w[1])))
+            with np.errstate(over="ignore"):
+                g, v = ref.product(a[0], a[1], w[0], w[1]), ref.product(a[0], a[1], u[0], u[1])
+                jobs.append((i, r.q8_gated, r.q8_gated_args(at(a[2]), at(a[3]), at(w[2]), at(w[3]), at(u[2]), at(u[3]), at(z), m=m, n=n, k=k, activation="relu", out_bf16=False), z,
+                             np.maximum(g, 0) * v))
+    order = np.random.default_rng(5).permutation(np.repeat(np.arange(len(jobs)), 20))
+    for j in order:
+        jobs[j][1](jobs[j][2])
+    for r in runs:
+        r.synchronize()
+    for _, _, _, y, want in jobs:
+        assert same(y.read(want.size * 4, np.float32).reshape(want.shape), want)
+    for d, r in zip(devs, runs):
+        d.free()
+        r.close()
+
+
 def test_a_decoder_layer(t0, rt, dev):
     """norm, q/k/v product, cache append, attention, rows into eight bits, output product, norm with residual: each step against the restatement of what it was given."""
     import kv4_reference as kv4
