@@ -138,14 +138,16 @@ enum { kNone = 0, kBf16 = 1, kF32 = 2 };               // the residual's type
 
 // Rows of up to kThreads * kChunks * 8 numbers, kThreads threads each (four rows to a block where a warp has a row).
 //   kRing = false: a row a group of threads, loaded straight into registers: the shortest way for few rows, and for short ones.
-//   kRing = true: groups walk over the rows, and copies bring the next ones into a ring in shared memory (P.slots rows), so that memory works while a row is reduced; a slot is filled again
-//     as soon as all threads have taken its numbers into registers.
+//   kRing = true: groups walk over the rows, and copies bring the next ones into a ring in shared memory (P.slots rows), so that memory works while a row is reduced.
 //   kExact: the row fills the threads' chunks, and nothing asks where it ends (8192 x 4096 through the norm 44.9 -> 41.4 us, into eight bits 18.9 -> 18.3).
 // (Six blocks of the norm's 256 threads an SM: with five, which a few registers more make, 47.9 us.)
 template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes, bool kRing, bool kExact>
-__global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : !kNorm || kThreads == 32 ? 1024 / (kThreads == 32 ? 128 : kThreads) : kChunks == 2 && kThreads <= 256 ? 1536 / kThreads : 768 / kThreads) q8_rows_kernel(const Rows P) {
+__global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : !kNorm || kThreads == 32 ? 1024 / (kThreads == 32 ? 128 : kThreads) : kChunks == 2 && kThreads <= 256 ? 1536 / kThreads : kThreads >= 512 ? 1024 / kThreads : 768 / kThreads) q8_rows_kernel(const Rows P) {
     constexpr int kWarps = kThreads / 32, kGroups = kThreads == 32 ? 4 : 1;
     constexpr bool kEarly = kNorm && !kRing && kChunks <= 2;       // the weight is asked for with the row, where registers allow
+    // A slot is filled again when the row's threads have met for the first time where there may be but one slot a block (2000 x 16384 through the norm 42.5 us, 50.1 with one block an SM and three
+    // slots), else when the row is done: thread 0's warp is then not held up in the row's chain (8192 x 14336 into eight bits 56.6 us, 61.2).
+    constexpr bool kSoon = kNorm && kThreads >= 512;
     constexpr uint32_t kXSize = kX32 ? 4 : 2, kRSize = kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0;
     __shared__ double sums[2][kWarps];
     __shared__ uint32_t tops[2][kWarps];
@@ -179,6 +181,10 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
                 if (first + s * groups < P.n_rows) fill(first + s * groups, s);
     }
     uint32_t slot = 0, phase = 0, turn = 0;
+    const auto refill = [&](uint64_t row) {
+        if constexpr (kRing)
+            if (t == 0 && row + P.slots * groups < P.n_rows) fill(row + P.slots * groups, slot);
+    };
     for (uint64_t row = first; row < P.n_rows; row += groups, turn ^= 1) {
         if constexpr (kRing) {
             if (!ptx::mbar_wait_warp(ptx::smem_u32(&full[group][slot]), phase, &abort_flag, P.wait_limit_ns) && (t & 31) == 0) atomicCAS(P.status, 0, kStatusProducerTimeout | (int)(row & 0xFFFFFF));
@@ -238,6 +244,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
             if constexpr (kWarps > 1) {
                 if ((t & 31) == 0) sums[turn][warp] = sum;
                 __syncthreads();
+                if constexpr (kSoon) refill(row);
                 double s[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < kWarps; ++i) s[i & 3] += sums[turn][i];
@@ -299,9 +306,8 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
             }
         }
         if constexpr (kRing) {
-            // all threads have met since they took the slot's numbers (a warp that has a row to itself meets here)
-            if constexpr (kWarps == 1) __syncwarp();
-            if (t == 0 && row + P.slots * groups < P.n_rows) fill(row + P.slots * groups, slot);
+            if constexpr (kWarps == 1) __syncwarp();               // (the others have met)
+            if constexpr (!kSoon) refill(row);
             if (++slot == P.slots) slot = 0, phase ^= 1;
         } else {
             break;
@@ -321,11 +327,11 @@ cudaError_t launch_few(t0_runtime* rt, const Rows& P) {
 }
 template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes, bool kExact>
 cudaError_t launch_ring(t0_runtime* rt, Rows& P) {
-    constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1, kRoom = 200u << 10, kAtOnce = std::max(1, (kNorm ? 1536 : 1024) / (int)(kGroups * kThreads));
+    constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1, kRoom = 200u << 10, kAtOnce = std::max(1, (kNorm && kThreads < 512 ? 1536 : 1024) / (int)(kGroups * kThreads));
     P.residual_at = ((P.dim & ~7u) * (kX32 ? 4 : 2) + 127) & ~127u;
     P.slot_bytes = P.residual_at + (((P.dim & ~7u) * (kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0) + 127) & ~127u);
     const uint32_t row_bytes = std::max(1u, kGroups * P.slot_bytes);
-    const uint32_t at_once = std::max(1u, std::min(kAtOnce, kRoom / (2 * row_bytes)));       // blocks an SM
+    const uint32_t at_once = std::max(1u, std::min(kAtOnce, kRoom / ((kNorm && kThreads >= 512 ? 1 : 2) * row_bytes)));       // blocks an SM
     P.slots = std::min(kMostSlots, std::max(1u, kRoom / at_once / row_bytes));
     auto kern = q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, true, kExact>;
     static std::atomic<bool> ready[64];
@@ -365,7 +371,7 @@ cudaError_t launch_by_dim(t0_runtime* rt, Rows& P) {
     if constexpr (!kNorm)
         if (d <= 1024) return launch_many<32, 4, kNorm, kX32, kRes>(rt, P);
     return d <= 2048 ? launch_many<kNorm ? 128 : 64, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : d <= 4096 ? launch_many<kNorm ? 256 : 128, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
-         : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P) : d <= 16384 ? launch_many<kNorm ? 1024 : 512, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
+         : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P) : d <= 16384 ? launch_many<512, 4, kNorm, kX32, kRes>(rt, P)
                      : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);
 }
 
