@@ -370,6 +370,10 @@ cudaError_t launch_by_dim(t0_runtime* rt, Rows& P) {
     if (d <= 512) return launch_many<32, 2, kNorm, kX32, kRes>(rt, P);
     if constexpr (!kNorm)
         if (d <= 1024) return launch_many<32, 4, kNorm, kX32, kRes>(rt, P);
+    if constexpr (kNorm) {                                         // three chunks a thread where they are enough (4000 x 5120 42.7 -> 36.2 us, 2000 x 12288 42.6 -> 33.9)
+        if (d > 4096 && d <= 6144) return launch_many<256, 3, kNorm, kX32, kRes>(rt, P);
+        if (d > 8192 && d <= 12288) return launch_many<512, 3, kNorm, kX32, kRes>(rt, P);
+    }
     return d <= 2048 ? launch_many<kNorm ? 128 : 64, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : d <= 4096 ? launch_many<kNorm ? 256 : 128, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
          : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P) : d <= 16384 ? launch_many<512, 4, kNorm, kX32, kRes>(rt, P)
                      : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);

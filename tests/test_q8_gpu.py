@@ -143,7 +143,8 @@ NORMS = [
     (4800, 500, True, "bf16", False, "qy", "residual"), (4737, 512, True, "f32", True, "q", "x"), (2500, 1021, False, "bf16", False, "q", "residual"), (1200, 2000, True, "f32", False, "qy", "x"),
     (1187, 2048, False, None, False, "y", ""), (600, 4096, True, "bf16", False, "q", "residual"), (610, 3001, False, "f32", True, "qy", ""), (298, 8192, False, "bf16", False, "q", "residual"),
     (300, 5000, True, "f32", False, "q", "residual"), (300, 16384, True, "bf16", True, "q", "residual"), (297, 9999, False, None, False, "qy", ""), (297, 32768, False, "bf16", False, "q", "residual"),
-    (298, 17000, True, "f32", False, "y", ""),
+    (298, 17000, True, "f32", False, "y", ""), (299, 6144, False, "bf16", False, "q", "residual"), (300, 6000, True, "f32", True, "qy", "x"), (301, 12288, False, "bf16", True, "q", ""),
+    (298, 10001, True, None, False, "q", ""),
 ]
 
 
