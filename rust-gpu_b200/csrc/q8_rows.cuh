@@ -146,8 +146,8 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
     constexpr int kWarps = kThreads / 32, kGroups = kThreads == 32 ? 4 : 1;
     constexpr bool kEarly = kNorm && !kRing && kChunks <= 2;       // the weight is asked for with the row, where registers allow
     // A slot is filled again when the row's threads have met for the first time where there may be but one slot a block (2000 x 16384 through the norm 42.5 us, 50.1 with one block an SM and three
-    // slots), else when the row is done: thread 0's warp is then not held up in the row's chain (8192 x 14336 into eight bits 56.6 us, 61.2).
-    constexpr bool kSoon = kNorm && kThreads >= 512;
+    // slots; 2000 x 28672 of f32 into eight bits 50.1, 62.2 the other way), else when the row is done: thread 0's warp is then not held up in the row's chain (8192 x 14336 into eight bits 56.6 us, 61.2).
+    constexpr bool kSoon = kThreads >= (kNorm ? 512 : 1024);
     constexpr uint32_t kXSize = kX32 ? 4 : 2, kRSize = kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0;
     __shared__ double sums[2][kWarps];
     __shared__ uint32_t tops[2][kWarps];
@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
             if constexpr (kWarps > 1) {
                 if ((t & 31) == 0) tops[turn][warp] = top;
                 __syncthreads();
+                if constexpr (kSoon && !kNorm) refill(row);
                 top = 0;
 #pragma unroll
                 for (int i = 0; i < kWarps; ++i) top = max(top, tops[turn][i]);
