@@ -15,6 +15,7 @@ namespace t0 {
 namespace q8 {
 
 constexpr uint32_t kMostSlots = 16;
+constexpr uint32_t kMostRing = 220u << 10;             // shared memory that a ring may have; what a block has beside it is a few hundred bytes
 
 struct Rows {
     const void *x, *residual, *weight;
@@ -326,11 +327,17 @@ cudaError_t launch_few(t0_runtime* rt, const Rows& P) {
     constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1;
     return gemm::launch_pdl(q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, false, false>, (P.n_rows + kGroups - 1) / kGroups, kGroups * kThreads, 0, rt->stream, P);
 }
+// A row of x and one of the residual in the ring, each from a 128-byte boundary on.
+template <bool kX32, int kRes>
+void lay_out_slot(Rows& P) {
+    P.residual_at = ((P.dim & ~7u) * (kX32 ? 4 : 2) + 127) & ~127u;
+    P.slot_bytes = P.residual_at + (((P.dim & ~7u) * (kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0) + 127) & ~127u);
+}
+// (The caller has seen to it that one slot for each group is no more than kMostRing.)
 template <int kThreads, int kChunks, bool kNorm, bool kX32, int kRes, bool kExact>
 cudaError_t launch_ring(t0_runtime* rt, Rows& P) {
     constexpr uint32_t kGroups = kThreads == 32 ? 4 : 1, kRoom = 200u << 10, kAtOnce = std::max(1, (kNorm && kThreads < 512 ? 1536 : 1024) / (int)(kGroups * kThreads));
-    P.residual_at = ((P.dim & ~7u) * (kX32 ? 4 : 2) + 127) & ~127u;
-    P.slot_bytes = P.residual_at + (((P.dim & ~7u) * (kRes == kF32 ? 4 : kRes == kBf16 ? 2 : 0) + 127) & ~127u);
+    lay_out_slot<kX32, kRes>(P);
     const uint32_t row_bytes = std::max(1u, kGroups * P.slot_bytes);
     const uint32_t at_once = std::max(1u, std::min(kAtOnce, kRoom / ((kNorm && kThreads >= 512 ? 1 : 2) * row_bytes)));       // blocks an SM
     P.slots = std::min(kMostSlots, std::max(1u, kRoom / at_once / row_bytes));
@@ -338,7 +345,7 @@ cudaError_t launch_ring(t0_runtime* rt, Rows& P) {
     static std::atomic<bool> ready[64];
     if (rt->device < 0 || rt->device >= 64) return cudaErrorInvalidDevice;
     if (!ready[rt->device].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostRing);
         if (e != cudaSuccess) return e;
         ready[rt->device].store(true, std::memory_order_release);
     }
@@ -375,9 +382,14 @@ cudaError_t launch_by_dim(t0_runtime* rt, Rows& P) {
         if (d > 4096 && d <= 6144) return launch_many<256, 3, kNorm, kX32, kRes>(rt, P);
         if (d > 8192 && d <= 12288) return launch_many<512, 3, kNorm, kX32, kRes>(rt, P);
     }
+    if (d > 16384) {
+        // rows of f32 with a residual of f32 from 28168 numbers on: one of each is longer than the ring can be, and every row goes straight into registers (1000 x 28672 82.0 us, 297 x 32768 37.1; with a ring
+        // of one slot 1000 x 28160 takes 88.9)
+        lay_out_slot<kX32, kRes>(P);
+        return P.slot_bytes > kMostRing ? launch_few<1024, 4, kNorm, kX32, kRes>(rt, P) : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);
+    }
     return d <= 2048 ? launch_many<kNorm ? 128 : 64, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P) : d <= 4096 ? launch_many<kNorm ? 256 : 128, kNorm ? 2 : 4, kNorm, kX32, kRes>(rt, P)
-         : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P) : d <= 16384 ? launch_many<512, 4, kNorm, kX32, kRes>(rt, P)
-                     : launch_many<1024, 4, kNorm, kX32, kRes>(rt, P);
+         : d <= 8192 ? launch_many<256, 4, kNorm, kX32, kRes>(rt, P) : launch_many<512, 4, kNorm, kX32, kRes>(rt, P);
 }
 
 }  // namespace
