@@ -5,6 +5,8 @@
 // Pure C++: nothing here touches the GPU.
 #include "common.h"
 
+#include <cuda_runtime_api.h>
+
 #include <algorithm>
 #include <vector>
 
@@ -28,6 +30,9 @@ int fail(int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     g_last_error = buf;
+    // The CUDA runtime keeps what a call of it has failed with until somebody asks: an error that this call answers with is not left for the next one, which would take it for its own.
+    // (What a kernel has done to the device stays an error of every call all the same.)
+    if (code == T0_ERR_CUDA) (void)cudaGetLastError();
     return code;
 }
 
