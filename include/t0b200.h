@@ -183,7 +183,8 @@ int t0_rt_wait_idle(t0_runtime* rt);
  * memory and write a status word; the next synchronising call returns T0_ERR_TIMEOUT and poisons the runtime. */
 int t0_rt_set_wait_limit_ns(t0_runtime* rt, uint64_t ns);
 /* Self-test of that path (no counterpart in the reference): the NEXT GEMM launch of this runtime (bf16, or t0_q8_gemm / t0_q8_gated) leaves out the first
- * operand load of its first tile, so that tile's accumulate wait runs out after the wait limit.  Nothing faults and the
+ * operand load of its first tile, so that tile's accumulate wait runs out after the wait limit; the next t0_q8_quant or t0_q8_rmsnorm whose rows are brought by
+ * copies (more rows than the GPU has threads for at once) leaves out row 0's.  Nothing faults and the
  * kernel returns by itself; the call that synchronises reports T0_ERR_TIMEOUT, the runtime is poisoned, the output of
  * that launch is incomplete.  Set a short limit first (milliseconds).  For tests of the error handling only. */
 int t0_rt_selftest_drop_one_load(t0_runtime* rt);

@@ -112,6 +112,12 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
         }
     }
 }
+// One thread's wait on its way out of a kernel that has given up: until the phase is over, or the time `until` has come.
+__device__ __forceinline__ void mbar_wait_until(uint32_t bar, uint32_t parity, uint64_t until) {
+    while (!mbar_try_wait(bar, parity) && globaltimer_ns() < until) {}
+}
+// All of `threads` threads (whole warps) arrive at the barrier, each warp from where it is: a warp that leaves a loop meets those that go on.
+__device__ __forceinline__ void bar_sync(uint32_t barrier, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory"); }
 // True in one lane of a converged warp, the same one every time: what the whole warp has computed is issued once.
 __device__ __forceinline__ bool elect_one() {
     uint32_t is;

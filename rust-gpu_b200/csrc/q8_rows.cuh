@@ -26,6 +26,7 @@ struct Rows {
     uint64_t x_stride, residual_stride, residual_out_stride, q_stride, y_stride;
     uint32_t n_rows, dim;
     uint32_t slots, slot_bytes, residual_at;           // the ring: rows, bytes a row, where in it the residual begins
+    uint32_t drop_load;
     int* status;
     uint64_t wait_limit_ns;
     double inv_dim, eps;
@@ -137,6 +138,11 @@ __device__ __forceinline__ double inverse_root(double m) {
 
 enum { kNone = 0, kBf16 = 1, kF32 = 2 };               // the residual's type
 
+// What a warp that has given up on a row leaves in the place of its sum of squares, or of its largest size: neither is ever one.  (With a sum of minus infinity among them the mean is that or NaN, so
+// that only rows of next to nothing and of NaNs look for it.)
+constexpr double kGone = -HUGE_VAL;
+constexpr uint32_t kGoneTop = 0xFFFFFFFFu;
+
 // Rows of up to kThreads * kChunks * 8 numbers, kThreads threads each (four rows to a block where a warp has a row).
 //   kRing = false: a row a group of threads, loaded straight into registers: the shortest way for few rows, and for short ones.
 //   kRing = true: groups walk over the rows, and copies bring the next ones into a ring in shared memory (P.slots rows), so that memory works while a row is reduced.
@@ -179,16 +185,26 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
     if constexpr (kRing) {
         if (t == 0)
             for (uint32_t s = 0; s < P.slots; ++s)
-                if (first + s * groups < P.n_rows) fill(first + s * groups, s);
+                if (first + s * groups < P.n_rows && !(P.drop_load && first + s * groups == 0)) fill(first + s * groups, s);     // (self-test of the failure path: row 0 is not brought)
     }
     uint32_t slot = 0, phase = 0, turn = 0;
     const auto refill = [&](uint64_t row) {
         if constexpr (kRing)
             if (t == 0 && row + P.slots * groups < P.n_rows) fill(row + P.slots * groups, slot);
     };
-    for (uint64_t row = first; row < P.n_rows; row += groups, turn ^= 1) {
+    uint64_t row = first;
+    for (; row < P.n_rows; row += groups, turn ^= 1) {
         if constexpr (kRing) {
-            if (!ptx::mbar_wait_warp(ptx::smem_u32(&full[group][slot]), phase, &abort_flag, P.wait_limit_ns) && (t & 31) == 0) atomicCAS(P.status, 0, kStatusProducerTimeout | (int)(row & 0xFFFFFF));
+            if (!ptx::mbar_wait_warp(ptx::smem_u32(&full[group][slot]), phase, &abort_flag, P.wait_limit_ns)) {
+                // The row's other warps may have had their answer before: they are told where they next meet, and all leave the loop at this row, with nothing of it written but what the sum is kept in.
+                if ((t & 31) == 0) {
+                    atomicCAS(P.status, 0, kStatusProducerTimeout | (int)(row & 0xFFFFFF));
+                    if constexpr (kNorm) sums[turn][warp] = kGone;
+                    else tops[turn][warp] = kGoneTop;
+                }
+                if constexpr (kWarps > 1) ptx::bar_sync(1, kThreads);
+                break;
+            }
         }
         const uint32_t in_ring = mine + slot * P.slot_bytes;
         const char* const x_row = (const char*)P.x + row * P.x_stride * kXSize;
@@ -244,14 +260,17 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
             if constexpr (kWarps > 1) {
                 if ((t & 31) == 0) sums[turn][warp] = sum;
-                __syncthreads();
+                ptx::bar_sync(1, kThreads);
                 if constexpr (kSoon) refill(row);
                 double s[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < kWarps; ++i) s[i & 3] += sums[turn][i];
                 sum = (s[0] + s[1]) + (s[2] + s[3]);
             }
-            const float r = (float)inverse_root(fma(sum, P.inv_dim, P.eps));
+            const double mean = fma(sum, P.inv_dim, P.eps);
+            if constexpr (kRing && kWarps > 1)
+                if (!((float)mean > 1e-30f) && __any_sync(0xFFFFFFFFu, (t & 31) < kWarps && sums[turn][t & 31] == kGone)) break;
+            const float r = (float)inverse_root(mean);
             const float2 r2 = make_float2(r, r);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
@@ -280,11 +299,12 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
             uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most) & 0x7FFFFFFFu);
             if constexpr (kWarps > 1) {
                 if ((t & 31) == 0) tops[turn][warp] = top;
-                __syncthreads();
+                ptx::bar_sync(1, kThreads);
                 if constexpr (kSoon && !kNorm) refill(row);
                 top = 0;
 #pragma unroll
                 for (int i = 0; i < kWarps; ++i) top = max(top, tops[turn][i]);
+                if (kRing && !kNorm && top == kGoneTop) break;
             }
             most = __uint_as_float(top);
             const bool held = most >= 0x1p-119f && top < 0x7F800000u;
@@ -316,8 +336,15 @@ __global__ void __launch_bounds__(kThreads == 32 ? 128 : kThreads, !kRing ? 0 : 
         }
     }
     if constexpr (kRing) {
-        if (*(volatile int*)&abort_flag)                           // copies that were given up on may still be on their way
-            for (int i = 0; i < 64; ++i) __nanosleep(1000);
+        // The rows were left: the copies that are on their way land before the block's shared memory is another's.  They are waited for again, a millisecond at most: the row's, those of the slots behind
+        // it, and the slot's next one where it may have been asked for.
+        if (row < P.n_rows && t == 0) {
+            const uint64_t until = ptx::globaltimer_ns() + 1000000;
+            for (uint32_t s = 0; s < P.slots + kSoon && row < P.n_rows; ++s, row += groups) {
+                ptx::mbar_wait_until(ptx::smem_u32(&full[group][slot]), phase, until);
+                if (++slot == P.slots) slot = 0, phase ^= 1;
+            }
+        }
     }
 }
 
@@ -341,6 +368,7 @@ cudaError_t launch_ring(t0_runtime* rt, Rows& P) {
     const uint32_t row_bytes = std::max(1u, kGroups * P.slot_bytes);
     const uint32_t at_once = std::max(1u, std::min(kAtOnce, kRoom / ((kNorm && kThreads >= 512 ? 1 : 2) * row_bytes)));       // blocks an SM
     P.slots = std::min(kMostSlots, std::max(1u, kRoom / at_once / row_bytes));
+    P.drop_load = rt->drop_next_load.exchange(0) != 0;
     auto kern = q8_rows_kernel<kThreads, kChunks, kNorm, kX32, kRes, true, kExact>;
     static std::atomic<bool> ready[64];
     if (rt->device < 0 || rt->device >= 64) return cudaErrorInvalidDevice;

@@ -4,6 +4,7 @@ import ctypes
 import numpy as np
 import pytest
 
+import q8_reference as ref
 import test_q8_gpu as q8
 from test_q8_gpu import dev  # noqa: F401  (a fixture)
 from test_recorded_launches_gpu import Driver
@@ -55,3 +56,67 @@ def test_an_error_is_one_calls_own(t0, rt, dev):  # noqa: F811
     rt.fill_uniform_bf16(filled.gpu_addr(), 100, 1)
     rt.synchronize()
     filled.free()
+
+
+# --------------------------------------------------------------------------- waits that run out
+
+@pytest.mark.parametrize("rows, dim, norm", [(4801, 300, False), (1201, 1500, False), (605, 3001, False), (300, 8192, False), (299, 16384, False), (297, 20001, False), (4800, 500, True), (1200, 2000, True),
+                                             (600, 4096, True), (300, 6000, True), (300, 8192, True), (301, 12288, True), (300, 16384, True), (297, 17000, True)])
+def test_rows_whose_wait_runs_out_are_left(t0, rt, dev, rows, dim, norm):  # noqa: F811
+    # The copy of row 0 is left out: the threads that wait for it give up after the limit, write nothing of it and no row behind it, and the call that synchronises says so.  The other blocks' rows are
+    # as ever, and another runtime goes on.
+    rng = np.random.default_rng(rows + dim)
+    f32 = dim % 2 == 0
+    x = rng.standard_normal((rows, dim)).astype(np.float32)
+    x = x if f32 else ref.bf16_round(x)
+    res = ref.bf16_round(rng.standard_normal((rows, dim)).astype(np.float32))
+    weight = ref.bf16_round(rng.uniform(0.5, 1.5, dim).astype(np.float32))
+    wide, q_wide = (dim + 7) // 8 * 8, q8.up16(dim)
+    bx, bw = dev.up(q8.padded(x if f32 else ref.bf16_bits(x), wide, 0)), dev.up(ref.bf16_bits(weight))
+    br = dev.up(q8.padded(ref.bf16_bits(res), wide, 0))
+    bh, bq, bs, by = (dev.up(np.zeros(shape, kind)) for shape, kind in (((rows, wide), np.uint16), ((rows, q_wide), np.uint8), (rows, np.float32), ((rows, wide), np.uint16)))
+    at = lambda b: b.gpu_addr()  # noqa: E731
+    if norm:
+        want_y, h = ref.rmsnorm(x, weight, 1e-5, res, True)
+        want = [*ref.hold(want_y), ref.bf16_bits(want_y), ref.bf16_bits(h)]
+    else:
+        want = list(ref.hold(x))
+
+    def run(r):
+        for b, fill, kind in ((bh, 0xABCD, np.uint16), (bq, 0x5A, np.uint8), (bs, -7, np.float32), (by, 0xABCD, np.uint16)):
+            b.write(np.full(rows * {2: wide, 1: q_wide, 4: 1}[kind().itemsize], fill, kind))
+        rt.synchronize()
+        if norm:
+            r.q8_rmsnorm(r.q8_rmsnorm_args(at(bx), at(bw), n_rows=rows, dim=dim, eps=1e-5, x_f32=f32, x_stride=wide, residual=at(br), residual_stride=wide, residual_out=at(bh), residual_out_stride=wide,
+                                           q=at(bq), scales=at(bs), y=at(by), y_stride=wide))
+        else:
+            r.q8_quant(r.q8_quant_args(at(bx), at(bq), at(bs), n_rows=rows, dim=dim, x_f32=f32, x_stride=wide))
+
+    def read():
+        got = [bq.read(rows * q_wide, np.int8).reshape(rows, -1)[:, :dim], bs.read(rows * 4, np.float32), by.read(rows * wide * 2, np.uint16).reshape(rows, -1)[:, :dim],
+               bh.read(rows * wide * 2, np.uint16).reshape(rows, -1)[:, :dim]]
+        return got[:len(want)]
+
+    def rows_of(parts, others):
+        return np.all([(a == b).reshape(rows, -1).all(1) for a, b in zip(parts, others)], axis=0)
+
+    r = t0.GpuRuntime(0)
+    run(r)
+    r.synchronize()
+    assert rows_of(read(), want).all()
+    r.set_wait_limit_ns(3_000_000)
+    r.selftest_drop_one_load()
+    run(r)
+    with pytest.raises(t0.T0Error) as e:
+        r.synchronize()
+    assert e.value.code == 4 and "wait expired" in str(e.value) and r.is_poisoned()
+    got = read()
+    right, untouched = rows_of(got, want), rows_of(got, [0x5A, -7, 0xABCD, 0xABCD])
+    assert untouched[0] and (right | untouched).all() and right.sum() >= rows // 2
+    with pytest.raises(t0.T0Error) as e:
+        run(r)
+    assert e.value.code == 3
+    r.close()
+    run(rt)
+    rt.synchronize()
+    assert rows_of(read(), want).all()
