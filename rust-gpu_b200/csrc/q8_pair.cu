@@ -267,12 +267,12 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             const uint32_t buf = iter & 1, acc_phase = (iter >> 1) & 1;
             const uint32_t row0 = t.m * 256 + cta_rank * kHalf + quarter * 32, row = row0 + lane;
             const float a_scale = row < P.m ? P.a_scales[row] : 0.0f;
-            if (!ptx::mbar_wait(ptx::smem_u32(&tmem_full_bar[buf]), acc_phase, abort_flag, p.wait_limit_ns)) {
+            __syncwarp();
+            if (!ptx::mbar_wait_warp(ptx::smem_u32(&tmem_full_bar[buf]), acc_phase, abort_flag, p.wait_limit_ns)) {
                 if (lane == 0) atomicCAS(p.status, 0, kStatusEpilogueTimeout | (int)(w & 0xFFFFFF));
                 break;
             }
             ptx::tc_fence_after_sync();
-            __syncwarp();
             const uint32_t tmem = tmem_base + ((quarter * 32) << 16) + buf * 256, wide = t.halved ? kWide / 2 : kWide;
 #pragma unroll 1
             for (uint32_t i = 0;; ++i) {

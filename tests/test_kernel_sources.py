@@ -25,3 +25,15 @@ def test_the_streaming_epilogue_follows_no_ring(t0):
     role = text[text.index("four warps: accumulators to y"):text.index("give copies and UMMAs already in flight")]
     waits = re.findall(r"mbar_wait\w*\((\w+)", role)
     assert sorted(set(waits)) == ["acc_full", "end_near"], waits
+
+
+def test_warps_of_the_eight_bit_kernels_wait_as_one(t0):
+    # A wait that may give up answers lane by lane (mbar_wait): where another role gives up just as the phase ends, lanes of one warp would go two ways, and what follows in these kernels (votes, loads from
+    # tensor memory) is for whole warps.  They ask with the warp's one answer.
+    csrc = os.path.join(os.path.dirname(os.path.dirname(t0.HEADER_PATH)), "rust-gpu_b200", "csrc")
+    paths = sorted(glob.glob(os.path.join(csrc, "q8_*.cu*")))
+    assert len(paths) >= 6
+    for path in paths:
+        text = open(path).read()
+        assert not re.search(r"\bmbar_wait\(", text), path
+    assert "mbar_wait_warp(" in open(os.path.join(csrc, "q8_pair.cu")).read()
