@@ -221,7 +221,8 @@ gemm_bf16_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const _
             const WorkItem wi = decode_work(tail ? tail_start + ((w - tail_start) >> 1) : w, p);
             const uint32_t n_chunks = tail ? kHalfN / 32 : kPairN / 32;
             const uint32_t buf = iter & 1, acc_phase = (iter >> 1) & 1;
-            if (!ptx::mbar_wait(ptx::smem_u32(&tmem_full_bar[buf]), acc_phase, abort_flag, p.wait_limit_ns)) {
+            __syncwarp();
+            if (!ptx::mbar_wait_warp(ptx::smem_u32(&tmem_full_bar[buf]), acc_phase, abort_flag, p.wait_limit_ns)) {      // (one answer for the warp, whose loads from tensor memory and stores follow)
                 if (lane == 0) atomicCAS(p.status, 0, kStatusEpilogueTimeout | (int)(w & 0xFFFFFF));
                 break;
             }

@@ -37,3 +37,9 @@ def test_warps_of_the_eight_bit_kernels_wait_as_one(t0):
         text = open(path).read()
         assert not re.search(r"\bmbar_wait\(", text), path
     assert "mbar_wait_warp(" in open(os.path.join(csrc, "q8_pair.cu")).read()
+
+
+def test_warps_of_the_pair_kernel_wait_as_one(t0):
+    # the same of the bf16 kernel on CTA pairs
+    csrc = os.path.join(os.path.dirname(os.path.dirname(t0.HEADER_PATH)), "rust-gpu_b200", "csrc")
+    assert not re.search(r"\bmbar_wait\(", open(os.path.join(csrc, "gemm_sm100_pair.cu")).read())
