@@ -713,7 +713,8 @@ typedef struct t0_q8_gemm_args {
 } t0_q8_gemm_args;
 int t0_q8_gemm(t0_runtime* rt, const t0_q8_gemm_args* args);
 /* The gated pair of products of a feed-forward block in one kernel: y = act(g) * u with g = a gate^T and u = a up^T as t0_q8_gemm gives them in f32 (gate and up: [n][k] each, one w_stride),
- * act of {T0_TEPI_RELU, T0_TEPI_SILU, T0_TEPI_GELU}, their meaning that of the epilogues: x sigmoid(x), x sigmoid(1.702 x).  y as in t0_q8_gemm. */
+ * act of {T0_TEPI_RELU, T0_TEPI_SILU, T0_TEPI_GELU}, their meaning that of the epilogues: x sigmoid(x), x sigmoid(1.702 x), the sigmoid zero from 2^-128 on; RELU leaves a NaN.  f32 rows hold the
+ * epilogues' bits times u; for bf16 rows the sigmoid's reciprocal is the hardware's (2^-23 of its value).  y as in t0_q8_gemm. */
 typedef struct t0_q8_gated_args {
     uint64_t a, a_scales;
     uint64_t gate, gate_scales;

@@ -298,14 +298,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     v[4 * j] = x.x, v[4 * j + 1] = x.y, v[4 * j + 2] = y.x, v[4 * j + 3] = y.y;
                 }
                 if constexpr (kGated) {
-                    if (P.act == T0_TEPI_RELU) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 32; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
-                    } else {
-                        const float slope = slope_of(P.act);
-#pragma unroll
-                        for (uint32_t j = 0; j < 32; ++j) v[j] = gate_of(v[j], slope);
-                    }
+                    gate(v, P.act, P.out_bf16);
 #pragma unroll
                     for (uint32_t j = 0; j < 8; ++j) {
                         const float4 s = spread4(cols + 128, j);

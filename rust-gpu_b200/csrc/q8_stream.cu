@@ -62,14 +62,7 @@ __device__ __forceinline__ void finish(const StreamParams& p, const Column& c, c
         v[j] = x.x, v[j + 1] = x.y;
     }
     if constexpr (kGated) {
-        if (p.P.act == T0_TEPI_RELU) {
-#pragma unroll
-            for (int j = 0; j < kCount; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
-        } else {
-            const float slope = slope_of(p.P.act);
-#pragma unroll
-            for (int j = 0; j < kCount; ++j) v[j] = gate_of(v[j], slope);
-        }
+        gate(v, p.P.act, p.P.out_bf16);
 #pragma unroll
         for (int j = 0; j < kCount; j += 2) {
             const float2 x = mul2(make_float2(v[j], v[j + 1]), scaled(sum2[j], sum2[j + 1], make_float2(a_scale[j], a_scale[j + 1]), w2));

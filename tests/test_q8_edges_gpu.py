@@ -6,6 +6,7 @@ import pytest
 
 import q8_reference as ref
 import test_q8_gpu as q8
+from test_kernel_edges_gpu import run_gemm
 from test_q8_gpu import dev  # noqa: F401  (a fixture)
 from test_recorded_launches_gpu import Driver
 
@@ -120,3 +121,53 @@ def test_rows_whose_wait_runs_out_are_left(t0, rt, dev, rows, dim, norm):  # noq
     run(rt)
     rt.synchronize()
     assert rows_of(read(), want).all()
+
+
+# --------------------------------------------------------------------------- gates far from zero
+
+@pytest.mark.parametrize("m", [3, 600])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_far_below_zero(t0, rt, dev, m, bf16, act):  # noqa: F811
+    # The sigmoid of the epilogues keeps its values down to 2^-128; times a large number of the other product they are ordinary numbers.  Gates of -0.7 * 127 .. 0.7 * 127 (gelu: through
+    # 1.702 of them), each from one code, the other product 2^107.
+    # The bound is the restatement's relative one, (14 + 11 |g|) 2^-24, and half a step of bf16; what it allows beside that where the sigmoid has no normal number is not granted here.
+    n, k, slope = 255, 16, 1.702 if act == "gelu" else 1.0
+    a, gate, up = np.zeros((m, k), np.int8), np.zeros((n, k), np.int8), np.zeros((n, k), np.int8)
+    a[:, 0], gate[:, 0], up[:, 0] = 1, np.arange(n) - 127, 64
+    one, gs, us = np.ones(m, np.float32), np.full(n, 0.7 / slope, np.float32), np.full(n, 2.0**101, np.float32)
+    y = dev.up(np.zeros((m, n), np.uint16 if bf16 else np.float32))
+    at = lambda v: dev.up(v).gpu_addr()  # noqa: E731
+    rt.q8_gated(rt.q8_gated_args(at(a), at(one), at(gate), at(gs), at(up), at(us), y.gpu_addr(), m=m, n=n, k=k, activation=act, out_bf16=bf16))
+    rt.synchronize()
+    got = y.read(m * n * (2 if bf16 else 4), np.uint16 if bf16 else np.float32).reshape(m, n)
+    got = (ref.from_bits(got) if bf16 else got).astype(np.float64)
+    g = (np.arange(n) - 127) * gs.astype(np.float64)
+    power = -g * slope * np.log2(np.e)                                       # the sigmoid is 1 / (1 + 2^power)
+    want = g / (1 + np.exp2(power)) * 2.0**107
+    bound = ((14 + 11 * np.abs(g)) * 2.0**-24 + (2.0**-8 if bf16 else 0)) * np.abs(want)
+    kept = power < 128 * (1 - 2.0**-20)
+    assert kept.sum() < n and (power[kept] > 126.5).any()                    # both sides of where it ends
+    assert (np.abs(got - want) <= bound)[:, kept].all()
+    assert ((np.abs(got - want) <= bound) | (got == 0))[:, ~kept].all()
+
+
+@pytest.mark.parametrize("m", [1, 600])
+@pytest.mark.parametrize("act, factor", [("silu", 1.0), ("gelu", 1.702)])
+def test_gates_are_what_the_epilogues_compute(t0, rt, dev, m, act, factor):  # noqa: F811
+    # rows of f32: the bits of the epilogue of the same name (its argument the bias of a product of zeros), whatever the argument; the other product is one
+    rng = np.random.default_rng(8)
+    edges = np.array([0.0, 87.2, 87.4, 88.0, 88.72, 88.73, 89.0, 103.0, 1e4, 3e38, np.inf, np.nan, 1e-30, 1e-40], np.float32) / np.float32(factor)
+    v = np.concatenate([edges, rng.uniform(0, 110, 3000), rng.uniform(86, 90, 500) / factor, np.exp(rng.uniform(-80, 6, 500))]).astype(np.float32)
+    n, k = 2 * v.size, 16
+    sign = np.repeat(np.array([1, -1], np.int8), v.size)
+    v = np.tile(v, 2)
+    a, gate, up = np.zeros((m, k), np.int8), np.zeros((n, k), np.int8), np.zeros((n, k), np.int8)
+    a[:, 0], gate[:, 0], up[:, 0] = 1, sign, 1
+    y = dev.up(np.zeros((m, n), np.float32))
+    at = lambda b: dev.up(b).gpu_addr()  # noqa: E731
+    rt.q8_gated(rt.q8_gated_args(at(a), at(np.ones(m, np.float32)), at(gate), at(v), at(up), at(np.ones(n, np.float32)), y.gpu_addr(), m=m, n=n, k=k, activation=act, out_bf16=False))
+    rt.synchronize()
+    got = y.read(m * n * 4, np.float32).reshape(m, n)
+    want = run_gemm(t0, rt, np.zeros((1, 64), np.float32), np.zeros((n, 64), np.float32), 1, n, 64, bias=v * sign, tile_epilogue=["bias", act])[0]
+    assert all(q8.same(row, want) for row in got)
