@@ -7,7 +7,7 @@ import pytest
 import q8_reference as ref
 import test_q8_gpu as q8
 from test_kernel_edges_gpu import run_gemm
-from test_q8_gpu import dev  # noqa: F401  (a fixture)
+from test_q8_gpu import dev, same  # noqa: F401  (dev is a fixture)
 from test_recorded_launches_gpu import Driver
 
 pytestmark = pytest.mark.gpu
@@ -171,3 +171,72 @@ def test_gates_are_what_the_epilogues_compute(t0, rt, dev, m, act, factor):  # n
     got = y.read(m * n * 4, np.float32).reshape(m, n)
     want = run_gemm(t0, rt, np.zeros((1, 64), np.float32), np.zeros((n, 64), np.float32), 1, n, 64, bias=v * sign, tile_epilogue=["bias", act])[0]
     assert all(q8.same(row, want) for row in got)
+
+
+# --------------------------------------------------------------------------- roundings
+
+def test_the_read_out_rounds_to_f32_and_then_to_bf16(t0, rt, dev):  # noqa: F811
+    # products next to half way between two numbers of bf16, which are half way as f32: the second rounding goes to the even one, whichever side the product was on
+    rng = np.random.default_rng(4)
+    codes = rng.integers(1, 128, 400000).astype(np.int8)
+    half_way = (2 * rng.integers(128, 256, codes.size) + 1).astype(np.float64)                 # nine bits, the last one set
+    scales = (half_way / codes).astype(np.float32)
+    exact = scales.astype(np.float64) * codes
+    beside = (exact != half_way) & (exact.astype(np.float32) == half_way)
+    codes, scales, exact, half_way = codes[beside], scales[beside], exact[beside], half_way[beside]
+    once = np.where(exact > half_way, half_way + 1, half_way - 1)
+    twice = ref.bf16_round(half_way.astype(np.float32))
+    assert codes.size > 10000 and 0.3 < (once != twice).mean() < 0.7
+    q = np.zeros((codes.size, 16), np.int8)
+    q[:, 0] = codes
+    y = dev.up(np.zeros((codes.size, 8), np.uint16))
+    rt.q8_dequant(rt.q8_dequant_args(dev.up(q).gpu_addr(), dev.up(scales).gpu_addr(), y.gpu_addr(), n_rows=codes.size, dim=1, y_stride=8))
+    rt.synchronize()
+    assert np.array_equal(ref.from_bits(y.read(codes.size * 16, np.uint16)).reshape(-1, 8)[:, 0], twice)
+
+
+def added(squares, threads, chunks):
+    """A row's sum of squares as `threads` threads with `chunks` chunks of eight numbers add it in 64 bits."""
+    x = squares.reshape(chunks, threads, 8)
+    part = [np.zeros(threads) for _ in range(4)]
+    for c in range(chunks):
+        for i in range(8):
+            part[i % 4] = part[i % 4] + x[c, :, i]
+    s = ((part[0] + part[1]) + (part[2] + part[3])).reshape(-1, 32)
+    for d in (16, 8, 4, 2, 1):
+        s = s + s[:, np.arange(32) ^ d]
+    four = [0.0] * 4
+    for i, v in enumerate(s[:, 0]):
+        four[i % 4] += v
+    return (four[0] + four[1]) + (four[2] + four[3])
+
+
+def test_a_norms_row_alone_and_among_many(t0, rt, dev):  # noqa: F811
+    # A row is added up by 512 threads where rows are few and by 256 where they are many.  What comes of it is the same, but for rows whose root lies half way between two f32 as closely as 64 bits show:
+    # there it may be the one or the other.  Row 0 is made one of those, by its eps.
+    rng = np.random.default_rng(12)
+    dim, many = 4096, 700
+    while True:
+        row = rng.standard_normal(dim).astype(np.float32)
+        squares = row.astype(np.float64)**2
+        sums = [added(squares, 512, 1), added(squares, 256, 2)]
+        root = np.float32(1 / np.sqrt(sums[0] / dim))
+        half_way = 1 / ((np.float64(root) + np.float64(np.nextafter(root, np.float32(0)))) / 2)**2         # the mean from which on the root is the next lower f32
+        eps = half_way - sums[0] / dim
+        if sums[0] != sums[1] and 2.0**-31 < eps < 2.0**-29:
+            break
+    x = np.vstack([row, rng.standard_normal((many - 1, dim)).astype(np.float32)])
+    weight = rng.uniform(0.5, 1.5, dim).astype(np.float32)
+    bx, bw = dev.up(x), dev.up(weight)
+    for step in range(-3, 4):
+        e = np.float32(eps) + step * np.spacing(np.float32(eps))
+        got = []
+        for n in (1, 7, many):
+            q, s = dev.up(np.zeros((n, dim), np.int8)), dev.up(np.zeros(n, np.float32))
+            rt.q8_rmsnorm(rt.q8_rmsnorm_args(bx.gpu_addr(), bw.gpu_addr(), n_rows=n, dim=dim, eps=float(e), x_f32=True, weight_f32=True, q=q.gpu_addr(), scales=s.gpu_addr()))
+            rt.synchronize()
+            got.append((q.read(n * dim, np.int8).reshape(n, dim), s.read(4 * n, np.float32)))
+        assert np.array_equal(got[1][0][1:], got[2][0][1:7]) and same(got[1][1][1:], got[2][1][1:7])
+        either = [ref.hold((row * r) * weight) for r in (root, np.nextafter(root, np.float32(0)))]
+        for codes, scales in got:
+            assert any(np.array_equal(codes[0], c) and scales[0] == w for c, w in either)
