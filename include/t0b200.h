@@ -685,7 +685,7 @@ int t0_q8_dequant(t0_runtime* rt, const t0_q8_dequant_args* args);
  *   h = x + residual, rounded to f32, then to the residual's type, written to residual_out (residual = 0: h = x);
  *   y = (h * r) * weight with r = 1 / sqrt(sum h^2 / dim + eps): the sum and r in f64, r rounded to f32 once, both products rounded to f32;
  *   y into eight bits (q, scales) as above, or rounded to bf16 rows (y), or both.
- * The order of the f64 sum depends on n_rows and dim: where 1 / sqrt lies half way between two f32 to within 2^-50 or so (one row in some 2^25), the rows that a row comes with may decide which of
+ * The order of the f64 sum depends on n_rows and dim: where 1 / sqrt lies half way between two f32 to within 2^-50 or so (one row in some 2^30), the rows that a row comes with may decide which of
  * the two r is.  Nothing else of a row's result depends on the others.
  * x f32 (x_f32) or bf16, residual and residual_out f32 (residual_f32) or bf16, weight [dim] f32 (weight_f32) or bf16; all 16-byte aligned, strides in numbers as in t0_q8_quant.
  * residual_out may be residual itself or, of one type, x itself (strides equal); 0 = the sum is not kept.  dim 1 .. 32768; eps finite and not negative. */

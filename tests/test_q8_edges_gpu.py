@@ -125,7 +125,7 @@ def test_rows_whose_wait_runs_out_are_left(t0, rt, dev, rows, dim, norm):  # noq
 
 # --------------------------------------------------------------------------- gates far from zero
 
-@pytest.mark.parametrize("m", [3, 600])
+@pytest.mark.parametrize("m", [3, 600, 1000])
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_gates_far_below_zero(t0, rt, dev, m, bf16, act):  # noqa: F811
@@ -152,7 +152,7 @@ def test_gates_far_below_zero(t0, rt, dev, m, bf16, act):  # noqa: F811
     assert ((np.abs(got - want) <= bound) | (got == 0))[:, ~kept].all()
 
 
-@pytest.mark.parametrize("m", [1, 600])
+@pytest.mark.parametrize("m", [1, 600, 1000])
 @pytest.mark.parametrize("act, factor", [("silu", 1.0), ("gelu", 1.702)])
 def test_gates_are_what_the_epilogues_compute(t0, rt, dev, m, act, factor):  # noqa: F811
     # rows of f32: the bits of the epilogue of the same name (its argument the bias of a product of zeros), whatever the argument; the other product is one
@@ -240,3 +240,105 @@ def test_a_norms_row_alone_and_among_many(t0, rt, dev):  # noqa: F811
         either = [ref.hold((row * r) * weight) for r in (root, np.nextafter(root, np.float32(0)))]
         for codes, scales in got:
             assert any(np.array_equal(codes[0], c) and scales[0] == w for c, w in either)
+
+
+# --------------------------------------------------------------------------- scales that are no numbers, rows far apart
+
+@pytest.mark.parametrize("m", [5, 600, 1000])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_products_of_scales_that_are_no_numbers(t0, rt, dev, m, bf16, act):  # noqa: F811
+    # tokens and channels of either matrix whose scales are zero, infinite and NaN: what the formula makes of them, and the others' numbers as ever.  (A row's
+    # codes have one sign, so that no sum is zero.)
+    rng = np.random.default_rng(6)
+    n, k = 130, 64
+    a, g, u = (rng.integers(1, 60, (rows, k)).astype(np.int8) * np.repeat(rng.choice([-2, 2], rows), k).reshape(rows, k).astype(np.int8) for rows in (m, n, n))
+    a_scales, g_scales, u_scales = (np.exp(rng.uniform(-1, 1, rows)).astype(np.float32) * np.float32(s) for rows, s in ((m, 1e-3), (n, 1e-3), (n, 1.0)))
+    a_scales[1:4] = 0, np.inf, np.nan
+    g_scales[2:5] = u_scales[7:10] = 0, np.inf, np.nan
+    y = dev.up(np.zeros((m, n), np.uint16 if bf16 else np.float32))
+    at = lambda b: dev.up(b).gpu_addr()  # noqa: E731
+    rt.q8_gated(rt.q8_gated_args(at(a), at(a_scales), at(g), at(g_scales), at(u), at(u_scales), y.gpu_addr(), m=m, n=n, k=k, activation=act, out_bf16=bf16))
+    rt.synchronize()
+    got = y.read(m * n * (2 if bf16 else 4), np.uint16 if bf16 else np.float32).reshape(m, n)
+    got = (ref.from_bits(got) if bf16 else got).astype(np.float64)
+    with np.errstate(invalid="ignore", over="ignore"):
+        gate, up = (((a.astype(np.float64) @ w.T.astype(np.float64)) * a_scales[:, None]) * s for w, s in ((g, g_scales), (u, u_scales)))
+        if act == "relu":
+            want = np.where(gate < 0, 0.0, gate) * up
+        else:
+            want = gate * (1 / (1 + np.exp(-gate * (1.702 if act == "gelu" else 1.0)))) * up
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want).any() and np.isinf(want).any()
+        ends = np.isinf(want)
+        assert np.array_equal(got[ends], want[ends])
+        fine = np.isfinite(want)
+        # the restatement's bound; its relative part is zero where the value is, which 0 * infinity does not say (relu of minus infinity, times a finite number)
+        relative = np.where(want == 0, 0, (14 + 11 * np.abs(gate)) * 2.0**-24 * np.abs(want))
+        bound = relative + 2.0**-118 * np.abs(up) + 2.0**-140 + (2.0**-8 * np.abs(want) if bf16 else 0)
+        assert (np.abs(got - want)[fine] <= bound[fine]).all()
+
+
+class Far:
+    """Rows `step` bytes apart in one buffer, several arrays beside one another in each step."""
+
+    def __init__(self, rt, rows, step):
+        self.rt, self.rows, self.step, self.used = rt, rows, step, 0
+        self.buf = rt.alloc(rows * step)
+
+    def put(self, data):
+        at = self.used
+        for i, row in enumerate(data):
+            self.buf.write_bytes(i * self.step + at, np.ascontiguousarray(row))
+        self.used += (data[0].nbytes + 255) // 256 * 256
+        assert self.used <= self.step
+        return at, self.buf.gpu_addr() + at
+
+    def get(self, at, n, count, kind):
+        return np.stack([self.buf.read_bytes(i * self.step + at, count * kind().itemsize, kind) for i in range(n)])
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("wide", [72, 75])
+def test_products_on_pairs_of_rows_far_apart(t0, rt, dev, gated, wide):  # noqa: F811
+    # offsets beyond 32 bits on CTA pairs, whose y goes out by copies (72 numbers a row) and row by row (75): rows of every array 8 MiB apart
+    rng = np.random.default_rng(wide)
+    m, n, k, step = 1700, wide, 200, 8 << 20
+    far = Far(rt, m, step)
+    a, g, u = (rng.integers(-127, 128, (rows, k)).astype(np.int8) for rows in (m, n, n))
+    scales = [np.exp(rng.uniform(-1, 1, rows)).astype(np.float32) * np.float32(1e-2) for rows in (m, n, n)]
+    (_, pa), (_, pg), (_, pu) = far.put(a), far.put(g), far.put(u)
+    y_at, py = far.put(np.zeros((m, n + 4), np.float32))
+    sa, sg, su = (dev.up(s).gpu_addr() for s in scales)
+    strides = dict(m=m, n=n, k=k, a_stride=step, w_stride=step, y_stride=step // 4)
+    if gated:
+        rt.q8_gated(rt.q8_gated_args(pa, sa, pg, sg, pu, su, py, activation="relu", out_bf16=False, **strides))
+        want = np.maximum(ref.product(a, scales[0], g, scales[1]), 0) * ref.product(a, scales[0], u, scales[2])
+    else:
+        rt.q8_gemm(rt.q8_gemm_args(pa, sa, pg, sg, py, **strides))
+        want = ref.product(a, scales[0], g, scales[1])
+    rt.synchronize()
+    got = far.get(y_at, m, n + 4, np.float32)
+    far.buf.free()
+    assert same(got[:, :n].copy(), want) and (got[:, n:] == 0).all()
+
+
+@pytest.mark.parametrize("rows, dim, step", [(6, 512, 1 << 30), (1300, 1500, 4 << 20), (300, 20000, 16 << 20)])
+def test_norms_of_rows_far_apart(t0, rt, dev, rows, dim, step):  # noqa: F811
+    # directly and with the ring: x, the residual in place, codes and bf16 rows, each beyond 32 bits
+    rng = np.random.default_rng(dim)
+    x, res = rng.standard_normal((rows, dim)).astype(np.float32), rng.standard_normal((rows, dim)).astype(np.float32)
+    weight = rng.uniform(0.5, 1.5, dim).astype(np.float32)
+    far = Far(rt, rows, step)
+    _, px = far.put(x)
+    r_at, pr = far.put(res)
+    q_at, pq = far.put(np.zeros((rows, q8.up16(dim)), np.int8))
+    y_at, py = far.put(np.zeros((rows, dim + 8), np.uint16))
+    s = dev.up(np.zeros(rows, np.float32))
+    rt.q8_rmsnorm(rt.q8_rmsnorm_args(px, dev.up(weight).gpu_addr(), n_rows=rows, dim=dim, eps=1e-5, x_f32=True, weight_f32=True, residual=pr, residual_out=pr, residual_f32=True, q=pq,
+                                     scales=s.gpu_addr(), y=py, x_stride=step // 4, residual_stride=step // 4, residual_out_stride=step // 4, q_stride=step, y_stride=step // 2))
+    rt.synchronize()
+    want, h = ref.rmsnorm(x, weight, 1e-5, res, False)
+    codes, scales = ref.hold(want)
+    got = [far.get(r_at, rows, dim, np.float32), far.get(q_at, rows, dim, np.int8), far.get(y_at, rows, dim, np.uint16)]
+    far.buf.free()
+    assert same(got[0], h) and np.array_equal(got[1], codes) and np.array_equal(got[2], ref.bf16_bits(want)) and same(s.read(4 * rows, np.float32), scales)
