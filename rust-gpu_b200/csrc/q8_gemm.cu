@@ -9,8 +9,10 @@ namespace t0 {
 namespace q8 {
 namespace {
 
-// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found so that its choices lose least over 430 shapes (1 .. 2200 rows, n 256 .. 16384,
-// k 256 .. 14336, plain and gated; 20 cuts each): 1.3 % over each shape's best on average, 24 % at most.  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
+// Which kernel takes a product, and how it is cut: by a model of both kernels' times, its constants found over 430 shapes (1 .. 2200 rows, n 256 .. 16384, k 256 .. 14336, plain and gated; 20
+// cuts each).  On those shapes the choice, with its bound on tiles, takes 3.6 % more time than each one's best on average and 44 % at most (gated 1015 x 500 x 13312: 27.8 us on pairs, 19.3 streamed; then 931 x 290 x 7711
+// 19.0 / 13.6: gated tiles hold half the tokens, and the bound sends them to pairs from 769 rows on).  Shapes that the constants were not found on have not been measured; with weights beyond what L2 holds the
+// rate that pairs are given is too high, and few rows go there (gated 48 x 8192 x 8192 30.0 on pairs, 24.3 streamed).  Nanoseconds, and bytes per nanosecond.  Both sides, plain, us on pairs / streamed:
 // 128 x 4096 x 4096 12.4 / 9.3, 256 x 4096 x 4096 12.8 / 13.2, 512 x 4096 x 4096 13.0 / 16.2, 400 x 1024 x 4096 11.8 / 9.7, 1024 x 11008 x 4096 35.5 / 50.1.
 //   streamed, a round of tiles: k blocks times the slowest of { issuing a block's copies and products, the weights' way from memory (slower with few CTAs), all operands' way from L2, the
 //     products, one SM's way from L2 }, then the epilogue by its tokens, and the adding of parts;

@@ -5,7 +5,7 @@
 // The gated pair of products takes 128 rows of each matrix as the two halves of B: the even CTA loads the gate's, the odd one the other's, and the sums of one output stand in one
 // lane of tensor memory, 128 columns apart.  The tile gives 256 x 128 outputs, and neither product leaves the SM.
 // A last round that would leave half of the pairs idle is taken in half tiles.
-// 8192 x 14336 x 4096 takes 300 to 347 us by how warm the GPU is (2.8 to 3.2 POP/s, twice its bf16 rate), the gated pair 4096 x 11008 x 4096 236 to 256: the tensor pipe is busy 89 to 91 % of
+// 8192 x 14336 x 4096 takes 300 to 347 us by how warm the GPU is (2.8 to 3.2 POP/s, twice its bf16 rate), the gated pair 4096 x 11008 x 4096 236 to 258: the tensor pipe is busy 89 to 91 % of
 // the time and the power limit sets its clock.  Tiles of half the columns are bound by their operands' way from L2 (24 KB a block and CTA at 104 bytes a nanosecond): 256 x 4096 x 4096 12.8 us.
 #include "gemm_common.cuh"
 #include "q8.cuh"

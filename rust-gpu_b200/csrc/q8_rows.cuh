@@ -1,8 +1,8 @@
 // Rows into eight bits with a scale for each, the root-mean-square norm that leaves such rows, and the way back.
 //
 // A row is read once and stays in its threads' registers between the two passes over it (its largest number, or for the norm the sum of its squares and then its largest
-// number; the codes).  What bounds these kernels is memory, a row's bytes in and out, and with the norm the issue of instructions beside it: 8192 x 14336 of bf16 into eight bits 56.6 us (6.2 TB/s, 94 %
-// of a plain copy's rate), the norm with residual of 8192 x 4096 of bf16 41.5 us (5.7 TB/s, 69 % of issue; a thread's fixed work is half of it).
+// number; the codes).  What bounds these kernels is memory, a row's bytes in and out, and with the norm the issue of instructions beside it: 8192 x 14336 of bf16 into eight bits 56.4 us (6.2 TB/s, 95 %
+// of a plain copy's rate), the norm with residual of 8192 x 4096 of bf16 41.4 us (5.7 TB/s, 69 % of issue; a thread's fixed work is half of it).
 #pragma once
 
 #include <cmath>
